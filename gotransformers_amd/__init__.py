@@ -20,6 +20,7 @@ LIB_PATH = os.path.join(HERE, "libgtmoe.so")
 FLOAT64, FLOAT32, INT8, FP4 = 0, 1, 2, 3
 PATH_AUTO, PATH_FP32, PATH_BF16 = 0, 1, 2
 KERNEL_GATEUP, KERNEL_DOWN = 0, 1
+VALUES_FLOAT32, VALUES_BFLOAT16, VALUES_FLOAT16 = 0, 1, 2
 
 ROLE_ROUTER = 0
 ROLES = {("shared", "gate"): 1, ("shared", "up"): 2, ("shared", "down"): 3,
@@ -41,6 +42,8 @@ EXPORTED = [
     "gtmoe_layer_load_weights", "gtmoe_layer_add_adapters", "gtmoe_layer_remove_adapters", "gtmoe_layer_adapter_rank",
     "gtmoe_layer_set_adapter", "gtmoe_layer_get_adapter", "gtmoe_layer_adapter_gradients",
     "gtmoe_layer_zero_adapter_gradients", "gtmoe_backward",
+    "gtmoe_grouped_forward", "gtmoe_grouped_input_gradient", "gtmoe_grouped_weight_gradient",
+    "gtmoe_adapted_workspace", "gtmoe_adapted_forward", "gtmoe_dropout",
 ]
 
 
@@ -64,6 +67,23 @@ class RowsStruct(C.Structure):
     _fields_ = [("precision", C.c_int32), ("rows", C.c_int32), ("width", C.c_int32), ("reserved", C.c_int32),
                 ("values", C.c_void_p), ("values_bytes", C.c_size_t), ("scales", C.c_void_p),
                 ("scale_count", C.c_size_t)]
+
+
+class GroupedDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("groups", C.c_int32), ("rows", C.c_int32), ("inputs", C.c_int32),
+                ("outputs", C.c_int32), ("reserved", C.c_int32), ("input_stride", C.c_int64),
+                ("output_stride", C.c_int64), ("weight_stride", C.c_int64), ("group_stride", C.c_int64)]
+
+
+class AdaptedDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("rows", C.c_int32), ("inputs", C.c_int32), ("outputs", C.c_int32),
+                ("adapters", C.c_int32), ("rank", C.c_int32), ("input_stride", C.c_int64),
+                ("output_stride", C.c_int64), ("weight_stride", C.c_int64)]
+
+
+class DropoutDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("rows", C.c_int32), ("columns", C.c_int32), ("reserved", C.c_int32),
+                ("input_stride", C.c_int64), ("base_stride", C.c_int64), ("output_stride", C.c_int64)]
 
 
 _lib = None
@@ -132,6 +152,12 @@ def library():
         "gtmoe_layer_adapter_gradients": ([P, i32, i32, P, P], i32),
         "gtmoe_layer_zero_adapter_gradients": ([P], i32),
         "gtmoe_backward": ([P, i32, P, P], i32),
+        "gtmoe_grouped_forward": ([P, P, P, P, P, P, P], i32),
+        "gtmoe_grouped_input_gradient": ([P, P, P, P, P, P, P], i32),
+        "gtmoe_grouped_weight_gradient": ([P, P, P, P, P, P, i32, i32, P], i32),
+        "gtmoe_adapted_workspace": ([P, P], i32),
+        "gtmoe_adapted_forward": ([P, P, P, P, P, P, P, P, P, P, P, C.c_size_t, P], i32),
+        "gtmoe_dropout": ([P, P, P, P, P, dbl, C.c_uint64, C.c_uint64, P], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -549,6 +575,81 @@ class Graph:
 
     def __exit__(self, *exc):
         self.destroy()
+
+
+# --------------------------------------------------------------------------
+# operators over plain rows (raw device addresses, as forward_device)
+# --------------------------------------------------------------------------
+
+def grouped_desc(values, groups, rows, inputs, outputs, input_stride=None, output_stride=None, weight_stride=None,
+                 group_stride=None):
+    """gtmoe_grouped_desc; strides in values, contiguous unless given."""
+    ws = inputs if weight_stride is None else weight_stride
+    return GroupedDesc(values, groups, rows, inputs, outputs, 0, inputs if input_stride is None else input_stride,
+                       outputs if output_stride is None else output_stride, ws,
+                       outputs * ws if group_stride is None else group_stride)
+
+
+def grouped_forward(ctx, desc, offsets_ptr, inputs_ptr, weights_ptr, outputs_ptr, stream=None):
+    """outputs[r] = W_g inputs[r] for the rows of every group (gtmoe_grouped_forward)."""
+    ctx.check(library().gtmoe_grouped_forward(ctx.handle, C.byref(desc), offsets_ptr, inputs_ptr, weights_ptr,
+                                              outputs_ptr, stream))
+
+
+def grouped_input_gradient(ctx, desc, offsets_ptr, output_gradients_ptr, weights_ptr, input_gradients_ptr, stream=None):
+    """input_gradients[r] = W_g^T output_gradients[r]."""
+    ctx.check(library().gtmoe_grouped_input_gradient(ctx.handle, C.byref(desc), offsets_ptr, output_gradients_ptr,
+                                                     weights_ptr, input_gradients_ptr, stream))
+
+
+def grouped_weight_gradient(ctx, desc, offsets_ptr, output_gradients_ptr, inputs_ptr, weight_gradients_ptr,
+                            gradient_values, accumulate=False, stream=None):
+    """weight_gradients[g] (+)= sum of output_gradients[r] inputs[r]^T, of type gradient_values."""
+    ctx.check(library().gtmoe_grouped_weight_gradient(ctx.handle, C.byref(desc), offsets_ptr, output_gradients_ptr,
+                                                      inputs_ptr, weight_gradients_ptr, gradient_values,
+                                                      1 if accumulate else 0, stream))
+
+
+def adapted_desc(values, rows, inputs, outputs, adapters, rank, input_stride=None, output_stride=None,
+                 weight_stride=None):
+    """gtmoe_adapted_desc; strides in values, contiguous unless given."""
+    return AdaptedDesc(values, rows, inputs, outputs, adapters, rank, inputs if input_stride is None else input_stride,
+                       outputs if output_stride is None else output_stride,
+                       inputs if weight_stride is None else weight_stride)
+
+
+def adapted_workspace_bytes(desc):
+    """Bytes of the workspace adapted_forward needs: the rows' products with
+    their Down matrices in fp32, padded to eight ranks."""
+    n = C.c_size_t(0)
+    _check(library().gtmoe_adapted_workspace(C.byref(desc), C.byref(n)))
+    return n.value
+
+
+def adapted_forward(ctx, desc, inputs_ptr, weights_ptr, biases_ptr, adapter_ptr, down_ptr, up_ptr, scales_ptr,
+                    outputs_ptr, workspace_ptr, stream=None, workspace_bytes=None):
+    """outputs[t] = W inputs[t] + b + s_a Up_a (Down_a inputs[t]) with each
+    row's own adapter a; weights_ptr None: added to outputs (gtmoe_adapted_forward).
+    workspace_bytes: the workspace's size, adapted_workspace_bytes(desc) unless given."""
+    n = adapted_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    ctx.check(library().gtmoe_adapted_forward(ctx.handle, C.byref(desc), inputs_ptr, weights_ptr, biases_ptr,
+                                              adapter_ptr, down_ptr, up_ptr, scales_ptr, outputs_ptr, workspace_ptr, n,
+                                              stream))
+
+
+def dropout_desc(values, rows, columns, input_stride=None, base_stride=None, output_stride=None):
+    """gtmoe_dropout_desc; strides in values, contiguous unless given."""
+    return DropoutDesc(values, rows, columns, 0, columns if input_stride is None else input_stride,
+                       columns if base_stride is None else base_stride,
+                       columns if output_stride is None else output_stride)
+
+
+def dropout(ctx, desc, inputs_ptr, base_ptr, outputs_ptr, rate, seed, offset, stream=None):
+    """outputs = [base +] dropout(inputs), the mask a function of (seed,
+    offset, row, column) (gtmoe_dropout); the same call on the output
+    gradients is the backward."""
+    ctx.check(library().gtmoe_dropout(ctx.handle, C.byref(desc), inputs_ptr, base_ptr, outputs_ptr, float(rate),
+                                      int(seed), int(offset), stream))
 
 
 # --------------------------------------------------------------------------

@@ -25,6 +25,8 @@ SOURCES = [
     ("experts_mfma.hip", []),
     ("misc.hip", []),
     ("lora.hip", []),
+    ("grouped.hip", []),
+    ("dropout.hip", []),
     ("api.cpp", []),
     ("encode.cpp", ["-ffp-contract=off"]),
     ("weightfile.cpp", []),

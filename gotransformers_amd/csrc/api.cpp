@@ -19,6 +19,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "grouped.h"
 #include "kernels.h"
 #include "gtmoe.h"
 #include "weightfile.h"
@@ -2842,6 +2843,449 @@ int32_t gtmoe_backward(gtmoe_layer *L, int32_t tokens, const double *output_grad
     if (!output_gradients || !input_gradients)
         return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "output or input gradients are null");
     return adapter_backward(L, tokens, output_gradients, input_gradients);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Operators over plain rows.  They keep nothing between calls: every buffer,
+// a workspace among them, is the caller's.
+// ---------------------------------------------------------------------------
+
+namespace {
+
+constexpr int kMaxPlainWidth = 1 << 20;  // widths and row strides: byte offsets inside a tile stay in 31 bits
+constexpr int kMaxPlainRows = 1 << 30;
+constexpr int kMaxPlainGroups = 4096;
+constexpr int kMaxAdapterRank = 256;
+
+// Rows of `width` bytes, `stride` bytes apart.
+struct Span {
+    const void *p;
+    int64_t rows, width, stride;
+};
+
+// Whether two sets of rows share a byte.  Rows of one stride may interleave
+// (column ranges of one matrix) without sharing any.
+bool overlap(const Span &a, const Span &b)
+{
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    const uintptr_t ea = pa + (uintptr_t)((a.rows - 1) * a.stride + a.width);
+    const uintptr_t eb = pb + (uintptr_t)((b.rows - 1) * b.stride + b.width);
+    if (ea <= pb || eb <= pa) return false;
+    if (a.stride != b.stride || a.rows == 1 || b.rows == 1) return true;
+    const int64_t st = a.stride;
+    const int64_t d = (int64_t)(pb - pa) % st, off = d < 0 ? d + st : d;
+    return !(off >= a.width && off + b.width <= st);
+}
+
+int32_t check_values(gtmoe_context *ctx, int32_t values)
+{
+    if (values < GTMOE_VALUES_FLOAT32 || values > GTMOE_VALUES_FLOAT16)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "unknown type of values %d", values);
+    return GTMOE_OK;
+}
+
+// A row stride in values: at least the row's width, at most the limit.
+int32_t check_stride(gtmoe_context *ctx, const char *what, int64_t stride, int64_t width)
+{
+    if (stride < width || stride > kMaxPlainWidth)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s stride %lld must be between the width %lld and %d", what,
+                    (long long)stride, (long long)width, kMaxPlainWidth);
+    return GTMOE_OK;
+}
+
+int32_t check_size(gtmoe_context *ctx, const char *what, int64_t v, int64_t lo, int64_t hi)
+{
+    if (v < lo || v > hi)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s must be between %lld and %lld, got %lld", what, (long long)lo,
+                    (long long)hi, (long long)v);
+    return GTMOE_OK;
+}
+
+int32_t check_apart(gtmoe_context *ctx, const char *what, const Span &out, std::initializer_list<Span> others)
+{
+    for (const Span &o : others)
+        if (overlap(out, o)) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s overlap another buffer of the call", what);
+    return GTMOE_OK;
+}
+
+// Pointers to values: multiples of their size.
+int32_t check_pointer(gtmoe_context *ctx, const char *what, const void *p, int bytes)
+{
+    if (!p) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s are null", what);
+    if ((uintptr_t)p % bytes != 0)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s are not aligned to %d bytes", what, bytes);
+    return GTMOE_OK;
+}
+
+#define TRY(expr)                               \
+    do {                                        \
+        const int32_t rc_ = (expr);             \
+        if (rc_ != GTMOE_OK) return rc_;        \
+    } while (0)
+
+int32_t check_grouped(gtmoe_context *ctx, const gtmoe_grouped_desc *d, const int32_t *offsets)
+{
+    if (!d) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+    TRY(check_values(ctx, d->values));
+    TRY(check_size(ctx, "groups", d->groups, 1, kMaxPlainGroups));
+    TRY(check_size(ctx, "rows", d->rows, 0, kMaxPlainRows));
+    TRY(check_size(ctx, "inputs", d->inputs, 1, kMaxPlainWidth));
+    TRY(check_size(ctx, "outputs", d->outputs, 1, kMaxPlainWidth));
+    if (d->reserved != 0) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "reserved must be 0");
+    TRY(check_stride(ctx, "input", d->input_stride, d->inputs));
+    TRY(check_stride(ctx, "output", d->output_stride, d->outputs));
+    TRY(check_stride(ctx, "weight", d->weight_stride, d->inputs));
+    const int64_t matrix = (d->outputs - 1) * d->weight_stride + d->inputs;
+    if (d->group_stride < matrix || d->group_stride > ((int64_t)1 << 48) / d->groups)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "group stride %lld is less than a matrix of %lld values or too large",
+                    (long long)d->group_stride, (long long)matrix);
+    return check_pointer(ctx, "offsets", offsets, 4);
+}
+
+Span rows_span(const void *p, int64_t rows, int64_t width, int64_t stride, int bytes)
+{
+    return {p, rows, width * bytes, stride * bytes};
+}
+
+Span offsets_span(const gtmoe_grouped_desc *d, const int32_t *offsets)
+{
+    return {offsets, 1, 4 * ((int64_t)d->groups + 1), 0};
+}
+
+Span grouped_matrices(const gtmoe_grouped_desc *d, const void *p, int bytes)
+{
+    const int64_t n = (d->groups - 1) * d->group_stride + (d->outputs - 1) * d->weight_stride + d->inputs;
+    return {p, 1, n * bytes, n * bytes};
+}
+
+// Without a context a call's arguments are checked and the call refused (text
+// in gtmoe_last_error(NULL)): nothing can run.
+template <class F>
+int32_t check_only(F &&check)
+{
+    TRY(check(nullptr));
+    return fail(nullptr, GTMOE_ERR_INVALID_ARGUMENT, "the context is null");
+}
+
+// Runs `fn`, whose kernels go to stream s: without event timing while s is
+// being captured into a graph (the events would become nodes of it).
+template <class F>
+int32_t run_plain(gtmoe_context *ctx, hipStream_t s, const char *name, F &&fn)
+{
+    const bool timing = ctx->timing;
+    if (timing) {
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+            (void)hipGetLastError();
+            ctx->timing = false;
+        }
+    }
+    const int32_t rc = run(ctx, s, name, fn);
+    ctx->timing = timing;
+    return rc;
+}
+
+GroupedArgs grouped_args(const gtmoe_grouped_desc *d, const int32_t *offsets)
+{
+    GroupedArgs a;
+    a.offsets = offsets;
+    a.groups = d->groups;
+    a.rows = d->rows;
+    a.inputs = d->inputs;
+    a.outputs = d->outputs;
+    a.group_stride = d->group_stride;
+    return a;
+}
+
+int32_t check_grid(gtmoe_context *ctx, const GroupedArgs &a, int direction, int values)
+{
+    if (!grouped_fits(a, direction, values))
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%d rows in %d groups of %d x %d are more tiles than one launch holds",
+                    a.rows, a.groups, a.outputs, a.inputs);
+    return GTMOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t gtmoe_grouped_forward(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                              const void *inputs, const void *weights, void *outputs, void *stream)
+{
+    GroupedArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_grouped(c, desc, offsets));
+        const int es = value_bytes(desc->values);
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "inputs", inputs, es));
+            TRY(check_pointer(c, "weights", weights, es));
+            TRY(check_pointer(c, "outputs", outputs, es));
+            TRY(check_apart(c, "outputs", rows_span(outputs, desc->rows, desc->outputs, desc->output_stride, es),
+                            {rows_span(inputs, desc->rows, desc->inputs, desc->input_stride, es),
+                             grouped_matrices(desc, weights, es), offsets_span(desc, offsets)}));
+        }
+        a = grouped_args(desc, offsets);
+        a.a = inputs;
+        a.lda = desc->input_stride;
+        a.b = weights;
+        a.ldb = desc->weight_stride;
+        a.out = outputs;
+        a.ldo = desc->output_stride;
+        return check_grid(c, a, kGroupedForward, desc->values);
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "grouped_forward", [&] { return launch_grouped(a, kGroupedForward, desc->values, s); });
+}
+
+int32_t gtmoe_grouped_input_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                                     const void *output_gradients, const void *weights, void *input_gradients,
+                                     void *stream)
+{
+    GroupedArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_grouped(c, desc, offsets));
+        const int es = value_bytes(desc->values);
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "output gradients", output_gradients, es));
+            TRY(check_pointer(c, "weights", weights, es));
+            TRY(check_pointer(c, "input gradients", input_gradients, es));
+            TRY(check_apart(c, "input gradients",
+                            rows_span(input_gradients, desc->rows, desc->inputs, desc->input_stride, es),
+                            {rows_span(output_gradients, desc->rows, desc->outputs, desc->output_stride, es),
+                             grouped_matrices(desc, weights, es), offsets_span(desc, offsets)}));
+        }
+        a = grouped_args(desc, offsets);
+        a.a = output_gradients;
+        a.lda = desc->output_stride;
+        a.b = weights;
+        a.ldb = desc->weight_stride;
+        a.out = input_gradients;
+        a.ldo = desc->input_stride;
+        return check_grid(c, a, kGroupedInputGradient, desc->values);
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "grouped_input_gradient",
+                     [&] { return launch_grouped(a, kGroupedInputGradient, desc->values, s); });
+}
+
+int32_t gtmoe_grouped_weight_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                                      const void *output_gradients, const void *inputs, void *weight_gradients,
+                                      int32_t gradient_values, int32_t accumulate, void *stream)
+{
+    GroupedArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_grouped(c, desc, offsets));
+        if (gradient_values != desc->values && gradient_values != GTMOE_VALUES_FLOAT32)
+            return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "weight gradients are of the values' type or float32, got %d",
+                        gradient_values);
+        const int es = value_bytes(desc->values), gs = value_bytes(gradient_values);
+        TRY(check_pointer(c, "weight gradients", weight_gradients, gs));
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "output gradients", output_gradients, es));
+            TRY(check_pointer(c, "inputs", inputs, es));
+        }
+        TRY(check_apart(c, "weight gradients", grouped_matrices(desc, weight_gradients, gs),
+                        {rows_span(output_gradients, desc->rows, desc->outputs, desc->output_stride, es),
+                         rows_span(inputs, desc->rows, desc->inputs, desc->input_stride, es),
+                         offsets_span(desc, offsets)}));
+        a = grouped_args(desc, offsets);
+        a.a = output_gradients;
+        a.lda = desc->output_stride;
+        a.b = inputs;
+        a.ldb = desc->input_stride;
+        a.out = weight_gradients;
+        a.ldo = desc->weight_stride;
+        a.out_f32 = gradient_values == GTMOE_VALUES_FLOAT32;
+        a.accumulate = accumulate != 0;
+        return check_grid(c, a, kGroupedWeightGradient, desc->values);
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "grouped_weight_gradient",
+                     [&] { return launch_grouped(a, kGroupedWeightGradient, desc->values, s); });
+}
+
+}  // extern "C"
+
+namespace {
+
+int32_t check_adapted(gtmoe_context *ctx, const gtmoe_adapted_desc *d)
+{
+    if (!d) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+    TRY(check_values(ctx, d->values));
+    TRY(check_size(ctx, "rows", d->rows, 0, kMaxPlainRows));
+    TRY(check_size(ctx, "inputs", d->inputs, 1, kMaxPlainWidth));
+    TRY(check_size(ctx, "outputs", d->outputs, 1, kMaxPlainWidth));
+    TRY(check_size(ctx, "adapters", d->adapters, 1, kMaxPlainWidth));
+    TRY(check_size(ctx, "rank", d->rank, 1, kMaxAdapterRank));
+    TRY(check_stride(ctx, "input", d->input_stride, d->inputs));
+    TRY(check_stride(ctx, "output", d->output_stride, d->outputs));
+    return check_stride(ctx, "weight", d->weight_stride, d->inputs);
+}
+
+int adapter_ldu(const gtmoe_adapted_desc *d) { return (d->rank + 7) / 8 * 8; }
+
+}  // namespace
+
+extern "C" {
+
+int32_t gtmoe_adapted_workspace(const gtmoe_adapted_desc *desc, size_t *bytes)
+{
+    if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
+    TRY(check_adapted(nullptr, desc));
+    *bytes = (size_t)std::max(desc->rows, 1) * adapter_ldu(desc) * sizeof(float);
+    return GTMOE_OK;
+}
+
+int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc, const void *inputs,
+                              const void *weights, const void *biases, const int32_t *adapter, const void *down,
+                              const void *up, const float *scales, void *outputs, void *workspace,
+                              size_t workspace_bytes, void *stream)
+{
+    GroupedArgs a;
+    AdapterDownArgs dargs;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_adapted(c, desc));
+        const int es = value_bytes(desc->values), ldu = adapter_ldu(desc);
+        const size_t need = (size_t)desc->rows * ldu * sizeof(float);
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "inputs", inputs, es));
+            if (weights) TRY(check_pointer(c, "weights", weights, es));
+            if (biases) TRY(check_pointer(c, "biases", biases, es));
+            TRY(check_pointer(c, "adapters of the rows", adapter, 4));
+            TRY(check_pointer(c, "down matrices", down, es));
+            TRY(check_pointer(c, "up matrices", up, es));
+            TRY(check_pointer(c, "scales", scales, 4));
+            TRY(check_pointer(c, "outputs", outputs, es));
+            TRY(check_pointer(c, "workspace bytes", workspace, 16));
+            if (workspace_bytes < need)
+                return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "the workspace has %zu bytes but the call needs %zu",
+                            workspace_bytes, need);
+        }
+        const int64_t n = desc->adapters, r = desc->rank;
+        const Span x = rows_span(inputs, desc->rows, desc->inputs, desc->input_stride, es);
+        const Span w = rows_span(weights, desc->outputs, desc->inputs, desc->weight_stride, es);
+        const Span b{biases, 1, (int64_t)desc->outputs * es, 0}, ad{adapter, 1, 4 * (int64_t)desc->rows, 0};
+        const Span dn{down, 1, n * r * desc->inputs * es, 0}, u{up, 1, n * r * desc->outputs * es, 0};
+        const Span sc{scales, 1, 4 * n, 0}, ws{workspace, 1, (int64_t)need, 0};
+        const Span y = rows_span(outputs, desc->rows, desc->outputs, desc->output_stride, es);
+        TRY(check_apart(c, "outputs", y, {x, w, b, ad, dn, u, sc, ws}));
+        TRY(check_apart(c, "the workspace's bytes", ws, {x, w, b, ad, dn, u, sc}));
+
+        a.rows = desc->rows;
+        a.inputs = desc->inputs;
+        a.outputs = desc->outputs;
+        a.a = inputs;
+        a.lda = desc->input_stride;
+        a.b = weights;
+        a.ldb = desc->weight_stride;
+        a.out = outputs;
+        a.ldo = desc->output_stride;
+        a.accumulate = weights == nullptr;
+        a.bias = biases;
+        a.term.u = reinterpret_cast<const float *>(workspace);
+        a.term.adapter = adapter;
+        a.term.up = up;
+        a.term.adapters = desc->adapters;
+        a.term.rank = desc->rank;
+        a.term.ldu = ldu;
+        dargs.x = inputs;
+        dargs.down = down;
+        dargs.scales = scales;
+        dargs.adapter = adapter;
+        dargs.u = reinterpret_cast<float *>(workspace);
+        dargs.ldx = desc->input_stride;
+        dargs.rows = desc->rows;
+        dargs.inputs = desc->inputs;
+        dargs.rank = desc->rank;
+        dargs.adapters = desc->adapters;
+        dargs.ldu = ldu;
+        return check_grid(c, a, kGroupedForward, desc->values);
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    TRY(run_plain(ctx, s, "adapter_down", [&] { return launch_adapter_down(dargs, desc->values, s); }));
+    return run_plain(ctx, s, "adapted_forward", [&] { return launch_grouped(a, kGroupedForward, desc->values, s); });
+}
+
+}  // extern "C"
+
+namespace {
+
+// 16-bit threshold and scale of a dropout rate.
+void dropout_rate(double rate, uint32_t &threshold, float &scale)
+{
+    threshold = std::min<uint32_t>((uint32_t)std::floor(rate * 65536.0 + 0.5), 65535u);
+    scale = (float)(65536.0 / (65536.0 - threshold));
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t gtmoe_dropout(gtmoe_context *ctx, const gtmoe_dropout_desc *desc, const void *inputs, const void *base,
+                      void *outputs, double rate, uint64_t seed, uint64_t offset, void *stream)
+{
+    DropoutArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        if (!desc) return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+        TRY(check_values(c, desc->values));
+        TRY(check_size(c, "rows", desc->rows, 0, kMaxPlainRows));
+        TRY(check_size(c, "columns", desc->columns, 1, kMaxPlainWidth));
+        if (desc->reserved != 0) return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "reserved must be 0");
+        TRY(check_stride(c, "input", desc->input_stride, desc->columns));
+        TRY(check_stride(c, "base", desc->base_stride, desc->columns));
+        TRY(check_stride(c, "output", desc->output_stride, desc->columns));
+        if (!(rate >= 0.0 && rate < 1.0))
+            return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "dropout rate must be at least 0 and less than 1, got %g", rate);
+        const int es = value_bytes(desc->values);
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "inputs", inputs, es));
+            if (base) TRY(check_pointer(c, "base values", base, es));
+            TRY(check_pointer(c, "outputs", outputs, es));
+        }
+        const Span y = rows_span(outputs, desc->rows, desc->columns, desc->output_stride, es);
+        // in place over the inputs or the base: the thread that writes a value is
+        // the one that read it
+        if (outputs != inputs || desc->output_stride != desc->input_stride)
+            TRY(check_apart(c, "outputs", y, {rows_span(inputs, desc->rows, desc->columns, desc->input_stride, es)}));
+        if (base && (outputs != base || desc->output_stride != desc->base_stride))
+            TRY(check_apart(c, "outputs", y, {rows_span(base, desc->rows, desc->columns, desc->base_stride, es)}));
+        a.x = inputs;
+        a.base = base;
+        a.out = outputs;
+        a.ldx = desc->input_stride;
+        a.ldbase = desc->base_stride;
+        a.ldo = desc->output_stride;
+        a.rows = desc->rows;
+        a.columns = desc->columns;
+        dropout_rate(rate, a.threshold, a.scale);
+        a.seed = seed;
+        a.offset = offset;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "dropout", [&] { return launch_dropout(a, desc->values, s); });
 }
 
 }  // extern "C"

@@ -127,7 +127,9 @@ int32_t gtmoe_close(gtmoe_context *ctx);
  * closed". */
 int32_t gtmoe_context_free(gtmoe_context *ctx);
 /* Text of the last failure on this context (Device.LastError,
- * gpu/device.go:749-753).  With ctx NULL: the last failure of gtmoe_open. */
+ * gpu/device.go:749-753).  With ctx NULL: the last failure on this thread of
+ * gtmoe_open, or of an operator over plain rows called without a context
+ * (such a call checks its arguments and then fails). */
 const char *gtmoe_last_error(const gtmoe_context *ctx);
 
 /* Test hook, no counterpart in the reference: the next call of the entry
@@ -415,6 +417,109 @@ int32_t gtmoe_layer_zero_adapter_gradients(gtmoe_layer *layer);
  * fails as the reference panics for compressed weights. */
 int32_t gtmoe_backward(gtmoe_layer *layer, int32_t tokens, const double *output_gradients,
                        double *input_gradients);
+
+/* ---------------------------------------------------------------------------
+ * Operators over plain rows: what a program that trains experts in full
+ * precision, or serves the adapters of many requests, needs beside a layer.
+ *
+ * Every buffer is device memory of the context's GPU and the caller's, a
+ * workspace among them: the library keeps nothing between calls, and calls on
+ * different streams or in different captured graphs share nothing.  A call
+ * enqueues its kernels on `stream` (a hipStream_t; NULL: the null stream)
+ * without synchronising, allocates nothing, and may be captured into a HIP
+ * graph.  Values are float32, bfloat16 or float16 and lie in rows: a stride is
+ * the distance between two rows in values, at least the width and at most
+ * 1048576; pointers are multiples of a value's size.  Outputs must not
+ * overlap another buffer of the call (GTMOE_ERR_INVALID_ARGUMENT) unless the
+ * entry point says so.  Sums are fp32; an output is rounded once.
+ * ------------------------------------------------------------------------- */
+enum gtmoe_values { GTMOE_VALUES_FLOAT32 = 0, GTMOE_VALUES_BFLOAT16 = 1, GTMOE_VALUES_FLOAT16 = 2 };
+
+/* Ragged products grouped by expert: the projections of experts whose rows
+ * are sorted by expert.  offsets (device, groups + 1 int32, ascending, as
+ * expert_offsets of gtmoe_last_routing): group g owns rows offsets[g] up to
+ * offsets[g + 1].  A group may be empty; rows in no group are neither read
+ * nor written.  Offsets outside [0, rows] or that descend are taken into the
+ * range (no access leaves the buffers), the results are then unspecified.
+ * weights: group g's outputs x inputs matrix (perceptron.Layer.Weights,
+ * perceptron/layer.go:12-25) at g * group_stride. */
+typedef struct gtmoe_grouped_desc {
+    int32_t values;  /* gtmoe_values of rows and weights */
+    int32_t groups;  /* 1 .. 4096 */
+    int32_t rows;    /* rows of the row buffers, 0 .. 2^30 */
+    int32_t inputs;  /* 1 .. 1048576 */
+    int32_t outputs; /* 1 .. 1048576 */
+    int32_t reserved;       /* 0 */
+    int64_t input_stride;   /* of inputs and input gradients */
+    int64_t output_stride;  /* of outputs and output gradients */
+    int64_t weight_stride;  /* of a matrix's rows, also in the weight gradients */
+    int64_t group_stride;   /* values between matrices, at least one matrix */
+} gtmoe_grouped_desc;
+
+/* outputs[r] = W_g inputs[r]: the product of Layer.Forward
+ * (perceptron/layer.go:133-162) for every group, without biases. */
+int32_t gtmoe_grouped_forward(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                              const void *inputs, const void *weights, void *outputs, void *stream);
+/* input_gradients[r] = W_g^T output_gradients[r] (Layer.Backward,
+ * perceptron/layer.go:164-210). */
+int32_t gtmoe_grouped_input_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                                     const void *output_gradients, const void *weights, void *input_gradients,
+                                     void *stream);
+/* weight_gradients[g] = sum over g's rows of output_gradients[r]
+ * inputs[r]^T (Layer.Backward), laid out as the weights; of type
+ * gradient_values, the rows' own or float32.  accumulate != 0 adds to what
+ * weight_gradients holds (micro-batches); otherwise an empty group's matrix
+ * becomes zero. */
+int32_t gtmoe_grouped_weight_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                                      const void *output_gradients, const void *inputs, void *weight_gradients,
+                                      int32_t gradient_values, int32_t accumulate, void *stream);
+
+/* A projection that all requests share beside the low-rank adapter of each
+ * row's own request (Layer.Forward with an adapter, perceptron/layer.go:133-162,
+ * perceptron/adapter.go:66-76):
+ *   outputs[t] = W inputs[t] + b + s_a Up_a (Down_a inputs[t]),  a = adapter[t]
+ * adapter (device, one int32 per row, in any order): a value outside
+ * [0, adapters) is a row without an adapter.  down [adapters][rank][inputs],
+ * up [adapters][outputs][rank], scales [adapters] (alpha / rank); an adapter
+ * of a smaller rank is padded with zeros.  biases may be NULL.  With weights
+ * NULL the shared product is what outputs holds already and the adapters'
+ * terms (and biases, if given) are added to it; without biases rows without
+ * an adapter are then left as they are.  Down_a inputs[t] is kept in fp32.
+ * The workspace holds gtmoe_adapted_workspace bytes (a host call that needs no
+ * context), 16-byte aligned, for the call's time on the stream. */
+typedef struct gtmoe_adapted_desc {
+    int32_t values;  /* gtmoe_values of everything but scales */
+    int32_t rows;    /* 0 .. 2^30 */
+    int32_t inputs, outputs; /* 1 .. 1048576 */
+    int32_t adapters;        /* 1 .. 1048576 */
+    int32_t rank;            /* 1 .. 256 */
+    int64_t input_stride, output_stride, weight_stride;
+} gtmoe_adapted_desc;
+int32_t gtmoe_adapted_workspace(const gtmoe_adapted_desc *desc, size_t *bytes);
+int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc, const void *inputs,
+                              const void *weights, const void *biases, const int32_t *adapter, const void *down,
+                              const void *up, const float *scales, void *outputs, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* Dropout (dropout/dropout.go) whose mask is never stored:
+ *   outputs[r][c] = base[r][c] + (keep(r, c) ? inputs[r][c] * scale : 0)
+ * base may be NULL (no first term).  The gradient of inputs is the same call
+ * on the output gradients (without base), with the same rate, seed and
+ * offset.  rate in [0, 1): threshold = rate * 65536 to the nearest integer (at
+ * most 65535), scale = 65536 / (65536 - threshold).  keep(r, c): 16 bits, the
+ * low (c even) or high half of word (c % 8) / 2 of Philox4x32-10 at counter
+ * (c / 8, r, offset's low 32 bits, offset's high) under key (seed's low 32
+ * bits, seed's high), are at least threshold.  outputs may be inputs or base
+ * themselves (same address and stride). */
+typedef struct gtmoe_dropout_desc {
+    int32_t values;
+    int32_t rows;    /* 0 .. 2^30 */
+    int32_t columns; /* 1 .. 1048576 */
+    int32_t reserved; /* 0 */
+    int64_t input_stride, base_stride, output_stride;
+} gtmoe_dropout_desc;
+int32_t gtmoe_dropout(gtmoe_context *ctx, const gtmoe_dropout_desc *desc, const void *inputs, const void *base,
+                      void *outputs, double rate, uint64_t seed, uint64_t offset, void *stream);
 
 #ifdef __cplusplus
 }
