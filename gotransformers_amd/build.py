@@ -26,6 +26,7 @@ SOURCES = [
     ("misc.hip", []),
     ("lora.hip", []),
     ("grouped.hip", []),
+    ("grouped_large.hip", []),
     ("dropout.hip", []),
     ("api.cpp", []),
     ("encode.cpp", ["-ffp-contract=off"]),

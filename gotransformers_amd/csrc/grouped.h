@@ -45,6 +45,11 @@ struct GroupedArgs {
 bool grouped_fits(const GroupedArgs &a, int direction, int values);
 hipError_t launch_grouped(const GroupedArgs &a, int direction, int values, hipStream_t s);
 
+// The same for many rows of 16-bit values with both operands staged by LDS-DMA
+// (grouped_large.hip).
+bool large_fits(const GroupedArgs &a, int direction, int value_bytes);
+hipError_t launch_large(const GroupedArgs &a, int direction, int values, hipStream_t s);
+
 // u[t][j] = scales[a] sum_k down[a][j][k] x[t][k] for the rows with an adapter a.
 struct AdapterDownArgs {
     const void *x = nullptr, *down = nullptr;
