@@ -22,6 +22,7 @@ namespace {
 
 constexpr long long kMaxBlocks = (1ll << 32) / 1024 - 1;  // a grid holds 2^32 - 1 threads
 constexpr int SB = 128;                                   // bytes of reduction per step
+constexpr int kCus = 256;
 
 // Tile of rows of block b (the hardware hands block b to XCD b % 8): XCD x
 // takes the x-th eighth of the row tiles in order, each with its `columns`
@@ -104,8 +105,9 @@ __device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NJ], void *ou
     }
 }
 
-// BM x BN tile by WM x WN waves; DA, DB: the operands staged by LDS-DMA.
-template <class T, int DIR, int BM, int BN, int WM, int WN, bool DA, bool DB, bool ADAPTED>
+// BM x BN tile by WM x WN waves; NS: stages; DA, DB: the operands staged by
+// LDS-DMA (both of them with more than two stages).
+template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, bool DB, bool ADAPTED>
 __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
 {
     constexpr int THREADS = 64 * WM * WN;
@@ -115,6 +117,10 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
     // one array per stage, so that the compiler tells their accesses apart
     __shared__ __attribute__((aligned(1024))) char s0[(BM + BN) * SB];
     __shared__ __attribute__((aligned(1024))) char s1[(BM + BN) * SB];
+    __shared__ __attribute__((aligned(1024))) char s2[NS > 2 ? (BM + BN) * SB : 16];
+    __shared__ __attribute__((aligned(1024))) char s3[NS > 2 ? (BM + BN) * SB : 16];
+    constexpr int L = (DA ? A::kLoads : 0) + (DB ? B::kLoads : 0);
+    static_assert(NS == 2 || (NS == 4 && DA && DB && 3 * L < 64), "");
 
     typedef typename T::Store Store;
     const Store *pa = reinterpret_cast<const Store *>(a.a), *pb = reinterpret_cast<const Store *>(a.b);
@@ -182,12 +188,13 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) acc[i][j] = T::mfma(fb[p][j], fa[p][i], acc[i][j]);
     };
-    // Stages 0 and 1 are filled up front, a stage again with step k + 2 once
-    // step k has been read from it.  A step's MFMA groups run with the next
+    // All stages are filled up front, a stage again with step k + NS once step
+    // k has been read from it.  A step's MFMA groups run with the next
     // group's operands already on their way from LDS; before its last group every
-    // wave has read all of the step and step k + 1 has landed, so that the
+    // wave has read all of the step and step k + 1 has landed (the loads of at
+    // most NS - 2 later steps are still pending), so that the
     // next step's first operands, too, load under MFMAs.  Steps past the end
-    // read zeros, and the loop takes two steps at a time without a way out
+    // read zeros, and the loop takes NS steps at a time without a way out
     // between them (with one, the accumulators were copied at the join).  An
     // operand staged through registers is loaded at the start of step k and
     // written where LDS-DMA loads are issued.
@@ -202,9 +209,10 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
         if constexpr (DB) ob.issue(s + BM * SB, ob.request(k));
         else ob.put(s + BM * SB, qb);
     };
-    auto landed = [&]() {
+    constexpr auto vm_wait = [](int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4); };  // vmcnt(n) lgkmcnt(0)
+    auto landed = [&](auto pending) {
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+        __builtin_amdgcn_s_waitcnt(vm_wait(decltype(pending)::value));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -223,19 +231,19 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
         }
     };
     auto body = [&](char *cur, const char *next, int k) {
-        fetch(k + 2);
+        fetch(k + NS);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
             if (kk + 1 < KK) {
                 read(cur, kk + 1, (kk + 1) & 1);
             } else {
-                landed();
-                fill(cur, k + 2);
+                landed(std::integral_constant<int, (NS - 2) * L>());
+                fill(cur, k + NS);
                 read(next, 0, 0);
             }
             multiply(kk & 1);
             if (kk + 1 < KK) interleave(std::integral_constant<int, 0>());
-            else interleave(std::integral_constant<int, (DA ? A::kLoads : 0) + (DB ? B::kLoads : 0)>());
+            else interleave(std::integral_constant<int, L>());
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -244,12 +252,20 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
         fill(s0, 0);
         fetch(1);
         fill(s1, 1);
-        landed();
+        if constexpr (NS > 2) {
+            fill(s2, 2);
+            fill(s3, 3);
+        }
+        landed(std::integral_constant<int, NS == 2 ? 0 : (NS - 1) * L>());
         read(s0, 0, 0);
     }
-    for (int k = 0; k < steps; k += 2) {
+    for (int k = 0; k < steps; k += NS) {
         body(s0, s1, k);
-        body(s1, s0, k + 1);
+        body(s1, NS > 2 ? s2 : s0, k + 1);
+        if constexpr (NS > 2) {
+            body(s2, s3, k + 2);
+            body(s3, s0, k + 3);
+        }
     }
     __builtin_amdgcn_s_waitcnt(0x0070);  // nothing may still be on its way into LDS
 
@@ -282,24 +298,40 @@ long long tile_blocks(const GroupedArgs &a, int direction, int bm, int bn)
     return (tiles + 7) / 8 * 8 * ((width + bn - 1) / bn);
 }
 
-template <class T, int DIR, int BM, int BN, int WM, int WN, bool DA, bool DB, bool ADAPTED>
+template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, bool DB, bool ADAPTED>
 hipError_t launch_tiles(const GroupedArgs &a, hipStream_t s)
 {
     const long long blocks = tile_blocks(a, DIR, BM, BN);
-    hipLaunchKernelGGL((grouped_kernel<T, DIR, BM, BN, WM, WN, DA, DB, ADAPTED>), dim3((unsigned)blocks),
+    hipLaunchKernelGGL((grouped_kernel<T, DIR, BM, BN, WM, WN, NS, DA, DB, ADAPTED>), dim3((unsigned)blocks),
                        dim3(64 * WM * WN), 0, s, a);
     return hipGetLastError();
 }
 
-template <class T, int DIR, int BM, int BN, int WM, int WN, bool ADAPTED = false>
+// NS: stages where both operands take LDS-DMA loads.
+template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool ADAPTED = false>
 hipError_t launch_staged(const GroupedArgs &a, bool da, bool db, hipStream_t s)
 {
-    if (da) return db ? launch_tiles<T, DIR, BM, BN, WM, WN, true, true, ADAPTED>(a, s)
-                      : launch_tiles<T, DIR, BM, BN, WM, WN, true, false, ADAPTED>(a, s);
-    return db ? launch_tiles<T, DIR, BM, BN, WM, WN, false, true, ADAPTED>(a, s)
-              : launch_tiles<T, DIR, BM, BN, WM, WN, false, false, ADAPTED>(a, s);
+    if (da && db) return launch_tiles<T, DIR, BM, BN, WM, WN, NS, true, true, ADAPTED>(a, s);
+    return db ? launch_tiles<T, DIR, BM, BN, WM, WN, 2, false, true, ADAPTED>(a, s)
+              : launch_tiles<T, DIR, BM, BN, WM, WN, 2, false, false, ADAPTED>(a, s);
 }
 
+// The tile by type, rows per group and number of tiles (times in us, MI355X):
+//   fp32  64 x 64: the matrix cores are so much slower here that small tiles lose
+//     nothing and waste less (14 experts of 1000 -> 1201, 2331 rows: forward 71
+//     against 126 with 128 x 128; 16 of 1024 -> 2048, 4096 rows: 159 against 230).
+//     Up to 32 rows per group 32 x 128 with four stages, to stream the weights
+//     (64 of 2048 -> 1024, 1024 rows: 107 against 150).
+//   16 bits, large tiles where large_fits says so; else
+//     64 x 64 up to 48 rows per group (16 of 1024 -> 2048, 512 rows: 14.2 against
+//     17.5 with 128 x 128) or while 128 x 128 would give fewer than 128 tiles
+//     (8 of 256 -> 512, 2048 rows: 6.0 against 7.7); with four stages while
+//     the tiles are at most two per CU, where the loads in flight bound it (16
+//     of 1024 -> 2048, 64 rows, input gradient: 13.5 against 20.0; 64 of 1024 ->
+//     512, 100 rows, 1024 tiles: 15.0 against 13.2),
+//     64 x 128 up to 192 rows per group (14 of 1000 -> 1201, 2331 rows: 25.8
+//     against 28.2), and for the weight gradient (12000 rows: 71 against 80),
+//     128 x 128 beyond (the same, input gradient: 61 against 69).
 template <class T, int DIR>
 hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
 {
@@ -310,9 +342,28 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
     const bool da = aligned16(a.a, a.lda * T::kBytes) && width_a % unit == 0;
     const bool db = aligned16(a.b, a.ldb * T::kBytes) && a.inputs % unit == 0 && (DIR == kGroupedWeightGradient || groups);
     if constexpr (DIR == kGroupedForward)
-        if (a.term.adapter) return launch_staged<T, DIR, 128, 128, 2, 2, true>(a, da, db, s);
-    if (da && db && large_fits(a, DIR, T::kBytes)) return launch_large(a, DIR, std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
-    return launch_staged<T, DIR, 128, 128, 2, 2>(a, da, db, s);
+        if (a.term.adapter) return launch_staged<T, DIR, 128, 128, 2, 2, 2, true>(a, da, db, s);
+    const long long each = a.rows / a.groups;
+    if constexpr (T::kBytes == 4) {
+        if constexpr (DIR != kGroupedWeightGradient)
+            if (each <= 32) return launch_staged<T, DIR, 32, 128, 1, 4, 4>(a, da, db, s);
+        return launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);
+    } else {
+        if (da && db && large_fits(a, DIR, T::kBytes))
+            return launch_large(a, DIR, std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
+        if constexpr (DIR == kGroupedWeightGradient) {
+            if (tile_blocks(a, DIR, 128, 128) < 256) return launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);
+            return launch_staged<T, DIR, 64, 128, 2, 2, 2>(a, da, db, s);
+        } else {
+            const int width = DIR == kGroupedForward ? a.outputs : a.inputs;
+            const long long likely = (a.rows / 128 + a.groups / 2) * ((width + 127) / 128);
+            if (each <= 48 || likely < 128)
+                return tile_blocks(a, DIR, 64, 64) <= 2 * kCus ? launch_staged<T, DIR, 64, 64, 2, 2, 4>(a, da, db, s)
+                                                               : launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);
+            if (each <= 192) return launch_staged<T, DIR, 64, 128, 2, 2, 2>(a, da, db, s);
+            return launch_staged<T, DIR, 128, 128, 2, 2, 2>(a, da, db, s);
+        }
+    }
 }
 
 template <class T>
@@ -329,7 +380,7 @@ hipError_t launch_values(const GroupedArgs &a, int direction, hipStream_t s)
 
 bool grouped_fits(const GroupedArgs &a, int direction, int values)
 {
-    return tile_blocks(a, direction, 128, 128) <= kMaxBlocks;
+    return tile_blocks(a, direction, 32, 64) <= kMaxBlocks;  // no tile is smaller
 }
 
 hipError_t launch_grouped(const GroupedArgs &a, int direction, int values, hipStream_t s)
