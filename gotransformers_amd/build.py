@@ -27,6 +27,7 @@ SOURCES = [
     ("lora.hip", []),
     ("grouped.hip", []),
     ("grouped_large.hip", []),
+    ("adapted.hip", []),
     ("dropout.hip", []),
     ("api.cpp", []),
     ("encode.cpp", ["-ffp-contract=off"]),

@@ -3221,7 +3221,7 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
     if (desc->rows == 0) return GTMOE_OK;
     hipStream_t s = (hipStream_t)stream;
     TRY(run_plain(ctx, s, "adapter_down", [&] { return launch_adapter_down(dargs, desc->values, s); }));
-    return run_plain(ctx, s, "adapted_forward", [&] { return launch_grouped(a, kGroupedForward, desc->values, s); });
+    return run_plain(ctx, s, "adapted_forward", [&] { return launch_adapted(a, desc->values, s); });
 }
 
 }  // extern "C"

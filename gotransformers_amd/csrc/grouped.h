@@ -60,6 +60,8 @@ struct AdapterDownArgs {
     int rows = 0, inputs = 0, rank = 0, adapters = 0, ldu = 0;
 };
 hipError_t launch_adapter_down(const AdapterDownArgs &a, int values, hipStream_t s);
+// The forward of one group with its adapters' term.
+hipError_t launch_adapted(const GroupedArgs &a, int values, hipStream_t s);
 
 // out[r][c] = base[r][c] + (keep(r, c) ? x[index ? index[r] : r][c] * scale : 0),
 // base null: no first term.

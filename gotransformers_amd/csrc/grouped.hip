@@ -342,7 +342,12 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
     const bool da = aligned16(a.a, a.lda * T::kBytes) && width_a % unit == 0;
     const bool db = aligned16(a.b, a.ldb * T::kBytes) && a.inputs % unit == 0 && (DIR == kGroupedWeightGradient || groups);
     if constexpr (DIR == kGroupedForward)
-        if (a.term.adapter) return launch_staged<T, DIR, 128, 128, 2, 2, 2, true>(a, da, db, s);
+        if (a.term.adapter) {
+            // 64 x 64: the adapters' term wants many waves (512 rows of 1024 -> 2048:
+            // 16.5 us against 25.7 with 128 x 128; 8192: 84.8 against 89.2)
+            return tile_blocks(a, DIR, 64, 64) <= 2 * kCus ? launch_staged<T, DIR, 64, 64, 2, 2, 4, true>(a, da, db, s)
+                                                           : launch_staged<T, DIR, 64, 64, 2, 2, 2, true>(a, da, db, s);
+        }
     const long long each = a.rows / a.groups;
     if constexpr (T::kBytes == 4) {
         if constexpr (DIR != kGroupedWeightGradient)
@@ -391,121 +396,6 @@ hipError_t launch_grouped(const GroupedArgs &a, int direction, int values, hipSt
     case kValuesF16: return launch_values<F16>(a, direction, s);
     default: return launch_values<F32>(a, direction, s);
     }
-}
-
-// ---------------------------------------------------------------------------
-// The adapters' first half: u[t] = s_a A_a x[t].
-// ---------------------------------------------------------------------------
-
-namespace {
-
-// 16 bytes of a row's reduction from value k on (zero at and past `length`),
-// any alignment.
-template <class T>
-__device__ __forceinline__ u32x4 load_unit(const typename T::Store *row, int k, int length)
-{
-    constexpr int unit = 16 / T::kBytes;
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (k + unit <= length) {
-        __builtin_memcpy(&v, row + k, 16);
-    } else if (k < length) {
-        if constexpr (T::kBytes == 2) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (k + e < length) v[e >> 1] |= (uint32_t)row[k + e] << (16 * (e & 1));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (k + e < length) v[e] = __float_as_uint(row[k + e]);
-        }
-    }
-    return v;
-}
-
-// c += a b^T over 64 bytes of reduction, 16 x 16: lane l holds 16 bytes
-// (quarter l / 16) of row l % 16 of both operands.
-template <class T>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c)
-{
-    if constexpr (std::is_same<T, Bf16>::value)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else if constexpr (std::is_same<T, F16>::value)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else {
-        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
-        return c;
-    }
-}
-
-constexpr int kDownWaves = 8;
-
-// A workgroup takes `tile` (at most 16) rows and 16 ranks (blockIdx.y): every
-// adapter among the rows in turn, its ranks times all the rows on 16 x 16
-// MFMAs, the waves splitting the reduction; a row keeps its own adapter's
-// products only.
-template <class T>
-__global__ __launch_bounds__(64 * kDownWaves) void adapter_down_kernel(AdapterDownArgs a, int tile)
-{
-    __shared__ float part[kDownWaves][16][17];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int q = lane >> 4, i = lane & 15;
-    const int t0 = blockIdx.x * tile, j0 = blockIdx.y * 16;
-    const int rows = min(tile, a.rows - t0);
-    constexpr int unit = 16 / T::kBytes, step = 4 * unit;
-    typedef typename T::Store Store;
-    int mine = -1;
-    if (i < rows) {
-        mine = a.adapter[t0 + i];
-        if (mine >= a.adapters) mine = -1;
-    }
-    const Store *x = reinterpret_cast<const Store *>(a.x) + (long long)(t0 + min(i, rows - 1)) * a.ldx;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    uint64_t todo = __ballot(mine >= 0);
-    while (todo) {
-        const int cur = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-        const bool here = mine == cur;
-        todo &= ~__ballot(here);
-        // ranks past the last repeat it: their results are not kept
-        const Store *d = reinterpret_cast<const Store *>(a.down) +
-                         ((long long)cur * a.rank + min(j0 + i, a.rank - 1)) * a.inputs;
-        f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int k = wave * step; k < a.inputs; k += kDownWaves * step)
-            p = mfma16<T>(load_unit<T>(d, k + q * unit, a.inputs), load_unit<T>(x, k + q * unit, a.inputs), p);
-        if (here) acc = p;
-    }
-    // lane l: row l % 16, ranks 4 (l / 16) ..
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][i][4 * q + e] = acc[e];
-    __syncthreads();
-    const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
-    if (r < rows && j0 + c < a.ldu) {
-        const int ad = a.adapter[t0 + r];
-        float v = 0.f;
-        if (ad >= 0 && ad < a.adapters && j0 + c < a.rank) {
-#pragma unroll
-            for (int w = 0; w < kDownWaves; ++w) v += part[w][r][c];
-            v *= a.scales[ad];
-        }
-        a.u[(long long)(t0 + r) * a.ldu + j0 + c] = v;
-    }
-}
-
-}  // namespace
-
-hipError_t launch_adapter_down(const AdapterDownArgs &a, int values, hipStream_t s)
-{
-    if (a.rows == 0) return hipSuccess;
-    const int tile = a.rows <= 512 ? 1 : a.rows >= 8192 ? 16 : (a.rows + 511) / 512;
-    const dim3 grid((a.rows + tile - 1) / tile, (a.ldu + 15) / 16), block(64 * kDownWaves);
-    switch (values) {
-    case kValuesBf16: hipLaunchKernelGGL(adapter_down_kernel<Bf16>, grid, block, 0, s, a, tile); break;
-    case kValuesF16: hipLaunchKernelGGL(adapter_down_kernel<F16>, grid, block, 0, s, a, tile); break;
-    default: hipLaunchKernelGGL(adapter_down_kernel<F32>, grid, block, 0, s, a, tile); break;
-    }
-    return hipGetLastError();
 }
 
 }  // namespace gtmoe

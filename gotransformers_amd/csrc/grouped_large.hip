@@ -219,7 +219,7 @@ __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int le
     }
 }
 
-template <class T, int DIR, bool ADAPTED>
+template <class T, int DIR>
 __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 {
     typedef Operand<T, DIR != kGroupedWeightGradient, kBm, kThreads, SB> A;
@@ -395,10 +395,6 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
             body(s1, s0);
         }
 
-        if constexpr (ADAPTED) {
-            if (a.bias) add_bias<T>(acc, a.bias, x.n0 + wn, a.outputs);
-            add_adapters<T, 2>(acc, a, x.m0 + wm, x.n0 + wn, x.m0 + x.m);
-        }
         // results: lane l holds row 64 i + wm + l % 32 and, in register r of
         // block (i, j), column wn + 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.  Through
         // LDS (rows of 128 bytes, 16-byte unit u of row r in slot u ^ (r / 2) % 8) to
@@ -463,11 +459,10 @@ hipError_t launch_values(const GroupedArgs &a, int direction, hipStream_t s)
     const dim3 grid(kCus), block(kThreads);
     switch (direction) {
     case kGroupedForward:
-        if (a.term.adapter) hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward>), grid, block, 0, s, a);
         break;
-    case kGroupedInputGradient: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedInputGradient, false>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedWeightGradient, false>), grid, block, 0, s, a); break;
+    case kGroupedInputGradient: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedInputGradient>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedWeightGradient>), grid, block, 0, s, a); break;
     }
     return hipGetLastError();
 }

@@ -303,51 +303,248 @@ __device__ __forceinline__ void load4(const typename T::Store *p, float (&v)[4],
     }
 }
 
+// Eight values of an adapter's up row from rank k on, zero at and past `rank`,
+// any alignment.
+template <class T>
+__device__ __forceinline__ void load_ranks(const typename T::Store *row, int k, int rank, float (&v)[8])
+{
+    typename T::Store w[8];
+    if (k + 8 <= rank) {
+        __builtin_memcpy(w, row + k, sizeof w);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = k + e < rank ? row[k + e] : (typename T::Store)0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = T::load(w[e]);
+}
+
+// Sixteen ranks' worth of one operand of the adapters' product: a lane of half
+// h = l / 32 holds ranks k .. k + 7, k = c + 8 h, of one row.
+//
+// 16-bit values: u enters the matrix cores as two 16-bit numbers, its leading
+// part and the rest of it, so that what is lost of a rank's product is 2^-16 of
+// it (bf16: the upper half of the word and the rest rounded; fp16: 2^-21), far
+// below the output's own rounding, at an eighth of the time of fp32 MFMAs.  fp16
+// has too few exponents for u: a row's ranks are scaled by a power of two, and
+// so is what they are added to (exactly).  What is not finite stays so in both parts.
+template <class T>
+struct RankRow {
+    u32x4 hi, lo;
+    float scale, unscale;  // fp16: the row's power of two and its inverse
+    __device__ __forceinline__ void load(const float *u, bool have)
+    {
+        f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if (have) {
+            v[0] = *reinterpret_cast<const f32x4 *>(u);
+            v[1] = *reinterpret_cast<const f32x4 *>(u + 4);
+        }
+        scale = unscale = 1.f;
+        if constexpr (std::is_same<T, F16>::value) {
+            float top = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = fabsf(v[e >> 2][e & 3]);
+                top = fmaxf(top, x < __builtin_inff() ? x : 0.f);
+            }
+            top = fmaxf(top, __shfl_xor(top, 32));  // the row's other half
+            if (top > 0.f) {
+                // 2^(exponent of top) held to where its inverse and both
+                // parts are normal numbers; scaled values are below 2
+                const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 252) - 127;
+                scale = __uint_as_float((uint32_t)(127 - ex) << 23);
+                unscale = __uint_as_float((uint32_t)(127 + ex) << 23);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            float h[2], l[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float x = v[p >> 1][2 * (p & 1) + e];
+                if constexpr (std::is_same<T, F16>::value) {
+                    const float y = x * scale;
+                    h[e] = T::load(T::round(y));
+                    l[e] = fabsf(x) < __builtin_inff() ? y - h[e] : x;
+                } else {
+                    h[e] = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+                    l[e] = fabsf(x) < __builtin_inff() ? x - h[e] : x;
+                }
+            }
+            hi[p] = T::pack(h[0], h[1]);
+            lo[p] = T::pack(l[0], l[1]);
+        }
+    }
+};
+
+// d += u B^T over ranks c .. c + 15 for one 32-row block of u and NJ 32-column
+// blocks of B (`up`: the lane's row of each, or null past the matrix).
+template <class T, int NJ>
+__device__ __forceinline__ void load_columns(const typename T::Store *const (&up)[NJ], int k, int rank, u32x4 (&b)[NJ])
+{
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        b[j] = u32x4{0u, 0u, 0u, 0u};
+        if (!up[j] || k >= rank) continue;
+        if (k + 8 <= rank) {
+            __builtin_memcpy(&b[j], up[j] + k, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < rank) b[j][e >> 1] |= (uint32_t)up[j][k + e] << (16 * (e & 1));
+        }
+    }
+}
+
 // acc += u B_a^T for the wave's blocks (block i's first row m0 + 32 EACH i, rows
-// from m on do not exist) and the rows that have an adapter: per 32-row block, every
-// adapter that occurs in it in turn, as fp32 MFMAs over the rank (u stays fp32
-// and a 16-bit B converts exactly), its products kept by the rows that are
-// its own only, so that no adapter's values reach another's rows.  Returns the
-// rows without an adapter (bit i: the lane's row of block i).
+// from m on do not exist) and the rows that have an adapter.  Returns the rows
+// without one (bit i: the lane's row of block i).  A row sees its own adapter's
+// values only, so that infinities in another's do not reach it:
+//   all the wave's rows with one adapter (prompts): B_a is loaded once for
+//     them and the products are added to acc directly;
+//   a 32-row block with at most kAdapterPasses adapters: each in turn, its rows
+//     keeping their own products;
+//   more (decode batches): every lane gathers its own row's adapter, eight ranks of a
+//     column at a time.
+constexpr int kAdapterPasses = 3;
+
 template <class T, int EACH, int MI, int NJ>
 __device__ __forceinline__ uint32_t add_adapters(f32x16 (&acc)[MI][NJ], const GroupedArgs &a, int m0, int n0, int m)
 {
-    uint32_t without = 0;
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const AdapterTerm &t = a.term;
-    const typename T::Store *up = reinterpret_cast<const typename T::Store *>(t.up);
+    const typename T::Store *const up = reinterpret_cast<const typename T::Store *>(t.up);
+    int mine[MI];
+    uint32_t without = 0;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int row = m0 + 32 * EACH * i + (lane & 31);
+        mine[i] = -2;  // past the rows
+        if (row < m) {
+            mine[i] = t.adapter[row];
+            if (mine[i] < 0 || mine[i] >= t.adapters) {
+                mine[i] = -1;
+                without |= 1u << i;
+            }
+        }
+    }
+    const int one = __builtin_amdgcn_readfirstlane(mine[0]);
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) same = same && (mine[i] == one || mine[i] == -2);
+    if (__ballot(!same) == 0) {
+        if (one < 0) return without;
+        if constexpr (T::kBytes == 2) {
+            const typename T::Store *rows[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int col = n0 + 32 * j + (lane & 31);
+                rows[j] = col < a.outputs ? up + ((long long)one * a.outputs + col) * t.rank : nullptr;
+            }
+            const typename T::Store *const(&cols)[NJ] = rows;
+            for (int c = 0; c < t.rank; c += 16) {
+                const int k = c + 8 * h;
+                u32x4 b[NJ];
+                load_columns<T, NJ>(cols, k, t.rank, b);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    RankRow<T> u;
+                    u.load(t.u + (long long)(m0 + 32 * EACH * i + (lane & 31)) * t.ldu + k, mine[i] >= 0 && k < t.ldu);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (std::is_same<T, F16>::value) acc[i][j] *= u.scale;
+                        acc[i][j] = T::mfma(b[j], u.hi, acc[i][j]);
+                        acc[i][j] = T::mfma(b[j], u.lo, acc[i][j]);
+                        if constexpr (std::is_same<T, F16>::value) acc[i][j] *= u.unscale;
+                    }
+                }
+            }
+            return without;
+        }
+    }
     const bool aligned = t.rank % 4 == 0 && (reinterpret_cast<uintptr_t>(t.up) & (4 * T::kBytes - 1)) == 0;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         const int row = m0 + 32 * EACH * i + (lane & 31);
-        int mine = -1;
-        if (row < m) {
-            mine = t.adapter[row];
-            if (mine >= t.adapters) mine = -1;
+        const uint64_t rows = __ballot(mine[i] >= 0);
+        uint64_t todo = rows;
+        int passes = 0;
+        while (todo && passes <= kAdapterPasses) {
+            todo &= ~__ballot(mine[i] == __builtin_amdgcn_readlane(mine[i], __builtin_ctzll(todo)));
+            ++passes;
         }
-        if (mine < 0) without |= 1u << i;
-        uint64_t todo = __ballot(mine >= 0);
+        if (passes > kAdapterPasses) {
+            if (mine[i] >= 0) {
+                const float *u = t.u + (long long)row * t.ldu;
+                const typename T::Store *mat = up + (long long)mine[i] * a.outputs * t.rank;
+                for (int c = 0; c < t.rank; c += 8) {
+                    const f32x4 u0 = *reinterpret_cast<const f32x4 *>(u + c), u1 = *reinterpret_cast<const f32x4 *>(u + c + 4);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int col = n0 + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3);
+                            if (col < a.outputs) {
+                                float b[8];
+                                load_ranks<T>(mat + (long long)col * t.rank, c, t.rank, b);
+                                float d = u0[0] * b[0];
+#pragma unroll
+                                for (int e = 1; e < 4; ++e) d = fmaf(u0[e], b[e], d);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) d = fmaf(u1[e], b[4 + e], d);
+                                acc[i][j][r] += d;
+                            }
+                        }
+                }
+            }
+            continue;
+        }
+        todo = rows;
         while (todo) {
-            const int cur = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-            const bool here = mine == cur;
+            const int cur = __builtin_amdgcn_readlane(mine[i], __builtin_ctzll(todo));
+            const bool here = mine[i] == cur;
             todo &= ~__ballot(here);
             f32x16 d[NJ];
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) d[j][r] = 0.f;
-            for (int c = 0; c < t.rank; c += 8) {
-                const int k = c + 4 * h;
-                f32x4 uv = {0.f, 0.f, 0.f, 0.f};
-                if (here) uv = *reinterpret_cast<const f32x4 *>(t.u + (long long)row * t.ldu + k);
+            if constexpr (T::kBytes == 2) {
+                const typename T::Store *crows[NJ];
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const int col = n0 + 32 * j + (lane & 31);
-                    float b[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (col < a.outputs && k < t.rank)
-                        load4<T>(up + ((long long)cur * a.outputs + col) * t.rank + k, b, t.rank - k, aligned);
+                    crows[j] = col < a.outputs ? up + ((long long)cur * a.outputs + col) * t.rank : nullptr;
+                }
+                const typename T::Store *const(&cols)[NJ] = crows;
+                for (int c = 0; c < t.rank; c += 16) {
+                    const int k = c + 8 * h;
+                    u32x4 b[NJ];
+                    load_columns<T, NJ>(cols, k, t.rank, b);
+                    RankRow<T> u;
+                    u.load(t.u + (long long)row * t.ldu + k, here && k < t.ldu);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) d[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[e], uv[e], d[j], 0, 0, 0);
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (std::is_same<T, F16>::value) d[j] *= u.scale;
+                        d[j] = T::mfma(b[j], u.hi, d[j]);
+                        d[j] = T::mfma(b[j], u.lo, d[j]);
+                        if constexpr (std::is_same<T, F16>::value) d[j] *= u.unscale;
+                    }
+                }
+            } else {
+                for (int c = 0; c < t.rank; c += 8) {
+                    const int k = c + 4 * h;
+                    f32x4 uv = {0.f, 0.f, 0.f, 0.f};
+                    if (here) uv = *reinterpret_cast<const f32x4 *>(t.u + (long long)row * t.ldu + k);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const int col = n0 + 32 * j + (lane & 31);
+                        float b[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (col < a.outputs && k < t.rank)
+                            load4<T>(up + ((long long)cur * a.outputs + col) * t.rank + k, b, t.rank - k, aligned);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[e], uv[e], d[j], 0, 0, 0);
+                    }
                 }
             }
             if (here) {
