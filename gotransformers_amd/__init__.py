@@ -41,7 +41,7 @@ EXPORTED = [
     "gtmoe_weights_file_entry", "gtmoe_weights_file_find", "gtmoe_weights_file_values", "gtmoe_weights_file_rows",
     "gtmoe_layer_load_weights", "gtmoe_layer_add_adapters", "gtmoe_layer_remove_adapters", "gtmoe_layer_adapter_rank",
     "gtmoe_layer_set_adapter", "gtmoe_layer_get_adapter", "gtmoe_layer_adapter_gradients",
-    "gtmoe_layer_zero_adapter_gradients", "gtmoe_backward",
+    "gtmoe_layer_zero_adapter_gradients", "gtmoe_backward", "gtmoe_layer_set_adapter_dropout",
     "gtmoe_grouped_forward", "gtmoe_grouped_input_gradient", "gtmoe_grouped_weight_gradient",
     "gtmoe_adapted_workspace", "gtmoe_adapted_forward", "gtmoe_dropout",
 ]
@@ -152,6 +152,7 @@ def library():
         "gtmoe_layer_adapter_gradients": ([P, i32, i32, P, P], i32),
         "gtmoe_layer_zero_adapter_gradients": ([P], i32),
         "gtmoe_backward": ([P, i32, P, P], i32),
+        "gtmoe_layer_set_adapter_dropout": ([P, dbl, C.c_uint64], i32),
         "gtmoe_grouped_forward": ([P, P, P, P, P, P, P], i32),
         "gtmoe_grouped_input_gradient": ([P, P, P, P, P, P, P], i32),
         "gtmoe_grouped_weight_gradient": ([P, P, P, P, P, P, i32, i32, P], i32),
@@ -410,6 +411,12 @@ class MixtureOfExperts:
 
     def remove_adapters(self):
         self.ctx.check(library().gtmoe_layer_remove_adapters(self.handle))
+
+    def set_adapter_dropout(self, rate, seed=0):
+        """Dropout on the adapters' inputs of later forwards and backwards
+        (rate 0: none); the masks are those of dropout() at the offsets
+        gtmoe.h gives."""
+        self.ctx.check(library().gtmoe_layer_set_adapter_dropout(self.handle, float(rate), int(seed)))
 
     def adapter_rank(self, kind, index=0, which=None):
         r = C.c_int32(0)

@@ -276,6 +276,13 @@ struct TrainWorkspace {
         int n = 0, nmulti = 0;
     } ot, rt;
     float *outer = nullptr;  // [P/64 + G][R][max(dp, hp, E)] tile sums of the adapter gradients
+    // dropout on the adapters' inputs (allocated with the first forward that
+    // has it): the dropped inputs of the role at hand, and t A before its mask
+    float *dropped = nullptr, *dropped_grad = nullptr;  // [max(P, T)][max(dp, hp)]
+    // what the last forward drew its masks from (threshold 0: no dropout)
+    uint32_t drop_threshold = 0;
+    float drop_scale = 1.f;
+    uint64_t drop_seed = 0, drop_offset = 0;
     int P = 0, ntiles_tr = 0, tile_tr = 4;
 };
 
@@ -320,6 +327,8 @@ struct gtmoe_layer {
     AdapterSet ad_gate, ad_up, ad_down, ad_router;
     TrainWorkspace tw;
     int adapter_T = -1;  // tokens of the last forward through the adapter path, -1: none
+    double dropout_rate = 0;  // on the adapters' inputs
+    uint64_t dropout_seed = 0, dropout_calls = 0;  // forwards since the rate was set
     // recorded graphs that hold pointers into this layer's workspace: while
     // any exists the workspace is never reallocated
     int live_graphs = 0;
@@ -1214,6 +1223,51 @@ int32_t ensure_train_workspace(gtmoe_layer *L, int T)
     return GTMOE_OK;
 }
 
+int32_t ensure_dropout_workspace(gtmoe_layer *L)
+{
+    TrainWorkspace &tw = L->tw;
+    if (tw.dropped) return GTMOE_OK;
+    gtmoe_context *ctx = L->ctx;
+    const size_t rows = (size_t)tw.cap * std::max(L->S + L->k, 1), width = std::max(L->dp, L->hp);
+    for (float **p : {&tw.dropped_grad, &tw.dropped}) {
+        void *block = nullptr;
+        HIP_TRY(ctx, dev_malloc(&block, rows * width * sizeof(float)));
+        tw.blocks.push_back(block);
+        *p = static_cast<float *>(block);
+    }
+    return GTMOE_OK;
+}
+
+// 16-bit threshold and scale of a dropout rate.
+void dropout_rate(double rate, uint32_t &threshold, float &scale)
+{
+    threshold = std::min<uint32_t>((uint32_t)std::floor(rate * 65536.0 + 0.5), 65535u);
+    scale = (float)(65536.0 / (65536.0 - threshold));
+}
+
+// The masks of one forward's adapters, by role.
+enum DropoutRole { kDropGate = 0, kDropUp = 1, kDropDown = 2, kDropRouter = 3 };
+
+// out = base + masked rows of in (gathered by index unless null), `columns` of
+// them with their padding (zeros stay zeros); base null: no first term.
+hipError_t adapter_dropout(const TrainWorkspace &tw, DropoutRole role, int rows, int columns, const float *in,
+                           const int32_t *index, const float *base, float *out, hipStream_t s)
+{
+    DropoutArgs a;
+    a.x = in;
+    a.base = base;
+    a.out = out;
+    a.index = index;
+    a.ldx = a.ldbase = a.ldo = columns;
+    a.rows = rows;
+    a.columns = columns;
+    a.threshold = tw.drop_threshold;
+    a.scale = tw.drop_scale;
+    a.seed = tw.drop_seed;
+    a.offset = tw.drop_offset + role;
+    return launch_dropout(a, kValuesF32, s);
+}
+
 LoraArgs lora_args(const AdapterSet &a, int P, const TrainWorkspace::OuterTiles &ot)
 {
     LoraArgs l{};
@@ -1320,6 +1374,15 @@ int32_t adapter_forward(gtmoe_layer *L, int T, const double *inputs, const int64
     int32_t rc = ensure_train_workspace(L, T);
     if (rc != GTMOE_OK) return rc;
     TrainWorkspace &tw = L->tw;
+    tw.drop_threshold = 0;
+    if (L->dropout_rate > 0) dropout_rate(L->dropout_rate, tw.drop_threshold, tw.drop_scale);
+    const bool drop = tw.drop_threshold > 0;
+    if (drop) {
+        rc = ensure_dropout_workspace(L);
+        if (rc != GTMOE_OK) return rc;
+        tw.drop_seed = L->dropout_seed;
+        tw.drop_offset = 4 * L->dropout_calls++;
+    }
     const int d = L->d, dp = L->dp, hp = L->hp, E = L->E, S = L->S, k = L->k, G = L->G;
     const bool hash = L->desc.use_hash_routing != 0;
     // The rows cross the bus as fp32 through pinned staging, as in a forward
@@ -1343,7 +1406,9 @@ int32_t adapter_forward(gtmoe_layer *L, int T, const double *inputs, const int64
         HIP_TRY(ctx, tables.send(s));
         RUN(ctx, s, "router", launch_router(w.xf, dp, T, d, L->router_w, dp, tw.zero_bias, E, w.logits, s));
         const LoraArgs ar = lora_args(L->ad_router, T, tw.rt);
-        RUN(ctx, s, "lora_down", launch_lora_down(ar, w.xf, dp, nullptr, tw.u_router, s));
+        if (drop)
+            RUN(ctx, s, "adapter_dropout", adapter_dropout(tw, kDropRouter, T, dp, w.xf, nullptr, nullptr, tw.dropped, s));
+        RUN(ctx, s, "lora_down", launch_lora_down(ar, drop ? tw.dropped : w.xf, dp, nullptr, tw.u_router, s));
         RUN(ctx, s, "lora_up_bias", launch_lora_up_bias_f64(ar, tw.u_router, w.logits, E, L->router_b, s));
         RUN(ctx, s, "topk", launch_topk(w.logits, T, E, k, L->balance, w.chosen, w.gates, w.gates32, s));
     }
@@ -1411,10 +1476,15 @@ int32_t adapter_forward(gtmoe_layer *L, int T, const double *inputs, const int64
         const DeviceMatrix &m;
         const AdapterSet &a;
         float *pre, *u;
+        DropoutRole drop;
     };
-    for (const Role &r : {Role{L->gate, L->ad_gate, tw.gpre, tw.u_gate}, Role{L->up, L->ad_up, tw.upre, tw.u_up}}) {
+    for (const Role &r : {Role{L->gate, L->ad_gate, tw.gpre, tw.u_gate, kDropGate},
+                          Role{L->up, L->ad_up, tw.upre, tw.u_up, kDropUp}}) {
         const LoraArgs la = lora_args(r.a, P, tw.ot);
-        RUN(ctx, s, "lora_down", launch_lora_down(la, w.xf, dp, w.tok, r.u, s));
+        if (drop)
+            RUN(ctx, s, "adapter_dropout", adapter_dropout(tw, r.drop, P, dp, w.xf, w.tok, nullptr, tw.dropped, s));
+        RUN(ctx, s, "lora_down",
+            launch_lora_down(la, drop ? tw.dropped : w.xf, dp, drop ? nullptr : w.tok, r.u, s));
         RUN(ctx, s, "lora_up_bias", launch_lora_up_bias(la, r.u, r.pre, hp, r.m.biases, s));
     }
     RUN(ctx, s, "swiglu", launch_swiglu_forward(tw.gpre, tw.upre, P, L->h, hp, limit, w.hidden32, s));
@@ -1437,7 +1507,9 @@ int32_t adapter_forward(gtmoe_layer *L, int T, const double *inputs, const int64
     b.raw = 1;
     RUN(ctx, s, "gemv_down", launch_gemv_down(b, L->down.precision, slices, s));
     const LoraArgs ld = lora_args(L->ad_down, P, tw.ot);
-    RUN(ctx, s, "lora_down", launch_lora_down(ld, w.hidden32, hp, nullptr, tw.u_down, s));
+    if (drop)
+        RUN(ctx, s, "adapter_dropout", adapter_dropout(tw, kDropDown, P, hp, w.hidden32, nullptr, nullptr, tw.dropped, s));
+    RUN(ctx, s, "lora_down", launch_lora_down(ld, drop ? tw.dropped : w.hidden32, hp, nullptr, tw.u_down, s));
     RUN(ctx, s, "lora_up_bias", launch_lora_up_bias(ld, tw.u_down, w.slot_out, d, L->down.biases, s));
     RUN(ctx, s, "combine",
         launch_combine(T, d, S, k, w.slot_out, false, w.pos, w.gates32, nullptr,
@@ -1478,23 +1550,40 @@ int32_t adapter_backward(gtmoe_layer *L, int T, const double *output_grads, doub
         return launch_rows_transposed(r, m.precision, tw.ntiles_tr, tw.tile_tr, chunks, tw.partial, s);
     };
     RUN(ctx, s, "rows_transposed", transposed(L->down, tw.eg, d, tw.hgrad, hp));
-    RUN(ctx, s, "lora_backward",
-        launch_lora_backward(lora_args(L->ad_down, P, tw.ot), tw.eg, d,
-                             tw.u_down, w.hidden32, hp, nullptr, tw.t, tw.hgrad, hp, L->ad_down.dA, L->ad_down.dB,
-                             tw.outer, s));
+    // An adapter's gradients with dropout: its inputs masked again as the
+    // forward masked them, and t A masked before it joins dx.
+    auto lora_backward = [&](const AdapterSet &ad, const TrainWorkspace::OuterTiles &ot, DropoutRole role, int rows,
+                             const float *grad, int ld_g, const float *u, const float *in, int ld, const int32_t *tok,
+                             float *dx) -> int32_t {
+        const LoraArgs la = lora_args(ad, rows, ot);
+        if (!tw.drop_threshold) {
+            RUN(ctx, s, "lora_backward",
+                launch_lora_backward(la, grad, ld_g, u, in, ld, tok, tw.t, dx, ld, ad.dA, ad.dB, tw.outer, s));
+            return GTMOE_OK;
+        }
+        RUN(ctx, s, "adapter_dropout", adapter_dropout(tw, role, rows, ld, in, tok, nullptr, tw.dropped, s));
+        RUN(ctx, s, "clear_gradient", hipMemsetAsync(tw.dropped_grad, 0, (size_t)rows * ld * sizeof(float), s));
+        RUN(ctx, s, "lora_backward",
+            launch_lora_backward(la, grad, ld_g, u, tw.dropped, ld, nullptr, tw.t, tw.dropped_grad, ld, ad.dA, ad.dB,
+                                 tw.outer, s));
+        RUN(ctx, s, "adapter_dropout", adapter_dropout(tw, role, rows, ld, tw.dropped_grad, nullptr, dx, dx, s));
+        return GTMOE_OK;
+    };
+    int32_t done = lora_backward(L->ad_down, tw.ot, kDropDown, P, tw.eg, d, tw.u_down, w.hidden32, hp, nullptr, tw.hgrad);
+    if (done != GTMOE_OK) return done;
     RUN(ctx, s, "swiglu_backward",
         launch_swiglu_backward(tw.hgrad, tw.gpre, tw.upre, P, L->h, hp, limit, tw.ggrad, tw.ugrad, s));
     struct Role {
         const DeviceMatrix &m;
         AdapterSet &a;
         float *grad, *u, *dx;
+        DropoutRole drop;
     };
-    for (const Role &r : {Role{L->gate, L->ad_gate, tw.ggrad, tw.u_gate, tw.dxg},
-                          Role{L->up, L->ad_up, tw.ugrad, tw.u_up, tw.dxu}}) {
+    for (const Role &r : {Role{L->gate, L->ad_gate, tw.ggrad, tw.u_gate, tw.dxg, kDropGate},
+                          Role{L->up, L->ad_up, tw.ugrad, tw.u_up, tw.dxu, kDropUp}}) {
         RUN(ctx, s, "rows_transposed", transposed(r.m, r.grad, hp, r.dx, dp));
-        RUN(ctx, s, "lora_backward",
-            launch_lora_backward(lora_args(r.a, P, tw.ot), r.grad, hp,
-                                 r.u, w.xf, dp, w.tok, tw.t, r.dx, dp, r.a.dA, r.a.dB, tw.outer, s));
+        done = lora_backward(r.a, tw.ot, r.drop, P, r.grad, hp, r.u, w.xf, dp, w.tok, r.dx);
+        if (done != GTMOE_OK) return done;
     }
     RUN(ctx, s, "gather_input_grad", launch_gather_input_grad(tw.dxg, tw.dxu, dp, d, T, S, k, w.pos, tw.dx, s));
     if (!L->desc.use_hash_routing) {
@@ -1502,10 +1591,8 @@ int32_t adapter_backward(gtmoe_layer *L, int T, const double *output_grads, doub
             launch_router_backward(tw.og, d, w.slot_out, d, w.chosen, w.gates, w.logits, w.pos, S, T, E, k, tw.lg,
                                    tw.lgf, s));
         RUN(ctx, s, "router_input_grad", launch_router_input_grad(tw.lgf, T, E, L->router_w, dp, d, tw.dxr, dp, s));
-        RUN(ctx, s, "lora_backward",
-            launch_lora_backward(lora_args(L->ad_router, T, tw.rt),
-                                 tw.lgf, E, tw.u_router, w.xf, dp, nullptr, tw.t, tw.dxr, dp, L->ad_router.dA,
-                                 L->ad_router.dB, tw.outer, s));
+        done = lora_backward(L->ad_router, tw.rt, kDropRouter, T, tw.lgf, E, tw.u_router, w.xf, dp, nullptr, tw.dxr);
+        if (done != GTMOE_OK) return done;
         RUN(ctx, s, "add_rows", launch_add_rows_f64(tw.dxr, dp, d, T, tw.dx, s));
     }
     HIP_TRY(ctx, hipMemcpyAsync(L->stage, tw.dx, sizeof(double) * T * d, hipMemcpyDeviceToHost, s));
@@ -2696,6 +2783,7 @@ int32_t gtmoe_layer_add_adapters(gtmoe_layer *L, int32_t rank, double alpha, uin
     free_train_workspace(L->tw);
     L->has_adapters = true;
     L->adapter_T = -1;
+    L->dropout_rate = 0;
     return GTMOE_OK;
 }
 
@@ -2706,6 +2794,20 @@ int32_t gtmoe_layer_remove_adapters(gtmoe_layer *L)
     ENTER(ctx);
     HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
     free_adapters(L);
+    return GTMOE_OK;
+}
+
+int32_t gtmoe_layer_set_adapter_dropout(gtmoe_layer *L, double rate, uint64_t seed)
+{
+    if (!L) return GTMOE_ERR_INVALID_ARGUMENT;
+    gtmoe_context *ctx = L->ctx;
+    ENTER_NODEV(ctx);
+    if (!(rate >= 0.0 && rate < 1.0))
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "dropout rate must be at least 0 and less than 1, got %g", rate);
+    if (!L->has_adapters) return fail(ctx, GTMOE_ERR_NOT_READY, "the layer has no low-rank adapters");
+    L->dropout_rate = rate;
+    L->dropout_seed = seed;
+    L->dropout_calls = 0;
     return GTMOE_OK;
 }
 
@@ -3223,21 +3325,6 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
     TRY(run_plain(ctx, s, "adapter_down", [&] { return launch_adapter_down(dargs, desc->values, s); }));
     return run_plain(ctx, s, "adapted_forward", [&] { return launch_adapted(a, desc->values, s); });
 }
-
-}  // extern "C"
-
-namespace {
-
-// 16-bit threshold and scale of a dropout rate.
-void dropout_rate(double rate, uint32_t &threshold, float &scale)
-{
-    threshold = std::min<uint32_t>((uint32_t)std::floor(rate * 65536.0 + 0.5), 65535u);
-    scale = (float)(65536.0 / (65536.0 - threshold));
-}
-
-}  // namespace
-
-extern "C" {
 
 int32_t gtmoe_dropout(gtmoe_context *ctx, const gtmoe_dropout_desc *desc, const void *inputs, const void *base,
                       void *outputs, double rate, uint64_t seed, uint64_t offset, void *stream)

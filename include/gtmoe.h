@@ -380,8 +380,8 @@ int32_t gtmoe_layer_load_weights(gtmoe_layer *layer, gtmoe_weights_file *file, c
  * the router) computes pre = (x W^T + s (x Down^T) Up^T) + b with s =
  * alpha / rank (perceptron/layer.go:133-162, perceptron/adapter.go:66-76),
  * in fp32, and keeps what gtmoe_backward needs.  gtmoe_forward_device, the
- * stack and graph entry points refuse such a layer.  Adapter dropout is not
- * supported (rate 0).
+ * stack and graph entry points refuse such a layer.  Adapter dropout is off
+ * until gtmoe_layer_set_adapter_dropout.
  * ------------------------------------------------------------------------- */
 
 /* Model.AddLowRankAdapters over MixtureOfExperts.Layers
@@ -394,6 +394,16 @@ int32_t gtmoe_layer_load_weights(gtmoe_layer *layer, gtmoe_weights_file *file, c
 int32_t gtmoe_layer_add_adapters(gtmoe_layer *layer, int32_t rank, double alpha, uint64_t seed);
 /* Model.RemoveAdapters (adapters.go:40-46). */
 int32_t gtmoe_layer_remove_adapters(gtmoe_layer *layer);
+/* Dropout on the adapters' inputs (AdapterDropout, perceptron/adapter.go:66-76)
+ * of this layer's later forwards and their backwards; rate 0 turns it off, as
+ * for evaluation.  The masks are gtmoe_dropout's, not the reference's random
+ * source: forward number c since this call (0, 1, ...) takes `seed` and offset
+ * 4 c + 0 for gate, + 1 for up, + 2 for down, + 3 for the router; a mask's row is
+ * the row's position (shared expert s: s tokens + token; routed: shared experts
+ * times tokens plus its place in rows_for_expert) or, for the router, the
+ * token.  gtmoe_backward makes the last forward's masks again.
+ * GTMOE_ERR_NOT_READY without adapters; adding adapters starts without dropout. */
+int32_t gtmoe_layer_set_adapter_dropout(gtmoe_layer *layer, double rate, uint64_t seed);
 /* Rank of one layer's adapter (LowRankAdapter.Rank); role/index as in
  * gtmoe_upload_rows. */
 int32_t gtmoe_layer_adapter_rank(gtmoe_layer *layer, int32_t role, int32_t index, int32_t *rank);

@@ -62,17 +62,18 @@ def _up_deriv(x, limit):
     return np.ones_like(x)
 
 
-def _layer_forward(W, b, ad, x):
-    """pre = (x W^T + s (x Down^T) Up^T) + b; returns (pre, u)."""
+def _layer_forward(W, b, ad, x, kept=1.0):
+    """pre = (x W^T + s ((kept x) Down^T) Up^T) + b; returns (pre, u).  kept:
+    the adapter's dropout on its inputs, 0 or its scale per value."""
     pre = x @ W.T
     u = None
     if ad is not None:
-        u = x @ ad.down.T
+        u = (x * kept) @ ad.down.T
         pre = pre + (ad.alpha / ad.down.shape[0]) * (u @ ad.up.T)
     return pre + b, u
 
 
-def _layer_backward(W, ad, x, u, pre_grad, grads, key):
+def _layer_backward(W, ad, x, u, pre_grad, grads, key, kept=1.0):
     """Frozen-base Layer.Backward from the pre-activation gradient."""
     dx = pre_grad @ W
     if ad is not None:
@@ -80,8 +81,8 @@ def _layer_backward(W, ad, x, u, pre_grad, grads, key):
         dA, dB = grads[key]
         dB += s * (pre_grad.T @ u)
         t = s * (pre_grad @ ad.up)
-        dA += t.T @ x
-        dx = dx + t @ ad.down
+        dA += t.T @ (x * kept)
+        dx = dx + (t @ ad.down) * kept
     return dx
 
 
@@ -90,24 +91,37 @@ def _expert_weights(e):
             for w in ("gate", "up", "down")}
 
 
-def _expert_forward(e, key, adapters, x, limit):
+def _no_dropout(which, positions, columns):
+    return 1.0
+
+
+def _masked(kept):
+    """_layer_backward's argument for an adapter's dropout (none without)."""
+    return {"kept": kept} if isinstance(kept, np.ndarray) else {}
+
+
+def _expert_forward(e, key, adapters, x, limit, dropout=_no_dropout, positions=None):
     W = _expert_weights(e)
     ad = {w: adapters.get(key + (w,)) for w in ("gate", "up", "down")}
-    gpre, ug = _layer_forward(*W["gate"], ad["gate"], x)
-    upre, uu = _layer_forward(*W["up"], ad["up"], x)
+    kept = {w: dropout(w, positions, W[w][0].shape[1]) for w in ("gate", "up", "down")}
+    gpre, ug = _layer_forward(*W["gate"], ad["gate"], x, kept["gate"])
+    upre, uu = _layer_forward(*W["up"], ad["up"], x, kept["up"])
     gout, uout = _gate_act(gpre, limit), _up_act(upre, limit)
     hidden = gout * uout
-    out, ud = _layer_forward(*W["down"], ad["down"], hidden)
-    return out, SimpleNamespace(W=W, ad=ad, x=x, gpre=gpre, upre=upre, gout=gout, uout=uout, hidden=hidden,
+    out, ud = _layer_forward(*W["down"], ad["down"], hidden, kept["down"])
+    return out, SimpleNamespace(W=W, ad=ad, kept=kept, x=x, gpre=gpre, upre=upre, gout=gout, uout=uout, hidden=hidden,
                                 u={"gate": ug, "up": uu, "down": ud})
 
 
 def _expert_backward(st, key, out_grad, grads, limit):
-    hg = _layer_backward(st.W["down"][0], st.ad["down"], st.hidden, st.u["down"], out_grad, grads, key + ("down",))
+    hg = _layer_backward(st.W["down"][0], st.ad["down"], st.hidden, st.u["down"], out_grad, grads, key + ("down",),
+                         **_masked(st.kept["down"]))
     gg = hg * st.uout * _gate_deriv(st.gpre, limit)
     ug = hg * st.gout * _up_deriv(st.upre, limit)
-    dx = _layer_backward(st.W["gate"][0], st.ad["gate"], st.x, st.u["gate"], gg, grads, key + ("gate",))
-    return dx + _layer_backward(st.W["up"][0], st.ad["up"], st.x, st.u["up"], ug, grads, key + ("up",))
+    dx = _layer_backward(st.W["gate"][0], st.ad["gate"], st.x, st.u["gate"], gg, grads, key + ("gate",),
+                         **_masked(st.kept["gate"]))
+    return dx + _layer_backward(st.W["up"][0], st.ad["up"], st.x, st.u["up"], ug, grads, key + ("up",),
+                                **_masked(st.kept["up"]))
 
 
 def _affinity(logits):
@@ -115,11 +129,15 @@ def _affinity(logits):
     return np.sqrt(sp)
 
 
-def forward(moe, adapters, x, token_ids=None, chosen=None):
+def forward(moe, adapters, x, token_ids=None, chosen=None, dropout=_no_dropout):
     """MixtureOfExperts.Forward with adapters.  `chosen` (T x k, ascending per
     row) replaces the top-k choice when given (to follow another
     implementation's routing at near-ties); the gates always come from this
-    forward's own logits.  Returns (outputs, state for backward)."""
+    forward's own logits.  dropout(which, positions, columns) gives the factors
+    of an adapter's inputs (perceptron/adapter.go:66-76 with AdapterDropout):
+    which "gate"/"up"/"down" and the positions of its rows (shared expert s on
+    s T + token, then the routed rows by expert and token), or "router" and the
+    tokens.  Returns (outputs, state for backward)."""
     x = np.atleast_2d(np.asarray(x, np.float64))
     T = x.shape[0]
     E, k = len(moe.routed), moe.experts_per_token
@@ -131,7 +149,7 @@ def forward(moe, adapters, x, token_ids=None, chosen=None):
     else:
         Wr = decode_rows(moe.router.weights)
         logits, u_router = _layer_forward(Wr, np.asarray(moe.router.biases, np.float64),
-                                          adapters.get(("router", 0, None)), x)
+                                          adapters.get(("router", 0, None)), x, dropout("router", np.arange(T), x.shape[1]))
         r = route_from_logits(logits, k, moe.balance_biases)
         ch = r.chosen if chosen is None else np.asarray(chosen, np.int32)
         aff = _affinity(logits)
@@ -140,16 +158,19 @@ def forward(moe, adapters, x, token_ids=None, chosen=None):
     out = np.zeros((T, moe.vector_size))
     shared_states = []
     for s, e in enumerate(moe.shared):
-        y, st = _expert_forward(e, ("shared", s), adapters, x, limit)
+        y, st = _expert_forward(e, ("shared", s), adapters, x, limit, dropout, s * T + np.arange(T))
         out = out + y
         shared_states.append(st)
     routed_states, rows_for = {}, {}
     expert_out = {}
+    first = len(moe.shared) * T
     for e in range(E):
         rows = [t for t in range(T) if e in ch[t]]
         rows_for[e] = rows
         if rows:
-            y, st = _expert_forward(moe.routed[e], ("routed", e), adapters, x[rows], limit)
+            y, st = _expert_forward(moe.routed[e], ("routed", e), adapters, x[rows], limit, dropout,
+                                    first + np.arange(len(rows)))
+            first += len(rows)
             routed_states[e] = st
             expert_out[e] = y
     for t in range(T):
@@ -157,7 +178,8 @@ def forward(moe, adapters, x, token_ids=None, chosen=None):
             e = int(ch[t, i])
             out[t] += gates[t, i] * expert_out[e][rows_for[e].index(t)]
     state = SimpleNamespace(x=x, chosen=ch, gates=gates, logits=logits, u_router=u_router, shared=shared_states,
-                            routed=routed_states, rows_for=rows_for, expert_out=expert_out, limit=limit)
+                            routed=routed_states, rows_for=rows_for, expert_out=expert_out, limit=limit,
+                            kept_router=1.0 if moe.use_hash_routing else dropout("router", np.arange(T), x.shape[1]))
     return out, state
 
 
@@ -195,24 +217,24 @@ def backward(moe, adapters, state, out_grad, grads):
             lg[t, e] = ag * (_sigmoid(state.logits[t, e]) / (2 * aff[t, e]))
     Wr = decode_rows(moe.router.weights)
     return dx + _layer_backward(Wr, adapters.get(("router", 0, None)), state.x, state.u_router, lg, grads,
-                                ("router", 0, None))
+                                ("router", 0, None), **_masked(state.kept_router))
 
 
-def gradient_check(moe, adapters, x, token_ids=None, seed=0, step=1e-6, allowed=1e-5):
+def gradient_check(moe, adapters, x, token_ids=None, seed=0, step=1e-6, allowed=1e-5, dropout=_no_dropout):
     """gradientcheck.Compare (gradientcheck/gradientcheck.go:17-61) on the
     adapters and the inputs: loss = sum(outputs * G) with G uniform in
     [-1, 1); central differences of step 1e-6 must agree with the backward to
     1e-5 * max(1, |numerical|).  Returns the list of problems."""
     rng = np.random.default_rng(seed)
     x = np.array(x, np.float64)
-    out, _ = forward(moe, adapters, x, token_ids)
+    out, _ = forward(moe, adapters, x, token_ids, dropout=dropout)
     G = rng.uniform(-1, 1, out.shape)
 
     def loss():
-        return float(np.sum(forward(moe, adapters, x, token_ids)[0] * G))
+        return float(np.sum(forward(moe, adapters, x, token_ids, dropout=dropout)[0] * G))
 
     grads = zero_grads(moe, adapters)
-    _, st = forward(moe, adapters, x, token_ids)
+    _, st = forward(moe, adapters, x, token_ids, dropout=dropout)
     dx = backward(moe, adapters, st, G, grads)
     problems = []
 
