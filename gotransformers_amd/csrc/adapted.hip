@@ -15,6 +15,91 @@ constexpr int kWaves = 8;
 // 2048 15.1 us against 24.3 with 64 x 64 tiles, 512 rows 29.5 against 16.5.
 constexpr int kFewRows = 256;
 
+// From this many rows times ranks on, with whole 16-byte rows and up to
+// kMaxSortedRank ranks, the rows are sorted by adapter (1024 -> 2048, 64 adapters,
+// bf16, us; runs of 1, 7 and 512 rows of one request):
+//                       sorted            in order
+//   8192 rows, rank 64  122, 122, 85      1270, 370, 102
+//   8192 rows, rank 16  113, 111, 79      225, 143, 82
+//   4096 rows, rank 64  92, 93, 60        585, 190, 57
+//   2048 rows, rank 64  84, 87, 53        257, 112, 36
+//   4096 rows, rank 16  86, 86, 57        103, 70, 44
+constexpr long long kSortedValues = 1 << 17;
+constexpr int kSortWaves = 16, kSortBins = 1024;
+
+// Rows by adapter (bin `adapters`: none), by one workgroup: every wave counts
+// the bins of its stretch of rows, the counts are summed over bins and waves,
+// and every wave places its rows.  64 rows of one bin keep their order; rows of
+// a bin among mixed ones take their places as they come, which changes no
+// result: a row's sums do not depend on the rows beside it.
+__global__ __launch_bounds__(64 * kSortWaves) void adapter_sort_kernel(const int32_t *__restrict__ adapter, int rows, int adapters,
+                                                                       int32_t *__restrict__ index, int32_t *__restrict__ offsets)
+{
+    __shared__ int place[kSortWaves][kSortBins];
+    __shared__ int sums[kSortWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bins = adapters + 1;
+    for (int i = threadIdx.x; i < kSortWaves * kSortBins; i += 64 * kSortWaves) (&place[0][0])[i] = 0;
+    const int each = ((rows + kSortWaves - 1) / kSortWaves + 63) & ~63;
+    const int begin = min(rows, wave * each), end = min(rows, begin + each);
+    auto bin_of = [&](int t) {
+        const int a = t < end ? adapter[t] : -1;
+        return a < 0 || a >= adapters ? adapters : a;
+    };
+    __syncthreads();
+    // eight times 64 rows of a wave's stretch are loaded together
+    auto each_chunk = [&](auto &&take) {
+        for (int t = begin; t < end; t += 512) {
+            int b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = bin_of(t + 64 * i + lane);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int n = min(64, end - (t + 64 * i));
+                if (n <= 0) break;
+                const int one = __builtin_amdgcn_readfirstlane(b[i]);
+                take(t + 64 * i, b[i], n, one, __ballot(b[i] != one && lane < n) == 0);
+            }
+        }
+    };
+    each_chunk([&](int t0, int b, int n, int one, bool same) {
+        if (same) {
+            if (lane == 0) place[wave][one] += n;
+        } else if (lane < n) {
+            atomicAdd(&place[wave][b], 1);
+        }
+    });
+    __syncthreads();
+    // a thread per bin: its rows before every wave's, then the bins before it
+    int total = 0;
+    if (threadIdx.x < bins)
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int n = place[w][threadIdx.x];
+            place[w][threadIdx.x] = total;
+            total += n;
+        }
+    int all;
+    int before = wave_sum_before(total, all);
+    if (lane == 0) sums[wave] = all;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) before += sums[w];
+    if (threadIdx.x < bins) {
+        offsets[threadIdx.x] = before;
+        for (int w = 0; w < kSortWaves; ++w) place[w][threadIdx.x] += before;
+        if (threadIdx.x == bins - 1) offsets[bins] = before + total;
+    }
+    __syncthreads();
+    each_chunk([&](int t0, int b, int n, int one, bool same) {
+        if (same) {
+            const int at = place[wave][one];
+            if (lane < n) index[at + lane] = t0 + lane;
+            if (lane == 0) place[wave][one] = at + n;
+        } else if (lane < n) {
+            index[atomicAdd(&place[wave][b], 1)] = t0 + lane;
+        }
+    });
+}
+
 // 16 bytes of a row's reduction from value k on (zero at and past `length`),
 // any alignment.
 template <class T>
@@ -131,11 +216,12 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(AdapterDownAr
     const int rows = min(tile, a.rows - t0);
     typedef typename T::Store Store;
     int mine = -1;
+    const int at = t0 + min(i, rows - 1), row = a.index ? a.index[at] : at;
     if (i < rows) {
-        mine = a.adapter[t0 + i];
+        mine = a.adapter[row];
         if (mine >= a.adapters) mine = -1;
     }
-    const Store *const x[1] = {reinterpret_cast<const Store *>(a.x) + (long long)(t0 + min(i, rows - 1)) * a.ldx};
+    const Store *const x[1] = {reinterpret_cast<const Store *>(a.x) + (long long)row * a.ldx};
     f32x4 acc[NR];
 #pragma unroll
     for (int p = 0; p < NR; ++p) acc[p] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -166,6 +252,45 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(AdapterDownAr
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[wave][i][16 * p + 4 * q + e] = acc[p][e];
     __syncthreads();
+    if constexpr (T::kBytes == 2) {
+        if (a.index) {
+            // u's two 16-bit parts (RankRow), of the row scaled to values below
+            // 2 for fp16: 32 lanes per row, two ranks or fewer each (blockIdx.y is 0)
+            const int r = threadIdx.x >> 5, c0 = threadIdx.x & 31;
+            static_assert(64 * kWaves / 32 == 16, "");
+            const int at = a.index[t0 + min(r, rows - 1)], ad = a.adapter[at];
+            const bool has = r < rows && ad >= 0 && ad < a.adapters;
+            float v[2] = {0.f, 0.f}, top = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = c0 + 32 * e;
+                if (has && c < 16 * NR && c < a.rank) {
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) v[e] += part[w][r][c];
+                    v[e] *= a.scales[ad];
+                }
+                top = fmaxf(top, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.f);
+            }
+#pragma unroll
+            for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+            if (!has) return;
+            const RowScale scale = row_scale<T>(top);
+            Store *hi = reinterpret_cast<Store *>(a.u_hi) + (long long)at * a.ldu;
+            Store *lo = reinterpret_cast<Store *>(a.u_lo) + (long long)at * a.ldu;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = c0 + 32 * e;
+                if (c < a.ldu) {
+                    float hv, lv;
+                    two_parts<T>(v[e], scale.down, hv, lv);
+                    hi[c] = T::round(hv);
+                    lo[c] = T::round(lv);
+                }
+            }
+            if (c0 == 0) a.unscale[t0 + r] = scale.up;  // in the sorted order
+            return;
+        }
+    }
     for (int o = threadIdx.x; o < 16 * 16 * NR; o += 64 * kWaves) {
         const int r = o / (16 * NR), c = o - r * (16 * NR);
         if (r < rows && j0 + c < a.ldu) {
@@ -275,6 +400,10 @@ hipError_t launch_down(const AdapterDownArgs &a, int tile, hipStream_t s)
 template <class T>
 hipError_t launch_down_values(const AdapterDownArgs &a, hipStream_t s)
 {
+    if (a.index) {
+        if (a.rank <= 16) return launch_down<T, 1>(a, 16, s);
+        return a.rank <= 32 ? launch_down<T, 2>(a, 16, s) : launch_down<T, 4>(a, 16, s);
+    }
     const int tile = a.rows <= 512 ? 1 : a.rows >= 8192 ? 16 : (a.rows + 511) / 512;
     if (a.rows < 512 || a.rank <= 16) return launch_down<T, 1>(a, tile, s);
     return a.rank <= 32 ? launch_down<T, 2>(a, tile, s) : launch_down<T, 4>(a, tile, s);
@@ -316,9 +445,26 @@ hipError_t launch_adapter_down(const AdapterDownArgs &a, int values, hipStream_t
     }
 }
 
+bool adapted_sorts(const GroupedArgs &a, int values)
+{
+    if (values == kValuesF32 || !a.b || (long long)a.rows * a.term.rank < kSortedValues || a.term.adapters >= kSortBins) return false;
+    const AdapterTerm &t = a.term;
+    auto whole = [](const void *p, long long stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; };
+    return whole(a.a, a.lda) && whole(a.b, a.ldb) && whole(t.up, t.rank) && a.inputs % 8 == 0 && t.rank <= kMaxSortedRank &&
+           (long long)a.rows * a.lda < 1 << 30 && (long long)a.rows * t.ldu < 1 << 30;
+}
+
+hipError_t launch_adapter_sort(const int32_t *adapter, int rows, int adapters, int32_t *index, int32_t *offsets,
+                               hipStream_t s)
+{
+    hipLaunchKernelGGL(adapter_sort_kernel, dim3(1), dim3(64 * kSortWaves), 0, s, adapter, rows, adapters, index, offsets);
+    return hipGetLastError();
+}
+
 hipError_t launch_adapted(const GroupedArgs &a, int values, hipStream_t s)
 {
     if (a.rows == 0) return hipSuccess;
+    if (a.term.index) return launch_large(a, kGroupedForward, values, s);
     if (a.rows > kFewRows) return launch_grouped(a, kGroupedForward, values, s);
     switch (values) {
     case kValuesBf16: return launch_few<Bf16>(a, s);

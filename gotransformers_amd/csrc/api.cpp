@@ -3240,6 +3240,23 @@ int32_t check_adapted(gtmoe_context *ctx, const gtmoe_adapted_desc *d)
 
 int adapter_ldu(const gtmoe_adapted_desc *d) { return (d->rank + 7) / 8 * 8; }
 
+// The workspace of one call: u in fp32, or its two 16-bit parts in the same
+// place; then, for rows sorted by adapter, each row's scale, the order and the
+// adapters' first places in it.
+struct AdaptedWorkspace {
+    size_t unscale, index, offsets, bytes;
+};
+AdaptedWorkspace adapted_workspace(const gtmoe_adapted_desc *d)
+{
+    const size_t rows = std::max(d->rows, 1);
+    AdaptedWorkspace w;
+    w.unscale = rows * adapter_ldu(d) * sizeof(float);
+    w.index = w.unscale + align_up(rows * sizeof(float), 16);
+    w.offsets = w.index + align_up(rows * sizeof(int32_t), 16);
+    w.bytes = w.offsets + align_up(((size_t)d->adapters + 2) * sizeof(int32_t), 16);
+    return w;
+}
+
 }  // namespace
 
 extern "C" {
@@ -3248,7 +3265,7 @@ int32_t gtmoe_adapted_workspace(const gtmoe_adapted_desc *desc, size_t *bytes)
 {
     if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
     TRY(check_adapted(nullptr, desc));
-    *bytes = (size_t)std::max(desc->rows, 1) * adapter_ldu(desc) * sizeof(float);
+    *bytes = adapted_workspace(desc).bytes;
     return GTMOE_OK;
 }
 
@@ -3262,7 +3279,8 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
     auto check = [&](gtmoe_context *c) -> int32_t {
         TRY(check_adapted(c, desc));
         const int es = value_bytes(desc->values), ldu = adapter_ldu(desc);
-        const size_t need = (size_t)desc->rows * ldu * sizeof(float);
+        const AdaptedWorkspace layout = adapted_workspace(desc);
+        const size_t need = layout.bytes;
         if (desc->rows > 0) {
             TRY(check_pointer(c, "inputs", inputs, es));
             if (weights) TRY(check_pointer(c, "weights", weights, es));
@@ -3315,6 +3333,15 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
         dargs.rank = desc->rank;
         dargs.adapters = desc->adapters;
         dargs.ldu = ldu;
+        if (adapted_sorts(a, desc->values)) {
+            char *base = reinterpret_cast<char *>(workspace);
+            a.offsets = reinterpret_cast<const int32_t *>(base + layout.offsets);
+            a.groups = desc->adapters + 1;  // the last: rows without an adapter
+            a.term.index = dargs.index = reinterpret_cast<const int32_t *>(base + layout.index);
+            a.term.u_hi = dargs.u_hi = base;
+            a.term.u_lo = dargs.u_lo = base + layout.unscale / 2;
+            a.term.unscale = dargs.unscale = reinterpret_cast<float *>(base + layout.unscale);
+        }
         return check_grid(c, a, kGroupedForward, desc->values);
     };
     if (!ctx) return check_only(check);
@@ -3322,6 +3349,11 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
     TRY(check(ctx));
     if (desc->rows == 0) return GTMOE_OK;
     hipStream_t s = (hipStream_t)stream;
+    if (a.term.index)
+        TRY(run_plain(ctx, s, "adapter_sort", [&] {
+            return launch_adapter_sort(adapter, a.rows, desc->adapters, const_cast<int32_t *>(a.term.index),
+                                       const_cast<int32_t *>(a.offsets), s);
+        }));
     TRY(run_plain(ctx, s, "adapter_down", [&] { return launch_adapter_down(dargs, desc->values, s); }));
     return run_plain(ctx, s, "adapted_forward", [&] { return launch_adapted(a, desc->values, s); });
 }

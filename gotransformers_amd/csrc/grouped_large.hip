@@ -194,6 +194,13 @@ struct MatrixTiles {
     }
 };
 
+__device__ __forceinline__ const char *scalar(const char *p)
+{
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<const char *>((uint64_t)hi << 32 | lo);
+}
+
 // Eight 16-bit or four fp32 values of a row as 16 bytes.
 template <class O>
 __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int left, bool aligned, bool add)
@@ -219,10 +226,13 @@ __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int le
     }
 }
 
-template <class T, int DIR>
+// ADAPTED (forward, one matrix for all groups): the groups are the adapters, their
+// rows at the places of a.term.index.  The adapter's term is two steps more of
+// the same stream, u's parts against the adapter's up matrix.
+template <class T, int DIR, bool ADAPTED>
 __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 {
-    typedef Operand<T, DIR != kGroupedWeightGradient, kBm, kThreads, SB> A;
+    typedef Operand<T, DIR != kGroupedWeightGradient, kBm, kThreads, SB, ADAPTED> A;
     typedef Operand<T, DIR == kGroupedForward, kBn, kThreads, SB> B;
     typedef typename T::Store Store;
     constexpr int NJ = 2, KK = SB / 32, L = A::kLoads + B::kLoads;
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
     // A tile: rows m0 .. + m of the output buffer (weight gradient: of the
     // group's matrix), columns n0 .. + n, its operands and steps.
     struct Tile {
-        int g, m0, n0, m, n, length, steps;
+        int g, m0, n0, m, n, length, steps, extra;  // extra: steps of an adapter's term
     };
     RowTiles rows_of(a, columns, (DIR == kGroupedForward ? a.inputs : a.outputs) * T::kBytes / SB + 1);
     const int strips = (a.outputs + kBm - 1) / kBm;
@@ -252,7 +262,7 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
             x.m0 = q / columns * kBm;
             x.n0 = (q - q / columns * columns) * kBn;
             int lo, hi;
-            group_rows(a, x.g, lo, hi);
+            wave_group_rows(a, x.g, lo, hi);
             x.length = hi - lo;
             x.m = min(kBm, a.outputs - x.m0);
         } else {
@@ -267,24 +277,35 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         x.m = __builtin_amdgcn_readfirstlane(x.m);
         x.length = __builtin_amdgcn_readfirstlane(x.length);
         x.steps = max(2, ((x.length + A::kStep - 1) / A::kStep + 1) / 2 * 2);
+        x.extra = ADAPTED && x.g < a.term.adapters ? 2 : 0;
         return x;
     };
     auto operand_a = [&](const Tile &x) {
         const Store *p = reinterpret_cast<const Store *>(a.a);
         if constexpr (DIR == kGroupedWeightGradient) {
             int lo, hi;
-            group_rows(a, x.g, lo, hi);
+            wave_group_rows(a, x.g, lo, hi);
             p += __builtin_amdgcn_readfirstlane(lo) * a.lda + x.m0;
-        } else {
+        } else if constexpr (!ADAPTED) {
             p += x.m0 * a.lda;
         }
-        return A(p, a.lda, x.m, x.length);
+        if constexpr (ADAPTED) return A(p, a.lda, a.rows, a.term.index + x.m0, x.m, x.length);
+        else return A(p, a.lda, x.m, x.length);
+    };
+    auto operand_u = [&](const Tile &x) {
+        if constexpr (ADAPTED) return A(a.term.u_hi, a.term.ldu, a.rows, a.term.index + x.m0, x.m, a.term.rank);
+        else return 0;
+    };
+    auto operand_up = [&](const Tile &x) {
+        const Store *p = reinterpret_cast<const Store *>(a.term.up) +
+                         ((long long)min(x.g, max(a.term.adapters - 1, 0)) * a.outputs + x.n0) * a.term.rank;
+        return B(p, a.term.rank, x.n, a.term.rank);
     };
     auto operand_b = [&](const Tile &x) {
         const Store *p = reinterpret_cast<const Store *>(a.b);
         if constexpr (DIR == kGroupedWeightGradient) {
             int lo, hi;
-            group_rows(a, x.g, lo, hi);
+            wave_group_rows(a, x.g, lo, hi);
             p += __builtin_amdgcn_readfirstlane(lo) * a.ldb + x.n0;
         } else {
             p += x.g * a.group_stride + (DIR == kGroupedForward ? x.n0 * a.ldb : (long long)x.n0);
@@ -297,26 +318,56 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
     else rows_of.range(begin, end);
     begin = __builtin_amdgcn_readfirstlane(begin);
     end = __builtin_amdgcn_readfirstlane(end);
-    int t = begin + place();  // the tile whose results are being made
+    int t = begin + place();
     if (t >= end) return;
 
     // the request stream: the tile whose steps are being requested, and the next of them
     Tile rt = find(t);
     A oa = operand_a(rt);
     B ob = operand_b(rt);
+    auto ou = operand_u(rt);
     int rk = 0, next_t = t + places();
     auto advance = [&]() {
-        if (rk < rt.steps) return;
+        if (rk < rt.steps + rt.extra) return;
         rk = 0;
         if (next_t < end) {
             rt = find(next_t);
             next_t += places();
             oa = operand_a(rt);
             ob = operand_b(rt);
+            ou = operand_u(rt);
         } else {
             oa.length = ob.length = 0;  // nothing more: requests of no bytes
             rt.steps = 1 << 30;
+            rt.extra = 0;
         }
+    };
+    // step rk of the request stream: of the operands, then u's parts and the
+    // adapter's up matrix (every field that is one for the wave kept scalar)
+    auto request_a = [&]() {
+        auto q = oa.request(rk);
+        if constexpr (ADAPTED) {
+            const bool more = rk >= rt.steps;
+            const auto e = ou.request(0);
+            const char *part = reinterpret_cast<const char *>(rk > rt.steps ? a.term.u_lo : a.term.u_hi);
+            q.p = scalar(more ? part : q.p);
+            q.bytes = __builtin_amdgcn_readfirstlane(more ? e.bytes : q.bytes);
+#pragma unroll
+            for (int i = 0; i < A::kLoads; ++i) q.off[i] = more ? e.off[i] : q.off[i];
+        }
+        return q;
+    };
+    auto request_b = [&]() {
+        auto q = ob.request(rk);
+        if constexpr (ADAPTED) {
+            const bool more = rk >= rt.steps;
+            const auto e = operand_up(rt).request(0);
+            q.p = scalar(more ? e.p : q.p);
+            q.bytes = __builtin_amdgcn_readfirstlane(more ? e.bytes : q.bytes);
+            q.row = __builtin_amdgcn_readfirstlane(more ? e.row : q.row);
+            q.off[0] = more ? e.off[0] : q.off[0];
+        }
+        return q;
     };
 
     u32x4 fa[2][4], fb[2][NJ];
@@ -327,14 +378,12 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    {
-        oa.issue(s0, oa.request(0));
-        ob.issue(s0 + kBm * SB, ob.request(0));
-        oa.issue(s1, oa.request(1));
-        ob.issue(s1 + kBm * SB, ob.request(1));
-        rk = 2;
-        landed();
-    }
+    A::issue(s0, oa.request(0));
+    B::issue(s0 + kBm * SB, ob.request(0));
+    A::issue(s1, oa.request(1));
+    B::issue(s1 + kBm * SB, ob.request(1));
+    rk = 2;
+    landed();
 
     Tile x = rt;
     auto run = [&](auto blocks) {
@@ -367,8 +416,8 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         // as in grouped_kernel; the requests run two steps ahead, into the next tile
         auto body = [&](char *cur, const char *next) {
             advance();
-            const auto qa = oa.request(rk);
-            const auto qb = ob.request(rk);
+            const auto qa = request_a();
+            const auto qb = request_b();
             ++rk;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
@@ -376,8 +425,8 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                     read(cur, kk + 1, (kk + 1) & 1);
                 } else {
                     landed();
-                    oa.issue(cur, qa);
-                    ob.issue(cur + kBm * SB, qb);
+                    A::issue(cur, qa);
+                    B::issue(cur + kBm * SB, qb);
                     read(next, 0, 0);
                 }
 #pragma unroll
@@ -389,24 +438,62 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
+        // ADAPTED, asked for now and used at the end: the places of the wave's rows
+        // (lane l: rows l and 64 + l of them) and, fp16, the scales of u's rows
+        const int r = lane & 31;
+        int at_rows[2];
+        float up[MI];
+        if constexpr (ADAPTED) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int row = 64 * (2 * q + h) + wm + r;
+                at_rows[q] = row < x.m ? a.term.index[x.m0 + row] : 0;
+            }
+            if constexpr (std::is_same<T, F16>::value) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const int row = 64 * i + wm + r;
+                    up[i] = x.extra && row < x.m ? a.term.unscale[x.m0 + row] : 1.f;
+                }
+            }
+        }
         read(s0, 0, 0);
         for (int k = 0; k < x.steps; k += 2) {
             body(s0, s1);
             body(s1, s0);
         }
-
+        if constexpr (ADAPTED) {
+            if (x.extra) {
+                // fp16: the row's accumulators in the scale of its u meanwhile
+                if constexpr (std::is_same<T, F16>::value) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc[i][j] *= 1.f / up[i];  // a power of two: exact
+                }
+                body(s0, s1);
+                body(s1, s0);
+                if constexpr (std::is_same<T, F16>::value) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc[i][j] *= up[i];
+                }
+            }
+            if (a.bias) add_bias<T>(acc, a.bias, x.n0 + wn, a.outputs);
+        }
         // results: lane l holds row 64 i + wm + l % 32 and, in register r of
         // block (i, j), column wn + 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.  Through
         // LDS (rows of 128 bytes, 16-byte unit u of row r in slot u ^ (r / 2) % 8) to
         // 16 bytes per lane, eight rows of 128 bytes at a time.
         char *stage = so + wave * 4096;
-        const int r = lane & 31;
         if (DIR == kGroupedWeightGradient && a.accumulate && x.length == 0) return;
         auto leave = [&](auto type) {
             typedef decltype(type) O;
             constexpr int unit = 16 / O::kBytes, each = O::kBytes == 2 ? 2 : 1;  // column blocks per pass
             typename O::Store *out = reinterpret_cast<typename O::Store *>(a.out) +
-                                     (DIR == kGroupedWeightGradient ? x.g * a.group_stride : 0) + x.m0 * a.ldo + x.n0;
+                                     (DIR == kGroupedWeightGradient ? x.g * a.group_stride : 0) +
+                                     (ADAPTED ? 0 : x.m0 * a.ldo) + x.n0;
             const bool aligned = a.ldo % unit == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
@@ -431,7 +518,9 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                         const int rr = 8 * p + (lane >> 3), u = lane & 7;
                         const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + rr * 128 + (u ^ ((rr >> 1) & 7)) * 16);
                         const int row = 64 * i + wm + rr, col = wn + 32 * j0 + unit * u;
-                        if (row < x.m && col < x.n) store_unit<O>(out + row * a.ldo + col, v, x.n - col, aligned, a.accumulate);
+                        int to = row;
+                        if constexpr (ADAPTED) to = __shfl(at_rows[i >> 1], 32 * (i & 1) + rr);
+                        if (row < x.m && col < x.n) store_unit<O>(out + to * a.ldo + col, v, x.n - col, aligned, a.accumulate);
                     }
                     __builtin_amdgcn_wave_barrier();
                 }
@@ -459,10 +548,11 @@ hipError_t launch_values(const GroupedArgs &a, int direction, hipStream_t s)
     const dim3 grid(kCus), block(kThreads);
     switch (direction) {
     case kGroupedForward:
-        hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward>), grid, block, 0, s, a);
+        if (a.term.index) hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, false>), grid, block, 0, s, a);
         break;
-    case kGroupedInputGradient: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedInputGradient>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedWeightGradient>), grid, block, 0, s, a); break;
+    case kGroupedInputGradient: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedInputGradient, false>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedWeightGradient, false>), grid, block, 0, s, a); break;
     }
     return hipGetLastError();
 }

@@ -94,6 +94,15 @@ __device__ __forceinline__ void group_rows(const GroupedArgs &a, int g, int &lo,
         hi = min(max(a.offsets[g + 1], lo), a.rows);
     }
 }
+// The same of a group that is one for the whole wave, by scalar loads: they do
+// not wait behind the wave's own loads and stores.
+__device__ __forceinline__ void wave_group_rows(const GroupedArgs &a, int g, int &lo, int &hi)
+{
+    const __attribute__((address_space(4))) int32_t *p =
+        (const __attribute__((address_space(4))) int32_t *)(a.offsets) + __builtin_amdgcn_readfirstlane(g);
+    lo = min(max(p[0], 0), a.rows);
+    hi = min(max(p[1], lo), a.rows);
+}
 
 __device__ __forceinline__ int wave_sum_before(int v, int &total)
 {
@@ -119,7 +128,8 @@ __device__ __forceinline__ int swizzle(int r)
 
 // One operand's way into LDS: ROWS of the tile's axis, SB of the
 // reduction per step, THREADS threads.
-template <class T, bool KC, int ROWS, int THREADS, int SB>
+// GATHER (KC only): the tile's rows lie at the places an index gives.
+template <class T, bool KC, int ROWS, int THREADS, int SB, bool GATHER = false>
 struct Operand {
     static constexpr int kUnit = 16 / T::kBytes;               // values per 16-byte unit
     static constexpr int kStep = SB / T::kBytes;       // reduction values per step
@@ -133,6 +143,8 @@ struct Operand {
     int length;         // reduction values that exist
     int r0, c;          // the thread's first LDS row, and its unit there (the same for all its rows)
     uint32_t off;       // byte offset of that unit from the step's base
+    int rows;           // GATHER: rows of the whole matrix
+    uint32_t offs[GATHER ? kLoads : 1];  // GATHER: the offsets of all the thread's units
 
     __device__ __forceinline__ Operand(const void *p, long long stride, int valid_, int length_)
         : base(reinterpret_cast<const char *>(p)), row(stride * T::kBytes), valid(valid_), length(length_)
@@ -142,6 +154,18 @@ struct Operand {
         c = (threadIdx.x % kRowUnits) ^ swizzle<T, KC, ROWS, SB>(r0);
         off = (uint32_t)r0 * (uint32_t)row + c * 16u;
     }
+    // rows index[0 .. valid_) of a matrix of rows_ rows (less than 2^31 bytes)
+    __device__ __forceinline__ Operand(const void *p, long long stride, int rows_, const int32_t *index, int valid_, int length_)
+        : Operand(p, stride, valid_, length_)
+    {
+        static_assert(GATHER && KC, "");
+        rows = rows_;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = r0 + i * kLoadRows;
+            offs[i] = r < valid ? (uint32_t)index[r] * (uint32_t)row + c * 16u : kOutside;
+        }
+    }
 
     // LDS-DMA of one step: the buffer its offsets are checked against (every
     // unit lies wholly inside its row or wholly outside) and the thread's
@@ -149,7 +173,8 @@ struct Operand {
     struct Request {
         const char *p;
         int bytes;
-        uint32_t off;
+        uint32_t row;
+        uint32_t off[GATHER ? kLoads : 1];
     };
     __device__ __forceinline__ Request request(int step) const
     {
@@ -158,16 +183,24 @@ struct Operand {
         const int bytes = left == 0 || valid <= 0 ? 0
                           : KC ? (int)((valid - 1) * row) + left * T::kBytes
                                : (int)((min(left, kStep) - 1) * row) + valid * T::kBytes;
-        // (kOutside plus the rows' offsets stays outside: they are below 2^30)
-        return {p, bytes, c * kUnit < (KC ? left : valid) ? off : kOutside};
+        const bool in = c * kUnit < (KC ? left : valid);
+        if constexpr (GATHER) {
+            Request q{p, left ? (int)((rows - 1) * row) + left * T::kBytes : 0, 0, {}};
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) q.off[i] = in ? offs[i] : kOutside;
+            return q;
+        } else {
+            // (kOutside plus the rows' offsets stays outside: they are below 2^30)
+            return {p, bytes, (uint32_t)row, {in ? off : kOutside}};
+        }
     }
-    __device__ __forceinline__ void issue(char *lds, const Request &q) const
+    static __device__ __forceinline__ void issue(char *lds, const Request &q)
     {
         const __amdgpu_buffer_rsrc_t src =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(q.p), 0, q.bytes, kRawBufferWord3);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const uint32_t o = q.off + (uint32_t)(i * kLoadRows) * (uint32_t)row;
+            const uint32_t o = GATHER ? q.off[GATHER ? i : 0] : q.off[0] + (uint32_t)(i * kLoadRows) * q.row;
             char *to = lds + (i * THREADS + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63)) * 16;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)to, 16, o, 0, 0, 0);
         }
@@ -328,10 +361,37 @@ __device__ __forceinline__ void load_ranks(const typename T::Store *row, int k, 
 // below the output's own rounding, at an eighth of the time of fp32 MFMAs.  fp16
 // has too few exponents for u: a row's ranks are scaled by a power of two, and
 // so is what they are added to (exactly).  What is not finite stays so in both parts.
+struct RowScale {
+    float down, up;  // the row's power of two and its inverse
+};
+// For values of at most `top`: scaled they are below 2.  The exponent is held to
+// -40 .. 100: what is added to u's product takes the same factors and may
+// neither overflow nor lose bits (an fp16 result's are between 2^-25 and 2^16),
+// and of smaller u the fp16 parts keep 2^-64, which no result shows.
+template <class T>
+__device__ __forceinline__ RowScale row_scale(float top)
+{
+    if (!std::is_same<T, F16>::value || !(top > 0.f)) return {1.f, 1.f};
+    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -40), 100);
+    return {__uint_as_float((uint32_t)(127 - ex) << 23), __uint_as_float((uint32_t)(127 + ex) << 23)};
+}
+template <class T>
+__device__ __forceinline__ void two_parts(float x, float scale, float &hi, float &lo)
+{
+    if constexpr (std::is_same<T, F16>::value) {
+        const float y = x * scale;
+        hi = T::load(T::round(y));
+        lo = fabsf(x) < __builtin_inff() ? y - hi : x;
+    } else {
+        hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+        lo = fabsf(x) < __builtin_inff() ? x - hi : x;
+    }
+}
+
 template <class T>
 struct RankRow {
     u32x4 hi, lo;
-    float scale, unscale;  // fp16: the row's power of two and its inverse
+    float scale, unscale;
     __device__ __forceinline__ void load(const float *u, bool have)
     {
         f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -339,38 +399,23 @@ struct RankRow {
             v[0] = *reinterpret_cast<const f32x4 *>(u);
             v[1] = *reinterpret_cast<const f32x4 *>(u + 4);
         }
-        scale = unscale = 1.f;
+        float top = 0.f;
         if constexpr (std::is_same<T, F16>::value) {
-            float top = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float x = fabsf(v[e >> 2][e & 3]);
                 top = fmaxf(top, x < __builtin_inff() ? x : 0.f);
             }
             top = fmaxf(top, __shfl_xor(top, 32));  // the row's other half
-            if (top > 0.f) {
-                // 2^(exponent of top) held to where its inverse and both
-                // parts are normal numbers; scaled values are below 2
-                const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 252) - 127;
-                scale = __uint_as_float((uint32_t)(127 - ex) << 23);
-                unscale = __uint_as_float((uint32_t)(127 + ex) << 23);
-            }
         }
+        const RowScale s = row_scale<T>(top);
+        scale = s.down;
+        unscale = s.up;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             float h[2], l[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float x = v[p >> 1][2 * (p & 1) + e];
-                if constexpr (std::is_same<T, F16>::value) {
-                    const float y = x * scale;
-                    h[e] = T::load(T::round(y));
-                    l[e] = fabsf(x) < __builtin_inff() ? y - h[e] : x;
-                } else {
-                    h[e] = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-                    l[e] = fabsf(x) < __builtin_inff() ? x - h[e] : x;
-                }
-            }
+            for (int e = 0; e < 2; ++e) two_parts<T>(v[p >> 1][2 * (p & 1) + e], scale, h[e], l[e]);
             hi[p] = T::pack(h[0], h[1]);
             lo[p] = T::pack(l[0], l[1]);
         }

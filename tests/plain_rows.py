@@ -60,10 +60,12 @@ def adapted(x, w, b, adapter, down, up, scales, base=None):
     size = np.abs(x) @ np.abs(w).T if w is not None else np.abs(base)
     if b is not None:
         y, size = y + b, size + np.abs(b)
-    for t, a in enumerate(adapter):
+    adapter = np.asarray(adapter)
+    for a in np.unique(adapter):
         if 0 <= a < len(scales):
-            y[t] += scales[a] * (up[a] @ (down[a] @ x[t]))
-            size[t] += abs(scales[a]) * (np.abs(up[a]) @ (np.abs(down[a]) @ np.abs(x[t])))
+            t = adapter == a
+            y[t] += scales[a] * (x[t] @ down[a].T @ up[a].T)
+            size[t] += abs(scales[a]) * (np.abs(x[t]) @ np.abs(down[a]).T @ np.abs(up[a]).T)
     return y, size
 
 

@@ -386,8 +386,53 @@ def check_adapted_whole(ctx, kind, T, K, N, rank, n, pattern, odd=False):
         assert np.array_equal(got, rounded(ref, kind)), (ww is None, bb is None)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("T, K, N, rank, n", [(1024, 72, 264, 16, 5), (8200, 72, 264, 16, 5), (16390, 72, 40, 8, 1),
+                                              (2100, 64, 520, 64, 1023), (5470, 136, 40, 24, 17),
+                                              (3300, 200, 300, 40, 100)])
+@pytest.mark.parametrize("pattern", ["one", "each its own", "runs", "none", "mixed"])
+def test_adapted_many_rows(ctx, kind, T, K, N, rank, n, pattern):
+    """Many rows, below and above where they are sorted by adapter, in every
+    order of them."""
+    check_adapted_whole(ctx, kind, T, K, N, rank, n, pattern)
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("T, rank", [(1, 16), (48, 16), (200, 32)])
+@pytest.mark.parametrize("K, N, rank, n, odd", [(64, 48, 72, 3, False), (64, 48, 36, 3, False), (68, 48, 40, 3, False),
+                                                (64, 48, 48, 1024, False), (64, 48, 64, 3, True)])
+def test_adapted_many_rows_that_cannot_be_sorted(ctx, kind, K, N, rank, n, odd):
+    """Ranks, widths, counts of adapters and strides the sorted form does not take."""
+    check_adapted_whole(ctx, kind, (1 << 17) // rank + 3, K, N, rank, n, "mixed", odd=odd)
+
+
+def test_adapted_scales_of_a_row_do_not_touch_another(ctx):
+    """fp16 parts of u are scaled by row: rows with u near 2^40 and 2^-20 side by
+    side, of one adapter, each exact to its own size."""
+    for T, rank in ((70, 8), (300, 8), (2200, 64)):
+        K, N = 64, 72
+        rng = np.random.default_rng(T)
+        x = np.zeros((T, K))
+        x[:, 0] = np.where(np.arange(T) % 2 == 0, 2.0 ** 10, 2.0 ** -10)
+        w, b = np.zeros((N, K)), whole(rng, N)
+        w[:, 0] = 2.0 ** -10
+        down, up = np.zeros((1, rank, K)), np.zeros((1, N, rank))
+        down[0, :, 0] = 2.0 ** 12
+        up[0, :, 0] = 2.0 ** -20 * whole(rng, N)
+        got = run_adapted(ctx, "f16", x, w, b, np.zeros(T, int), down, up, [1.0])
+        ref, _ = adapted(x, w, b, np.zeros(T, int), down, up, [1.0])
+        assert np.array_equal(got, rounded(ref, "f16"))
+        got = run_adapted(ctx, "f16", x, w, b, np.zeros(T, int), down, up, [2.0 ** 18])
+        ref, _ = adapted(x, w, b, np.zeros(T, int), down, up, [2.0 ** 18])
+        # Up's values are fp16 subnormals here.  The matrix cores align a sum to
+        # its products' exponents before normalising, a subnormal factor's being
+        # that of 2^-14: a sum with |u| = 2^20 keeps what is above 2^20 2^-14 2^-24
+        # per product (two parts of one rank), whatever the product's value
+        bound = HALF_STEP["f16"] * np.abs(ref) + 2 * 2.0 ** (20 - 14 - 24)
+        assert np.all(np.abs(got - ref)[1::2] <= bound[1::2])
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T, rank", [(1, 16), (48, 16), (300, 32), (4200, 32)])
 def test_adapted_normal_values(ctx, kind, T, rank):
     K, N, n = 520, 392, 7
     rng = np.random.default_rng(11)
@@ -398,18 +443,20 @@ def test_adapted_normal_values(ctx, kind, T, rank):
     adapter = adapters_of(rng, "mixed", T, n)
     got = run_adapted(ctx, kind, x, w, b, adapter, down, up, scales)
     ref, size = adapted(x, w, b, adapter, down, up, scales)
-    # K terms of the shared sum; K, the scale and rank terms of the adapter's; bias and the two parts' sum
+    # K terms of the shared sum; K, the scale and rank terms of the adapter's; bias and the two parts' sum;
+    # bf16: u in two parts loses 2^-16 of it (the rest of 8 bits cut off, rounded to 8), fp16 2^-22
     bound = HALF_STEP[kind] * np.abs(ref) + HALF_LAST_STEP[kind] + (K + rank + 4) * 2.0 ** -24 * size
+    bound += {"bf16": 2.0 ** -16, "f16": 2.0 ** -22, "f32": 0.0}[kind] * size
     assert np.all(np.abs(got - ref) <= bound * (1 + 2.0 ** -7))
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("T", [20, 140])
-def test_adapted_nan_stays_with_its_request(ctx, kind, T):
+@pytest.mark.parametrize("T, rank", [(20, 8), (140, 8), (300, 8), (2100, 64)])
+def test_adapted_nan_stays_with_its_request(ctx, kind, T, rank):
     """A request whose row or adapter holds NaN or infinity leaves the other
     requests' rows as they are without it."""
     rng = np.random.default_rng(12)
-    K, N, n, rank = 136, 72, 6, 8
+    K, N, n = 136, 72, 6
     sparse = lambda *s: whole(rng, *s, top=1) * (rng.random(s) < 0.25)
     x, w = whole(rng, T, K, top=1), whole(rng, N, K)
     down, up, scales = sparse(n, rank, K), sparse(n, N, rank), np.ones(n)

@@ -140,9 +140,11 @@ def adapted_desc(**changes):
 
 
 def test_adapted_workspace_size():
-    assert gt.adapted_workspace_bytes(adapted_desc()) == 50 * 16 * 4
-    assert gt.adapted_workspace_bytes(adapted_desc(rank=16)) == 50 * 16 * 4
-    assert gt.adapted_workspace_bytes(adapted_desc(rank=17)) == 50 * 24 * 4
+    # u, the rows' scales and order (16-byte multiples), the adapters' places
+    rest = 2 * 208 + 32
+    assert gt.adapted_workspace_bytes(adapted_desc()) == 50 * 16 * 4 + rest
+    assert gt.adapted_workspace_bytes(adapted_desc(rank=16)) == 50 * 16 * 4 + rest
+    assert gt.adapted_workspace_bytes(adapted_desc(rank=17)) == 50 * 24 * 4 + rest
     assert gt.adapted_workspace_bytes(adapted_desc(rows=0)) > 0
     with pytest.raises(gt.InvalidArgument, match="rank must be"):
         gt.adapted_workspace_bytes(adapted_desc(rank=257))
