@@ -608,14 +608,18 @@ __device__ __forceinline__ void add_bias(f32x16 (&acc)[MI][NJ], const void *bias
 {
     const int h = (threadIdx.x >> 5) & 1;
     const typename T::Store *b = reinterpret_cast<const typename T::Store *>(bias);
+    const bool aligned = (reinterpret_cast<uintptr_t>(bias) & (4 * T::kBytes - 1)) == 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int col = n0 + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3);
-            const float v = col < n ? T::load(b[col]) : 0.f;
+        for (int q = 0; q < 4; ++q) {
+            const int col = n0 + 32 * j + 8 * q + 4 * h;
+            float v[4];
+            load4<T>(b + col, v, n - col, aligned);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) acc[i][j][r] += v;
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
         }
 }
 
