@@ -110,13 +110,13 @@ struct RowTiles {
     {
         const int tile = t / columns;
         column = t - tile * columns;
-        while (tile >= before + count) {
+        while (tile >= before + count && e0 + 64 < a.groups) {
             before += count;
             load(e0 + 64);
             place_tiles();
         }
         const uint64_t hit = __ballot(tile >= first && tile < first + n);
-        const int src = __builtin_ctzll(hit);
+        const int src = hit ? __builtin_ctzll(hit) : 0;
         g = e0 + src;
         const int rows = __builtin_amdgcn_readlane(per, src);
         p0 = __builtin_amdgcn_readlane(lo, src) + (tile - __builtin_amdgcn_readlane(first, src)) * rows;
@@ -124,7 +124,8 @@ struct RowTiles {
     }
     __device__ __forceinline__ void range(int &begin, int &end) const
     {
-        const long long all = (long long)total * columns;
+        // (more than the 2^30 tiles a launch is held to: only of offsets that descend)
+        const long long all = min((long long)total * columns, 1ll << 30);
         begin = (int)(all * xcd() / kXcds);
         end = (int)(all * (xcd() + 1) / kXcds);
     }
@@ -201,28 +202,37 @@ __device__ __forceinline__ const char *scalar(const char *p)
     return reinterpret_cast<const char *>((uint64_t)hi << 32 | lo);
 }
 
-// Eight 16-bit or four fp32 values of a row as 16 bytes.
-template <class O>
+// 16 bytes of a row's results as they were staged: eight values of a 16-bit type S
+// = O, or four fp32 ones, to which `add` adds what out holds before the one
+// rounding to O.  `left` of them exist.
+template <class S, class O>
 __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int left, bool aligned, bool add)
 {
-    constexpr int unit = 16 / O::kBytes;
-    typedef typename O::Store Store;
-    Store w[unit];
-    __builtin_memcpy(w, &v, 16);
+    constexpr int unit = 16 / S::kBytes;
     if (left >= unit && aligned) {
-        if (add) {
-            const u32x4 old = *reinterpret_cast<const u32x4 *>(p);
-            Store o[unit];
-            __builtin_memcpy(o, &old, 16);
-#pragma unroll
-            for (int e = 0; e < unit; ++e) w[e] = O::round(O::load(o[e]) + O::load(w[e]));
-            __builtin_memcpy(&v, w, 16);
+        if constexpr (S::kBytes == 2) {
+            *reinterpret_cast<u32x4 *>(p) = v;
+        } else {
+            f32x4 w = __builtin_bit_cast(f32x4, v);
+            if constexpr (O::kBytes == 4) {
+                if (add) w += *reinterpret_cast<const f32x4 *>(p);
+                *reinterpret_cast<f32x4 *>(p) = w;
+            } else {
+                if (add) {
+                    const uint2 o = *reinterpret_cast<const uint2 *>(p);
+                    w += f32x4{O::load((uint16_t)o.x), O::load((uint16_t)(o.x >> 16)), O::load((uint16_t)o.y),
+                               O::load((uint16_t)(o.y >> 16))};
+                }
+                *reinterpret_cast<uint2 *>(p) = make_uint2(O::pack(w[0], w[1]), O::pack(w[2], w[3]));
+            }
         }
-        *reinterpret_cast<u32x4 *>(p) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < unit; ++e)
-            if (e < left) p[e] = add ? O::round(O::load(p[e]) + O::load(w[e])) : w[e];
+            if (e < left) {
+                if constexpr (S::kBytes == 2) p[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+                else p[e] = O::round((add ? O::load(p[e]) : 0.f) + __uint_as_float(v[e]));
+            }
     }
 }
 
@@ -488,13 +498,14 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         // 16 bytes per lane, eight rows of 128 bytes at a time.
         char *stage = so + wave * 4096;
         if (DIR == kGroupedWeightGradient && a.accumulate && x.length == 0) return;
-        auto leave = [&](auto type) {
+        auto leave = [&](auto staged, auto type) {
+            typedef decltype(staged) S;  // the values' type in LDS
             typedef decltype(type) O;
-            constexpr int unit = 16 / O::kBytes, each = O::kBytes == 2 ? 2 : 1;  // column blocks per pass
+            constexpr int unit = 16 / S::kBytes, each = S::kBytes == 2 ? 2 : 1;  // column blocks per pass
             typename O::Store *out = reinterpret_cast<typename O::Store *>(a.out) +
                                      (DIR == kGroupedWeightGradient ? x.g * a.group_stride : 0) +
                                      (ADAPTED ? 0 : x.m0 * a.ldo) + x.n0;
-            const bool aligned = a.ldo % unit == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+            const bool aligned = a.ldo % unit == 0 && (reinterpret_cast<uintptr_t>(out) & (unit * O::kBytes - 1)) == 0;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -504,9 +515,9 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const f32x16 &v = acc[i][j];
-                            if constexpr (O::kBytes == 2) {
+                            if constexpr (S::kBytes == 2) {
                                 *reinterpret_cast<uint2 *>(stage + r * 128 + ((4 * (j - j0) + q) ^ ((r >> 1) & 7)) * 16 + h * 8) =
-                                    make_uint2(O::pack(v[4 * q], v[4 * q + 1]), O::pack(v[4 * q + 2], v[4 * q + 3]));
+                                    make_uint2(S::pack(v[4 * q], v[4 * q + 1]), S::pack(v[4 * q + 2], v[4 * q + 3]));
                             } else {
                                 *reinterpret_cast<float4 *>(stage + r * 128 + ((2 * q + h) ^ ((r >> 1) & 7)) * 16) =
                                     make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -520,13 +531,15 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                         const int row = 64 * i + wm + rr, col = wn + 32 * j0 + unit * u;
                         int to = row;
                         if constexpr (ADAPTED) to = __shfl(at_rows[i >> 1], 32 * (i & 1) + rr);
-                        if (row < x.m && col < x.n) store_unit<O>(out + to * a.ldo + col, v, x.n - col, aligned, a.accumulate);
+                        if (row < x.m && col < x.n) store_unit<S, O>(out + to * a.ldo + col, v, x.n - col, aligned, a.accumulate);
                     }
                     __builtin_amdgcn_wave_barrier();
                 }
         };
-        if (DIR == kGroupedWeightGradient && a.out_f32) leave(F32());
-        else leave(T());
+        // (a weight gradient in fp32 up to its one rounding, for what it may be added to)
+        if (DIR == kGroupedWeightGradient && a.out_f32) leave(F32(), F32());
+        else if (DIR == kGroupedWeightGradient) leave(F32(), T());
+        else leave(T(), T());
     };
     for (;;) {
         switch ((x.m + 63) / 64) {

@@ -705,6 +705,145 @@ def test_operators_on_two_streams_at_once(ctx):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("G, K, N", [(3, 136, 72), (40, 520, 264)])
+def test_grouped_weight_gradients_accumulate_with_one_rounding(ctx, kind, G, K, N):
+    """A 16-bit gradient that is added to: the sum of both in fp32, rounded once.
+    Whole numbers up to 4 * 300 + 4000 < 2^24 are exact in fp32; in the type
+    neither the new sum nor the result is, so a second rounding would show."""
+    rng = np.random.default_rng(21)
+    off = offsets_of([300, 0, 41] + [7] * (G - 3))
+    R = int(off[-1])
+    x, dy = whole(rng, R, K), whole(rng, R, N)
+    before = rounded(rng.integers(-4000, 4001, size=(G, N, K)), kind)
+    say(f"accumulate {kind} {G} of {K} x {N}")
+    dw = torch.as_tensor(before).to(TYPES[kind]).cuda()
+    hx, hdy, o = Rows(kind, R, K, data=x), Rows(kind, R, N, data=dy), device_offsets(off)
+    gt.grouped_weight_gradient(ctx, gt.grouped_desc(VALUES[kind], G, R, K, N), o.data_ptr(), hdy.ptr, hx.ptr,
+                               dw.data_ptr(), VALUES[kind], True, stream())
+    want = rounded(before + grouped(off, x, np.zeros((G, N, K)), dy)[2], kind)
+    assert np.array_equal(dw.double().cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("bad", [[0, 4096] * 10 + [0], [4096] * 20 + [0], [-1, 1 << 30] * 10 + [-(1 << 31)],
+                                 [0] * 19 + [(1 << 31) - 1, 5]])
+def test_many_rows_offsets_that_descend_stay_inside_the_buffers(ctx, bad):
+    rng = np.random.default_rng(22)
+    G, R, K, N = 20, 4096, 72, 2048
+    x, w, dy = whole(rng, R, K), whole(rng, G, N, K), whole(rng, R, N)
+    say("offsets", bad)
+    y, dx, _ = run_grouped(ctx, "bf16", bad, x, w, dy)
+    assert y.outside_is_untouched() and dx.outside_is_untouched()
+
+
+def test_adapted_rows_beyond_two_gigabytes(ctx):
+    """Row offsets that pass 2^31 values: rows 2^20 values apart."""
+    R, K, N, st, n, rank = 2200, 64, 48, 1 << 20, 5, 64
+    rng = np.random.default_rng(23)
+    x, w = whole(rng, R, K, top=1), whole(rng, N, K)
+    down, up = whole(rng, n, rank, K, top=1), whole(rng, n, N, rank, top=1) * (rng.random((n, N, rank)) < 0.25)
+    adapter = adapters_of(rng, "mixed", R, n)
+    ref, _ = adapted(x, w, None, adapter, down, up, np.ones(n))
+    view = torch.empty(R * st, dtype=torch.bfloat16, device="cuda").view(R, st)
+    hx, hy = view[:, :K], view[:, 512:512 + N]
+    hx.copy_(torch.as_tensor(x))
+    dev = lambda v: torch.as_tensor(v).bfloat16().cuda()
+    hw, hd, hu, hs = dev(w), dev(down), dev(up), torch.ones(n, device="cuda")
+    ha = torch.as_tensor(adapter.astype(np.int32)).cuda()
+    d = gt.adapted_desc(gt.VALUES_BFLOAT16, R, K, N, n, rank, st, st)
+    ws = torch.empty(gt.adapted_workspace_bytes(d), dtype=torch.uint8, device="cuda")
+    gt.adapted_forward(ctx, d, hx.data_ptr(), hw.data_ptr(), None, ha.data_ptr(), hd.data_ptr(), hu.data_ptr(),
+                       hs.data_ptr(), hy.data_ptr(), ws.data_ptr(), stream())
+    # |u| <= 64, |y| < 2^24: exact in fp32, one rounding
+    assert np.array_equal(hy.double().cpu().numpy(), rounded(ref, "bf16"))
+
+
+def many_rows(kind, seed):
+    """The operators' forms for many rows: a training step and an adapted
+    projection with its rows sorted, each with its own buffers."""
+    rng = np.random.default_rng(seed)
+    off = device_offsets(offsets_of([900, 0, 1300, 77, 2500, 0, 400, 1100]))
+    make = lambda *s: torch.as_tensor(rng.normal(size=s)).to(TYPES[kind]).cuda()
+    R, G, K, N, n, rank = 6277, 8, 520, 2056, 9, 32
+    x, w, dy = make(R, K), make(G, N, K), make(R, N)
+    down, up, sc = make(n, rank, K), make(n, N, rank), torch.ones(n, device="cuda")
+    ad = torch.as_tensor(rng.integers(-1, n, size=R).astype(np.int32)).cuda()
+    d = gt.adapted_desc(VALUES[kind], R, K, N, n, rank)
+    ws = torch.empty(gt.adapted_workspace_bytes(d), dtype=torch.uint8, device="cuda")
+    z = torch.empty_like(dy)
+
+    def make_step(ctx):
+        step, outs = layer_step(ctx, kind, off, x, w, dy, 0.25, seed)
+
+        def both():
+            step()
+            gt.adapted_forward(ctx, d, x.data_ptr(), w[0].data_ptr(), None, ad.data_ptr(), down.data_ptr(),
+                               up.data_ptr(), sc.data_ptr(), z.data_ptr(), ws.data_ptr(), stream())
+
+        return both, (*outs, z)
+
+    return make_step, (x, w, dy, ad)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_many_rows_do_not_change_between_runs(ctx, kind):
+    """Mixed rows of an adapter are sorted in any order; their sums are the same."""
+    make_step, _ = many_rows(kind, 24)
+    step, outs = make_step(ctx)
+    step()
+    first = [o.clone() for o in outs]
+    for _ in range(5):
+        for o in outs:
+            o.fill_(float("nan"))
+        step()
+        for a, b in zip(first, outs):
+            assert torch.equal(a, b)
+
+
+def test_many_rows_in_a_replayed_graph(ctx):
+    make_step, data = many_rows("bf16", 25)
+    step, outs = make_step(ctx)
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for i in range(3):
+        for t in data[:3]:
+            t.copy_(torch.randn_like(t.float()))
+        data[3].copy_(torch.randint(-1, 9, data[3].shape, device="cuda", dtype=torch.int32))
+        step()
+        torch.cuda.synchronize()
+        want = [o.clone() for o in outs]
+        for o in outs:
+            o.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_many_rows_on_two_streams_at_once(ctx):
+    jobs = [many_rows("bf16", 26 + i)[0](ctx) for i in range(2)]
+    want = []
+    for step, outs in jobs:
+        step()
+        torch.cuda.synchronize()
+        want.append([o.clone() for o in outs])
+        for o in outs:
+            o.fill_(float("nan"))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        for s, (step, _) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                step()
+    torch.cuda.synchronize()
+    for w, (_, outs) in zip(want, jobs):
+        for a, b in zip(w, outs):
+            assert torch.equal(a, b)
+
+
 def test_results_do_not_change_between_runs(ctx):
     """Sums have one order: normal numbers give the same bits every time."""
     rng = np.random.default_rng(16)
