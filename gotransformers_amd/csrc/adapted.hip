@@ -48,6 +48,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void adapter_sort_kernel(const int
     };
     __syncthreads();
     // eight times 64 rows of a wave's stretch are loaded together
+    // (a wave's LDS operations stay in order; the fence keeps the compiler to it,
+    // for lane 0's writes are the other lanes' next reads)
     auto each_chunk = [&](auto &&take) {
         for (int t = begin; t < end; t += 512) {
             int b[8];
@@ -59,6 +61,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void adapter_sort_kernel(const int
                 if (n <= 0) break;
                 const int one = __builtin_amdgcn_readfirstlane(b[i]);
                 take(t + 64 * i, b[i], n, one, __ballot(b[i] != one && lane < n) == 0);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
         }
     };
@@ -443,6 +446,12 @@ hipError_t launch_adapter_down(const AdapterDownArgs &a, int values, hipStream_t
     case kValuesF16: return launch_down_values<F16>(a, s);
     default: return launch_down_values<F32>(a, s);
     }
+}
+
+bool adapted_fits(const GroupedArgs &a, int values)
+{
+    // launch_down's 16 rows per workgroup; a grid holds 2^32 - 1 threads
+    return ((long long)a.rows + 15) / 16 * (64 * kWaves) < 1ll << 32 && grouped_fits(a, kGroupedForward, values);
 }
 
 bool adapted_sorts(const GroupedArgs &a, int values)

@@ -3102,9 +3102,9 @@ GroupedArgs grouped_args(const gtmoe_grouped_desc *d, const int32_t *offsets)
     return a;
 }
 
-int32_t check_grid(gtmoe_context *ctx, const GroupedArgs &a, int direction, int values)
+int32_t check_grid(gtmoe_context *ctx, const GroupedArgs &a, bool fits)
 {
-    if (!grouped_fits(a, direction, values))
+    if (!fits)
         return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%d rows in %d groups of %d x %d are more tiles than one launch holds",
                     a.rows, a.groups, a.outputs, a.inputs);
     return GTMOE_OK;
@@ -3136,7 +3136,7 @@ int32_t gtmoe_grouped_forward(gtmoe_context *ctx, const gtmoe_grouped_desc *desc
         a.ldb = desc->weight_stride;
         a.out = outputs;
         a.ldo = desc->output_stride;
-        return check_grid(c, a, kGroupedForward, desc->values);
+        return check_grid(c, a, grouped_fits(a, kGroupedForward, desc->values));
     };
     if (!ctx) return check_only(check);
     ENTER(ctx);
@@ -3170,7 +3170,7 @@ int32_t gtmoe_grouped_input_gradient(gtmoe_context *ctx, const gtmoe_grouped_des
         a.ldb = desc->weight_stride;
         a.out = input_gradients;
         a.ldo = desc->input_stride;
-        return check_grid(c, a, kGroupedInputGradient, desc->values);
+        return check_grid(c, a, grouped_fits(a, kGroupedInputGradient, desc->values));
     };
     if (!ctx) return check_only(check);
     ENTER(ctx);
@@ -3210,7 +3210,7 @@ int32_t gtmoe_grouped_weight_gradient(gtmoe_context *ctx, const gtmoe_grouped_de
         a.ldo = desc->weight_stride;
         a.out_f32 = gradient_values == GTMOE_VALUES_FLOAT32;
         a.accumulate = accumulate != 0;
-        return check_grid(c, a, kGroupedWeightGradient, desc->values);
+        return check_grid(c, a, grouped_fits(a, kGroupedWeightGradient, desc->values));
     };
     if (!ctx) return check_only(check);
     ENTER(ctx);
@@ -3342,7 +3342,7 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
             a.term.u_lo = dargs.u_lo = base + layout.unscale / 2;
             a.term.unscale = dargs.unscale = reinterpret_cast<float *>(base + layout.unscale);
         }
-        return check_grid(c, a, kGroupedForward, desc->values);
+        return check_grid(c, a, adapted_fits(a, desc->values));
     };
     if (!ctx) return check_only(check);
     ENTER(ctx);

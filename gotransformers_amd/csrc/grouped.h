@@ -74,6 +74,8 @@ struct AdapterDownArgs {
 hipError_t launch_adapter_down(const AdapterDownArgs &a, int values, hipStream_t s);
 // The forward of one group with its adapters' term.
 hipError_t launch_adapted(const GroupedArgs &a, int values, hipStream_t s);
+// Whether both kernels' workgroups fit one launch each.
+bool adapted_fits(const GroupedArgs &a, int values);
 // Whether a forward with adapters takes its rows sorted by adapter (a.term.index
 // and parts of u instead of u): launch_adapter_sort first.
 bool adapted_sorts(const GroupedArgs &a, int values);

@@ -20,7 +20,8 @@ namespace gtmoe {
 
 namespace {
 
-constexpr long long kMaxBlocks = (1ll << 32) / 1024 - 1;  // a grid holds 2^32 - 1 threads
+constexpr int kThreads = 256;                               // of every grouped_kernel
+constexpr long long kMaxBlocks = (1ll << 32) / kThreads - 1;  // a grid holds 2^32 - 1 threads
 constexpr int SB = 128;                                   // bytes of reduction per step
 constexpr int kCus = 256;
 
@@ -111,6 +112,7 @@ template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, boo
 __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
 {
     constexpr int THREADS = 64 * WM * WN;
+    static_assert(THREADS == kThreads, "");
     constexpr int MI = BM / WM / 32, NJ = BN / WN / 32;
     typedef Operand<T, DIR != kGroupedWeightGradient, BM, THREADS, SB> A;
     typedef Operand<T, DIR == kGroupedForward, BN, THREADS, SB> B;

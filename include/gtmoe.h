@@ -439,7 +439,9 @@ int32_t gtmoe_backward(gtmoe_layer *layer, int32_t tokens, const double *output_
  * without synchronising, allocates nothing, and may be captured into a HIP
  * graph.  Values are float32, bfloat16 or float16 and lie in rows: a stride is
  * the distance between two rows in values, at least the width and at most
- * 1048576; pointers are multiples of a value's size.  Outputs must not
+ * 1048576, also of a buffer that is NULL; pointers are multiples of a value's
+ * size.  A call of more work than one launch holds (2^24 tiles of 32 x 64
+ * outputs, or with adapters 2^27 rows) is refused.  Outputs must not
  * overlap another buffer of the call (GTMOE_ERR_INVALID_ARGUMENT) unless the
  * entry point says so.  Sums are fp32; an output is rounded once.
  * ------------------------------------------------------------------------- */
