@@ -12,6 +12,12 @@
 // 65536 / (65536 - threshold), the inverse of the share that is kept exactly.
 // A dropped value is selected away, not multiplied by zero: infinities and
 // NaN in dropped places do not reach the output.
+//
+// What bounds it (MI355X): memory, with the ten rounds' quarter-rate products
+// close behind.  8192 x 2048 in bf16, with and without a base, 39 us for both calls:
+// 168 MB at 4.3 TB/s, where a large copy reaches 5.1.  A thread that steps
+// through rows and columns without the 64-bit division per item, on as many
+// workgroups as the chip holds, took 40 us.
 #include "grouped.h"
 
 namespace gtmoe {

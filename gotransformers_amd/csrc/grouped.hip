@@ -6,11 +6,21 @@
 // and, for one group of all rows, the shared projection beside many requests'
 // adapters, whose second half (B_a u) the epilogue adds.
 //
-// One workgroup computes a BM x BN tile of one group's product on the matrix
-// cores, fp32 accumulation: v_mfma_f32_32x32x16 for 16-bit values,
+// One workgroup of four waves computes a BM x BN tile of one group's product on
+// the matrix cores, fp32 accumulation: v_mfma_f32_32x32x16 for 16-bit values,
 // v_mfma_f32_32x32x2_f32 for fp32.  A step takes 128 bytes of reduction (64
 // 16-bit values, 32 fp32) of both operands into LDS; two stages, the next
-// step's loads in flight while this one multiplies.
+// step's loads in flight while this one multiplies, or four where few
+// workgroups share a CU and the loads' latency would show.  Tiles by the rules
+// above launch_direction; many 16-bit rows go to grouped_large.hip.
+//
+// What bounds it (MI355X): few rows, the matrices' bytes: 64 rows over 16
+// matrices of 2048 x 1024 in bf16 13.1 us, 67 MB at 5.1 TB/s, what a large copy
+// reaches.  fp32, the matrix cores: 2331 rows over 14 matrices of 1201 x 1000
+// 72 us per direction, 78 TFLOP/s of the 154 a large product reaches; a group's 166
+// rows fill 2.6 of its 3 row tiles and 1201 columns 18.8 of 19, and the
+// scattered LDS reads of fp32 operands with the tile's axis contiguous do the
+// rest.
 //
 // Row groups are found on the device: the grid holds the most tiles the rows
 // can need, every wave scans the offsets for its tile, surplus workgroups end.

@@ -9,10 +9,22 @@
 // the tile's results leave through 4 KiB of LDS per wave as whole 128-byte
 // row pieces.
 //
-// What bounds it: with 128 x 64 per wave the LDS moves 64 KiB of operands
-// and writes 64 KiB / 4 per group of 32 bytes of reduction and 512 cycles of MFMA,
-// which is its whole 128 bytes per cycle; smaller tiles need more of it per
-// MFMA (kRowCost).
+// What bounds it (MI355X, bf16): a step's 64 KiB per CU on their way from L2
+// into LDS take about 1.5 us however few of the tile's rows exist, which is
+// about what the 256 x 256 tile's MFMAs take (kRowCost), and a launch about 15 us
+// before its first results.  Long tiles reach 1050 to 1190 TFLOP/s (8 groups
+// of 2048 x 2048, 16384 rows: weight gradient 131 us, forward 152, input gradient
+// 158; a large library product 1010 to 1296), skewed small groups 850 (fp16,
+// 131072 rows over 128 matrices of 768 x 2048: 434 us forward).  The weight
+// gradient of short groups is bound by its results' bytes: 64 fp32 matrices of
+// 2048 x 1024 from 16384 rows 175 us, 3.6 TB/s, the four steps of a tile and the
+// stores of its 256 KiB mostly one after the other (loads and stores return in one
+// order).
+//
+// ADAPTED costs more than the product beside it (8192 rows of 1024 -> 2048 with
+// 12 adapters of rank 64, fp16, 95 us; the plain product 41): thirteen
+// groups' rows make some 400 tiles where 256 would do, two rounds of them, rows
+// are gathered, and two steps are added to sixteen.
 //
 // Tiles: rows of a group by bm, every XCD an eighth of them in order (the
 // hardware hands block b to XCD b % 8), its blocks taking them in turn, so
@@ -216,7 +228,9 @@ __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int le
             f32x4 w = __builtin_bit_cast(f32x4, v);
             if constexpr (O::kBytes == 4) {
                 if (add) w += *reinterpret_cast<const f32x4 *>(p);
-                *reinterpret_cast<f32x4 *>(p) = w;
+                // not kept in L2, which the operands want (64 matrices of 2048 x 1024,
+                // 16384 rows: 176 us against 182)
+                __builtin_nontemporal_store(w, reinterpret_cast<f32x4 *>(p));
             } else {
                 if (add) {
                     const uint2 o = *reinterpret_cast<const uint2 *>(p);

@@ -422,8 +422,8 @@ struct RankRow {
     }
 };
 
-// d += u B^T over ranks c .. c + 15 for one 32-row block of u and NJ 32-column
-// blocks of B (`up`: the lane's row of each, or null past the matrix).
+// Eight ranks of B from rank k on, 16-bit values, for NJ 32-column blocks (`up`:
+// the lane's row of each, or null past the matrix); zero at and past `rank`.
 template <class T, int NJ>
 __device__ __forceinline__ void load_columns(const typename T::Store *const (&up)[NJ], int k, int rank, u32x4 (&b)[NJ])
 {
