@@ -18,8 +18,7 @@
 // 131072 rows over 128 matrices of 768 x 2048: 434 us forward).  The weight
 // gradient of short groups is bound by its results' bytes: 64 fp32 matrices of
 // 2048 x 1024 from 16384 rows 175 us, 3.6 TB/s, the four steps of a tile and the
-// stores of its 256 KiB mostly one after the other (loads and stores return in one
-// order).
+// stores of its 256 KiB mostly one after the other, in all CUs at about the same time.
 //
 // ADAPTED costs more than the product beside it (8192 rows of 1024 -> 2048 with
 // 12 adapters of rank 64, fp16, 95 us; the plain product 41): thirteen
