@@ -9,8 +9,8 @@
 // 4.6 and 5.0, which is a launch and two dependent trips to memory each (W's
 // 8 MiB alone: 1.6); 64 rows of 48 adapters 4.8 and 8.8, the gathered Up
 // rows (2 MiB per 32 of them) in the epilogue; 8192 rows, 12 adapters of rank 64, fp16, sort
-// 6.2, down 17.5 (17 MB of rows and, per 16 of them, 128 KiB of Down from L2),
-// tiles 95 (grouped_large.hip).
+// 6.1, down 17.5 (17 MB of rows and, per 16 of them, 128 KiB of Down from L2),
+// tiles 76 (grouped_large.hip).
 #include "grouped_tile.h"
 
 namespace gtmoe {

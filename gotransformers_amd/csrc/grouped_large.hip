@@ -13,15 +13,16 @@
 // into LDS take about 1.5 us however few of the tile's rows exist, which is
 // about what the 256 x 256 tile's MFMAs take (kRowCost), and a launch about 15 us
 // before its first results.  Long tiles reach 1050 to 1190 TFLOP/s (8 groups
-// of 2048 x 2048, 16384 rows: weight gradient 131 us, forward 152, input gradient
-// 158; a large library product 1010 to 1296), skewed small groups 850 (fp16,
-// 131072 rows over 128 matrices of 768 x 2048: 434 us forward).  The weight
+// of 2048 x 2048, 16384 rows: weight gradient 131 us, forward 148, input gradient
+// 156; a large library product 1010 to 1296), skewed small groups 800 to 940 (fp16,
+// 131072 rows over 128 matrices of 768 x 2048: 440 us forward, 488 input gradient,
+// 510 weight gradient).  The weight
 // gradient of short groups is bound by its results' bytes: 64 fp32 matrices of
 // 2048 x 1024 from 16384 rows 175 us, 3.6 TB/s, the four steps of a tile and the
 // stores of its 256 KiB mostly one after the other, in all CUs at about the same time.
 //
 // ADAPTED costs more than the product beside it (8192 rows of 1024 -> 2048 with
-// 12 adapters of rank 64, fp16, 95 us; the plain product 41): thirteen
+// 12 adapters of rank 64, fp16, 76 us; the plain product 38): thirteen
 // groups' rows make some 400 tiles where 256 would do, two rounds of them, rows
 // are gathered, and two steps are added to sixteen.
 //
@@ -509,7 +510,22 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         // block (i, j), column wn + 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.  Through
         // LDS (rows of 128 bytes, 16-byte unit u of row r in slot u ^ (r / 2) % 8) to
         // 16 bytes per lane, eight rows of 128 bytes at a time.
+        // What the epilogue uses of the lane is made again here, hidden from the
+        // compiler: made ahead it was spilled over the steps, and every reload waited
+        // for the stores before it (24576 rows over 64 matrices of 512 x 1024 44.8
+        // -> 40.5 us, with 12 adapters 114 -> 94).
         char *stage = so + wave * 4096;
+        int el = lane;
+        asm volatile("" : "+v"(el));
+        const int er = el & 31, slot = er * 128 + ((er >> 1) & 7) * 16;
+        int places_of[2] = {0, 0};
+        if constexpr (ADAPTED) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                places_of[q] = at_rows[q];
+                asm volatile("" : "+v"(places_of[q]));
+            }
+        }
         if (DIR == kGroupedWeightGradient && a.accumulate && x.length == 0) return;
         auto leave = [&](auto staged, auto type) {
             typedef decltype(staged) S;  // the values' type in LDS
@@ -529,21 +545,21 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                         for (int q = 0; q < 4; ++q) {
                             const f32x16 &v = acc[i][j];
                             if constexpr (S::kBytes == 2) {
-                                *reinterpret_cast<uint2 *>(stage + r * 128 + ((4 * (j - j0) + q) ^ ((r >> 1) & 7)) * 16 + h * 8) =
+                                *reinterpret_cast<uint2 *>(stage + ((slot ^ (4 * (j - j0) + q) * 16) + (el >> 5) * 8)) =
                                     make_uint2(S::pack(v[4 * q], v[4 * q + 1]), S::pack(v[4 * q + 2], v[4 * q + 3]));
                             } else {
-                                *reinterpret_cast<float4 *>(stage + r * 128 + ((2 * q + h) ^ ((r >> 1) & 7)) * 16) =
+                                *reinterpret_cast<float4 *>(stage + (slot ^ (2 * q + (el >> 5)) * 16)) =
                                     make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
                             }
                         }
                     __builtin_amdgcn_wave_barrier();
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int rr = 8 * p + (lane >> 3), u = lane & 7;
+                        const int rr = 8 * p + (el >> 3), u = el & 7;
                         const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + rr * 128 + (u ^ ((rr >> 1) & 7)) * 16);
                         const int row = 64 * i + wm + rr, col = wn + 32 * j0 + unit * u;
                         int to = row;
-                        if constexpr (ADAPTED) to = __shfl(at_rows[i >> 1], 32 * (i & 1) + rr);
+                        if constexpr (ADAPTED) to = __builtin_amdgcn_ds_bpermute(4 * (32 * (i & 1) + rr), places_of[i >> 1]);
                         if (row < x.m && col < x.n) store_unit<S, O>(out + to * a.ldo + col, v, x.n - col, aligned, a.accumulate);
                     }
                     __builtin_amdgcn_wave_barrier();
