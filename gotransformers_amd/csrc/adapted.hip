@@ -26,11 +26,13 @@ constexpr int kFewRows = 256;
 // kMaxSortedRank ranks, the rows are sorted by adapter (1024 -> 2048, 64 adapters,
 // bf16, us; runs of 1, 7 and 512 rows of one request):
 //                       sorted            in order
-//   8192 rows, rank 64  122, 122, 85      1270, 370, 102
-//   8192 rows, rank 16  113, 111, 79      225, 143, 82
-//   4096 rows, rank 64  92, 93, 60        585, 190, 57
-//   2048 rows, rank 64  84, 87, 53        257, 112, 36
-//   4096 rows, rank 16  86, 86, 57        103, 70, 44
+//   8192 rows, rank 64  104, 101, 69      1270, 370, 102
+//   8192 rows, rank 16  87, 86, 62        225, 143, 82
+//   4096 rows, rank 64  76, 76, 49        585, 190, 57
+//   2048 rows, rank 64  71, 74, 45        257, 112, 36
+//   4096 rows, rank 16  73, 72, 47        110, 71, 43
+//   2048 rows, rank 32  67, 69, 43        100, 59, 29
+//   1024 rows, rank 64  74, 74, 43        184, 85, 27
 constexpr long long kSortedValues = 1 << 17;
 constexpr int kSortWaves = 16, kSortBins = 1024;
 
