@@ -11,8 +11,7 @@
 //
 // What bounds it (MI355X, bf16): a step's 64 KiB per CU on their way from L2
 // into LDS take about 1.5 us however few of the tile's rows exist, which is
-// about what the 256 x 256 tile's MFMAs take (kRowCost), and a launch some 10 us
-// before its first results.  Long tiles reach 1050 to 1190 TFLOP/s (8 groups
+// about what the 256 x 256 tile's MFMAs take (kRowCost).  Long tiles reach 1050 to 1190 TFLOP/s (8 groups
 // of 2048 x 2048, 16384 rows: weight gradient 131 us, forward 148, input gradient
 // 156; a large library product 1010 to 1296), skewed small groups 800 to 940 (fp16,
 // 131072 rows over 128 matrices of 768 x 2048: 440 us forward, 488 input gradient,
