@@ -11,14 +11,14 @@
 //
 // What bounds it (MI355X, bf16): a step's 64 KiB per CU on their way from L2
 // into LDS take about 1.5 us however few of the tile's rows exist, which is
-// about what the 256 x 256 tile's MFMAs take (kRowCost).  Long tiles reach 1050 to 1190 TFLOP/s (8 groups
-// of 2048 x 2048, 16384 rows: weight gradient 131 us, forward 148, input gradient
-// 156; a large library product 1010 to 1296), skewed small groups 800 to 940 (fp16,
-// 131072 rows over 128 matrices of 768 x 2048: 440 us forward, 488 input gradient,
-// 510 weight gradient).  The weight
-// gradient of short groups is bound by its results' bytes: 64 fp32 matrices of
-// 2048 x 1024 from 16384 rows 175 us, 3.6 TB/s, the four steps of a tile and the
-// stores of its 256 KiB mostly one after the other, in all CUs at about the same time.
+// about what the 256 x 256 tile's MFMAs take (kRowCost).  Long tiles reach 870 to
+// 1190 TFLOP/s (8 groups of 2048 x 2048, 16384 rows: weight gradient 131 us,
+// forward 148, input gradient 156; a large library product 1010 to 1296), skewed
+// small groups 800 to 940 (fp16, 131072 rows over 128 matrices of 768 x 2048:
+// forward 440 us, input gradient 488, weight gradient 510).  The weight gradient
+// of short groups is bound by its results' bytes: 64 fp32 matrices of 2048 x 1024
+// from 16384 rows 175 us, 3.6 TB/s, the four steps of a tile and the stores of
+// its 256 KiB mostly one after the other, in all CUs at about the same time.
 //
 // ADAPTED costs more than the product beside it (8192 rows of 1024 -> 2048 with
 // 12 adapters of rank 64, fp16, 76 us; the plain product 38): thirteen

@@ -736,6 +736,48 @@ def test_many_rows_offsets_that_descend_stay_inside_the_buffers(ctx, bad):
     assert y.outside_is_untouched() and dx.outside_is_untouched()
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("stride, shift", [(2059, 1), (2064, 4), (2056, 0)])
+def test_many_rows_to_outputs_of_any_alignment(ctx, kind, stride, shift):
+    """Aligned operands, outputs whose rows are not: the large tiles of every
+    direction and of sorted adapters, with a last column tile of eight."""
+    rng = np.random.default_rng(27)
+    G, K, N = 8, 520, 2056
+    off = offsets_of([900, 0, 1300, 77, 500, 0, 400, 511])
+    R = int(off[-1])
+    x, w, dy = whole(rng, R, K, top=1), whole(rng, G, N, K, top=1), whole(rng, R, N, top=1)
+    say(f"any alignment {kind} stride={stride} shift={shift}")
+    ry, rdx, rdw = grouped(off, x, w, dy)
+    hx, hdy, o = Rows(kind, R, K, data=x), Rows(kind, R, N, data=dy), device_offsets(off)
+    hw = torch.as_tensor(w).to(TYPES[kind]).cuda()
+    narrow = stride - N + K
+    y, dx = Rows(kind, R, N, stride, shift), Rows(kind, R, K, narrow, shift)
+    dw = Rows(kind, G * N, K, narrow, shift)
+    v = VALUES[kind]
+    gt.grouped_forward(ctx, gt.grouped_desc(v, G, R, K, N, K, stride), o.data_ptr(), hx.ptr, hw.data_ptr(), y.ptr, stream())
+    gt.grouped_input_gradient(ctx, gt.grouped_desc(v, G, R, K, N, narrow, N), o.data_ptr(), hdy.ptr, hw.data_ptr(), dx.ptr,
+                              stream())
+    gt.grouped_weight_gradient(ctx, gt.grouped_desc(v, G, R, K, N, K, N, narrow, N * narrow), o.data_ptr(), hdy.ptr,
+                               hx.ptr, dw.ptr, v, False, stream())
+    for got, ref in ((y, ry), (dx, rdx), (dw, rdw.reshape(G * N, K))):
+        assert np.array_equal(got.get(), rounded(ref, kind)) and got.outside_is_untouched()
+    n, rank = 5, 64
+    down = whole(rng, n, rank, K, top=1) * (rng.random((n, rank, K)) < 0.25)
+    up = whole(rng, n, N, rank, top=1) * (rng.random((n, N, rank)) < 0.25)
+    adapter = adapters_of(rng, "mixed", R, n)
+    ref, _ = adapted(x, w[0], None, adapter, down, up, np.ones(n))
+    dev = lambda a: torch.as_tensor(a).to(TYPES[kind]).cuda()
+    hd, hu, hs = dev(down), dev(up), torch.ones(n, device="cuda")
+    ha = torch.as_tensor(adapter.astype(np.int32)).cuda()
+    d = gt.adapted_desc(v, R, K, N, n, rank, K, stride)
+    ws = torch.empty(gt.adapted_workspace_bytes(d), dtype=torch.uint8, device="cuda")
+    z = Rows(kind, R, N, stride, shift)
+    gt.adapted_forward(ctx, d, hx.ptr, hw.data_ptr(), None, ha.data_ptr(), hd.data_ptr(), hu.data_ptr(), hs.data_ptr(),
+                       z.ptr, ws.data_ptr(), stream())
+    # |u| <= 520, |y| <= 520 + 64 * 520 < 2^24 and below fp16's 65504: exact in fp32, one rounding
+    assert np.array_equal(z.get(), rounded(ref, kind)) and z.outside_is_untouched()
+
+
 def test_adapted_rows_beyond_two_gigabytes(ctx):
     """Row offsets that pass 2^31 values: rows 2^20 values apart."""
     R, K, N, st, n, rank = 2200, 64, 48, 1 << 20, 5, 64
