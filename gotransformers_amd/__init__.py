@@ -184,7 +184,8 @@ def _check(code, ctx_handle=None):
 
 def inject_failure(entry_point, status):
     """Test hook: the next call of `entry_point` on this thread answers
-    `status` instead of running (gtmoe_test_inject_failure)."""
+    `status` instead of running ("hipMalloc": the next device allocation finds
+    no memory; gtmoe_test_inject_failure)."""
     _check(library().gtmoe_test_inject_failure(entry_point.encode(), status))
 
 

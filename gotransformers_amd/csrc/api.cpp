@@ -43,6 +43,21 @@ thread_local std::string g_open_error;
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+// One failure armed by gtmoe_test_inject_failure on this thread: the next
+// call of the named entry point answers `status` instead of running ("hipMalloc": the next device
+// allocation finds no memory).
+thread_local std::string g_inject_entry;
+thread_local int32_t g_inject_status = GTMOE_OK;
+
+bool take_injection(const char *entry, int32_t *status)
+{
+    if (g_inject_status == GTMOE_OK || g_inject_entry != entry) return false;
+    *status = g_inject_status;
+    g_inject_status = GTMOE_OK;
+    g_inject_entry.clear();
+    return true;
+}
+
 // Every device allocation and free the library makes goes through these two,
 // which count them for gtmoe_test_device_allocations.
 std::atomic<long long> g_device_allocations{0}, g_device_frees{0};
@@ -50,6 +65,8 @@ std::atomic<long long> g_device_allocations{0}, g_device_frees{0};
 template <class T>
 hipError_t dev_malloc(T **p, size_t bytes)
 {
+    int32_t injected = GTMOE_OK;
+    if (take_injection("hipMalloc", &injected)) return hipErrorOutOfMemory;
     g_device_allocations.fetch_add(1, std::memory_order_relaxed);
     return hipMalloc(reinterpret_cast<void **>(p), bytes);
 }
@@ -172,20 +189,6 @@ int32_t run(gtmoe_context *ctx, hipStream_t s, const char *name, F &&fn)
         int32_t rc_ = run((ctx), (s), (name), [&]() { return (expr); }); \
         if (rc_ != GTMOE_OK) return rc_;                             \
     } while (0)
-
-// One failure armed by gtmoe_test_inject_failure on this thread: the next
-// call of the named entry point answers `status` instead of running.
-thread_local std::string g_inject_entry;
-thread_local int32_t g_inject_status = GTMOE_OK;
-
-bool take_injection(const char *entry, int32_t *status)
-{
-    if (g_inject_status == GTMOE_OK || g_inject_entry != entry) return false;
-    *status = g_inject_status;
-    g_inject_status = GTMOE_OK;
-    g_inject_entry.clear();
-    return true;
-}
 
 // Entry into a call on a context: its lock, then the refusals every call
 // shares (a closed context, an injected failure), then its device current.
@@ -328,7 +331,7 @@ struct gtmoe_layer {
     TrainWorkspace tw;
     int adapter_T = -1;  // tokens of the last forward through the adapter path, -1: none
     double dropout_rate = 0;  // on the adapters' inputs
-    uint64_t dropout_seed = 0, dropout_calls = 0;  // forwards since the rate was set
+    uint64_t dropout_seed = 0, dropout_calls = 0;  // forwards that succeeded since the rate was set
     // recorded graphs that hold pointers into this layer's workspace: while
     // any exists the workspace is never reallocated
     int live_graphs = 0;
@@ -495,6 +498,7 @@ size_t layout_workspace(const gtmoe_layer *L, int cap, bool host_staging, char *
 int32_t ensure_workspace(gtmoe_layer *L, int T)
 {
     gtmoe_context *ctx = L->ctx;
+    L->adapter_T = -1;  // the call writes over what the last adapter forward kept for its backward
     if (T <= L->ws.cap) return GTMOE_OK;
     if (L->live_graphs > 0)
         return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT,
@@ -1228,13 +1232,12 @@ int32_t ensure_dropout_workspace(gtmoe_layer *L)
     TrainWorkspace &tw = L->tw;
     if (tw.dropped) return GTMOE_OK;
     gtmoe_context *ctx = L->ctx;
-    const size_t rows = (size_t)tw.cap * std::max(L->S + L->k, 1), width = std::max(L->dp, L->hp);
-    for (float **p : {&tw.dropped_grad, &tw.dropped}) {
-        void *block = nullptr;
-        HIP_TRY(ctx, dev_malloc(&block, rows * width * sizeof(float)));
-        tw.blocks.push_back(block);
-        *p = static_cast<float *>(block);
-    }
+    const size_t values = align_up((size_t)tw.cap * std::max(L->S + L->k, 1) * std::max(L->dp, L->hp), 64);
+    void *block = nullptr;
+    HIP_TRY(ctx, dev_malloc(&block, 2 * values * sizeof(float)));
+    tw.blocks.push_back(block);
+    tw.dropped = static_cast<float *>(block);
+    tw.dropped_grad = tw.dropped + values;
     return GTMOE_OK;
 }
 
@@ -1374,14 +1377,15 @@ int32_t adapter_forward(gtmoe_layer *L, int T, const double *inputs, const int64
     int32_t rc = ensure_train_workspace(L, T);
     if (rc != GTMOE_OK) return rc;
     TrainWorkspace &tw = L->tw;
-    tw.drop_threshold = 0;
-    if (L->dropout_rate > 0) dropout_rate(L->dropout_rate, tw.drop_threshold, tw.drop_scale);
+    // what the masks are made from, here and in the backward of this forward
+    // (until this one is through there is none: ensure_workspace)
+    dropout_rate(L->dropout_rate, tw.drop_threshold, tw.drop_scale);
+    tw.drop_seed = L->dropout_seed;
+    tw.drop_offset = 4 * L->dropout_calls;
     const bool drop = tw.drop_threshold > 0;
     if (drop) {
         rc = ensure_dropout_workspace(L);
         if (rc != GTMOE_OK) return rc;
-        tw.drop_seed = L->dropout_seed;
-        tw.drop_offset = 4 * L->dropout_calls++;
     }
     const int d = L->d, dp = L->dp, hp = L->hp, E = L->E, S = L->S, k = L->k, G = L->G;
     const bool hash = L->desc.use_hash_routing != 0;
@@ -1523,6 +1527,7 @@ int32_t adapter_forward(gtmoe_layer *L, int T, const double *inputs, const int64
     L->load_on_host = true;
     L->relaunch_ready = false;
     L->adapter_T = T;
+    ++L->dropout_calls;
     return GTMOE_OK;
 }
 

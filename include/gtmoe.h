@@ -137,7 +137,9 @@ const char *gtmoe_last_error(const gtmoe_context *ctx);
  * answers `status` with the text "injected failure in <entry point>" instead
  * of running, as a failing HIP call would; later calls run normally.  For
  * testing a caller's fallback (the CPU answer and lastError of
- * gpu/device.go:733-737).  Armed per thread; one failure at a time. */
+ * gpu/device.go:733-737).  Armed per thread; one failure at a time.  With
+ * "hipMalloc" the library's next device allocation on this thread finds no
+ * memory, whatever the status: a call that fails halfway. */
 int32_t gtmoe_test_inject_failure(const char *entry_point, int32_t status);
 
 /* Test hook, no counterpart in the reference: how many device allocations
@@ -397,11 +399,12 @@ int32_t gtmoe_layer_remove_adapters(gtmoe_layer *layer);
 /* Dropout on the adapters' inputs (AdapterDropout, perceptron/adapter.go:66-76)
  * of this layer's later forwards and their backwards; rate 0 turns it off, as
  * for evaluation.  The masks are gtmoe_dropout's, not the reference's random
- * source: forward number c since this call (0, 1, ...) takes `seed` and offset
- * 4 c + 0 for gate, + 1 for up, + 2 for down, + 3 for the router; a mask's row is
- * the row's position (shared expert s: s tokens + token; routed: shared experts
- * times tokens plus its place in rows_for_expert) or, for the router, the
- * token.  gtmoe_backward makes the last forward's masks again.
+ * source: forward number c since this call (0, 1, ...; one that fails or has no
+ * tokens does not count) takes `seed` and offset 4 c + 0 for gate, + 1 for up,
+ * + 2 for down, + 3 for the router; a mask's row is the row's position (shared
+ * expert s: s tokens + token; routed: shared experts times tokens plus its place
+ * in rows_for_expert) or, for the router, the token.  gtmoe_backward makes the
+ * last forward's masks again.
  * GTMOE_ERR_NOT_READY without adapters; adding adapters starts without dropout. */
 int32_t gtmoe_layer_set_adapter_dropout(gtmoe_layer *layer, double rate, uint64_t seed);
 /* Rank of one layer's adapter (LowRankAdapter.Rank); role/index as in
@@ -424,7 +427,8 @@ int32_t gtmoe_layer_zero_adapter_gradients(gtmoe_layer *layer);
  * added to.  Base weights are frozen (Layer.Backward with FreezeBase,
  * layer.go:164-210): input gradients go through them with
  * Rows.AddScaledRowTo (lowprecision/rows.go:285-324).  Without adapters it
- * fails as the reference panics for compressed weights. */
+ * fails as the reference panics for compressed weights; after a forward that
+ * failed halfway there is nothing to go back through (GTMOE_ERR_NOT_READY). */
 int32_t gtmoe_backward(gtmoe_layer *layer, int32_t tokens, const double *output_gradients,
                        double *input_gradients);
 

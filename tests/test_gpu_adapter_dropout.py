@@ -118,3 +118,70 @@ def test_adapter_dropout_refusals():
                     m.set_adapter_dropout(rate)
         finally:
             m.destroy()
+
+
+@pytest.mark.gpu
+def test_failed_forward_leaves_nothing_for_the_backward():
+    """A forward that runs out of memory -- where the masked inputs are
+    allocated, the training buffers or the forward's own -- leaves no state of
+    the forward before it behind: the backward answers that there is none.  The
+    next forward takes the masks the failed one would have taken."""
+    d, h, S, k, T, rank = 40, 56, 1, 2, 9, 4
+    spec = make_moe(gt.encode_rows, d=d, h=h, E=4, k=k, S=S, precision=INT8, seed=9)
+    rng = np.random.default_rng(10)
+    adapters = lora.make_adapters(spec, rank, 2.0 * rank, rng, up_scale=0.2)
+    x, g = rng.normal(size=(T, d)), rng.uniform(-1, 1, (T, d))
+    big = rng.normal(size=(300, d))
+    rate, seed = 0.4, 1234567
+    with gt.Context(0) as ctx:
+        m = gt.MixtureOfExperts.from_spec(ctx, spec)
+        try:
+            m.add_adapters(rank, 2.0 * rank)
+            for (kind, i, which), ad in adapters.items():
+                m.set_adapter(kind, i, which, ad.down, ad.up)
+
+            def check(call):
+                """A forward and its backward with the masks of forward number `call`."""
+                m.zero_adapter_gradients()
+                y, r = m.forward(x), m.last_routing()
+                dx = m.backward(g)
+                grads = lora.zero_grads(spec, adapters)
+                ref_y, st = lora.forward(spec, adapters, x, chosen=r.chosen, dropout=masks(rate, seed, call, T * (S + k)))
+                ref_dx = lora.backward(spec, adapters, st, g, grads)
+                assert rel(y, ref_y) <= FWD_TOL and rel(dx, ref_dx) <= GRAD_TOL
+                got, ref = m.adapter_gradients("shared", 0, "down"), grads[("shared", 0, "down")]
+                assert rel(got[0], ref[0]) <= GRAD_TOL and rel(got[1], ref[1]) <= GRAD_TOL
+
+            def fails(rows):
+                print(f"adapter dropout: a forward of {rows.shape[0]} rows without memory", flush=True)
+                gt.inject_failure("hipMalloc", gt.ERR_OUT_OF_MEMORY)
+                with pytest.raises(gt.GtmoeError, match="out of memory"):
+                    m.forward(rows)
+                for tokens in (x, big):
+                    with pytest.raises(gt.GtmoeError, match="call Forward before Backward") as info:
+                        m.backward(np.zeros_like(tokens))
+                    assert info.value.code == gt.ERR_NOT_READY
+
+            m.forward(x)  # without dropout: its allocations are all but the masked inputs'
+            m.set_adapter_dropout(rate, seed)
+            fails(x)
+            fails(x)
+            check(0)
+            check(1)
+            fails(big)  # the forward's workspace
+            m.remove_adapters()
+            m.forward(big)  # the workspace has room now
+            m.add_adapters(rank, 2.0 * rank)
+            for (kind, i, which), ad in adapters.items():
+                m.set_adapter(kind, i, which, ad.down, ad.up)
+            m.set_adapter_dropout(rate, seed)
+            check(0)
+            fails(big)  # the training buffers
+            check(1)
+            # a call that is refused before it starts changes nothing
+            y = m.forward(x)
+            with pytest.raises(gt.InvalidArgument):
+                m.backward(np.zeros((T + 1, d)))
+            assert y.shape == m.backward(g).shape
+        finally:
+            m.destroy()
