@@ -510,6 +510,11 @@ int32_t ensure_workspace(gtmoe_layer *L, int T)
         HIP_TRY(ctx, hipDeviceSynchronize());
         (void)dev_free(L->ws.base);
         L->ws = Workspace{};
+        // the last forward's state goes with it, also where the next one fails
+        L->last_T = -1;
+        L->relaunch_ready = false;
+        L->dispatch_pending = false;
+        L->load_on_host = false;
     }
     Workspace w{};
     const size_t total = layout_workspace(L, cap, true, nullptr, w);

@@ -132,3 +132,41 @@ def test_host_forward_waits_for_a_device_forward_on_another_stream():
     eb, ea = rel_err(yb, ref_b.outputs), rel_err(ya, ref_a.outputs)
     say(f"host forward {eb:.2e}, device forward {ea:.2e}")
     assert eb <= 1e-4 and ea <= 1e-4
+
+
+@pytest.mark.parametrize("path", [gt.PATH_FP32, gt.PATH_BF16])
+def test_forward_without_memory_leaves_no_state_of_the_one_before(path):
+    """A forward that needs a larger workspace and finds no memory has given up
+    the old one: nothing of the last forward can be read or launched again,
+    and the layer works on."""
+    say(f"forward without memory, path {path}")
+    spec = make_moe(gt.encode_rows, d=64, h=96, E=4, k=2, S=1, precision=INT8, seed=88)
+    rng = np.random.default_rng(89)
+    x, big = rng.standard_normal((5, 64)), rng.standard_normal((200, 64))
+    with gt.Context(0) as ctx:
+        m = gt.MixtureOfExperts.from_spec(ctx, spec)
+        try:
+            xd = torch.from_numpy(x.astype(np.float32)).cuda()
+            yd = torch.empty(5, 64, device="cuda")
+            torch.cuda.synchronize()
+            m.forward_device(5, xd.data_ptr(), yd.data_ptr(), path=path)
+            torch.cuda.synchronize()
+            want = yd.clone()
+            gt.inject_failure("hipMalloc", gt.ERR_OUT_OF_MEMORY)
+            with pytest.raises(gt.GtmoeError, match="out of memory") as info:
+                m.forward(big, path=path)
+            assert info.value.code == gt.ERR_OUT_OF_MEMORY
+            for call in (m.last_routing, m.last_expert_load, lambda: m.relaunch(gt.KERNEL_GATEUP),
+                         lambda: m.relaunch(gt.KERNEL_DOWN)):
+                with pytest.raises(gt.GtmoeError) as info:
+                    call()
+                assert info.value.code == gt.ERR_NOT_READY
+            m.update_balance(0.1)  # nothing before the first forward
+            assert np.array_equal(m.balance_biases, spec.balance_biases)
+            m.forward_device(5, xd.data_ptr(), yd.data_ptr(), path=path)
+            torch.cuda.synchronize()
+            assert torch.equal(yd, want)
+            assert m.last_routing().load.sum() == 10
+            assert m.forward(big, path=path).shape == big.shape
+        finally:
+            m.destroy()
