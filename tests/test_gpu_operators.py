@@ -932,3 +932,26 @@ def test_operators_are_timed_by_name(ctx):
     ctx.timing(False)
     ctx.timing_reset()
     assert times["dropout"][1] == 1 and times["dropout"][0] > 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("stride, shift", [(520, 0), (524, 4), (523, 1)])
+def test_many_tiles_of_weight_gradients_accumulate_in_fp32(ctx, kind, stride, shift):
+    """Micro-batches summed in fp32 matrices of any alignment, an empty group
+    among them: whole numbers up to 2 * 4 * 300 + 50, exact in fp32."""
+    rng = np.random.default_rng(31)
+    G, K, N = 40, 520, 264
+    off = offsets_of([300, 0, 41] + [7] * (G - 3))
+    R = int(off[-1])
+    x, dy, before = whole(rng, R, K), whole(rng, R, N), whole(rng, G, N, K, top=50)
+    say(f"accumulate fp32 {kind} stride={stride} shift={shift}")
+    dw = Rows("f32", G * N, K, stride, shift, before.reshape(G * N, K))
+    hx, hdy, o = Rows(kind, R, K, data=x), Rows(kind, R, N, data=dy), device_offsets(off)
+    d = gt.grouped_desc(VALUES[kind], G, R, K, N, K, N, stride, N * stride)
+    want = before
+    for _ in range(2):
+        gt.grouped_weight_gradient(ctx, d, o.data_ptr(), hdy.ptr, hx.ptr, dw.ptr, gt.VALUES_FLOAT32, True, stream())
+        want = want + grouped(off, x, np.zeros((G, N, K)), dy)[2]
+    assert np.array_equal(dw.get(), want.reshape(G * N, K)) and dw.outside_is_untouched()
+    gt.grouped_weight_gradient(ctx, d, o.data_ptr(), hdy.ptr, hx.ptr, dw.ptr, gt.VALUES_FLOAT32, False, stream())
+    assert np.array_equal(dw.get(), ((want - before) / 2).reshape(G * N, K)) and dw.outside_is_untouched()
