@@ -42,7 +42,8 @@ constexpr int kSortWaves = 16, kSortBins = 1024;
 // a bin among mixed ones take their places as they come, which changes no
 // result: a row's sums do not depend on the rows beside it.
 __global__ __launch_bounds__(64 * kSortWaves) void adapter_sort_kernel(const int32_t *__restrict__ adapter, int rows, int adapters,
-                                                                       int32_t *__restrict__ index, int32_t *__restrict__ offsets)
+                                                                       int32_t *__restrict__ index, int32_t *__restrict__ sorted,
+                                                                       int32_t *__restrict__ offsets)
 {
     __shared__ int place[kSortWaves][kSortBins];
     __shared__ int sums[kSortWaves];
@@ -104,10 +105,15 @@ __global__ __launch_bounds__(64 * kSortWaves) void adapter_sort_kernel(const int
     each_chunk([&](int t0, int b, int n, int one, bool same) {
         if (same) {
             const int at = place[wave][one];
-            if (lane < n) index[at + lane] = t0 + lane;
+            if (lane < n) {
+                index[at + lane] = t0 + lane;
+                sorted[at + lane] = one;
+            }
             if (lane == 0) place[wave][one] = at + n;
         } else if (lane < n) {
-            index[atomicAdd(&place[wave][b], 1)] = t0 + lane;
+            const int at = atomicAdd(&place[wave][b], 1);
+            index[at] = t0 + lane;
+            sorted[at] = b;
         }
     });
 }
@@ -230,7 +236,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(AdapterDownAr
     int mine = -1;
     const int at = t0 + min(i, rows - 1), row = a.index ? a.index[at] : at;
     if (i < rows) {
-        mine = a.adapter[row];
+        mine = a.adapter[at];
         if (mine >= a.adapters) mine = -1;
     }
     const Store *const x[1] = {reinterpret_cast<const Store *>(a.x) + (long long)row * a.ldx};
@@ -264,56 +270,17 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(AdapterDownAr
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[wave][i][16 * p + 4 * q + e] = acc[p][e];
     __syncthreads();
-    if constexpr (T::kBytes == 2) {
-        if (a.index) {
-            // u's two 16-bit parts (RankRow), of the row scaled to values below
-            // 2 for fp16: 32 lanes per row, two ranks or fewer each (blockIdx.y is 0)
-            const int r = threadIdx.x >> 5, c0 = threadIdx.x & 31;
-            static_assert(64 * kWaves / 32 == 16, "");
-            const int at = a.index[t0 + min(r, rows - 1)], ad = a.adapter[at];
-            const bool has = r < rows && ad >= 0 && ad < a.adapters;
-            float v[2] = {0.f, 0.f}, top = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = c0 + 32 * e;
-                if (has && c < 16 * NR && c < a.rank) {
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w) v[e] += part[w][r][c];
-                    v[e] *= a.scales[ad];
-                }
-                top = fmaxf(top, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.f);
-            }
-#pragma unroll
-            for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-            if (!has) return;
-            const RowScale scale = row_scale<T>(top);
-            Store *hi = reinterpret_cast<Store *>(a.u_hi) + (long long)at * a.ldu;
-            Store *lo = reinterpret_cast<Store *>(a.u_lo) + (long long)at * a.ldu;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = c0 + 32 * e;
-                if (c < a.ldu) {
-                    float hv, lv;
-                    two_parts<T>(v[e], scale.down, hv, lv);
-                    hi[c] = T::round(hv);
-                    lo[c] = T::round(lv);
-                }
-            }
-            if (c0 == 0) a.unscale[t0 + r] = scale.up;  // in the sorted order
-            return;
-        }
-    }
     for (int o = threadIdx.x; o < 16 * 16 * NR; o += 64 * kWaves) {
         const int r = o / (16 * NR), c = o - r * (16 * NR);
         if (r < rows && j0 + c < a.ldu) {
-            const int ad = a.adapter[t0 + r];
+            const int ad = a.adapter[t0 + r], to = a.index ? a.index[t0 + r] : t0 + r;
             float v = 0.f;
             if (ad >= 0 && ad < a.adapters && j0 + c < a.rank) {
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) v += part[w][r][c];
                 v *= a.scales[ad];
             }
-            a.u[(long long)(t0 + r) * a.ldu + j0 + c] = v;
+            a.u[(long long)to * a.ldu + j0 + c] = v;
         }
     }
 }
@@ -469,13 +436,14 @@ bool adapted_sorts(const GroupedArgs &a, int values)
     const AdapterTerm &t = a.term;
     auto whole = [](const void *p, long long stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; };
     return whole(a.a, a.lda) && whole(a.b, a.ldb) && whole(t.up, t.rank) && a.inputs % 8 == 0 && t.rank <= kMaxSortedRank &&
-           (long long)a.rows * a.lda < 1 << 30 && (long long)a.rows * t.ldu < 1 << 30;
+           (long long)a.rows * a.lda < 1 << 30 && (long long)a.rows * t.ldu < 1 << 29;
 }
 
-hipError_t launch_adapter_sort(const int32_t *adapter, int rows, int adapters, int32_t *index, int32_t *offsets,
-                               hipStream_t s)
+hipError_t launch_adapter_sort(const int32_t *adapter, int rows, int adapters, int32_t *index, int32_t *sorted,
+                               int32_t *offsets, hipStream_t s)
 {
-    hipLaunchKernelGGL(adapter_sort_kernel, dim3(1), dim3(64 * kSortWaves), 0, s, adapter, rows, adapters, index, offsets);
+    hipLaunchKernelGGL(adapter_sort_kernel, dim3(1), dim3(64 * kSortWaves), 0, s, adapter, rows, adapters, index, sorted,
+                       offsets);
     return hipGetLastError();
 }
 

@@ -3250,18 +3250,17 @@ int32_t check_adapted(gtmoe_context *ctx, const gtmoe_adapted_desc *d)
 
 int adapter_ldu(const gtmoe_adapted_desc *d) { return (d->rank + 7) / 8 * 8; }
 
-// The workspace of one call: u in fp32, or its two 16-bit parts in the same
-// place; then, for rows sorted by adapter, each row's scale, the order and the
-// adapters' first places in it.
+// The workspace of one call: u; then, for rows sorted by adapter, their
+// adapters, the order and the adapters' first places in it.
 struct AdaptedWorkspace {
-    size_t unscale, index, offsets, bytes;
+    size_t sorted, index, offsets, bytes;
 };
 AdaptedWorkspace adapted_workspace(const gtmoe_adapted_desc *d)
 {
     const size_t rows = std::max(d->rows, 1);
     AdaptedWorkspace w;
-    w.unscale = rows * adapter_ldu(d) * sizeof(float);
-    w.index = w.unscale + align_up(rows * sizeof(float), 16);
+    w.sorted = rows * adapter_ldu(d) * sizeof(float);
+    w.index = w.sorted + align_up(rows * sizeof(int32_t), 16);
     w.offsets = w.index + align_up(rows * sizeof(int32_t), 16);
     w.bytes = w.offsets + align_up(((size_t)d->adapters + 2) * sizeof(int32_t), 16);
     return w;
@@ -3348,9 +3347,7 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
             a.offsets = reinterpret_cast<const int32_t *>(base + layout.offsets);
             a.groups = desc->adapters + 1;  // the last: rows without an adapter
             a.term.index = dargs.index = reinterpret_cast<const int32_t *>(base + layout.index);
-            a.term.u_hi = dargs.u_hi = base;
-            a.term.u_lo = dargs.u_lo = base + layout.unscale / 2;
-            a.term.unscale = dargs.unscale = reinterpret_cast<float *>(base + layout.unscale);
+            dargs.adapter = reinterpret_cast<const int32_t *>(base + layout.sorted);
         }
         return check_grid(c, a, adapted_fits(a, desc->values));
     };
@@ -3362,7 +3359,7 @@ int32_t gtmoe_adapted_forward(gtmoe_context *ctx, const gtmoe_adapted_desc *desc
     if (a.term.index)
         TRY(run_plain(ctx, s, "adapter_sort", [&] {
             return launch_adapter_sort(adapter, a.rows, desc->adapters, const_cast<int32_t *>(a.term.index),
-                                       const_cast<int32_t *>(a.offsets), s);
+                                       const_cast<int32_t *>(dargs.adapter), const_cast<int32_t *>(a.offsets), s);
         }));
     TRY(run_plain(ctx, s, "adapter_down", [&] { return launch_adapter_down(dargs, desc->values, s); }));
     return run_plain(ctx, s, "adapted_forward", [&] { return launch_adapted(a, desc->values, s); });

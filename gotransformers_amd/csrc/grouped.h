@@ -20,12 +20,8 @@ struct AdapterTerm {
     const int32_t *adapter = nullptr;  // [rows]; outside [0, adapters): none
     const void *up = nullptr;
     int adapters = 0, rank = 0, ldu = 0;
-    // rows sorted by adapter (grouped_large.hip): u as two 16-bit parts
-    // [rows][ldu] of a row scaled by a power of two, whose inverse unscale holds in
-    // the sorted order, and the sorted rows' places, group `adapters` those without
-    // an adapter
-    const void *u_hi = nullptr, *u_lo = nullptr;
-    const float *unscale = nullptr;
+    // rows sorted by adapter (grouped_large.hip): the sorted rows' places, group
+    // `adapters` those without an adapter
     const int32_t *index = nullptr;
 };
 
@@ -56,9 +52,10 @@ hipError_t launch_grouped(const GroupedArgs &a, int direction, int values, hipSt
 // (grouped_large.hip).
 bool large_fits(const GroupedArgs &a, int direction, int value_bytes);
 hipError_t launch_large(const GroupedArgs &a, int direction, int values, hipStream_t s);
-constexpr int kMaxSortedRank = 64;  // ranks of a part of u in one step
+constexpr int kMaxSortedRank = 64;  // ranks of u in two steps
 
-// u[t][j] = scales[a] sum_k down[a][j][k] x[t][k] for the rows with an adapter a.
+// u[t][j] = scales[a] sum_k down[a][j][k] x[t][k] for the rows with an adapter a,
+// zero for the others.
 struct AdapterDownArgs {
     const void *x = nullptr, *down = nullptr;
     const float *scales = nullptr;
@@ -66,23 +63,21 @@ struct AdapterDownArgs {
     float *u = nullptr;
     long long ldx = 0;
     int rows = 0, inputs = 0, rank = 0, adapters = 0, ldu = 0;
-    // with sorted rows: their order, and u's parts (AdapterTerm) instead of u
-    const int32_t *index = nullptr;
-    void *u_hi = nullptr, *u_lo = nullptr;
-    float *unscale = nullptr;
+    const int32_t *index = nullptr;  // with sorted rows: their places, and adapter in the sorted order
 };
 hipError_t launch_adapter_down(const AdapterDownArgs &a, int values, hipStream_t s);
 // The forward of one group with its adapters' term.
 hipError_t launch_adapted(const GroupedArgs &a, int values, hipStream_t s);
 // Whether both kernels' workgroups fit one launch each.
 bool adapted_fits(const GroupedArgs &a, int values);
-// Whether a forward with adapters takes its rows sorted by adapter (a.term.index
-// and parts of u instead of u): launch_adapter_sort first.
+// Whether a forward with adapters takes its rows sorted by adapter
+// (a.term.index): launch_adapter_sort first.
 bool adapted_sorts(const GroupedArgs &a, int values);
-// index [rows]: the rows by adapter, those without one last; offsets
-// [adapters + 2]: where each adapter's begin.
-hipError_t launch_adapter_sort(const int32_t *adapter, int rows, int adapters, int32_t *index, int32_t *offsets,
-                               hipStream_t s);
+// index [rows]: the rows by adapter, those without one last; sorted [rows]: the
+// adapters in that order (`adapters`: none); offsets [adapters + 2]: where each
+// adapter's begin.
+hipError_t launch_adapter_sort(const int32_t *adapter, int rows, int adapters, int32_t *index, int32_t *sorted,
+                               int32_t *offsets, hipStream_t s);
 
 // out[r][c] = base[r][c] + (keep(r, c) ? x[index ? index[r] : r][c] * scale : 0),
 // base null: no first term.

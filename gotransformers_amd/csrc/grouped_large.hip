@@ -257,6 +257,7 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 {
     typedef Operand<T, DIR != kGroupedWeightGradient, kBm, kThreads, SB, ADAPTED> A;
     typedef Operand<T, DIR == kGroupedForward, kBn, kThreads, SB> B;
+    typedef Operand<F32, true, kBm, kThreads, SB, ADAPTED> U;  // of an adapter's term
     typedef typename T::Store Store;
     constexpr int NJ = 2, KK = SB / 32, L = A::kLoads + B::kLoads;
     __shared__ __attribute__((aligned(1024))) char s0[(kBm + kBn) * SB];
@@ -316,13 +317,14 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         else return A(p, a.lda, x.m, x.length);
     };
     auto operand_u = [&](const Tile &x) {
-        if constexpr (ADAPTED) return A(a.term.u_hi, a.term.ldu, a.rows, a.term.index + x.m0, x.m, a.term.rank);
+        if constexpr (ADAPTED) return U(a.term.u, a.term.ldu, a.rows, a.term.index + x.m0, x.m, a.term.rank);
         else return 0;
     };
-    auto operand_up = [&](const Tile &x) {
+    // step e of the adapter's up matrix: as many ranks as a step of u has
+    auto operand_up = [&](const Tile &x, int e) {
         const Store *p = reinterpret_cast<const Store *>(a.term.up) +
-                         ((long long)min(x.g, max(a.term.adapters - 1, 0)) * a.outputs + x.n0) * a.term.rank;
-        return B(p, a.term.rank, x.n, a.term.rank);
+                         ((long long)min(x.g, max(a.term.adapters - 1, 0)) * a.outputs + x.n0) * a.term.rank + e * U::kStep;
+        return B(p, a.term.rank, x.n, min(U::kStep, a.term.rank - e * U::kStep));
     };
     auto operand_b = [&](const Tile &x) {
         const Store *p = reinterpret_cast<const Store *>(a.b);
@@ -365,15 +367,15 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
             rt.extra = 0;
         }
     };
-    // step rk of the request stream: of the operands, then u's parts and the
-    // adapter's up matrix (every field that is one for the wave kept scalar)
+    // step rk of the request stream: of the operands, then of u and the adapter's
+    // up matrix (every field that is one for the wave kept scalar)
     auto request_a = [&]() {
         auto q = oa.request(rk);
         if constexpr (ADAPTED) {
             const bool more = rk >= rt.steps;
-            const auto e = ou.request(0);
-            const char *part = reinterpret_cast<const char *>(rk > rt.steps ? a.term.u_lo : a.term.u_hi);
-            q.p = scalar(more ? part : q.p);
+            static_assert(U::kLoads == A::kLoads, "");
+            const auto e = ou.request(more ? rk - rt.steps : 0);
+            q.p = scalar(more ? e.p : q.p);
             q.bytes = __builtin_amdgcn_readfirstlane(more ? e.bytes : q.bytes);
 #pragma unroll
             for (int i = 0; i < A::kLoads; ++i) q.off[i] = more ? e.off[i] : q.off[i];
@@ -384,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         auto q = ob.request(rk);
         if constexpr (ADAPTED) {
             const bool more = rk >= rt.steps;
-            const auto e = operand_up(rt).request(0);
+            const auto e = operand_up(rt, more ? rk - rt.steps : 0).request(0);
             q.p = scalar(more ? e.p : q.p);
             q.bytes = __builtin_amdgcn_readfirstlane(more ? e.bytes : q.bytes);
             q.row = __builtin_amdgcn_readfirstlane(more ? e.row : q.row);
@@ -395,6 +397,9 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 
     u32x4 fa[2][4], fb[2][NJ];
     const uint32_t la = A::lane_offset(wm), lb = B::lane_offset(wn);
+    // the lane's first eight ranks of u in a step: units 2 h and 2 h + 1 of its row
+    const int ur = wm + (lane & 31);
+    const uint32_t lu = ur * SB + ((2 * h) ^ swizzle<F32, true, kBm, SB>(ur)) * 16;
     auto landed = [&]() {
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
@@ -461,23 +466,42 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
+        // a step of the adapter's term: 32 ranks of u, split as they leave LDS
+        auto ranks = [&](char *cur, int e) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                if (e * U::kStep + 16 * g >= a.term.rank) break;
+                UpRow<T> b[NJ];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) b[j].split(B::read(cur + kBm * SB, lb, j, g));
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    f32x4 v[2];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        v[p] = *reinterpret_cast<const f32x4 *>(cur + ((lu ^ (64 * g + 16 * p)) + i * (64 * SB)));
+                    RankRow u;
+                    u.split(v);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = multiply_ranks<T>(b[j], u, acc[i][j]);
+                }
+            }
+            advance();
+            const auto qa = request_a();
+            const auto qb = request_b();
+            ++rk;
+            landed();
+            A::issue(cur, qa);
+            B::issue(cur + kBm * SB, qb);
+        };
         // ADAPTED, asked for now and used at the end: the places of the wave's rows
-        // (lane l: rows l and 64 + l of them) and, fp16, the scales of u's rows
-        const int r = lane & 31;
+        // (lane l: rows l and 64 + l of them)
         int at_rows[2];
-        float up[MI];
         if constexpr (ADAPTED) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int row = 64 * (2 * q + h) + wm + r;
+                const int row = 64 * (2 * q + h) + wm + (lane & 31);
                 at_rows[q] = row < x.m ? a.term.index[x.m0 + row] : 0;
-            }
-            if constexpr (std::is_same<T, F16>::value) {
-#pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    const int row = 64 * i + wm + r;
-                    up[i] = x.extra && row < x.m ? a.term.unscale[x.m0 + row] : 1.f;
-                }
             }
         }
         read(s0, 0, 0);
@@ -487,21 +511,8 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         }
         if constexpr (ADAPTED) {
             if (x.extra) {
-                // fp16: the row's accumulators in the scale of its u meanwhile
-                if constexpr (std::is_same<T, F16>::value) {
-#pragma unroll
-                    for (int i = 0; i < MI; ++i)
-#pragma unroll
-                        for (int j = 0; j < NJ; ++j) acc[i][j] *= 1.f / up[i];  // a power of two: exact
-                }
-                body(s0, s1);
-                body(s1, s0);
-                if constexpr (std::is_same<T, F16>::value) {
-#pragma unroll
-                    for (int i = 0; i < MI; ++i)
-#pragma unroll
-                        for (int j = 0; j < NJ; ++j) acc[i][j] *= up[i];
-                }
+                ranks(s0, 0);
+                ranks(s1, 1);
             }
             if (a.bias) add_bias<T>(acc, a.bias, x.n0 + wn, a.outputs);
         }

@@ -352,46 +352,34 @@ __device__ __forceinline__ void load_ranks(const typename T::Store *row, int k, 
     for (int e = 0; e < 8; ++e) v[e] = T::load(w[e]);
 }
 
-// Sixteen ranks' worth of one operand of the adapters' product: a lane of half
-// h = l / 32 holds ranks k .. k + 7, k = c + 8 h, of one row.
-//
-// 16-bit values: u enters the matrix cores as two 16-bit numbers, its leading
-// part and the rest of it, so that what is lost of a rank's product is 2^-16 of
-// it (bf16: the upper half of the word and the rest rounded; fp16: 2^-21), far
-// below the output's own rounding, at an eighth of the time of fp32 MFMAs.  fp16
-// has too few exponents for u: a row's ranks are scaled by a power of two, and
-// so is what they are added to (exactly).  What is not finite stays so in both parts.
-struct RowScale {
-    float down, up;  // the row's power of two and its inverse
-};
-// For values of at most `top`: scaled they are below 2.  The exponent is held to
-// -40 .. 100: what is added to u's product takes the same factors and may
-// neither overflow nor lose bits (an fp16 result's are between 2^-25 and 2^16),
-// and of smaller u the fp16 parts keep 2^-64, which no result shows.
-template <class T>
-__device__ __forceinline__ RowScale row_scale(float top)
-{
-    if (!std::is_same<T, F16>::value || !(top > 0.f)) return {1.f, 1.f};
-    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -40), 100);
-    return {__uint_as_float((uint32_t)(127 - ex) << 23), __uint_as_float((uint32_t)(127 + ex) << 23)};
-}
-template <class T>
-__device__ __forceinline__ void two_parts(float x, float scale, float &hi, float &lo)
-{
-    if constexpr (std::is_same<T, F16>::value) {
-        const float y = x * scale;
-        hi = T::load(T::round(y));
-        lo = fabsf(x) < __builtin_inff() ? y - hi : x;
-    } else {
-        hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-        lo = fabsf(x) < __builtin_inff() ? x - hi : x;
-    }
-}
-
-template <class T>
+// The adapters' product on the 16-bit matrix cores, sixteen ranks at a time: a
+// lane of half h = l / 32 holds ranks k .. k + 7, k = c + 8 h, of one row of u and
+// of one row of the adapter's up matrix.  u, which is fp32, enters as three bf16
+// numbers whose sum it is (each cut off after eight bits, the rest exact, 24 bits in
+// all), Up's values as they are or, fp16, as two (eight and three bits).  Products
+// of bf16 numbers are exact in fp32, so the term is as if made there, whatever a
+// row's ranks' sizes beside each other, for three or five MFMAs; fp32 ones would
+// take as long as sixteen.  (Of fp16 the smallest parts' product, below 2^-24 of the
+// whole, is left out.)  What is not finite stays so.
 struct RankRow {
-    u32x4 hi, lo;
-    float scale, unscale;
+    u32x4 part[3];
+    __device__ __forceinline__ void split(const f32x4 (&v)[2])
+    {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            uint32_t w[2][3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float x = v[p >> 1][2 * (p & 1) + e];
+                const float r = fabsf(x) < __builtin_inff() ? x - upper(x) : 0.f;
+                w[e][0] = __float_as_uint(x);
+                w[e][1] = __float_as_uint(r);
+                w[e][2] = __float_as_uint(r - upper(r));
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q) part[q][p] = upper_halves(w[0][q], w[1][q]);
+        }
+    }
     __device__ __forceinline__ void load(const float *u, bool have)
     {
         f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -399,45 +387,64 @@ struct RankRow {
             v[0] = *reinterpret_cast<const f32x4 *>(u);
             v[1] = *reinterpret_cast<const f32x4 *>(u + 4);
         }
-        float top = 0.f;
+        split(v);
+    }
+    // the bf16 number that x's upper half is
+    static __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+    static __device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi)
+    {
+        return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+    }
+};
+
+// Eight ranks of a row of Up for the same product.
+template <class T>
+struct UpRow {
+    u32x4 part[std::is_same<T, F16>::value ? 2 : 1];
+    __device__ __forceinline__ void split(u32x4 v)
+    {
         if constexpr (std::is_same<T, F16>::value) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = fabsf(v[e >> 2][e & 3]);
-                top = fmaxf(top, x < __builtin_inff() ? x : 0.f);
+            for (int p = 0; p < 4; ++p) {
+                const float x = T::load((uint16_t)v[p]), y = T::load((uint16_t)(v[p] >> 16));
+                part[0][p] = RankRow::upper_halves(__float_as_uint(x), __float_as_uint(y));
+                part[1][p] = RankRow::upper_halves(__float_as_uint(x - RankRow::upper(x)), __float_as_uint(y - RankRow::upper(y)));
             }
-            top = fmaxf(top, __shfl_xor(top, 32));  // the row's other half
-        }
-        const RowScale s = row_scale<T>(top);
-        scale = s.down;
-        unscale = s.up;
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            float h[2], l[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) two_parts<T>(v[p >> 1][2 * (p & 1) + e], scale, h[e], l[e]);
-            hi[p] = T::pack(h[0], h[1]);
-            lo[p] = T::pack(l[0], l[1]);
+        } else {
+            part[0] = v;
         }
     }
 };
 
+// c += b u^T over sixteen ranks of 32 rows each.
+template <class T>
+__device__ __forceinline__ f32x16 multiply_ranks(const UpRow<T> &b, const RankRow &u, f32x16 c)
+{
+#pragma unroll
+    for (int q = 0; q < 3; ++q) c = Bf16::mfma(b.part[0], u.part[q], c);
+    if constexpr (std::is_same<T, F16>::value) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) c = Bf16::mfma(b.part[1], u.part[q], c);
+    }
+    return c;
+}
+
 // Eight ranks of B from rank k on, 16-bit values, for NJ 32-column blocks (`up`:
 // the lane's row of each, or null past the matrix); zero at and past `rank`.
 template <class T, int NJ>
-__device__ __forceinline__ void load_columns(const typename T::Store *const (&up)[NJ], int k, int rank, u32x4 (&b)[NJ])
+__device__ __forceinline__ void load_columns(const typename T::Store *const (&up)[NJ], int k, int rank, UpRow<T> (&b)[NJ])
 {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        b[j] = u32x4{0u, 0u, 0u, 0u};
-        if (!up[j] || k >= rank) continue;
-        if (k + 8 <= rank) {
-            __builtin_memcpy(&b[j], up[j] + k, 16);
-        } else {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (up[j] && k + 8 <= rank) {
+            __builtin_memcpy(&v, up[j] + k, 16);
+        } else if (up[j] && k < rank) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (k + e < rank) b[j][e >> 1] |= (uint32_t)up[j][k + e] << (16 * (e & 1));
+                if (k + e < rank) v[e >> 1] |= (uint32_t)up[j][k + e] << (16 * (e & 1));
         }
+        b[j].split(v);
     }
 }
 
@@ -489,19 +496,14 @@ __device__ __forceinline__ uint32_t add_adapters(f32x16 (&acc)[MI][NJ], const Gr
             const typename T::Store *const(&cols)[NJ] = rows;
             for (int c = 0; c < t.rank; c += 16) {
                 const int k = c + 8 * h;
-                u32x4 b[NJ];
+                UpRow<T> b[NJ];
                 load_columns<T, NJ>(cols, k, t.rank, b);
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    RankRow<T> u;
+                    RankRow u;
                     u.load(t.u + (long long)(m0 + 32 * EACH * i + (lane & 31)) * t.ldu + k, mine[i] >= 0 && k < t.ldu);
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        if constexpr (std::is_same<T, F16>::value) acc[i][j] *= u.scale;
-                        acc[i][j] = T::mfma(b[j], u.hi, acc[i][j]);
-                        acc[i][j] = T::mfma(b[j], u.lo, acc[i][j]);
-                        if constexpr (std::is_same<T, F16>::value) acc[i][j] *= u.unscale;
-                    }
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = multiply_ranks<T>(b[j], u, acc[i][j]);
                 }
             }
             return without;
@@ -564,17 +566,12 @@ __device__ __forceinline__ uint32_t add_adapters(f32x16 (&acc)[MI][NJ], const Gr
                 const typename T::Store *const(&cols)[NJ] = crows;
                 for (int c = 0; c < t.rank; c += 16) {
                     const int k = c + 8 * h;
-                    u32x4 b[NJ];
+                    UpRow<T> b[NJ];
                     load_columns<T, NJ>(cols, k, t.rank, b);
-                    RankRow<T> u;
+                    RankRow u;
                     u.load(t.u + (long long)row * t.ldu + k, here && k < t.ldu);
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        if constexpr (std::is_same<T, F16>::value) d[j] *= u.scale;
-                        d[j] = T::mfma(b[j], u.hi, d[j]);
-                        d[j] = T::mfma(b[j], u.lo, d[j]);
-                        if constexpr (std::is_same<T, F16>::value) d[j] *= u.unscale;
-                    }
+                    for (int j = 0; j < NJ; ++j) d[j] = multiply_ranks<T>(b[j], u, d[j]);
                 }
             } else {
                 for (int c = 0; c < t.rank; c += 8) {

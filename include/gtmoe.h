@@ -500,7 +500,12 @@ int32_t gtmoe_grouped_weight_gradient(gtmoe_context *ctx, const gtmoe_grouped_de
  * of a smaller rank is padded with zeros.  biases may be NULL.  With weights
  * NULL the shared product is what outputs holds already and the adapters'
  * terms (and biases, if given) are added to it; without biases rows without
- * an adapter are then left as they are.  Down_a inputs[t] is kept in fp32.
+ * an adapter are then left as they are.  Down_a inputs[t] is kept in fp32 and
+ * multiplied with Up's values as such, whatever its ranks' sizes beside each
+ * other.  What is not finite in a row or its adapter leaves that row's outputs
+ * not finite (an infinity may come out as NaN) and reaches no other row.  A row's
+ * last bits may depend on how many rows a call has and on their adapters, which
+ * choose the order of the sums; the same call gives the same bits.
  * The workspace holds gtmoe_adapted_workspace bytes (a host call that needs no
  * context), 16-byte aligned, for the call's time on the stream. */
 typedef struct gtmoe_adapted_desc {

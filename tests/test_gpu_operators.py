@@ -955,3 +955,56 @@ def test_many_tiles_of_weight_gradients_accumulate_in_fp32(ctx, kind, stride, sh
     assert np.array_equal(dw.get(), want.reshape(G * N, K)) and dw.outside_is_untouched()
     gt.grouped_weight_gradient(ctx, d, o.data_ptr(), hdy.ptr, hx.ptr, dw.ptr, gt.VALUES_FLOAT32, False, stream())
     assert np.array_equal(dw.get(), ((want - before) / 2).reshape(G * N, K)) and dw.outside_is_untouched()
+
+
+# rows and ranks: few rows; tiles with the rows in order; rows sorted by adapter
+FORMS = [(20, 8), (300, 8), (300, 24), (2100, 64), (8200, 16), (5470, 24)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T, rank", FORMS)
+@pytest.mark.parametrize("pattern", ["one", "runs", "each its own"])
+def test_adapted_holds_the_ranks_products_in_fp32_in_every_form(ctx, kind, T, rank, pattern):
+    """Down x is 1 + 2^-9 + 2^-18 in one rank and 1 + 2^-9 in another, whose Up
+    values cancel up to their last bits: 2^10 2^-18 is left, and nothing where
+    Down x is held in 16 bits."""
+    K, N, n = 16, 40, 7
+    rng = np.random.default_rng(T + rank)
+    x = np.zeros((T, K))
+    x[:, 0], x[:, 1], x[:, 2] = 1.0, 2.0 ** -9, 2.0 ** -9
+    down, up = np.zeros((n, rank, K)), np.zeros((n, N, rank))
+    for a in range(n):
+        i, j = rng.choice(rank, 2, replace=False)
+        down[a, [i, j], 0], down[a, [i, j], 1], down[a, i, 2] = 1.0, 1.0, 2.0 ** -9
+        up[a, :, i] = 2.0 ** 10 * rng.choice([-1.0, 1.0], N)
+        up[a, :, j] = -up[a, :, i]
+    adapter = adapters_of(rng, pattern, T, n)
+    say(f"fp32 ranks {kind} T={T} rank={rank} {pattern}")
+    for w, base in ((np.zeros((N, K)), None), (None, np.zeros((T, N)))):
+        got = run_adapted(ctx, kind, x, w, None, adapter, down, up, np.ones(n), base=base)
+        ref, _ = adapted(x, w, None, adapter, down, up, np.ones(n), base=base)
+        assert set(np.unique(np.abs(ref))) <= {0.0, 2.0 ** -8}
+        assert np.array_equal(got, ref)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T, rank", FORMS)
+@pytest.mark.parametrize("pattern", ["one", "runs", "each its own"])
+def test_adapted_ranks_of_unlike_sizes(ctx, kind, T, rank, pattern):
+    """Ranks whose products with the row are up to 2^24 apart, Up's values as far
+    apart the other way: every rank weighs the same in the output."""
+    K, N, n = 64, 72, 7
+    rng = np.random.default_rng(T * 3 + rank)
+    make = lambda *s, f=1.0: rounded(rng.normal(size=s) * f, kind)
+    x, w, b = make(T, K), make(N, K), make(N)
+    size_of = 2.0 ** (12 - 24 * rng.permutation(rank) / max(rank - 1, 1)).round()
+    down, up = make(n, rank, K, f=size_of[:, None]), make(n, N, rank, f=1 / size_of)
+    scales = np.float32(rng.uniform(0.5, 2, size=n)).astype(np.float64)
+    adapter = adapters_of(rng, pattern, T, n)
+    say(f"unlike ranks {kind} T={T} rank={rank} {pattern}")
+    for ww, base in ((w, None), (None, make(T, N))):
+        got = run_adapted(ctx, kind, x, ww, b, adapter, down, up, scales, base=base)
+        ref, size = adapted(x, ww, b, adapter, down, up, scales, base=base)
+        # K terms of the shared sum; K, the scale and rank terms of the adapter's; bias and the two parts' sum
+        bound = HALF_STEP[kind] * np.abs(ref) + HALF_LAST_STEP[kind] + (K + rank + 4) * 2.0 ** -24 * size
+        assert np.all(np.abs(got - ref) <= bound * (1 + 2.0 ** -7))
