@@ -628,7 +628,8 @@ def adapted_desc(values, rows, inputs, outputs, adapters, rank, input_stride=Non
 
 def adapted_workspace_bytes(desc):
     """Bytes of the workspace adapted_forward needs: the rows' products with
-    their Down matrices in fp32, padded to eight ranks."""
+    their Down matrices in fp32, padded to eight ranks, the rows' order by
+    adapter with their adapters, and where each adapter's rows begin."""
     n = C.c_size_t(0)
     _check(library().gtmoe_adapted_workspace(C.byref(desc), C.byref(n)))
     return n.value

@@ -6,11 +6,11 @@
 // with their adapters' epilogue.
 //
 // The three kernels' times on an MI355X (us): one row of 2048 -> 2048, rank 16, bf16,
-// 4.6 and 5.0, which is a launch and two dependent trips to memory each (W's
-// 8 MiB alone: 1.6); 64 rows of 48 adapters 4.8 and 8.8, the gathered Up
+// 4.6 and 5.2, which is a launch and two dependent trips to memory each (W's
+// 8 MiB alone: 1.6); 64 rows of 48 adapters 4.8 and 9.0, the gathered Up
 // rows (2 MiB per 32 of them) in the epilogue; 8192 rows, 12 adapters of rank 64, fp16, sort
-// 6.1, down 17.5 (17 MB of rows and, per 16 of them, 128 KiB of Down from L2),
-// tiles 76 (grouped_large.hip).
+// 6.4, down 17.2 (17 MB of rows and, per 16 of them, 128 KiB of Down from L2),
+// tiles 82 (grouped_large.hip).
 #include "grouped_tile.h"
 
 namespace gtmoe {
@@ -22,17 +22,24 @@ constexpr int kWaves = 8;
 // 2048 15.1 us against 24.3 with 64 x 64 tiles, 512 rows 29.5 against 16.5.
 constexpr int kFewRows = 256;
 
-// From this many rows times ranks on, with whole 16-byte rows and up to
-// kMaxSortedRank ranks, the rows are sorted by adapter (1024 -> 2048, 64 adapters,
-// bf16, us; runs of 1, 7 and 512 rows of one request):
-//                       sorted            in order
-//   8192 rows, rank 64  104, 101, 69      1270, 370, 102
-//   8192 rows, rank 16  87, 86, 62        225, 143, 82
-//   4096 rows, rank 64  76, 76, 49        585, 190, 57
-//   2048 rows, rank 64  71, 74, 45        257, 112, 36
-//   4096 rows, rank 16  73, 72, 47        110, 71, 43
-//   2048 rows, rank 32  67, 69, 43        100, 59, 29
-//   1024 rows, rank 64  74, 74, 43        184, 85, 27
+// From this many rows times ranks on, with a shared matrix, whole 16-byte rows and up
+// to kMaxSortedRank ranks, the rows are sorted by adapter (64 adapters, bf16, us;
+// runs of 1, 7, 512 and 700 rows of one request):
+//                                     sorted             in order
+//   8192 rows, 1024 -> 2048, rank 64  97, 106, 73, 96    1269, 374, 95, 98
+//   8192 rows, 1024 -> 2048, rank 16  78, 83, 62, 80     212, 133, 73, 75
+//   8192 rows, 2048 -> 1024, rank 64  91, 109, 81, 93    760, 249, 85, 93
+//   8192 rows, 512 -> 1024, rank 64   49, 52, 43, 48     403, 164, 40, 42
+//   4096 rows, 1024 -> 2048, rank 64  72, 78, 50, 57     578, 193, 55, 60
+//   2048 rows, 1024 -> 2048, rank 64  67, 72, 44, 50     260, 111, 35, 35
+//   2048 rows, 512 -> 1024, rank 64   34, 36, 32, 34     100, 78, 18, 19
+// and below it
+//   4096 rows, 1024 -> 2048, rank 16  65, 67, 45, 49     101, 68, 41, 43
+//   2048 rows, 1024 -> 2048, rank 32  63, 66, 42, 45     100, 59, 29, 29
+//   1024 rows, 1024 -> 2048, rank 64  66, 74, 43, 47     190, 86, 28, 29
+// Which order the rows come in is known on the device alone.  Near the limit the
+// wrong form costs up to 1.8 times the better one when sorted (long runs) and up
+// to three times in order (mixed rows).
 constexpr long long kSortedValues = 1 << 17;
 constexpr int kSortWaves = 16, kSortBins = 1024;
 
@@ -40,7 +47,9 @@ constexpr int kSortWaves = 16, kSortBins = 1024;
 // the bins of its stretch of rows, the counts are summed over bins and waves,
 // and every wave places its rows.  64 rows of one bin keep their order; rows of
 // a bin among mixed ones take their places as they come, which changes no
-// result: a row's sums do not depend on the rows beside it.
+// result: among sorted rows a row's sums do not depend on the rows beside it.
+// (One workgroup: mixed rows of 64 adapters take 6.4 us at 8192 rows of runs of 700, 12
+// with every row another's, 63 at 65536 and 224 at 262144.)
 __global__ __launch_bounds__(64 * kSortWaves) void adapter_sort_kernel(const int32_t *__restrict__ adapter, int rows, int adapters,
                                                                        int32_t *__restrict__ index, int32_t *__restrict__ sorted,
                                                                        int32_t *__restrict__ offsets)

@@ -14,13 +14,17 @@
 // workgroups share a CU and the loads' latency would show.  Tiles by the rules
 // above launch_direction; many 16-bit rows go to grouped_large.hip.
 //
-// What bounds it (MI355X): few rows, the matrices' bytes: 64 rows over 16
-// matrices of 2048 x 1024 in bf16 13.1 us, 67 MB at 5.1 TB/s, what a large copy
-// reaches.  fp32, the matrix cores: 2331 rows over 14 matrices of 1201 x 1000
-// 72 us per direction, 78 TFLOP/s of the 154 a large product reaches; a group's 166
-// rows fill 2.6 of its 3 row tiles and 1201 columns 18.8 of 19, and the
-// scattered LDS reads of fp32 operands with the tile's axis contiguous do the
-// rest.
+// What bounds it (MI355X): a decode batch, the matrices' bytes: 64 rows over 16
+// matrices of 2048 x 1024 in bf16 13.0 us, 67 MB at 5.1 TB/s, what a large copy
+// reaches.  Fewer row tiles than that leave XCDs idle, each tile's columns being
+// one XCD's: two rows of two matrices (8.4 MB, 1.6 us) take 8.4 us, ten of ten
+// (42 MB, 8.2 us) 13.5.  fp32, the matrix cores and the tiles' shares: 2331 rows over
+// 14 matrices of 1201 x 1000 83, 80 and 89 us (forward, input and weight
+// gradient), 63 to 70 TFLOP/s of the 154 a large product reaches.  By the
+// counters 28 % of the products are of ragged tiles' missing rows and columns,
+// the matrix cores are busy 82, 77 and 68 % of the time their CU has work, and CUs
+// have work for 72 to 81 % of the kernel: of 42 to 44 row tiles seven XCDs take six
+// each and the last what is left.
 //
 // Row groups are found on the device: the grid holds the most tiles the rows
 // can need, every wave scans the offsets for its tile, surplus workgroups end.
@@ -36,9 +40,10 @@ constexpr int SB = 128;                                   // bytes of reduction 
 constexpr int kCus = 256;
 
 // Tile of rows of block b (the hardware hands block b to XCD b % 8): XCD x
-// takes the x-th eighth of the row tiles in order, each with its `columns`
-// column tiles back to back, so that a group's matrix and a tile's rows are
-// fetched once per XCD.  False for the blocks past the last tile.
+// takes the x-th eighth of the row tiles (rounded up: the last XCDs may get less or
+// none) in order, each with its `columns` column tiles back to back, so that a
+// group's matrix and a tile's rows are fetched once per XCD.  False for the blocks
+// past the last tile.
 __device__ __forceinline__ bool find_row_tile(const GroupedArgs &a, int bm, int columns, int &g, int &p0, int &m,
                                               int &column)
 {
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
     uint32_t skip = 0;
     if constexpr (ADAPTED) {
         if (a.bias) add_bias<T>(acc, a.bias, tile_n + wn, a.outputs);
-        const uint32_t without = add_adapters<T, 1>(acc, a, tile_m + wm, tile_n + wn, tile_m + m);
+        const uint32_t without = add_adapters<T>(acc, a, tile_m + wm, tile_n + wn, tile_m + m);
         if (!a.b && !a.bias) skip = without;
     }
     if (DIR == kGroupedWeightGradient && a.out_f32)

@@ -11,19 +11,24 @@
 //
 // What bounds it (MI355X, bf16): a step's 64 KiB per CU on their way from L2
 // into LDS take about 1.5 us however few of the tile's rows exist, which is
-// about what the 256 x 256 tile's MFMAs take (kRowCost).  Long tiles reach 870 to
-// 1190 TFLOP/s (8 groups of 2048 x 2048, 16384 rows: weight gradient 131 us,
+// about what the 256 x 256 tile's MFMAs take (kRowCost).  Long tiles reach 880 to
+// 1050 TFLOP/s (8 groups of 2048 x 2048, 16384 rows: weight gradient 131 us,
 // forward 148, input gradient 156; a large library product 1010 to 1296), skewed
-// small groups 800 to 940 (fp16, 131072 rows over 128 matrices of 768 x 2048:
-// forward 440 us, input gradient 488, weight gradient 510).  The weight gradient
-// of short groups is bound by its results' bytes: 64 fp32 matrices of 2048 x 1024
-// from 16384 rows 175 us, 3.6 TB/s, the four steps of a tile and the stores of
-// its 256 KiB mostly one after the other, in all CUs at about the same time.
+// small groups 640 to 980 (fp16, 131072 rows over 128 matrices of 768 x 2048:
+// forward 421 us, input gradient 483, weight gradient 640).  A last round of tiles
+// that does not fill the chip costs as much as a full one: 16 groups of 1024 rows,
+// 2048 -> 1024, are 384 tiles for 256 CUs, 85 us in which a CU has work 65 % of the
+// time.  The weight gradient of short groups is bound by its results' bytes: 64 fp32
+// matrices of 2048 x 1024 from 16384 rows 174 us, 3.6 TB/s, the four steps of a
+// tile and the stores of its 256 KiB mostly one after the other, in all CUs at about
+// the same time.
 //
 // ADAPTED costs more than the product beside it (8192 rows of 1024 -> 2048 with
-// 12 adapters of rank 64, fp16, 76 us; the plain product 38): thirteen
-// groups' rows make some 400 tiles where 256 would do, two rounds of them, rows
-// are gathered, and two steps are added to sixteen.
+// 12 adapters of rank 64, fp16, 82 us; the plain product 38): thirteen
+// groups' rows make some 380 tiles where 256 would do, two rounds of them, rows
+// are gathered, and two steps are added to sixteen, whose MFMAs are five times (bf16:
+// three) a plain product's of as many ranks.  (With u in two fp16 parts 76 us, but
+// a rank far below the row's largest lost its bits.)
 //
 // Tiles: rows of a group by bm, every XCD an eighth of them in order (the
 // hardware hands block b to XCD b % 8), its blocks taking them in turn, so

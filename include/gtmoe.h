@@ -114,7 +114,8 @@ typedef struct gtmoe_rows {
  * on the context or its layers answers GTMOE_ERR_INVALID_ARGUMENT with "the
  * context is closed" in gtmoe_last_error, and gtmoe_layer_destroy still frees
  * a layer.  A closed context's own few hundred bytes stay allocated until
- * gtmoe_context_free. */
+ * gtmoe_context_free.  A call on a context makes its device the calling thread's
+ * current one, as hipSetDevice does, and leaves it so. */
 int32_t gtmoe_abi_version(void);
 int32_t gtmoe_device_count(int32_t *count);
 int32_t gtmoe_open(int32_t device, gtmoe_context **out);
@@ -447,7 +448,8 @@ int32_t gtmoe_backward(gtmoe_layer *layer, int32_t tokens, const double *output_
  * size.  A call of more work than one launch holds (2^24 tiles of 32 x 64
  * outputs, or with adapters 2^27 rows) is refused.  Outputs must not
  * overlap another buffer of the call (GTMOE_ERR_INVALID_ARGUMENT) unless the
- * entry point says so.  Sums are fp32; an output is rounded once.
+ * entry point says so.  Sums are fp32; an output is rounded once.  (A sum with a
+ * float16 factor below 2^-14 is held to 2^-38 of the other factor.)
  * ------------------------------------------------------------------------- */
 enum gtmoe_values { GTMOE_VALUES_FLOAT32 = 0, GTMOE_VALUES_BFLOAT16 = 1, GTMOE_VALUES_FLOAT16 = 2 };
 
