@@ -1008,3 +1008,30 @@ def test_adapted_ranks_of_unlike_sizes(ctx, kind, T, rank, pattern):
         # K terms of the shared sum; K, the scale and rank terms of the adapter's; bias and the two parts' sum
         bound = HALF_STEP[kind] * np.abs(ref) + HALF_LAST_STEP[kind] + (K + rank + 4) * 2.0 ** -24 * size
         assert np.all(np.abs(got - ref) <= bound * (1 + 2.0 ** -7))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T, rank", [(20, 8), (140, 8), (300, 24), (2100, 64), (8200, 16)])
+def test_adapted_infinities_of_a_row_stay_in_it(ctx, kind, T, rank):
+    """A row with an infinity, or whose Down product overflows fp32, is not finite;
+    the rows beside it, of the same adapter or another, are as without it."""
+    rng = np.random.default_rng(33)
+    K, N, n = 72, 40, 4
+    sparse = lambda *s: whole(rng, *s, top=1) * (rng.random(s) < 0.25)
+    x, w = whole(rng, T, K, top=1), whole(rng, N, K)
+    down, up, scales = sparse(n, rank, K), sparse(n, N, rank), np.ones(n)
+    down[:, :, 5] = up[:, :, 0] = 1.0
+    scales[3] = 2.0 ** 125
+    x[:, 5] = 0.0
+    adapter = np.where(np.arange(T) % 4 == 3, -1, np.arange(T) % 3)
+    base = whole(rng, T, N)
+    say(f"infinities {kind} T={T} rank={rank}")
+    for ww, start in ((w, None), (None, base)):
+        clean = run_adapted(ctx, kind, x, ww, None, adapter, down, up, scales, base=start)
+        bad, a = x.copy(), adapter.copy()
+        bad[4, 5], bad[9, 5] = np.inf, -np.inf
+        a[10], bad[10, 5] = 3, 4096.0  # 2^125 4096
+        got = run_adapted(ctx, kind, bad, ww, None, a, down, up, scales, base=start)
+        keep = ~np.isin(np.arange(T), [4, 9, 10])
+        assert np.array_equal(got[keep], clean[keep])
+        assert not np.any(np.isfinite(got[[4, 9, 10]]))
