@@ -21,6 +21,9 @@ FLOAT64, FLOAT32, INT8, FP4 = 0, 1, 2, 3
 PATH_AUTO, PATH_FP32, PATH_BF16 = 0, 1, 2
 KERNEL_GATEUP, KERNEL_DOWN = 0, 1
 VALUES_FLOAT32, VALUES_BFLOAT16, VALUES_FLOAT16 = 0, 1, 2
+CODES_NONE, CODES_INT8, CODES_E4M3 = 0, 1, 2
+ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_SILU, ACTIVATION_GELU, ACTIVATION_GELU_TANH = range(5)
+SCORES_SOFTMAX, SCORES_SIGMOID = 0, 1
 
 ROLE_ROUTER = 0
 ROLES = {("shared", "gate"): 1, ("shared", "up"): 2, ("shared", "down"): 3,
@@ -44,6 +47,10 @@ EXPORTED = [
     "gtmoe_layer_zero_adapter_gradients", "gtmoe_backward", "gtmoe_layer_set_adapter_dropout",
     "gtmoe_grouped_forward", "gtmoe_grouped_input_gradient", "gtmoe_grouped_weight_gradient",
     "gtmoe_adapted_workspace", "gtmoe_adapted_forward", "gtmoe_dropout",
+    "gtmoe_pack_rows", "gtmoe_unpack_rows", "gtmoe_norm_forward", "gtmoe_norm_workspace", "gtmoe_norm_gradient",
+    "gtmoe_activation_forward", "gtmoe_activation_gradient", "gtmoe_grouped_fused_forward",
+    "gtmoe_grouped_bias_workspace", "gtmoe_grouped_bias_gradient",
+    "gtmoe_route_workspace", "gtmoe_route_forward", "gtmoe_route_gradient",
 ]
 
 
@@ -84,6 +91,39 @@ class AdaptedDesc(C.Structure):
 class DropoutDesc(C.Structure):
     _fields_ = [("values", C.c_int32), ("rows", C.c_int32), ("columns", C.c_int32), ("reserved", C.c_int32),
                 ("input_stride", C.c_int64), ("base_stride", C.c_int64), ("output_stride", C.c_int64)]
+
+
+class PackedDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("rows", C.c_int32), ("columns", C.c_int32), ("codes", C.c_int32),
+                ("scale_columns", C.c_int32), ("reserved", C.c_int32), ("value_stride", C.c_int64),
+                ("code_stride", C.c_int64), ("scale_stride", C.c_int64)]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("rows", C.c_int32), ("columns", C.c_int32), ("codes", C.c_int32),
+                ("scale_columns", C.c_int32), ("reserved", C.c_int32), ("epsilon", C.c_double),
+                ("input_stride", C.c_int64), ("residual_stride", C.c_int64), ("sum_stride", C.c_int64),
+                ("output_stride", C.c_int64), ("code_stride", C.c_int64), ("scale_stride", C.c_int64)]
+
+
+class ActivationDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("rows", C.c_int32), ("columns", C.c_int32), ("activation", C.c_int32),
+                ("codes", C.c_int32), ("scale_columns", C.c_int32), ("limit", C.c_double), ("gate_stride", C.c_int64),
+                ("up_stride", C.c_int64), ("output_stride", C.c_int64), ("code_stride", C.c_int64),
+                ("scale_stride", C.c_int64)]
+
+
+class Epilogue(C.Structure):
+    _fields_ = [("activation", C.c_int32), ("reserved", C.c_int32), ("biases", C.c_void_p), ("factors", C.c_void_p),
+                ("residuals", C.c_void_p), ("products", C.c_void_p), ("bias_stride", C.c_int64),
+                ("factor_stride", C.c_int64), ("residual_stride", C.c_int64), ("product_stride", C.c_int64)]
+
+
+class RouteDesc(C.Structure):
+    _fields_ = [("values", C.c_int32), ("tokens", C.c_int32), ("experts", C.c_int32), ("experts_per_token", C.c_int32),
+                ("expert_groups", C.c_int32), ("chosen_groups", C.c_int32), ("group_best", C.c_int32),
+                ("scores", C.c_int32), ("renormalize", C.c_int32), ("reserved", C.c_int32), ("scale", C.c_double),
+                ("logit_stride", C.c_int64)]
 
 
 _lib = None
@@ -159,6 +199,19 @@ def library():
         "gtmoe_adapted_workspace": ([P, P], i32),
         "gtmoe_adapted_forward": ([P, P, P, P, P, P, P, P, P, P, P, C.c_size_t, P], i32),
         "gtmoe_dropout": ([P, P, P, P, P, dbl, C.c_uint64, C.c_uint64, P], i32),
+        "gtmoe_pack_rows": ([P] * 6, i32),
+        "gtmoe_unpack_rows": ([P] * 6, i32),
+        "gtmoe_norm_forward": ([P] * 10, i32),
+        "gtmoe_norm_workspace": ([P, P], i32),
+        "gtmoe_norm_gradient": ([P, P, P, P, P, P, P, P, i32, i32, P, C.c_size_t, P], i32),
+        "gtmoe_activation_forward": ([P] * 10, i32),
+        "gtmoe_activation_gradient": ([P] * 11, i32),
+        "gtmoe_grouped_fused_forward": ([P] * 8, i32),
+        "gtmoe_grouped_bias_workspace": ([P, P], i32),
+        "gtmoe_grouped_bias_gradient": ([P, P, P, P, P, i32, i32, P, C.c_size_t, P], i32),
+        "gtmoe_route_workspace": ([P, P], i32),
+        "gtmoe_route_forward": ([P, P, P, P, P, P, P, P, P, P, C.c_size_t, P], i32),
+        "gtmoe_route_gradient": ([P] * 7, i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -659,6 +712,151 @@ def dropout(ctx, desc, inputs_ptr, base_ptr, outputs_ptr, rate, seed, offset, st
     gradients is the backward."""
     ctx.check(library().gtmoe_dropout(ctx.handle, C.byref(desc), inputs_ptr, base_ptr, outputs_ptr, float(rate),
                                       int(seed), int(offset), stream))
+
+
+# --------------------------------------------------------------------------
+# a block in plain rows (raw device addresses)
+# --------------------------------------------------------------------------
+
+def _scales_per_row(columns, scale_columns):
+    return -(-columns // scale_columns) if scale_columns else 1
+
+
+def packed_desc(values, rows, columns, codes, scale_columns=128, value_stride=None, code_stride=None, scale_stride=None):
+    """gtmoe_packed_desc; strides in values, codes and scales, contiguous unless given."""
+    return PackedDesc(values, rows, columns, codes, scale_columns, 0, columns if value_stride is None else value_stride,
+                      columns if code_stride is None else code_stride,
+                      _scales_per_row(columns, scale_columns) if scale_stride is None else scale_stride)
+
+
+def pack_rows(ctx, desc, inputs_ptr, codes_ptr, scales_ptr, stream=None):
+    """Rows into 8-bit codes with scales (gtmoe_pack_rows)."""
+    ctx.check(library().gtmoe_pack_rows(ctx.handle, C.byref(desc), inputs_ptr, codes_ptr, scales_ptr, stream))
+
+
+def unpack_rows(ctx, desc, codes_ptr, scales_ptr, outputs_ptr, stream=None):
+    """outputs = code * scale (gtmoe_unpack_rows)."""
+    ctx.check(library().gtmoe_unpack_rows(ctx.handle, C.byref(desc), codes_ptr, scales_ptr, outputs_ptr, stream))
+
+
+def norm_desc(values, rows, columns, epsilon=1e-6, codes=CODES_NONE, scale_columns=None, input_stride=None,
+              residual_stride=None, sum_stride=None, output_stride=None, code_stride=None, scale_stride=None):
+    """gtmoe_norm_desc; strides contiguous unless given, 128 columns per scale with codes."""
+    if scale_columns is None:
+        scale_columns = 128 if codes else 0
+    strides = [columns if v is None else v for v in (input_stride, residual_stride, sum_stride, output_stride, code_stride)]
+    return NormDesc(values, rows, columns, codes, scale_columns, 0, float(epsilon), *strides,
+                    _scales_per_row(columns, scale_columns) if scale_stride is None else scale_stride)
+
+
+def norm_forward(ctx, desc, inputs_ptr, residuals_ptr, weights_ptr, sums_ptr, outputs_ptr, codes_ptr=None,
+                 scales_ptr=None, stream=None):
+    """sums = inputs + residuals, outputs and codes their RMS norm times weights (gtmoe_norm_forward)."""
+    ctx.check(library().gtmoe_norm_forward(ctx.handle, C.byref(desc), inputs_ptr, residuals_ptr, weights_ptr, sums_ptr,
+                                           outputs_ptr, codes_ptr, scales_ptr, stream))
+
+
+def norm_workspace_bytes(desc):
+    """Bytes of the workspace norm_gradient needs for weight gradients."""
+    n = C.c_size_t(0)
+    _check(library().gtmoe_norm_workspace(C.byref(desc), C.byref(n)))
+    return n.value
+
+
+def norm_gradient(ctx, desc, output_gradients_ptr, sums_ptr, weights_ptr, sum_gradients_ptr, input_gradients_ptr,
+                  weight_gradients_ptr, gradient_values, accumulate=False, workspace_ptr=None, stream=None,
+                  workspace_bytes=None):
+    """The gradients of inputs and weights (gtmoe_norm_gradient).
+    workspace_bytes: the workspace's size, norm_workspace_bytes(desc) unless given."""
+    n = norm_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    ctx.check(library().gtmoe_norm_gradient(ctx.handle, C.byref(desc), output_gradients_ptr, sums_ptr, weights_ptr,
+                                            sum_gradients_ptr, input_gradients_ptr, weight_gradients_ptr, gradient_values,
+                                            1 if accumulate else 0, workspace_ptr, n, stream))
+
+
+def activation_desc(values, rows, columns, activation, limit=0.0, codes=CODES_NONE, scale_columns=None, gate_stride=None,
+                    up_stride=None, output_stride=None, code_stride=None, scale_stride=None):
+    """gtmoe_activation_desc; strides contiguous unless given, 128 columns per scale with codes."""
+    if scale_columns is None:
+        scale_columns = 128 if codes else 0
+    strides = [columns if v is None else v for v in (gate_stride, up_stride, output_stride, code_stride)]
+    return ActivationDesc(values, rows, columns, activation, codes, scale_columns, float(limit), *strides,
+                          _scales_per_row(columns, scale_columns) if scale_stride is None else scale_stride)
+
+
+def activation_forward(ctx, desc, gates_ptr, ups_ptr, outputs_ptr, gate_codes_ptr=None, gate_scales_ptr=None,
+                       up_codes_ptr=None, up_scales_ptr=None, stream=None):
+    """outputs = act(gates) * ups, both kept in 8 bits where the description has codes (gtmoe_activation_forward)."""
+    ctx.check(library().gtmoe_activation_forward(ctx.handle, C.byref(desc), gates_ptr, ups_ptr, outputs_ptr, gate_codes_ptr,
+                                                 gate_scales_ptr, up_codes_ptr, up_scales_ptr, stream))
+
+
+def activation_gradient(ctx, desc, output_gradients_ptr, gates_ptr, gate_scales_ptr, ups_ptr, up_scales_ptr,
+                        gate_gradients_ptr, up_gradients_ptr, outputs_ptr=None, stream=None):
+    """The gradients of gates and ups, from values or from what was kept, and the outputs
+    again (gtmoe_activation_gradient)."""
+    ctx.check(library().gtmoe_activation_gradient(ctx.handle, C.byref(desc), output_gradients_ptr, gates_ptr,
+                                                  gate_scales_ptr, ups_ptr, up_scales_ptr, gate_gradients_ptr,
+                                                  up_gradients_ptr, outputs_ptr, stream))
+
+
+def epilogue(activation=ACTIVATION_NONE, biases_ptr=None, factors_ptr=None, residuals_ptr=None, products_ptr=None, width=0,
+             bias_stride=None, factor_stride=None, residual_stride=None, product_stride=None):
+    """gtmoe_epilogue; strides `width` (the product's outputs) unless given."""
+    strides = [width if v is None else v for v in (bias_stride, factor_stride, residual_stride, product_stride)]
+    return Epilogue(activation, 0, biases_ptr, factors_ptr, residuals_ptr, products_ptr, *strides)
+
+
+def grouped_fused_forward(ctx, desc, epilogue, offsets_ptr, inputs_ptr, weights_ptr, outputs_ptr, stream=None):
+    """outputs[r] = act(W_g inputs[r] + b_g) * factors[r] + residuals[r] (gtmoe_grouped_fused_forward)."""
+    ctx.check(library().gtmoe_grouped_fused_forward(ctx.handle, C.byref(desc), C.byref(epilogue), offsets_ptr, inputs_ptr,
+                                                    weights_ptr, outputs_ptr, stream))
+
+
+def grouped_bias_workspace_bytes(desc):
+    """Bytes of the workspace grouped_bias_gradient needs."""
+    n = C.c_size_t(0)
+    _check(library().gtmoe_grouped_bias_workspace(C.byref(desc), C.byref(n)))
+    return n.value
+
+
+def grouped_bias_gradient(ctx, desc, offsets_ptr, output_gradients_ptr, bias_gradients_ptr, gradient_values,
+                          accumulate=False, workspace_ptr=None, stream=None, workspace_bytes=None):
+    """bias_gradients[g] (+)= sum of output_gradients[r] over the group's rows.
+    workspace_bytes: the workspace's size, grouped_bias_workspace_bytes(desc) unless given."""
+    n = grouped_bias_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    ctx.check(library().gtmoe_grouped_bias_gradient(ctx.handle, C.byref(desc), offsets_ptr, output_gradients_ptr,
+                                                    bias_gradients_ptr, gradient_values, 1 if accumulate else 0,
+                                                    workspace_ptr, n, stream))
+
+
+def route_desc(values, tokens, experts, experts_per_token, expert_groups=1, chosen_groups=1, group_best=1,
+               scores=SCORES_SOFTMAX, renormalize=True, scale=1.0, logit_stride=None):
+    """gtmoe_route_desc; logit rows contiguous unless given."""
+    return RouteDesc(values, tokens, experts, experts_per_token, expert_groups, chosen_groups, group_best, scores,
+                     1 if renormalize else 0, 0, float(scale), experts if logit_stride is None else logit_stride)
+
+
+def route_workspace_bytes(desc):
+    """Bytes of the workspace route_forward needs for the rows in expert order."""
+    n = C.c_size_t(0)
+    _check(library().gtmoe_route_workspace(C.byref(desc), C.byref(n)))
+    return n.value
+
+
+def route_forward(ctx, desc, logits_ptr, biases_ptr, chosen_ptr, gates_ptr, expert_offsets_ptr=None,
+                  rows_for_expert_ptr=None, places_ptr=None, workspace_ptr=None, stream=None, workspace_bytes=None):
+    """Every token's experts and gates, and the rows in expert order (gtmoe_route_forward).
+    workspace_bytes: the workspace's size, route_workspace_bytes(desc) unless given."""
+    n = route_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    ctx.check(library().gtmoe_route_forward(ctx.handle, C.byref(desc), logits_ptr, biases_ptr, chosen_ptr, gates_ptr,
+                                            expert_offsets_ptr, rows_for_expert_ptr, places_ptr, workspace_ptr, n, stream))
+
+
+def route_gradient(ctx, desc, logits_ptr, chosen_ptr, gate_gradients_ptr, logit_gradients_ptr, stream=None):
+    """The logits' gradients from the gates' (gtmoe_route_gradient)."""
+    ctx.check(library().gtmoe_route_gradient(ctx.handle, C.byref(desc), logits_ptr, chosen_ptr, gate_gradients_ptr,
+                                             logit_gradients_ptr, stream))
 
 
 # --------------------------------------------------------------------------

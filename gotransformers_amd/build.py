@@ -27,8 +27,12 @@ SOURCES = [
     ("lora.hip", []),
     ("grouped.hip", []),
     ("grouped_large.hip", []),
+    ("grouped_few.hip", []),
     ("adapted.hip", []),
     ("dropout.hip", []),
+    ("norm.hip", []),
+    ("packed.hip", []),
+    ("choose.hip", []),
     ("api.cpp", []),
     ("encode.cpp", ["-ffp-contract=off"]),
     ("weightfile.cpp", []),

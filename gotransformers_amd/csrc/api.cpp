@@ -3415,3 +3415,714 @@ int32_t gtmoe_dropout(gtmoe_context *ctx, const gtmoe_dropout_desc *desc, const 
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// A block in plain rows.
+// ---------------------------------------------------------------------------
+
+namespace {
+
+constexpr int kMostRouted = 1 << 24;
+
+int32_t check_reserved(gtmoe_context *ctx, int32_t reserved)
+{
+    if (reserved != 0) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "reserved must be 0");
+    return GTMOE_OK;
+}
+
+int64_t scales_of(int32_t columns, int32_t scale_columns)
+{
+    return scale_columns ? ((int64_t)columns + scale_columns - 1) / scale_columns : 1;
+}
+
+// Codes of rows, and the rows of codes and scales.  whole_rows: one scale per row is offered.
+int32_t check_codes(gtmoe_context *ctx, int32_t codes, int32_t columns, int32_t scale_columns, bool whole_rows,
+                    int64_t code_stride, int64_t scale_stride)
+{
+    if (codes != GTMOE_CODES_INT8 && codes != GTMOE_CODES_E4M3)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "unknown type of codes %d", codes);
+    if (!(scale_columns == 16 || scale_columns == 32 || scale_columns == 64 || scale_columns == 128 ||
+          (whole_rows && scale_columns == 0)))
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "scale columns must be %s16, 32, 64 or 128, got %d",
+                    whole_rows ? "0, " : "", scale_columns);
+    TRY(check_stride(ctx, "code", code_stride, columns));
+    return check_stride(ctx, "scale", scale_stride, scales_of(columns, scale_columns));
+}
+
+Span codes_span(const void *p, int64_t rows, int64_t columns, int64_t stride) { return {p, rows, columns, stride}; }
+Span scales_span(const void *p, int64_t rows, int32_t columns, int32_t scale_columns, int64_t stride)
+{
+    return rows_span(p, rows, scales_of(columns, scale_columns), stride, 4);
+}
+
+// An output apart from the buffers of the call, or the very rows of one that may be
+// written over (same address and stride).
+struct Shared {
+    Span span;
+    bool may;
+};
+int32_t check_output(gtmoe_context *ctx, const char *what, const Span &out, std::initializer_list<Shared> others)
+{
+    for (const Shared &o : others) {
+        if (o.may && o.span.p == out.p && o.span.stride == out.stride) continue;
+        if (overlap(out, o.span)) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s overlap another buffer of the call", what);
+    }
+    return GTMOE_OK;
+}
+
+int32_t check_workspace(gtmoe_context *ctx, const void *workspace, size_t have, size_t need)
+{
+    if (need == 0) return GTMOE_OK;
+    TRY(check_pointer(ctx, "workspace bytes", workspace, 16));
+    if (have < need)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the workspace has %zu bytes but the call needs %zu", have, need);
+    return GTMOE_OK;
+}
+
+int32_t check_gradient_values(gtmoe_context *ctx, const char *what, int32_t gradient_values, int32_t values)
+{
+    if (gradient_values != values && gradient_values != GTMOE_VALUES_FLOAT32)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%s are of the values' type or float32, got %d", what, gradient_values);
+    return GTMOE_OK;
+}
+
+int32_t check_packed(gtmoe_context *ctx, const gtmoe_packed_desc *d)
+{
+    if (!d) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+    TRY(check_values(ctx, d->values));
+    TRY(check_size(ctx, "rows", d->rows, 0, kMaxPlainRows));
+    TRY(check_size(ctx, "columns", d->columns, 1, kMaxPlainWidth));
+    TRY(check_reserved(ctx, d->reserved));
+    TRY(check_codes(ctx, d->codes, d->columns, d->scale_columns, true, d->code_stride, d->scale_stride));
+    return check_stride(ctx, "value", d->value_stride, d->columns);
+}
+
+PackArgs pack_args(const gtmoe_packed_desc *d, const void *codes, const float *scales)
+{
+    PackArgs a;
+    a.ldx = d->value_stride;
+    a.rows = d->rows;
+    a.columns = d->columns;
+    a.kept.codes = (uint8_t *)codes;
+    a.kept.scales = (float *)scales;
+    a.kept.ldcodes = d->code_stride;
+    a.kept.ldscales = d->scale_stride;
+    a.kept.code_type = d->codes;
+    a.kept.scale_columns = d->scale_columns;
+    return a;
+}
+
+int32_t check_norm(gtmoe_context *ctx, const gtmoe_norm_desc *d)
+{
+    if (!d) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+    TRY(check_values(ctx, d->values));
+    TRY(check_size(ctx, "rows", d->rows, 0, kMaxPlainRows));
+    TRY(check_size(ctx, "columns", d->columns, 1, kMaxPlainWidth));
+    TRY(check_reserved(ctx, d->reserved));
+    if (!(d->epsilon >= 0.0 && d->epsilon <= 1e30))
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "epsilon must be at least 0 and at most 1e30, got %g", d->epsilon);
+    if (d->codes != GTMOE_CODES_NONE)
+        TRY(check_codes(ctx, d->codes, d->columns, d->scale_columns, true, d->code_stride, d->scale_stride));
+    return GTMOE_OK;
+}
+
+int32_t check_activation(gtmoe_context *ctx, int32_t activation)
+{
+    if (activation < GTMOE_ACTIVATION_NONE || activation > GTMOE_ACTIVATION_GELU_TANH)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "unknown activation %d", activation);
+    return GTMOE_OK;
+}
+
+int32_t check_activation_desc(gtmoe_context *ctx, const gtmoe_activation_desc *d)
+{
+    if (!d) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+    TRY(check_values(ctx, d->values));
+    TRY(check_size(ctx, "rows", d->rows, 0, kMaxPlainRows));
+    TRY(check_size(ctx, "columns", d->columns, 1, kMaxPlainWidth));
+    TRY(check_activation(ctx, d->activation));
+    if (!(d->limit == 0.0 || (d->limit > 0.0 && (float)d->limit > 0.f)))
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the limit must be 0 (none) or a positive float32, got %g", d->limit);
+    if (d->codes != GTMOE_CODES_NONE)
+        return check_codes(ctx, d->codes, d->columns, d->scale_columns, false, d->code_stride, d->scale_stride);
+    return GTMOE_OK;
+}
+
+ActivationArgs activation_args(const gtmoe_activation_desc *d)
+{
+    ActivationArgs a;
+    a.rows = d->rows;
+    a.columns = d->columns;
+    a.activation = d->activation;
+    a.limit = d->limit > 0.0 ? (float)d->limit : INFINITY;
+    a.ldgate = a.lddgate = d->gate_stride;
+    a.ldup = a.lddup = d->up_stride;
+    a.ldo = a.lddy = d->output_stride;
+    return a;
+}
+
+PackedRows kept_rows(const gtmoe_activation_desc *d, const void *codes, const float *scales)
+{
+    PackedRows k;
+    k.codes = (uint8_t *)codes;
+    k.scales = (float *)scales;
+    k.ldcodes = d->code_stride;
+    k.ldscales = d->scale_stride;
+    k.code_type = d->codes;
+    k.scale_columns = d->scale_columns;
+    return k;
+}
+
+int32_t check_route(gtmoe_context *ctx, const gtmoe_route_desc *d)
+{
+    if (!d) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the description is null");
+    TRY(check_values(ctx, d->values));
+    TRY(check_size(ctx, "tokens", d->tokens, 0, kMostRouted));
+    TRY(check_size(ctx, "experts", d->experts, 1, 1024));
+    TRY(check_size(ctx, "expert groups", d->expert_groups, 1, 64));
+    if (d->experts % d->expert_groups != 0)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "%d experts are not whole in %d groups", d->experts, d->expert_groups);
+    TRY(check_size(ctx, "chosen groups", d->chosen_groups, 1, d->expert_groups));
+    TRY(check_size(ctx, "experts per token", d->experts_per_token, 1,
+                   std::min(32, d->experts / d->expert_groups * d->chosen_groups)));
+    TRY(check_size(ctx, "a group's best", d->group_best, 1, 2));
+    if (d->scores != GTMOE_SCORES_SOFTMAX && d->scores != GTMOE_SCORES_SIGMOID)
+        return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "unknown scores %d", d->scores);
+    TRY(check_reserved(ctx, d->reserved));
+    if (!std::isfinite((float)d->scale)) return fail(ctx, GTMOE_ERR_INVALID_ARGUMENT, "the scale is not finite");
+    return check_stride(ctx, "logit", d->logit_stride, d->experts);
+}
+
+// Offsets, which one group of all rows does without.
+int32_t check_grouped_or_whole(gtmoe_context *ctx, const gtmoe_grouped_desc *d, const int32_t *offsets)
+{
+    static const int32_t whole[2] = {0, 0};
+    return check_grouped(ctx, d, d && d->groups == 1 && !offsets ? whole : offsets);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t gtmoe_pack_rows(gtmoe_context *ctx, const gtmoe_packed_desc *desc, const void *inputs, void *codes, float *scales,
+                        void *stream)
+{
+    PackArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_packed(c, desc));
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "inputs", inputs, value_bytes(desc->values)));
+            TRY(check_pointer(c, "codes", codes, 1));
+            TRY(check_pointer(c, "scales", scales, 4));
+        }
+        const Span x = rows_span(inputs, desc->rows, desc->columns, desc->value_stride, value_bytes(desc->values));
+        const Span q = codes_span(codes, desc->rows, desc->columns, desc->code_stride);
+        const Span k = scales_span(scales, desc->rows, desc->columns, desc->scale_columns, desc->scale_stride);
+        TRY(check_apart(c, "codes", q, {x, k}));
+        TRY(check_apart(c, "scales", k, {x}));
+        a = pack_args(desc, codes, scales);
+        a.x = inputs;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "pack_rows", [&] { return launch_pack(a, desc->values, s); });
+}
+
+int32_t gtmoe_unpack_rows(gtmoe_context *ctx, const gtmoe_packed_desc *desc, const void *codes, const float *scales,
+                          void *outputs, void *stream)
+{
+    PackArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_packed(c, desc));
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "codes", codes, 1));
+            TRY(check_pointer(c, "scales", scales, 4));
+            TRY(check_pointer(c, "outputs", outputs, value_bytes(desc->values)));
+        }
+        TRY(check_apart(c, "outputs",
+                        rows_span(outputs, desc->rows, desc->columns, desc->value_stride, value_bytes(desc->values)),
+                        {codes_span(codes, desc->rows, desc->columns, desc->code_stride),
+                         scales_span(scales, desc->rows, desc->columns, desc->scale_columns, desc->scale_stride)}));
+        a = pack_args(desc, codes, scales);
+        a.out = outputs;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "unpack_rows", [&] { return launch_unpack(a, desc->values, s); });
+}
+
+int32_t gtmoe_norm_forward(gtmoe_context *ctx, const gtmoe_norm_desc *desc, const void *inputs, const void *residuals,
+                           const void *weights, void *sums, void *outputs, void *codes, float *scales, void *stream)
+{
+    NormArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_norm(c, desc));
+        const int es = value_bytes(desc->values);
+        const bool coded = desc->codes != GTMOE_CODES_NONE;
+        TRY(check_stride(c, "input", desc->input_stride, desc->columns));
+        if (residuals) TRY(check_stride(c, "residual", desc->residual_stride, desc->columns));
+        if (sums) TRY(check_stride(c, "sum", desc->sum_stride, desc->columns));
+        if (outputs) TRY(check_stride(c, "output", desc->output_stride, desc->columns));
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "inputs", inputs, es));
+            if (residuals) {
+                TRY(check_pointer(c, "residuals", residuals, es));
+                if (!sums) return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "sums are null, but there are residuals");
+            }
+            if (weights) TRY(check_pointer(c, "weights", weights, es));
+            if (sums) TRY(check_pointer(c, "sums", sums, es));
+            if (outputs || !coded) TRY(check_pointer(c, "outputs", outputs, es));
+            if (coded) {
+                TRY(check_pointer(c, "codes", codes, 1));
+                TRY(check_pointer(c, "scales", scales, 4));
+            }
+        }
+        const int64_t n = desc->rows, w = desc->columns;
+        const Span x = rows_span(inputs, n, w, desc->input_stride, es), r = rows_span(residuals, n, w, desc->residual_stride, es);
+        const Span s = rows_span(sums, n, w, desc->sum_stride, es), y = rows_span(outputs, n, w, desc->output_stride, es);
+        const Span wt{weights, 1, w * es, w * es};
+        const Span q = codes_span(coded ? codes : nullptr, n, w, desc->code_stride);
+        const Span k = scales_span(coded ? scales : nullptr, n, desc->columns, desc->scale_columns, desc->scale_stride);
+        TRY(check_output(c, "sums", s, {{x, true}, {r, true}, {wt, false}}));
+        TRY(check_apart(c, "outputs", y, {x, r, s, wt}));
+        TRY(check_apart(c, "codes", q, {x, r, s, y, wt}));
+        TRY(check_apart(c, "scales", k, {x, r, s, y, wt, q}));
+        a.x = inputs;
+        a.residual = residuals;
+        a.w = weights;
+        a.sums = sums;
+        a.out = outputs;
+        a.ldx = desc->input_stride;
+        a.ldresidual = desc->residual_stride;
+        a.ldsums = desc->sum_stride;
+        a.ldo = desc->output_stride;
+        a.rows = desc->rows;
+        a.columns = desc->columns;
+        a.epsilon = desc->epsilon;
+        if (coded) {
+            a.codes = (uint8_t *)codes;
+            a.scales = scales;
+            a.ldcodes = desc->code_stride;
+            a.ldscales = desc->scale_stride;
+            a.code_type = desc->codes;
+            a.scale_columns = desc->scale_columns;
+        }
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "norm_forward", [&] { return launch_norm_forward(a, desc->values, s); });
+}
+
+int32_t gtmoe_norm_workspace(const gtmoe_norm_desc *desc, size_t *bytes)
+{
+    if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
+    TRY(check_norm(nullptr, desc));
+    *bytes = norm_gradient_floats(desc->rows, desc->columns) * 4;
+    return GTMOE_OK;
+}
+
+int32_t gtmoe_norm_gradient(gtmoe_context *ctx, const gtmoe_norm_desc *desc, const void *output_gradients, const void *sums,
+                            const void *weights, const void *sum_gradients, void *input_gradients, void *weight_gradients,
+                            int32_t gradient_values, int32_t accumulate, void *workspace, size_t workspace_bytes, void *stream)
+{
+    NormGradientArgs a;
+    AddPartialsArgs into;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_norm(c, desc));
+        const int es = value_bytes(desc->values);
+        TRY(check_stride(c, "output", desc->output_stride, desc->columns));
+        TRY(check_stride(c, "sum", desc->sum_stride, desc->columns));
+        TRY(check_stride(c, "input", desc->input_stride, desc->columns));
+        int gs = 4;
+        size_t need = 0;
+        if (weight_gradients) {
+            TRY(check_gradient_values(c, "weight gradients", gradient_values, desc->values));
+            gs = value_bytes(gradient_values);
+            TRY(check_pointer(c, "weight gradients", weight_gradients, gs));
+            need = norm_gradient_floats(desc->rows, desc->columns) * 4;
+            TRY(check_workspace(c, workspace, workspace_bytes, need));
+        }
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "output gradients", output_gradients, es));
+            TRY(check_pointer(c, "sums", sums, es));
+            if (weights) TRY(check_pointer(c, "weights", weights, es));
+            if (sum_gradients) TRY(check_pointer(c, "sum gradients", sum_gradients, es));
+            TRY(check_pointer(c, "input gradients", input_gradients, es));
+        }
+        const int64_t n = desc->rows, w = desc->columns;
+        const Span dy = rows_span(output_gradients, n, w, desc->output_stride, es), s = rows_span(sums, n, w, desc->sum_stride, es);
+        const Span ds = rows_span(sum_gradients, n, w, desc->sum_stride, es), dx = rows_span(input_gradients, n, w, desc->input_stride, es);
+        const Span wt{weights, 1, w * es, w * es}, dw{weight_gradients, 1, w * gs, w * gs};
+        const Span ws{need ? workspace : nullptr, 1, (int64_t)need, 0};
+        TRY(check_output(c, "input gradients", dx, {{dy, false}, {s, false}, {ds, true}, {wt, false}}));
+        TRY(check_apart(c, "weight gradients", dw, {dy, s, ds, dx, wt}));
+        TRY(check_apart(c, "the workspace's bytes", ws, {dy, s, ds, dx, wt, dw}));
+        a.dy = output_gradients;
+        a.s = sums;
+        a.w = weights;
+        a.ds = sum_gradients;
+        a.dx = input_gradients;
+        a.lddy = desc->output_stride;
+        a.lds = a.ldds = desc->sum_stride;
+        a.lddx = desc->input_stride;
+        a.rows = desc->rows;
+        a.columns = desc->columns;
+        a.epsilon = desc->epsilon;
+        into.out = weight_gradients;
+        into.out_f32 = gradient_values == GTMOE_VALUES_FLOAT32;
+        into.accumulate = accumulate != 0;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0 && !weight_gradients) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "norm_gradient", [&] { return launch_norm_gradient(a, (float *)workspace, into, desc->values, s); });
+}
+
+int32_t gtmoe_activation_forward(gtmoe_context *ctx, const gtmoe_activation_desc *desc, const void *gates, const void *ups,
+                                 void *outputs, void *gate_codes, float *gate_scales, void *up_codes, float *up_scales,
+                                 void *stream)
+{
+    ActivationArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_activation_desc(c, desc));
+        const int es = value_bytes(desc->values);
+        const bool coded = desc->codes != GTMOE_CODES_NONE;
+        TRY(check_stride(c, "gate", desc->gate_stride, desc->columns));
+        if (ups) TRY(check_stride(c, "up", desc->up_stride, desc->columns));
+        TRY(check_stride(c, "output", desc->output_stride, desc->columns));
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "gates", gates, es));
+            if (ups) TRY(check_pointer(c, "ups", ups, es));
+            TRY(check_pointer(c, "outputs", outputs, es));
+            if (coded) {
+                TRY(check_pointer(c, "gate codes", gate_codes, 1));
+                TRY(check_pointer(c, "gate scales", gate_scales, 4));
+                if (ups) {
+                    TRY(check_pointer(c, "up codes", up_codes, 1));
+                    TRY(check_pointer(c, "up scales", up_scales, 4));
+                }
+            }
+        }
+        const int64_t n = desc->rows, w = desc->columns;
+        const bool both = coded && ups;
+        const Span g = rows_span(gates, n, w, desc->gate_stride, es), u = rows_span(ups, n, w, desc->up_stride, es);
+        const Span y = rows_span(outputs, n, w, desc->output_stride, es);
+        const Span gq = codes_span(coded ? gate_codes : nullptr, n, w, desc->code_stride);
+        const Span uq = codes_span(both ? up_codes : nullptr, n, w, desc->code_stride);
+        const Span gk = scales_span(coded ? gate_scales : nullptr, n, desc->columns, desc->scale_columns, desc->scale_stride);
+        const Span uk = scales_span(both ? up_scales : nullptr, n, desc->columns, desc->scale_columns, desc->scale_stride);
+        TRY(check_output(c, "outputs", y, {{g, true}, {u, true}}));
+        TRY(check_apart(c, "gate codes", gq, {g, u, y}));
+        TRY(check_apart(c, "up codes", uq, {g, u, y, gq}));
+        TRY(check_apart(c, "gate scales", gk, {g, u, y, gq, uq}));
+        TRY(check_apart(c, "up scales", uk, {g, u, y, gq, uq, gk}));
+        a = activation_args(desc);
+        a.gate = gates;
+        a.up = ups;
+        a.out = outputs;
+        if (coded) a.kept_gate = kept_rows(desc, gate_codes, gate_scales);
+        if (both) a.kept_up = kept_rows(desc, up_codes, up_scales);
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "activation_forward", [&] { return launch_activation(a, false, desc->values, s); });
+}
+
+int32_t gtmoe_activation_gradient(gtmoe_context *ctx, const gtmoe_activation_desc *desc, const void *output_gradients,
+                                  const void *gates, const float *gate_scales, const void *ups, const float *up_scales,
+                                  void *gate_gradients, void *up_gradients, void *outputs, void *stream)
+{
+    ActivationArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_activation_desc(c, desc));
+        const int es = value_bytes(desc->values);
+        const bool coded = desc->codes != GTMOE_CODES_NONE;
+        if (up_gradients && !ups) return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "up gradients without ups");
+        if (!coded || gate_gradients) TRY(check_stride(c, "gate", desc->gate_stride, desc->columns));
+        if ((!coded && ups) || up_gradients) TRY(check_stride(c, "up", desc->up_stride, desc->columns));
+        TRY(check_stride(c, "output", desc->output_stride, desc->columns));
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "output gradients", output_gradients, es));
+            TRY(check_pointer(c, coded ? "gate codes" : "gates", gates, coded ? 1 : es));
+            if (ups) TRY(check_pointer(c, coded ? "up codes" : "ups", ups, coded ? 1 : es));
+            if (coded) {
+                TRY(check_pointer(c, "gate scales", gate_scales, 4));
+                if (ups) TRY(check_pointer(c, "up scales", up_scales, 4));
+            }
+            if (gate_gradients) TRY(check_pointer(c, "gate gradients", gate_gradients, es));
+            if (up_gradients) TRY(check_pointer(c, "up gradients", up_gradients, es));
+            if (outputs) TRY(check_pointer(c, "outputs", outputs, es));
+        }
+        const int64_t n = desc->rows, w = desc->columns;
+        const Span dy = rows_span(output_gradients, n, w, desc->output_stride, es);
+        const Span g = coded ? codes_span(gates, n, w, desc->code_stride) : rows_span(gates, n, w, desc->gate_stride, es);
+        const Span u = coded ? codes_span(ups, n, w, desc->code_stride) : rows_span(ups, n, w, desc->up_stride, es);
+        const Span gk = scales_span(coded ? gate_scales : nullptr, n, desc->columns, desc->scale_columns, desc->scale_stride);
+        const Span uk = scales_span(coded && ups ? up_scales : nullptr, n, desc->columns, desc->scale_columns, desc->scale_stride);
+        const Span dg = rows_span(gate_gradients, n, w, desc->gate_stride, es), du = rows_span(up_gradients, n, w, desc->up_stride, es);
+        const Span y = rows_span(outputs, n, w, desc->output_stride, es);
+        // in place over values: the thread that writes them is the one that read them
+        TRY(check_output(c, "gate gradients", dg, {{dy, true}, {g, !coded}, {u, !coded}, {gk, false}, {uk, false}}));
+        TRY(check_output(c, "up gradients", du, {{dy, true}, {g, !coded}, {u, !coded}, {gk, false}, {uk, false}, {dg, false}}));
+        TRY(check_output(c, "outputs", y, {{dy, true}, {g, !coded}, {u, !coded}, {gk, false}, {uk, false}, {dg, false}, {du, false}}));
+        a = activation_args(desc);
+        a.dy = output_gradients;
+        a.dgate = gate_gradients;
+        a.dup = up_gradients;
+        a.out = outputs;
+        if (coded) {
+            a.kept_gate = kept_rows(desc, gates, gate_scales);
+            if (ups) a.kept_up = kept_rows(desc, ups, up_scales);
+        } else {
+            a.gate = gates;
+            a.up = ups;
+        }
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "activation_gradient", [&] { return launch_activation(a, true, desc->values, s); });
+}
+
+int32_t gtmoe_grouped_fused_forward(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const gtmoe_epilogue *epilogue,
+                                    const int32_t *offsets, const void *inputs, const void *weights, void *outputs,
+                                    void *stream)
+{
+    GroupedArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_grouped_or_whole(c, desc, offsets));
+        if (!epilogue) return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "the epilogue is null");
+        TRY(check_activation(c, epilogue->activation));
+        TRY(check_reserved(c, epilogue->reserved));
+        const gtmoe_epilogue &e = *epilogue;
+        const int es = value_bytes(desc->values);
+        const int64_t n = desc->rows, w = desc->outputs;
+        if (e.biases && desc->groups > 1) TRY(check_stride(c, "bias", e.bias_stride, w));
+        if (e.factors) TRY(check_stride(c, "factor", e.factor_stride, w));
+        if (e.residuals) TRY(check_stride(c, "residual", e.residual_stride, w));
+        if (e.products) TRY(check_stride(c, "product", e.product_stride, w));
+        const int64_t ldbias = desc->groups > 1 ? e.bias_stride : 0;
+        if (desc->rows > 0) {
+            TRY(check_pointer(c, "inputs", inputs, es));
+            TRY(check_pointer(c, "weights", weights, es));
+            TRY(check_pointer(c, "outputs", outputs, es));
+            if (e.biases) TRY(check_pointer(c, "biases", e.biases, es));
+            if (e.factors) TRY(check_pointer(c, "factors", e.factors, es));
+            if (e.residuals) TRY(check_pointer(c, "residuals", e.residuals, es));
+            if (e.products) TRY(check_pointer(c, "products", e.products, es));
+            const Span x = rows_span(inputs, n, desc->inputs, desc->input_stride, es), m = grouped_matrices(desc, weights, es);
+            const Span o = offsets ? offsets_span(desc, offsets) : Span{nullptr, 0, 0, 0};
+            const Span b = rows_span(e.biases, desc->groups, w, ldbias, es);
+            const Span f = rows_span(e.factors, n, w, e.factor_stride, es), r = rows_span(e.residuals, n, w, e.residual_stride, es);
+            const Span z = rows_span(e.products, n, w, e.product_stride, es), y = rows_span(outputs, n, w, desc->output_stride, es);
+            TRY(check_output(c, "outputs", y,
+                             {{x, false}, {m, false}, {o, false}, {b, false}, {f, true}, {r, true}, {z, false}}));
+            TRY(check_apart(c, "products", z, {x, m, o, b, f, r}));
+        }
+        a = grouped_args(desc, offsets);
+        a.a = inputs;
+        a.lda = desc->input_stride;
+        a.b = weights;
+        a.ldb = desc->weight_stride;
+        a.out = outputs;
+        a.ldo = desc->output_stride;
+        a.epilogue.on = 1;
+        a.epilogue.activation = e.activation;
+        a.epilogue.bias = e.biases;
+        a.epilogue.factor = e.factors;
+        a.epilogue.residual = e.residuals;
+        a.epilogue.products = e.products;
+        a.epilogue.ldbias = ldbias;
+        a.epilogue.ldfactor = e.factor_stride;
+        a.epilogue.ldresidual = e.residual_stride;
+        a.epilogue.ldproducts = e.product_stride;
+        return check_grid(c, a, grouped_fits(a, kGroupedForward, desc->values));
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->rows == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "grouped_fused_forward", [&] { return launch_grouped(a, kGroupedForward, desc->values, s); });
+}
+
+int32_t gtmoe_grouped_bias_workspace(const gtmoe_grouped_desc *desc, size_t *bytes)
+{
+    static const int32_t offsets[2] = {0, 0};
+    if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
+    TRY(check_grouped(nullptr, desc, offsets));
+    *bytes = sum_floats(desc->rows, desc->groups, desc->outputs) * 4;
+    return GTMOE_OK;
+}
+
+int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                                    const void *output_gradients, void *bias_gradients, int32_t gradient_values,
+                                    int32_t accumulate, void *workspace, size_t workspace_bytes, void *stream)
+{
+    ColumnSumsArgs a;
+    AddPartialsArgs add;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_grouped_or_whole(c, desc, offsets));
+        TRY(check_gradient_values(c, "bias gradients", gradient_values, desc->values));
+        const int es = value_bytes(desc->values), gs = value_bytes(gradient_values);
+        const size_t need = sum_floats(desc->rows, desc->groups, desc->outputs) * 4;
+        TRY(check_pointer(c, "bias gradients", bias_gradients, gs));
+        if (desc->rows > 0) TRY(check_pointer(c, "output gradients", output_gradients, es));
+        TRY(check_workspace(c, workspace, workspace_bytes, need));
+        const Span dy = rows_span(output_gradients, desc->rows, desc->outputs, desc->output_stride, es);
+        const Span o = offsets ? offsets_span(desc, offsets) : Span{nullptr, 0, 0, 0};
+        const Span db{bias_gradients, 1, (int64_t)desc->groups * desc->outputs * gs, 0}, ws{workspace, 1, (int64_t)need, 0};
+        TRY(check_apart(c, "bias gradients", db, {dy, o, ws}));
+        TRY(check_apart(c, "the workspace's bytes", ws, {dy, o}));
+        a.x = output_gradients;
+        a.ldx = desc->output_stride;
+        a.offsets = add.offsets = offsets;
+        a.partial = (float *)workspace;
+        add.partial = a.partial;
+        a.rows = add.rows = desc->rows;
+        a.columns = add.columns = desc->outputs;
+        a.groups = add.groups = desc->groups;
+        a.each = add.each = sum_rows_each(desc->rows, desc->groups, desc->outputs);
+        add.out = bias_gradients;
+        add.ldo = desc->outputs;
+        add.out_f32 = gradient_values == GTMOE_VALUES_FLOAT32;
+        add.accumulate = accumulate != 0;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "grouped_bias_gradient", [&] { return launch_column_sums(a, add, desc->values, s); });
+}
+
+int32_t gtmoe_route_workspace(const gtmoe_route_desc *desc, size_t *bytes)
+{
+    if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
+    TRY(check_route(nullptr, desc));
+    *bytes = choose_layout(desc->tokens, desc->experts).bytes;
+    return GTMOE_OK;
+}
+
+int32_t gtmoe_route_forward(gtmoe_context *ctx, const gtmoe_route_desc *desc, const void *logits, const float *biases,
+                            int32_t *chosen, float *gates, int32_t *expert_offsets, int32_t *rows_for_expert,
+                            int32_t *places, void *workspace, size_t workspace_bytes, void *stream)
+{
+    ChooseArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_route(c, desc));
+        if (!expert_offsets && (rows_for_expert || places))
+            return fail(c, GTMOE_ERR_INVALID_ARGUMENT, "rows or places without expert offsets");
+        const int es = value_bytes(desc->values);
+        size_t need = 0;
+        if (expert_offsets) {
+            TRY(check_pointer(c, "expert offsets", expert_offsets, 4));
+            need = choose_layout(desc->tokens, desc->experts).bytes;
+            TRY(check_workspace(c, workspace, workspace_bytes, need));
+        }
+        if (desc->tokens > 0) {
+            TRY(check_pointer(c, "logits", logits, es));
+            if (biases) TRY(check_pointer(c, "biases", biases, 4));
+            TRY(check_pointer(c, "chosen", chosen, 4));
+            TRY(check_pointer(c, "gates", gates, 4));
+            if (rows_for_expert) TRY(check_pointer(c, "rows of the experts", rows_for_expert, 4));
+            if (places) TRY(check_pointer(c, "places", places, 4));
+        }
+        const int64_t n = 4 * (int64_t)desc->tokens * desc->experts_per_token;
+        const Span l = rows_span(logits, desc->tokens, desc->experts, desc->logit_stride, es);
+        const Span b{biases, 1, 4 * (int64_t)desc->experts, 0}, ch{chosen, 1, n, 0}, g{gates, 1, n, 0};
+        const Span o{expert_offsets, 1, 4 * ((int64_t)desc->experts + 1), 0}, r{rows_for_expert, 1, n, 0}, p{places, 1, n, 0};
+        const Span ws{need ? workspace : nullptr, 1, (int64_t)need, 0};
+        TRY(check_apart(c, "chosen", ch, {l, b}));
+        TRY(check_apart(c, "gates", g, {l, b, ch}));
+        TRY(check_apart(c, "expert offsets", o, {l, b, ch, g}));
+        TRY(check_apart(c, "rows of the experts", r, {l, b, ch, g, o}));
+        TRY(check_apart(c, "places", p, {l, b, ch, g, o, r}));
+        TRY(check_apart(c, "the workspace's bytes", ws, {l, b, ch, g, o, r, p}));
+        a.logits = logits;
+        a.biases = biases;
+        a.chosen = chosen;
+        a.gates = gates;
+        a.offsets = expert_offsets;
+        a.rows = rows_for_expert;
+        a.places = places;
+        a.ldlogits = desc->logit_stride;
+        a.tokens = desc->tokens;
+        a.experts = desc->experts;
+        a.k = desc->experts_per_token;
+        a.groups = desc->expert_groups;
+        a.chosen_groups = desc->chosen_groups;
+        a.group_best = desc->group_best;
+        a.logistic = desc->scores == GTMOE_SCORES_SIGMOID;
+        a.renormalize = desc->renormalize != 0;
+        a.scale = (float)desc->scale;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->tokens == 0 && !expert_offsets) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "route_forward", [&] { return launch_choose(a, desc->values, workspace, s); });
+}
+
+int32_t gtmoe_route_gradient(gtmoe_context *ctx, const gtmoe_route_desc *desc, const void *logits, const int32_t *chosen,
+                             const float *gate_gradients, void *logit_gradients, void *stream)
+{
+    ChooseGradientArgs a;
+    auto check = [&](gtmoe_context *c) -> int32_t {
+        TRY(check_route(c, desc));
+        const int es = value_bytes(desc->values);
+        if (desc->tokens > 0) {
+            TRY(check_pointer(c, "logits", logits, es));
+            TRY(check_pointer(c, "chosen", chosen, 4));
+            TRY(check_pointer(c, "gate gradients", gate_gradients, 4));
+            TRY(check_pointer(c, "logit gradients", logit_gradients, es));
+        }
+        const int64_t n = 4 * (int64_t)desc->tokens * desc->experts_per_token;
+        TRY(check_apart(c, "logit gradients", rows_span(logit_gradients, desc->tokens, desc->experts, desc->logit_stride, es),
+                        {rows_span(logits, desc->tokens, desc->experts, desc->logit_stride, es), Span{chosen, 1, n, 0},
+                         Span{gate_gradients, 1, n, 0}}));
+        a.logits = logits;
+        a.chosen = chosen;
+        a.gate_gradients = gate_gradients;
+        a.logit_gradients = logit_gradients;
+        a.ldlogits = a.ldgradients = desc->logit_stride;
+        a.tokens = desc->tokens;
+        a.experts = desc->experts;
+        a.k = desc->experts_per_token;
+        a.logistic = desc->scores == GTMOE_SCORES_SIGMOID;
+        a.renormalize = desc->renormalize != 0;
+        a.scale = (float)desc->scale;
+        return GTMOE_OK;
+    };
+    if (!ctx) return check_only(check);
+    ENTER(ctx);
+    TRY(check(ctx));
+    if (desc->tokens == 0) return GTMOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    return run_plain(ctx, s, "route_gradient", [&] { return launch_choose_gradient(a, desc->values, s); });
+}
+
+}  // extern "C"

@@ -28,7 +28,7 @@
 //
 // Row groups are found on the device: the grid holds the most tiles the rows
 // can need, every wave scans the offsets for its tile, surplus workgroups end.
-#include "grouped_tile.h"
+#include "grouped_rows.h"
 
 namespace gtmoe {
 
@@ -123,7 +123,7 @@ __device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NJ], void *ou
 
 // BM x BN tile by WM x WN waves; NS: stages; DA, DB: the operands staged by
 // LDS-DMA (both of them with more than two stages).
-template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, bool DB, bool ADAPTED>
+template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, bool DB, bool ADAPTED, bool FUSED>
 __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
 {
     constexpr int THREADS = 64 * WM * WN;
@@ -292,6 +292,24 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
         const uint32_t without = add_adapters<T>(acc, a, tile_m + wm, tile_n + wn, tile_m + m);
         if (!a.b && !a.bias) skip = without;
     }
+    if constexpr (FUSED) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int row = wm + 32 * i + (lane & 31);
+            if (row >= m) continue;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int col = wn + 32 * j + 8 * q + 4 * h;
+                    if (col >= n) continue;
+                    float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    store_fused<T>(a, g, (long long)tile_m + row, tile_n + col, v, n - col);
+                }
+        }
+        return;
+    }
     if (DIR == kGroupedWeightGradient && a.out_f32)
         store_tile<F32>(acc, out, a.ldo, wm, wn, m, n, a.accumulate, skip);
     else
@@ -315,22 +333,24 @@ long long tile_blocks(const GroupedArgs &a, int direction, int bm, int bn)
     return (tiles + 7) / 8 * 8 * ((width + bn - 1) / bn);
 }
 
-template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, bool DB, bool ADAPTED>
+template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool DA, bool DB, bool ADAPTED, bool FUSED>
 hipError_t launch_tiles(const GroupedArgs &a, hipStream_t s)
 {
     const long long blocks = tile_blocks(a, DIR, BM, BN);
-    hipLaunchKernelGGL((grouped_kernel<T, DIR, BM, BN, WM, WN, NS, DA, DB, ADAPTED>), dim3((unsigned)blocks),
+    hipLaunchKernelGGL((grouped_kernel<T, DIR, BM, BN, WM, WN, NS, DA, DB, ADAPTED, FUSED>), dim3((unsigned)blocks),
                        dim3(64 * WM * WN), 0, s, a);
     return hipGetLastError();
 }
 
 // NS: stages where both operands take LDS-DMA loads.
-template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool ADAPTED = false>
+template <class T, int DIR, int BM, int BN, int WM, int WN, int NS, bool ADAPTED = false, bool FUSED = false>
 hipError_t launch_staged(const GroupedArgs &a, bool da, bool db, hipStream_t s)
 {
-    if (da && db) return launch_tiles<T, DIR, BM, BN, WM, WN, NS, true, true, ADAPTED>(a, s);
-    return db ? launch_tiles<T, DIR, BM, BN, WM, WN, 2, false, true, ADAPTED>(a, s)
-              : launch_tiles<T, DIR, BM, BN, WM, WN, 2, false, false, ADAPTED>(a, s);
+    if constexpr (DIR == kGroupedForward && !ADAPTED && !FUSED)
+        if (a.epilogue.on) return launch_staged<T, DIR, BM, BN, WM, WN, NS, false, true>(a, da, db, s);
+    if (da && db) return launch_tiles<T, DIR, BM, BN, WM, WN, NS, true, true, ADAPTED, FUSED>(a, s);
+    return db ? launch_tiles<T, DIR, BM, BN, WM, WN, 2, false, true, ADAPTED, FUSED>(a, s)
+              : launch_tiles<T, DIR, BM, BN, WM, WN, 2, false, false, ADAPTED, FUSED>(a, s);
 }
 
 // The tile by type, rows per group and number of tiles (times in us, MI355X):
@@ -365,6 +385,9 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
             return tile_blocks(a, DIR, 64, 64) <= 2 * kCus ? launch_staged<T, DIR, 64, 64, 2, 2, 4, true>(a, da, db, s)
                                                            : launch_staged<T, DIR, 64, 64, 2, 2, 2, true>(a, da, db, s);
         }
+    if constexpr (DIR == kGroupedForward)
+        if (a.epilogue.on && few_fits(a))
+            return launch_few(a, T::kBytes == 4 ? kValuesF32 : std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
     const long long each = a.rows / a.groups;
     if constexpr (T::kBytes == 4) {
         if constexpr (DIR != kGroupedWeightGradient)

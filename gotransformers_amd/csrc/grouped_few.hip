@@ -1,0 +1,116 @@
+// Ragged products of few rows with an epilogue (grouped.hip has the others'): W
+// streams from memory into MFMA operands, no LDS on its way, and the epilogue's
+// thread has four columns of a row.
+//
+// A workgroup takes NC times 16 columns of one group's matrix and up to RT times 16
+// of its rows, the waves splitting the reduction.  Its group is found on the
+// device, as in grouped.hip; columns are dealt to the XCDs in turn, so that
+// however few rows there are every XCD streams its share of W, and the row tiles of
+// a group, a multiple of eight workgroups apart, find W in the same L2.
+#include "grouped_rows.h"
+
+namespace gtmoe {
+
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kMostRows = 256;
+
+template <class T, int NC, int RT>
+__global__ __launch_bounds__(64 * kWaves) void grouped_few_kernel(GroupedArgs a, int columns)
+{
+    __shared__ float part[kWaves][16 * RT][16 * NC + 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int q = lane >> 4, i = lane & 15;
+    const int tile = blockIdx.x / columns, n0 = (blockIdx.x - tile * columns) * (16 * NC);
+    if (n0 >= a.outputs) return;
+    // the tile's group: its rows in tiles of 16 RT
+    int g = -1, t0 = 0, rows = 0, before = 0;
+    for (int e0 = 0; e0 < a.groups; e0 += 64) {
+        int lo = 0, hi = 0;
+        if (e0 + lane < a.groups) group_rows(a, e0 + lane, lo, hi);
+        const int n = (hi - lo + 16 * RT - 1) / (16 * RT);
+        int total;
+        const int first = before + wave_sum_before(n, total);
+        const uint64_t hit = __ballot(tile >= first && tile < first + n);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            g = e0 + src;
+            t0 = __builtin_amdgcn_readlane(lo, src) + (tile - __builtin_amdgcn_readlane(first, src)) * (16 * RT);
+            rows = min(16 * RT, __builtin_amdgcn_readlane(hi, src) - t0);
+            break;
+        }
+        before += total;
+    }
+    if (g < 0) return;
+    typedef typename T::Store Store;
+    f32x4 acc[NC][RT];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int p = 0; p < RT; ++p) acc[c][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // columns and rows past the last repeat it: their results are not kept
+    const Store *w[NC], *x[RT];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+        w[c] = reinterpret_cast<const Store *>(a.b) + g * a.group_stride + min(n0 + 16 * c + i, a.outputs - 1) * a.ldb;
+#pragma unroll
+    for (int p = 0; p < RT; ++p) x[p] = reinterpret_cast<const Store *>(a.a) + (long long)(t0 + min(16 * p + i, rows - 1)) * a.lda;
+    const Store *const(&wc)[NC] = w;
+    const Store *const(&xc)[RT] = x;
+    multiply_rows<T, kWaves, NC, RT>(wc, xc, a.inputs, wave, acc);
+    // lane l: row l % 16 of each row tile, columns 4 (l / 16) .. of each column tile
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int p = 0; p < RT; ++p)
+            *reinterpret_cast<f32x4 *>(&part[wave][16 * p + i][16 * c + 4 * q]) = acc[c][p];
+    __syncthreads();
+    for (int o = threadIdx.x; o < 16 * RT * 4 * NC; o += 64 * kWaves) {
+        const int r = o / (4 * NC), c = (o - r * (4 * NC)) * 4;
+        if (r >= rows || n0 + c >= a.outputs) continue;
+        f32x4 s = *reinterpret_cast<const f32x4 *>(&part[0][r][c]);
+#pragma unroll
+        for (int v = 1; v < kWaves; ++v) s += *reinterpret_cast<const f32x4 *>(&part[v][r][c]);
+        float y[4] = {s[0], s[1], s[2], s[3]};
+        store_fused<T>(a, g, (long long)t0 + r, n0 + c, y, a.outputs - n0 - c);
+    }
+}
+
+// Row tiles of a call: at most one partial tile per group.
+long long row_tiles(const GroupedArgs &a, int rows) { return a.rows / rows + (a.groups < a.rows ? a.groups : a.rows); }
+int columns_of(const GroupedArgs &a, int width) { return ((a.outputs + width - 1) / width + 7) / 8 * 8; }
+
+template <class T, int NC, int RT>
+hipError_t launch_shape(const GroupedArgs &a, hipStream_t s)
+{
+    const int columns = columns_of(a, 16 * NC);
+    hipLaunchKernelGGL((grouped_few_kernel<T, NC, RT>), dim3((unsigned)(row_tiles(a, 16 * RT) * columns)), dim3(64 * kWaves), 0, s, a,
+                       columns);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_values(const GroupedArgs &a, hipStream_t s)
+{
+    if (a.rows / a.groups <= 16) return launch_shape<T, 1, 1>(a, s);
+    return launch_shape<T, 1, 2>(a, s);
+}
+
+}  // namespace
+
+bool few_fits(const GroupedArgs &a)
+{
+    return a.rows <= kMostRows && a.groups <= 64 && row_tiles(a, 16) * columns_of(a, 16) <= 1 << 22;
+}
+
+hipError_t launch_few(const GroupedArgs &a, int values, hipStream_t s)
+{
+    switch (values) {
+    case kValuesBf16: return launch_values<Bf16>(a, s);
+    case kValuesF16: return launch_values<F16>(a, s);
+    default: return launch_values<F32>(a, s);
+    }
+}
+
+}  // namespace gtmoe

@@ -37,7 +37,7 @@
 // rounds of tiles an XCD's CUs go through (kRowCost cycles per step, measured
 // against each other, and kTileCost per tile).  The weight gradient's XCDs take
 // eighths of the work instead: groups differ in their rows.
-#include "grouped_tile.h"
+#include "grouped_rows.h"
 
 namespace gtmoe {
 
@@ -257,7 +257,8 @@ __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int le
 // ADAPTED (forward, one matrix for all groups): the groups are the adapters, their
 // rows at the places of a.term.index.  The adapter's term is two steps more of
 // the same stream, u's parts against the adapter's up matrix.
-template <class T, int DIR, bool ADAPTED>
+// FUSED (forward): the results leave LDS in fp32 and pass the epilogue on their way.
+template <class T, int DIR, bool ADAPTED, bool FUSED = false>
 __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 {
     typedef Operand<T, DIR != kGroupedWeightGradient, kBm, kThreads, SB, ADAPTED> A;
@@ -575,14 +576,22 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
                         const int row = 64 * i + wm + rr, col = wn + 32 * j0 + unit * u;
                         int to = row;
                         if constexpr (ADAPTED) to = __builtin_amdgcn_ds_bpermute(4 * (32 * (i & 1) + rr), places_of[i >> 1]);
-                        if (row < x.m && col < x.n) store_unit<S, O>(out + to * a.ldo + col, v, x.n - col, aligned, a.accumulate);
+                        if (row < x.m && col < x.n) {
+                            if constexpr (FUSED) {
+                                const f32x4 f = __builtin_bit_cast(f32x4, v);
+                                float w[4] = {f[0], f[1], f[2], f[3]};
+                                store_fused<T>(a, x.g, (long long)x.m0 + row, x.n0 + col, w, x.n - col);
+                            } else {
+                                store_unit<S, O>(out + to * a.ldo + col, v, x.n - col, aligned, a.accumulate);
+                            }
+                        }
                     }
                     __builtin_amdgcn_wave_barrier();
                 }
         };
         // (a weight gradient in fp32 up to its one rounding, for what it may be added to)
         if (DIR == kGroupedWeightGradient && a.out_f32) leave(F32(), F32());
-        else if (DIR == kGroupedWeightGradient) leave(F32(), T());
+        else if (DIR == kGroupedWeightGradient || FUSED) leave(F32(), T());
         else leave(T(), T());
     };
     for (;;) {
@@ -606,6 +615,7 @@ hipError_t launch_values(const GroupedArgs &a, int direction, hipStream_t s)
     switch (direction) {
     case kGroupedForward:
         if (a.term.index) hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, true>), grid, block, 0, s, a);
+        else if (a.epilogue.on) hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, false, true>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedForward, false>), grid, block, 0, s, a);
         break;
     case kGroupedInputGradient: hipLaunchKernelGGL((grouped_large_kernel<T, kGroupedInputGradient, false>), grid, block, 0, s, a); break;

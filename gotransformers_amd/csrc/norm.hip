@@ -1,0 +1,587 @@
+// Root-mean-square norm over plain rows with the residual's addition
+// (normalization/rmsnorm.go:33-53 around transformer/block.go:76-77):
+//   s = x + residual, rounded to the values' type as it is kept
+//   y = s r w, r = 1 / sqrt(mean(s^2) + epsilon), in the values' type and / or in 8 bits
+// its gradients, from s:
+//   n = s r, g = dy w
+//   dx = r (g - n mean(g n)) + ds       (ds: what reaches s past the norm)
+//   dw = sum over the rows of dy n
+// and the packing of rows that need no norm.
+//
+// A row stays in registers between its sum and its use: 16 lanes, a wave or a
+// workgroup hold one (`TEAM` threads of `NV` times eight values), rows wider than
+// 65536 are read again.  The gradient keeps dw's sums in registers over the rows
+// of a team, one partial row per workgroup, which a second kernel adds in a fixed
+// order.
+#include "rows.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace gtmoe {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWideThreads = 1024;
+
+// The team's total of v: 16 lanes, a wave, or the whole workgroup.
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float *shared)
+{
+    if constexpr (TEAM == 16) return sixteen_sum(v);
+    v = wave_sum(v);
+    if constexpr (TEAM > 64) {
+        __syncthreads();  // the last total has been read
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < TEAM / 64; ++w) v += shared[w];
+    }
+    return v;
+}
+template <int TEAM>
+__device__ __forceinline__ uint32_t team_max(uint32_t v, float *shared)
+{
+    if constexpr (TEAM == 16) return lanes_max(v, 16);
+    v = wave_max(v);
+    if constexpr (TEAM > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = __uint_as_float(v);
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int w = 0; w < TEAM / 64; ++w) v = max(v, __float_as_uint(shared[w]));
+    }
+    return v;
+}
+
+// Sums in 64 bits, for squares that fp32 does not hold: two halves through the
+// 32-bit exchanges would round, so lanes exchange whole doubles.
+template <int TEAM>
+__device__ double team_sum64(double v, float *shared)
+{
+#pragma unroll
+    for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) v += __shfl_xor(v, d);
+    if constexpr (TEAM > 64) {
+        double *s = reinterpret_cast<double *>(shared);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0;
+        for (int w = 0; w < TEAM / 64; ++w) v += s[w];
+        __syncthreads();
+    }
+    return v;
+}
+
+constexpr int team_threads(int team) { return team > kThreads ? team : kThreads; }
+
+// A row in a team's registers (NV > 0) or read again each time.
+template <int VALUES, int TEAM, int NV>
+struct Row {
+    Eight<VALUES> v[NV ? NV : 1];
+    const void *base;
+    long long at;
+    int columns, thread;
+
+    __device__ __forceinline__ Row(const void *base_, long long at_, int columns_)
+        : base(base_), at(at_), columns(columns_), thread(threadIdx.x % TEAM)
+    {
+    }
+    __device__ __forceinline__ int chunks() const { return NV ? NV : ((columns + 7) / 8 + TEAM - 1) / TEAM; }
+    __device__ __forceinline__ int column(int i) const { return 8 * (i * TEAM + thread); }
+    __device__ __forceinline__ void fill(const void *from, long long row)
+    {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load_eight(v[i], from, row + column(i), columns - column(i));
+        }
+    }
+    __device__ __forceinline__ Eight<VALUES> get(int i) const
+    {
+        if constexpr (NV > 0) {
+            return v[i];
+        } else {
+            Eight<VALUES> e;
+            load_eight(e, base, at + column(i), columns - column(i));
+            return e;
+        }
+    }
+    // f(i) for every group of eight of the thread; i is a constant of the compiler's
+    // where the row is in registers
+    template <class F>
+    __device__ __forceinline__ void each(F &&f) const
+    {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) f(i);
+        } else {
+            for (int i = 0; i < chunks(); ++i) f(i);
+        }
+    }
+};
+
+// 1 / sqrt(mean(s^2) + epsilon) of a row.  Squares beyond fp32, or all below it
+// beside no epsilon, are added in 64 bits.
+template <int VALUES, int TEAM, int NV>
+__device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, double epsilon, float *shared)
+{
+    float sum = 0.f;
+    row.each([&](int i) {
+        const Eight<VALUES> e = row.get(i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(e.get(j), e.get(j), sum);
+    });
+    sum = team_sum<TEAM>(sum, shared);
+    float r = 1.f / sqrtf(sum / (float)row.columns + (float)epsilon);
+    const bool narrow = sum <= 1e37f && (sum >= 1e-25f || epsilon >= 1e-15);
+    // (the lanes of a wave exchange values below: all of them go if one has to)
+    if (TEAM > 64 ? !narrow : __ballot(!narrow) != 0) {
+        double wide = 0;
+        row.each([&](int i) {
+            const Eight<VALUES> e = row.get(i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wide += (double)e.get(j) * (double)e.get(j);
+        });
+        wide = team_sum64<TEAM>(wide, shared);
+        const float again = (float)(1.0 / sqrt(wide / row.columns + epsilon));
+        if (!narrow) r = again;
+    }
+    return r;
+}
+
+template <int VALUES, int TEAM, int NV>
+__global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormArgs a)
+{
+    constexpr int TEAMS = team_threads(TEAM) / TEAM;
+    __shared__ float shared[2 * kWideThreads / 64];
+    const int scale_bits = a.scale_columns ? __builtin_ctz(a.scale_columns) : 31;
+    for (long long r0 = (long long)blockIdx.x * TEAMS; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS) {
+        // teams past the last row work on a row of no columns
+        const long long r = r0 + threadIdx.x / TEAM;
+        const bool have = r < a.rows;
+        const int columns = have ? a.columns : 0;
+        Row<VALUES, TEAM, NV> row(a.sums ? a.sums : a.x, r * (a.sums ? a.ldsums : a.ldx), columns);
+        if (a.residual || a.sums) {
+            row.fill(a.x, r * a.ldx);
+            row.each([&](int i) {
+                const int c = row.column(i), n = columns - c;
+                if (n <= 0) return;
+                Eight<VALUES> e;
+                if constexpr (NV > 0) e = row.v[i];
+                else load_eight(e, a.x, r * a.ldx + c, n);
+                if (a.residual) {
+                    Eight<VALUES> b;
+                    load_eight(b, a.residual, r * a.ldresidual + c, n);
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = e.get(j) + b.get(j);
+                    e.set(v);
+                }
+                if constexpr (NV > 0) row.v[i] = e;
+                store_eight(e, a.sums, r * a.ldsums + c, n);
+            });
+        } else {
+            row.fill(a.x, r * a.ldx);
+        }
+        float inverse = 1.f;
+        if (a.norm) {
+            row.columns = have ? a.columns : 1;  // (of the mean; no value is read)
+            if constexpr (NV == 0) row.columns = columns;
+            inverse = inverse_size(row, a.epsilon, shared);
+            row.columns = columns;
+        }
+        auto value = [&](int i, float (&y)[8]) {
+            const int c = row.column(i), n = columns - c;
+            const Eight<VALUES> e = row.get(i);
+            if (a.norm) {
+                Eight<VALUES> w;
+                if (a.w) load_eight(w, a.w, c, n);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = a.w ? e.get(j) * inverse * w.get(j) : e.get(j) * inverse;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = e.get(j);
+            }
+        };
+        auto largest = [](const float (&y)[8]) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, size_bits(y[j]));
+            return m;
+        };
+        uint32_t most = 0;
+        if (a.codes && !a.scale_columns) {
+            row.each([&](int i) {
+                float y[8];
+                value(i, y);
+                most = max(most, largest(y));
+            });
+            most = team_max<TEAM>(most, shared);
+        }
+        row.each([&](int i) {
+            const int c = row.column(i), n = columns - c;
+            float y[8];
+            value(i, y);
+            if (a.out && n > 0) {
+                Eight<VALUES> e;
+                e.set(y);
+                store_eight(e, a.out, r * a.ldo + c, n);
+            }
+            if (a.codes) {
+                const Scale s(a.scale_columns ? lanes_max(largest(y), a.scale_columns / 8) : most, a.code_type);
+                if (n > 0) {
+                    store_codes(encode_eight(y, s, a.code_type), a.codes + r * a.ldcodes + c, n);
+                    if ((c & ((1u << scale_bits) - 1)) == 0) a.scales[r * a.ldscales + (c >> scale_bits)] = s.value;
+                }
+            }
+        });
+    }
+}
+
+// One partial row of dw per workgroup (a.partial), none without it.
+template <int VALUES, int TEAM, int NV>
+__global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormGradientArgs a)
+{
+    constexpr int THREADS = team_threads(TEAM), TEAMS = THREADS / TEAM;
+    __shared__ float shared[2 * kWideThreads / 64];
+    __shared__ float part[TEAMS > 1 ? TEAMS : 1][TEAMS > 1 ? TEAM * NV * 8 : 1];
+    float dw[NV ? NV : 1][8];
+#pragma unroll
+    for (int i = 0; i < (NV ? NV : 1); ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+    const float mean = 1.f / (float)a.columns;
+    for (long long r0 = (long long)blockIdx.x * TEAMS; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS) {
+        const long long r = r0 + threadIdx.x / TEAM;
+        const bool have = r < a.rows;
+        const int columns = have ? a.columns : 0;
+        Row<VALUES, TEAM, NV> s(a.s, r * a.lds, columns), dy(a.dy, r * a.lddy, columns);
+        s.fill(a.s, r * a.lds);
+        dy.fill(a.dy, r * a.lddy);
+        s.columns = NV && !have ? 1 : columns;
+        const float inverse = inverse_size(s, a.epsilon, shared);
+        s.columns = columns;
+        if (NV == 0 && a.inverse && threadIdx.x == 0) a.inverse[r] = inverse;
+        float dot = 0.f;
+        s.each([&](int i) {
+            const int c = s.column(i), n = columns - c;
+            const Eight<VALUES> v = s.get(i), g = dy.get(i);
+            Eight<VALUES> w;
+            if (a.w) load_eight(w, a.w, c, n);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float t = g.get(j) * (v.get(j) * inverse);
+                dot = a.w ? fmaf(w.get(j), t, dot) : dot + t;
+                if constexpr (NV > 0) dw[i][j] += t;
+            }
+        });
+        dot = team_sum<TEAM>(dot, shared) * mean;
+        s.each([&](int i) {
+            const int c = s.column(i), n = columns - c;
+            if (n <= 0) return;
+            const Eight<VALUES> v = s.get(i), g = dy.get(i);
+            Eight<VALUES> w, e;
+            if (a.w) load_eight(w, a.w, c, n);
+            if (a.ds) load_eight(e, a.ds, r * a.ldds + c, n);
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float m = v.get(j) * inverse, t = a.w ? g.get(j) * w.get(j) : g.get(j);
+                y[j] = inverse * fmaf(-m, dot, t) + (a.ds ? e.get(j) : 0.f);
+            }
+            e.set(y);
+            store_eight(e, a.dx, r * a.lddx + c, n);
+        });
+    }
+    if constexpr (NV > 0) {
+        if (!a.partial) return;
+        const int thread = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+        float *out = a.partial + (long long)blockIdx.x * a.columns;
+        if constexpr (TEAMS > 1) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) part[team][8 * (i * TEAM + thread) + j] = dw[i][j];
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.columns; c += THREADS) {
+                float v = 0.f;
+#pragma unroll
+                for (int t = 0; t < TEAMS; ++t) v += part[t][c];
+                out[c] = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int c = 8 * (i * TEAM + thread) + j;
+                    if (c < a.columns) out[c] = dw[i][j];
+                }
+        }
+    }
+}
+
+// Sums over rows by group, in two steps: a workgroup adds `each` consecutive rows of
+// 512 columns, one partial row for every group among them; the pair (workgroup b,
+// group g) has slot b + g, and no other pair has it, since rows are in group order.
+// With v: of the rows' values times v's times inverse[r].
+constexpr int kSumColumns = 512;
+
+template <int VALUES>
+__global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
+{
+    __shared__ float part[kThreads / 64][kSumColumns];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = blockIdx.x * kSumColumns + 8 * lane, n = a.columns - c;
+    const int first = blockIdx.y * a.each, last = min(first + a.each, a.rows);
+    for (int g0 = 0; g0 < a.groups; g0 += 64) {
+        int lo = 0, hi = 0;
+        if (g0 + lane < a.groups) {
+            lo = a.offsets ? min(max(a.offsets[g0 + lane], 0), a.rows) : 0;
+            hi = a.offsets ? min(max(a.offsets[g0 + lane + 1], lo), a.rows) : a.rows;
+        }
+        lo = max(lo, first);
+        hi = min(hi, last);
+        uint64_t todo = __ballot(lo < hi);
+        while (todo) {
+            const int src = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const int begin = __builtin_amdgcn_readlane(lo, src), end = __builtin_amdgcn_readlane(hi, src);
+            float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (n > 0) {
+#pragma unroll 4
+                for (int r = begin + wave; r < end; r += kThreads / 64) {
+                    Eight<VALUES> e;
+                    load_eight(e, a.x, r * a.ldx + c, n);
+                    if (a.v) {
+                        Eight<VALUES> v;
+                        load_eight(v, a.v, r * a.ldv + c, n);
+                        const float inverse = a.inverse[r];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum[j] += e.get(j) * (v.get(j) * inverse);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum[j] += e.get(j);
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) part[wave][8 * lane + j] = sum[j];
+            __syncthreads();
+            float *out = a.partial + (long long)(blockIdx.y + g0 + src) * a.columns + blockIdx.x * kSumColumns;
+            for (int i = threadIdx.x; i < min(kSumColumns, a.columns - blockIdx.x * kSumColumns); i += kThreads) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < kThreads / 64; ++w) v += part[w][i];
+                out[i] = v;
+            }
+        }
+    }
+}
+
+// out[g][c] (+)= the sum of partial rows: 16 columns per workgroup, 16 threads each.
+// The partial rows of group g are those of the row ranges it touches.
+template <int VALUES>
+__global__ __launch_bounds__(kThreads) void add_partials_kernel(AddPartialsArgs a)
+{
+    __shared__ float part[16][17];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, g = blockIdx.y;
+    const int c = blockIdx.x * 16 + x;
+    int begin = 0, end = a.count;
+    if (a.each) {
+        int lo = a.offsets ? min(max(a.offsets[g], 0), a.rows) : 0;
+        int hi = a.offsets ? min(max(a.offsets[g + 1], lo), a.rows) : a.rows;
+        begin = lo < hi ? lo / a.each + g : 0;
+        end = lo < hi ? (hi - 1) / a.each + g + 1 : 0;
+    }
+    float sum = 0.f;
+    if (c < a.columns) {
+#pragma unroll 8
+        for (int p = begin + y; p < end; p += 16) sum += a.partial[(long long)p * a.columns + c];
+    }
+    part[y][x] = sum;
+    __syncthreads();
+    if (y == 0 && c < a.columns) {
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += part[i][x];
+        if (begin == end && a.accumulate) return;
+        const long long at = g * a.ldo + c;
+        if (a.out_f32) {
+            float *o = reinterpret_cast<float *>(a.out) + at;
+            *o = a.accumulate ? *o + sum : sum;
+        } else {
+            typedef typename Eight<VALUES>::Store Store;
+            Eight<VALUES> e;
+            Store *o = reinterpret_cast<Store *>(a.out) + at, w[8] = {};
+            if (a.accumulate) {
+                w[0] = *o;
+                __builtin_memcpy(e.raw, w, sizeof w);
+                sum += e.get(0);
+            }
+            const float v[8] = {sum, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            e.set(v);
+            __builtin_memcpy(w, e.raw, sizeof w);
+            *o = w[0];
+        }
+    }
+}
+
+// Threads and groups of eight values per thread that hold a row.  One wave per
+// row up to 2048 columns; from there, and while there are few rows, a workgroup.
+constexpr int kFewRows = 512;
+struct Shape {
+    int team, nv;
+};
+Shape shape_of(int rows, int columns)
+{
+    const int eights = (columns + 7) / 8;
+    if (eights <= 16) return {16, 1};
+    if (eights <= 64) return {64, 1};
+    if (rows > kFewRows && eights <= 128) return {64, 2};
+    if (rows > kFewRows && eights <= 256) return {64, 4};
+    if (eights <= 256) return {256, 1};
+    if (eights <= 512) return {256, 2};
+    if (eights <= 1024) return {256, 4};
+    if (eights <= 2048) return {256, 8};
+    if (eights <= 8192) return {1024, 8};
+    return {1024, 0};
+}
+
+// f(team, nv) as constants
+template <class F>
+hipError_t with_shape(Shape s, F &&f)
+{
+#define GTMOE_SHAPE(T, N) \
+    if (s.team == T && s.nv == N) return f(std::integral_constant<int, T>(), std::integral_constant<int, N>());
+    GTMOE_SHAPE(16, 1)
+    GTMOE_SHAPE(64, 1)
+    GTMOE_SHAPE(64, 2)
+    GTMOE_SHAPE(64, 4)
+    GTMOE_SHAPE(256, 1)
+    GTMOE_SHAPE(256, 2)
+    GTMOE_SHAPE(256, 4)
+    GTMOE_SHAPE(256, 8)
+    GTMOE_SHAPE(1024, 8)
+#undef GTMOE_SHAPE
+    return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>());
+}
+template <class F>
+hipError_t with_values(int values, F &&f)
+{
+    switch (values) {
+    case kValuesBf16: return f(std::integral_constant<int, kValuesBf16>());
+    case kValuesF16: return f(std::integral_constant<int, kValuesF16>());
+    default: return f(std::integral_constant<int, kValuesF32>());
+    }
+}
+
+constexpr int kMostBlocks = 1 << 20;
+
+int blocks_of(long long rows, int team)
+{
+    const int teams = team_threads(team) / team;
+    return (int)std::min<long long>((rows + teams - 1) / teams, kMostBlocks);
+}
+
+// Workgroups of the gradient with dw: as many partial rows.
+int gradient_blocks(int rows, int columns)
+{
+    const Shape s = shape_of(rows, columns);
+    return std::min(blocks_of(rows, s.team), 512);
+}
+
+}  // namespace
+
+hipError_t launch_norm_forward(const NormArgs &a, int values, hipStream_t s)
+{
+    const Shape shape = shape_of(a.rows, a.columns);
+    return with_values(values, [&](auto v) {
+        return with_shape(shape, [&](auto team, auto nv) {
+            constexpr int T = decltype(team)::value;
+            hipLaunchKernelGGL((norm_forward_kernel<decltype(v)::value, T, decltype(nv)::value>), dim3(blocks_of(a.rows, T)),
+                               dim3(team_threads(T)), 0, s, a);
+            return hipGetLastError();
+        });
+    });
+}
+
+int sum_rows_each(int rows, int groups, int columns)
+{
+    // about 1024 workgroups, of 32 rows at least
+    const int strips = (columns + kSumColumns - 1) / kSumColumns;
+    const int slices = std::max(1, std::min(1024 / std::min(strips, 1024), 65535));
+    return std::max(32, (rows + slices - 1) / slices);
+}
+size_t sum_floats(int rows, int groups, int columns)
+{
+    const int each = sum_rows_each(rows, groups, columns);
+    return (size_t)((rows + each - 1) / each + groups) * columns;
+}
+
+hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &add, int values, hipStream_t s)
+{
+    return with_values(values, [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        if (a.rows > 0)
+            hipLaunchKernelGGL(column_sums_kernel<V>, dim3((a.columns + kSumColumns - 1) / kSumColumns, (a.rows + a.each - 1) / a.each),
+                               dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16, a.groups), dim3(kThreads), 0, s, add);
+        return hipGetLastError();
+    });
+}
+
+size_t norm_gradient_floats(int rows, int columns)
+{
+    if (rows == 0) return 0;
+    if (shape_of(rows, columns).nv) return (size_t)gradient_blocks(rows, columns) * columns;
+    return (size_t)rows + sum_floats(rows, 1, columns);
+}
+
+hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddPartialsArgs &into, int values, hipStream_t s)
+{
+    const Shape shape = shape_of(a.rows, a.columns);
+    const bool weights = into.out != nullptr;
+    if (weights) (shape.nv ? a.partial : a.inverse) = workspace;
+    const int blocks = weights && shape.nv ? gradient_blocks(a.rows, a.columns) : blocks_of(a.rows, shape.team);
+    return with_values(values, [&](auto v) -> hipError_t {
+        constexpr int V = decltype(v)::value;
+        if (a.rows > 0) {
+            const hipError_t e = with_shape(shape, [&](auto team, auto nv) {
+                constexpr int T = decltype(team)::value;
+                hipLaunchKernelGGL((norm_gradient_kernel<V, T, decltype(nv)::value>), dim3(blocks), dim3(team_threads(T)), 0, s, a);
+                return hipGetLastError();
+            });
+            if (e != hipSuccess) return e;
+        }
+        if (!weights) return hipSuccess;
+        AddPartialsArgs add = into;
+        add.columns = a.columns;
+        add.groups = 1;
+        if (shape.nv || a.rows == 0) {
+            add.partial = workspace;
+            add.count = a.rows ? blocks : 0;
+            hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16), dim3(kThreads), 0, s, add);
+            return hipGetLastError();
+        }
+        ColumnSumsArgs c;
+        c.x = a.dy;
+        c.ldx = a.lddy;
+        c.v = a.s;
+        c.ldv = a.lds;
+        c.inverse = a.inverse;
+        c.partial = workspace + a.rows;
+        c.rows = add.rows = a.rows;
+        c.columns = a.columns;
+        c.groups = 1;
+        c.each = add.each = sum_rows_each(a.rows, 1, a.columns);
+        add.partial = c.partial;
+        return launch_column_sums(c, add, V, s);
+    });
+}
+
+}  // namespace gtmoe

@@ -1,0 +1,277 @@
+// Rows kept in 8 bits, and what a gated activation's backward takes from them:
+//   y = act(min(gate, L)) clamp(up, -L, L)          (feedforward/gatedfeedforward.go:49-57,
+//                                                    clamped: moreactivationfunctions.go:207-244)
+//   dgate = dy clamp(up) act'(gate) [gate <= L],  dup = dy act(min(gate, L)) [|up| <= L]
+// The forward writes y and, in the same pass, gate and up as codes with a scale per
+// scale_columns columns; the gradient reads those instead of the 16-bit rows and
+// makes y again, which the next product's weight gradient wants.
+//
+// A thread takes eight columns of a row; a scale's columns are two to sixteen
+// neighbouring lanes, whose maximum they find by DPP.
+#include <algorithm>
+#include <type_traits>
+
+#include "rows.h"
+
+namespace gtmoe {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Eight columns of a row per thread: rows are padded to whole scales, `per`
+// threads each.
+struct Place {
+    long long row;
+    int column;
+};
+__device__ __forceinline__ Place place_of(long long i, int per, bool narrow)
+{
+    if (narrow) {
+        const uint32_t r = (uint32_t)i / (uint32_t)per;
+        return {(long long)r, (int)((uint32_t)i - r * (uint32_t)per) * 8};
+    }
+    const long long r = i / per;
+    return {r, (int)(i - r * per) * 8};
+}
+
+__device__ __forceinline__ uint32_t largest_of(const float (&v)[8])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, size_bits(v[e]));
+    return m;
+}
+
+// Codes of eight values and, by its first lane, their block's scale.  Every lane of
+// the block calls it.
+__device__ __forceinline__ void keep_eight(const float (&v)[8], const Place &p, int n, const PackedRows &k)
+{
+    const Scale s(lanes_max(largest_of(v), k.scale_columns / 8), k.code_type);
+    if (n <= 0) return;
+    store_codes(encode_eight(v, s, k.code_type), k.codes + p.row * k.ldcodes + p.column, n);
+    const int bits = __builtin_ctz(k.scale_columns);
+    if ((p.column & (k.scale_columns - 1)) == 0) k.scales[p.row * k.ldscales + (p.column >> bits)] = s.value;
+}
+
+// The eight values that codes stand for (scale_columns 0: one scale per row).
+__device__ __forceinline__ void kept_eight(float (&v)[8], const Place &p, int n, const PackedRows &k)
+{
+    const int bits = k.scale_columns ? __builtin_ctz(k.scale_columns) : 31;
+    decode_eight(load_codes(k.codes + p.row * k.ldcodes + p.column, n), k.scales[p.row * k.ldscales + (p.column >> bits)],
+                 k.code_type, v);
+}
+
+template <int VALUES>
+__global__ __launch_bounds__(kThreads) void pack_kernel(PackArgs a, int per, long long total, bool narrow)
+{
+    for (long long i0 = (long long)blockIdx.x * kThreads; i0 < total; i0 += (long long)gridDim.x * kThreads) {
+        const Place p = place_of(i0 + threadIdx.x, per, narrow);
+        const int n = p.row < a.rows ? a.columns - p.column : 0;
+        Eight<VALUES> e;
+        load_eight(e, a.x, p.row * a.ldx + p.column, n);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = e.get(j);
+        keep_eight(v, p, n, a.kept);
+    }
+}
+
+template <int VALUES>
+__global__ __launch_bounds__(kThreads) void unpack_kernel(PackArgs a, int per, long long total, bool narrow)
+{
+    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
+        const Place p = place_of(i, per, narrow);
+        const int n = a.columns - p.column;
+        if (n <= 0) continue;
+        float v[8];
+        kept_eight(v, p, n, a.kept);
+        Eight<VALUES> e;
+        e.set(v);
+        store_eight(e, a.out, p.row * a.ldx + p.column, n);
+    }
+}
+
+// gate and up within the limit (a NaN stays one), and whether they were
+template <int ACT>
+__device__ __forceinline__ void limited(float &g, float &u, float limit, bool &g_in, bool &u_in)
+{
+    g_in = !(g > limit);
+    u_in = !(fabsf(u) > limit);
+    g = g_in ? g : limit;
+    u = u_in ? u : copysignf(limit, u);
+}
+
+template <int VALUES, int ACT>
+__global__ __launch_bounds__(kThreads) void activation_forward_kernel(ActivationArgs a, int per, long long total, bool narrow)
+{
+    for (long long i0 = (long long)blockIdx.x * kThreads; i0 < total; i0 += (long long)gridDim.x * kThreads) {
+        const Place p = place_of(i0 + threadIdx.x, per, narrow);
+        const int n = p.row < a.rows ? a.columns - p.column : 0;
+        Eight<VALUES> ge, ue;
+        load_eight(ge, a.gate, p.row * a.ldgate + p.column, n);
+        if (a.up) load_eight(ue, a.up, p.row * a.ldup + p.column, n);
+        float g[8], u[8], y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            g[j] = ge.get(j);
+            u[j] = a.up ? ue.get(j) : 1.f;
+            float gl = g[j], ul = u[j];
+            bool gi, ui;
+            limited<ACT>(gl, ul, a.limit, gi, ui);
+            y[j] = a.up ? activated<ACT>(gl) * ul : activated<ACT>(gl);
+        }
+        if (n > 0) {
+            Eight<VALUES> e;
+            e.set(y);
+            store_eight(e, a.out, p.row * a.ldo + p.column, n);
+        }
+        if (a.kept_gate.codes) {
+            keep_eight(g, p, n, a.kept_gate);
+            if (a.up) keep_eight(u, p, n, a.kept_up);
+        }
+    }
+}
+
+template <int VALUES, int ACT>
+__global__ __launch_bounds__(kThreads) void activation_gradient_kernel(ActivationArgs a, int per, long long total, bool narrow)
+{
+    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
+        const Place p = place_of(i, per, narrow);
+        const int n = a.columns - p.column;
+        if (n <= 0) continue;
+        const bool gated = a.up || a.kept_up.codes;
+        Eight<VALUES> de;
+        load_eight(de, a.dy, p.row * a.lddy + p.column, n);
+        float g[8], u[8];
+        if (a.kept_gate.codes) {
+            kept_eight(g, p, n, a.kept_gate);
+            if (gated) kept_eight(u, p, n, a.kept_up);
+        } else {
+            Eight<VALUES> ge, ue;
+            load_eight(ge, a.gate, p.row * a.ldgate + p.column, n);
+            if (gated) load_eight(ue, a.up, p.row * a.ldup + p.column, n);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                g[j] = ge.get(j);
+                if (gated) u[j] = ue.get(j);
+            }
+        }
+        float y[8], dg[8], du[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (!gated) u[j] = 1.f;
+            bool gi, ui;
+            limited<ACT>(g[j], u[j], a.limit, gi, ui);
+            if (!gated) u[j] = 1.f;
+            float act, slope;
+            activation_of<ACT, true>(g[j], act, slope);
+            const float d = de.get(j);
+            y[j] = act * u[j];
+            dg[j] = gi ? d * u[j] * slope : 0.f;
+            du[j] = ui ? d * act : 0.f;
+        }
+        Eight<VALUES> e;
+        if (a.dgate) {
+            e.set(dg);
+            store_eight(e, a.dgate, p.row * a.lddgate + p.column, n);
+        }
+        if (a.dup) {
+            e.set(du);
+            store_eight(e, a.dup, p.row * a.lddup + p.column, n);
+        }
+        if (a.out) {
+            e.set(y);
+            store_eight(e, a.out, p.row * a.ldo + p.column, n);
+        }
+    }
+}
+
+// Threads of a row: whole scales, or groups of eight where there are none.
+struct Grid {
+    int per;
+    long long total;
+    bool narrow;
+    dim3 blocks;
+    Grid(int rows, int columns, int scale_columns)
+    {
+        const int unit = std::max(scale_columns, 8);
+        per = (columns + unit - 1) / unit * (unit / 8);
+        total = (long long)rows * per;
+        narrow = total < (1ll << 31);
+        blocks = dim3((unsigned)std::min<long long>((total + kThreads - 1) / kThreads, 1 << 20));
+    }
+};
+
+template <class F>
+hipError_t with_values(int values, F &&f)
+{
+    switch (values) {
+    case kValuesBf16: return f(std::integral_constant<int, kValuesBf16>());
+    case kValuesF16: return f(std::integral_constant<int, kValuesF16>());
+    default: return f(std::integral_constant<int, kValuesF32>());
+    }
+}
+template <class F>
+hipError_t with_activation(int act, F &&f)
+{
+    switch (act) {
+    case kActivationRelu: return f(std::integral_constant<int, kActivationRelu>());
+    case kActivationSilu: return f(std::integral_constant<int, kActivationSilu>());
+    case kActivationGelu: return f(std::integral_constant<int, kActivationGelu>());
+    case kActivationGeluTanh: return f(std::integral_constant<int, kActivationGeluTanh>());
+    default: return f(std::integral_constant<int, kActivationNone>());
+    }
+}
+
+}  // namespace
+
+hipError_t launch_pack(const PackArgs &a, int values, hipStream_t s)
+{
+    if (!a.kept.scale_columns) {
+        // a scale per row: the norm's rows without a norm
+        NormArgs n;
+        n.x = a.x;
+        n.ldx = a.ldx;
+        n.codes = a.kept.codes;
+        n.scales = a.kept.scales;
+        n.ldcodes = a.kept.ldcodes;
+        n.ldscales = a.kept.ldscales;
+        n.rows = a.rows;
+        n.columns = a.columns;
+        n.norm = 0;
+        n.code_type = a.kept.code_type;
+        return launch_norm_forward(n, values, s);
+    }
+    const Grid g(a.rows, a.columns, a.kept.scale_columns);
+    return with_values(values, [&](auto v) {
+        hipLaunchKernelGGL(pack_kernel<decltype(v)::value>, g.blocks, dim3(kThreads), 0, s, a, g.per, g.total, g.narrow);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_unpack(const PackArgs &a, int values, hipStream_t s)
+{
+    const Grid g(a.rows, a.columns, 0);
+    return with_values(values, [&](auto v) {
+        hipLaunchKernelGGL(unpack_kernel<decltype(v)::value>, g.blocks, dim3(kThreads), 0, s, a, g.per, g.total, g.narrow);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_activation(const ActivationArgs &a, bool gradient, int values, hipStream_t s)
+{
+    const Grid g(a.rows, a.columns, gradient ? 0 : a.kept_gate.scale_columns);
+    return with_values(values, [&](auto v) {
+        return with_activation(a.activation, [&](auto act) {
+            constexpr int V = decltype(v)::value, A = decltype(act)::value;
+            if (gradient)
+                hipLaunchKernelGGL((activation_gradient_kernel<V, A>), g.blocks, dim3(kThreads), 0, s, a, g.per, g.total, g.narrow);
+            else
+                hipLaunchKernelGGL((activation_forward_kernel<V, A>), g.blocks, dim3(kThreads), 0, s, a, g.per, g.total, g.narrow);
+            return hipGetLastError();
+        });
+    });
+}
+
+}  // namespace gtmoe

@@ -1,0 +1,322 @@
+// Parts the operators over plain rows share: the values' types, eight values of
+// a row at a time, sums and maxima over neighbouring lanes, 8-bit codes with
+// scales, and activations.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "grouped.h"
+
+namespace gtmoe {
+
+namespace {
+
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+
+// Eight consecutive values of a row as they lie in memory.
+template <int VALUES>
+struct Eight;
+template <>
+struct Eight<kValuesF32> {
+    typedef float Store;
+    float raw[8];
+    __device__ __forceinline__ float get(int e) const { return raw[e]; }
+    __device__ __forceinline__ void set(const float (&v)[8])
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = v[e];
+    }
+    static __device__ __forceinline__ float rounded(float v) { return v; }
+};
+template <>
+struct Eight<kValuesBf16> {
+    typedef uint16_t Store;
+    uint32_t raw[4];
+    __device__ __forceinline__ float get(int e) const
+    {
+        return __uint_as_float(e & 1 ? raw[e >> 1] & 0xffff0000u : raw[e >> 1] << 16);
+    }
+    __device__ __forceinline__ void set(const float (&v)[8])
+    {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[2 * e], v[2 * e + 1]}, b2));
+    }
+    static __device__ __forceinline__ float rounded(float v) { return (float)(__bf16)v; }
+};
+template <>
+struct Eight<kValuesF16> {
+    typedef uint16_t Store;
+    uint32_t raw[4];
+    __device__ __forceinline__ float get(int e) const
+    {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[e >> 1] >> (16 * (e & 1))));
+    }
+    __device__ __forceinline__ void set(const float (&v)[8])
+    {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[2 * e], v[2 * e + 1]}, h2));
+    }
+    static __device__ __forceinline__ float rounded(float v) { return (float)(_Float16)v; }
+};
+
+// Eight values from p on, any alignment; n of them exist, the others are zero.
+template <int VALUES>
+__device__ __forceinline__ void load_eight(Eight<VALUES> &v, const void *base, long long at, int n)
+{
+    typedef typename Eight<VALUES>::Store Store;
+    const Store *p = reinterpret_cast<const Store *>(base) + at;
+    if (n >= 8) {
+        __builtin_memcpy(v.raw, p, sizeof v.raw);
+    } else {
+        Store w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = e < n ? p[e] : (Store)0;
+        __builtin_memcpy(v.raw, w, sizeof v.raw);
+    }
+}
+template <int VALUES>
+__device__ __forceinline__ void store_eight(const Eight<VALUES> &v, void *base, long long at, int n)
+{
+    typedef typename Eight<VALUES>::Store Store;
+    Store *p = reinterpret_cast<Store *>(base) + at;
+    if (n >= 8) {
+        __builtin_memcpy(p, v.raw, sizeof v.raw);
+    } else {
+        Store w[8];
+        __builtin_memcpy(w, v.raw, sizeof w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = w[e];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Neighbouring lanes, by DPP: after the exchanges with the lane beside, two and
+// four (half mirrored) and eight (mirrored) away the 16 lanes of a row agree.
+// ---------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kDppPairs = 0xB1, kDppFours = 0x4E, kDppEights = 0x141, kDppSixteens = 0x140;
+
+// The largest of the `lanes` (a power of two up to 16) lanes' values.
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes)
+{
+    if (lanes > 1) v = max(v, moved<kDppPairs>(v));
+    if (lanes > 2) v = max(v, moved<kDppFours>(v));
+    if (lanes > 4) v = max(v, moved<kDppEights>(v));
+    if (lanes > 8) v = max(v, moved<kDppSixteens>(v));
+    return v;
+}
+__device__ __forceinline__ float sixteen_sum(float v)
+{
+    v += __uint_as_float(moved<kDppPairs>(__float_as_uint(v)));
+    v += __uint_as_float(moved<kDppFours>(__float_as_uint(v)));
+    v += __uint_as_float(moved<kDppEights>(__float_as_uint(v)));
+    v += __uint_as_float(moved<kDppSixteens>(__float_as_uint(v)));
+    return v;
+}
+__device__ __forceinline__ float lane_value(float v, int lane)
+{
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+__device__ __forceinline__ float wave_sum(float v)
+{
+    v = sixteen_sum(v);
+    return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+    v = lanes_max(v, 16);
+    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+    const uint32_t b = max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
+    return max(a, b);
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit codes: the values of a block share scale = max|v| / 127 (int8) or / 448
+// (e4m3), rounded to fp32.
+//   int8  v / scale to the nearest whole number, halves away from zero, at most 127
+//         in size (lowprecision.encodeInt8, lowprecision.go:66-78, for the same scale)
+//   e4m3  v / scale rounded to fp32, then to the nearest e4m3, halves to even, at most
+//         448 in size
+// A block of zeros has scale 0 and codes 0; one with a value that is not finite
+// has scale NaN and codes 0, so that all of it reads back as NaN.
+// ---------------------------------------------------------------------------
+enum Codes { kCodesNone = 0, kCodesInt8 = 1, kCodesE4m3 = 2 };
+
+// max |v| as bits: the order of finite, infinite and NaN values in one comparison.
+__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct Scale {
+    float value;   // as it is stored
+    float times;   // a power of two that keeps value * times and its inverse normal
+    float scaled;  // value * times
+    float inverse; // 1 / scaled, rounded; 0 for codes of 0
+    __device__ __forceinline__ Scale(uint32_t most_bits, int codes)
+    {
+        const float most = __uint_as_float(most_bits);
+        value = codes == kCodesInt8 ? most / 127.f : most / 448.f;
+        if (most_bits >= 0x7f800000u) value = __uint_as_float(0x7fc00000u);
+        times = value < 0x1p-60f ? 0x1p90f : 1.f;
+        scaled = value * times;
+        inverse = value > 0.f ? 1.f / scaled : 0.f;
+    }
+};
+
+// The code of v as a number.  A quotient by its inverse may be off by a unit in the
+// last place; the remainder v - q scale, exact in an fma, puts it right.
+__device__ __forceinline__ float int8_code(float v, const Scale &s)
+{
+    const float a = fabsf(v) * s.times;
+    float q = rintf(a * s.inverse);
+    const float left = fmaf(-q, s.scaled, a), half = 0.5f * s.scaled;
+    q += left >= half ? 1.f : 0.f;
+    q -= left < -half ? 1.f : 0.f;
+    q = s.inverse > 0.f ? fminf(q, 127.f) : 0.f;
+    return copysignf(q, v);
+}
+__device__ __forceinline__ float e4m3_quotient(float v, const Scale &s)
+{
+    const float a = v * s.times, q = a * s.inverse;
+    const float r = fmaf(fmaf(-q, s.scaled, a), s.inverse, q);
+    return s.inverse > 0.f ? fminf(fmaxf(r, -448.f), 448.f) : 0.f;
+}
+
+__device__ __forceinline__ uint2 encode_eight(const float (&v)[8], const Scale &s, int codes)
+{
+    uint32_t w[2];
+    if (codes == kCodesInt8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            w[i] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[i] |= ((uint32_t)(int)int8_code(v[4 * i + e], s) & 0xffu) << (8 * e);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_quotient(v[4 * i], s), e4m3_quotient(v[4 * i + 1], s), 0, false);
+            p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_quotient(v[4 * i + 2], s), e4m3_quotient(v[4 * i + 3], s), p, true);
+            w[i] = (uint32_t)p;
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void decode_eight(uint2 c, float scale, int codes, float (&v)[8])
+{
+    const uint32_t w[2] = {c.x, c.y};
+    if (codes == kCodesInt8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * scale;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+            v[4 * i] = lo[0] * scale;
+            v[4 * i + 1] = lo[1] * scale;
+            v[4 * i + 2] = hi[0] * scale;
+            v[4 * i + 3] = hi[1] * scale;
+        }
+    }
+}
+__device__ __forceinline__ uint2 load_codes(const uint8_t *p, int n)
+{
+    uint2 c = make_uint2(0, 0);
+    if (n >= 8) {
+        __builtin_memcpy(&c, p, 8);
+    } else {
+        uint8_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = e < n ? p[e] : (uint8_t)0;
+        __builtin_memcpy(&c, w, 8);
+    }
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint2 c, uint8_t *p, int n)
+{
+    if (n >= 8) {
+        __builtin_memcpy(p, &c, 8);
+    } else {
+        uint8_t w[8];
+        __builtin_memcpy(w, &c, 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = w[e];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Activations and their derivatives in fp32.
+// ---------------------------------------------------------------------------
+enum Activation { kActivationNone = 0, kActivationRelu = 1, kActivationSilu = 2, kActivationGelu = 3, kActivationGeluTanh = 4 };
+
+// e^-|x|, about a unit in the last place: the exponent's product with log2 e in two
+// parts.  The hardware's power of two gives zero where the result is below 2^-126:
+// there it takes 64 less, and the product with 2^-64 keeps the subnormal bits.
+__device__ __forceinline__ float exp_minus(float x)
+{
+    constexpr float log2e = 1.44269504088896340736f, rest = (float)(1.44269504088896340736 - (double)1.44269504088896340736f);
+    const float a = -fabsf(x), t = a * log2e;
+    const float lo = fmaf(a, rest, fmaf(a, log2e, -t));
+    const bool small = t < -125.f;
+    const float e = __builtin_amdgcn_exp2f(small ? t + 64.f : t);
+    return a < -1e4f ? 0.f : fmaf(e, lo * 0.69314718055994530942f, e) * (small ? 0x1p-64f : 1.f);
+}
+__device__ __forceinline__ float inverse_of(float d)  // d in [1, 2]
+{
+    const float x = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, x, 1.f), x, x);
+}
+// 1 / (1 + e^-z)
+__device__ __forceinline__ float logistic(float z)
+{
+    const float e = exp_minus(z), r = inverse_of(1.f + e);
+    return z != z ? z : z >= 0.f ? r : e * r;
+}
+
+// act(z) and, where asked for, act'(z).  A NaN stays one.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void activation_of(float z, float &a, float &slope)
+{
+    if constexpr (ACT == kActivationNone) {
+        a = z;
+        slope = 1.f;
+    } else if constexpr (ACT == kActivationRelu) {
+        a = z <= 0.f ? 0.f : z;
+        slope = z <= 0.f ? 0.f : z != z ? z : 1.f;
+    } else if constexpr (ACT == kActivationSilu) {
+        const float s = logistic(z);
+        a = z * s;
+        if constexpr (SLOPE) slope = fmaf(a, 1.f - s, s);
+    } else if constexpr (ACT == kActivationGelu) {
+        // the normal distribution from its smaller tail: nothing cancels
+        const float c = 0.5f * erfcf(-0.70710678118654752440f * z);
+        a = z * c;
+        if constexpr (SLOPE) slope = fmaf(z * 0.39894228040143267794f, exp_minus(0.5f * z * z), c);
+    } else {
+        // 0.5 z (1 + tanh(u)) = z logistic(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+        constexpr float k = 1.59576912160573071176f, c3 = 0.044715f;
+        const float s = logistic(k * z * fmaf(c3 * z, z, 1.f));
+        a = z * s;
+        if constexpr (SLOPE) slope = fmaf(a * (1.f - s), k * fmaf(3.f * c3 * z, z, 1.f), s);
+    }
+}
+template <int ACT>
+__device__ __forceinline__ float activated(float z)
+{
+    float a, slope;
+    activation_of<ACT, false>(z, a, slope);
+    return a;
+}
+
+}  // namespace
+
+}  // namespace gtmoe

@@ -544,6 +544,209 @@ typedef struct gtmoe_dropout_desc {
 int32_t gtmoe_dropout(gtmoe_context *ctx, const gtmoe_dropout_desc *desc, const void *inputs, const void *base,
                       void *outputs, double rate, uint64_t seed, uint64_t offset, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A block in plain rows: the choice of experts, the norm, products with an
+ * epilogue, activations and rows kept in 8 bits.  Everything said above of the
+ * operators over plain rows holds for these, but for the launch limit: rows of
+ * the norm, of activations and of packed rows may be as many as the description
+ * allows.  A buffer that may be NULL takes its stride's check with it.
+ * ------------------------------------------------------------------------- */
+
+/* 8-bit codes of rows.  Every scale_columns columns of a row (16, 32, 64 or 128; 0:
+ * the whole row) share scale = max|v| / 127 (INT8) or / 448 (E4M3: 8-bit floats of
+ * four exponent and three mantissa bits, largest 448, no infinities), rounded to
+ * float32.
+ *   INT8  v / scale to the nearest whole number, halves away from zero, at most
+ *         127 in size: lowprecision.Rows.Append (lowprecision/rows.go:38-79), to the
+ *         bit of float32 values with scale_columns 16
+ *   E4M3  v / scale rounded to float32, then to the nearest E4M3 value, halves to
+ *         even, at most 448 in size
+ * A block of zeros has scale 0.  A block with a value that is not finite has a NaN
+ * for its scale and reads back as NaN.  Codes are one byte each in rows
+ * code_stride bytes apart; scales float32, ceil(columns / scale_columns) per row
+ * (one with scale_columns 0), rows scale_stride apart. */
+enum gtmoe_codes { GTMOE_CODES_NONE = 0, GTMOE_CODES_INT8 = 1, GTMOE_CODES_E4M3 = 2 };
+
+typedef struct gtmoe_packed_desc {
+    int32_t values;
+    int32_t rows;          /* 0 .. 2^30 */
+    int32_t columns;       /* 1 .. 1048576 */
+    int32_t codes;         /* GTMOE_CODES_INT8 or GTMOE_CODES_E4M3 */
+    int32_t scale_columns; /* 0, 16, 32, 64 or 128 */
+    int32_t reserved;      /* 0 */
+    int64_t value_stride, code_stride, scale_stride;
+} gtmoe_packed_desc;
+int32_t gtmoe_pack_rows(gtmoe_context *ctx, const gtmoe_packed_desc *desc, const void *inputs, void *codes, float *scales,
+                        void *stream);
+/* outputs = code * scale, rounded to the values' type. */
+int32_t gtmoe_unpack_rows(gtmoe_context *ctx, const gtmoe_packed_desc *desc, const void *codes, const float *scales,
+                          void *outputs, void *stream);
+
+/* RMSNorm with the residual's addition (RMSNorm.Forward,
+ * normalization/rmsnorm.go:33-53; Block.Forward, transformer/block.go:71-77):
+ *   s = inputs + residuals                  (residuals may be NULL)
+ *   outputs = s / sqrt(mean(s^2) + epsilon) * weights   (weights may be NULL: 1)
+ * s is rounded to the values' type before it is normed, and written to sums, which
+ * may be NULL without residuals and may be inputs or residuals themselves (same
+ * address and stride).  With codes other than NONE the result, before it is rounded
+ * to the values' type, also goes to codes and scales; outputs may then be NULL.
+ * Squares that float32 does not hold are added in 64 bits. */
+typedef struct gtmoe_norm_desc {
+    int32_t values;
+    int32_t rows;          /* 0 .. 2^30 */
+    int32_t columns;       /* 1 .. 1048576 */
+    int32_t codes;         /* gtmoe_codes */
+    int32_t scale_columns; /* with codes: 0, 16, 32, 64 or 128; else 0 */
+    int32_t reserved;      /* 0 */
+    double epsilon;        /* at least 0 */
+    int64_t input_stride;    /* of inputs and input gradients */
+    int64_t residual_stride; /* of residuals */
+    int64_t sum_stride;      /* of sums and their gradients */
+    int64_t output_stride;   /* of outputs and their gradients */
+    int64_t code_stride, scale_stride;
+} gtmoe_norm_desc;
+int32_t gtmoe_norm_forward(gtmoe_context *ctx, const gtmoe_norm_desc *desc, const void *inputs, const void *residuals,
+                           const void *weights, void *sums, void *outputs, void *codes, float *scales, void *stream);
+/* The gradients of what gtmoe_norm_forward normed (RMSNorm.Backward), with n = s / sqrt(mean(s^2)
+ * + epsilon), g = output_gradients * weights:
+ *   input_gradients = (g - n mean(g n)) / sqrt(mean(s^2) + epsilon) + sum_gradients
+ *   weight_gradients (+)= sum over the rows of output_gradients n
+ * sums is s.  sum_gradients, what reaches s past the norm, may be NULL; input_gradients,
+ * the gradient of inputs and residuals alike, may be sum_gradients themselves where
+ * the strides are the same.  weight_gradients (one row, of type gradient_values: the
+ * values' own or float32) may be NULL.  The workspace, of gtmoe_norm_workspace
+ * bytes, 16-byte aligned, is only for them.  The codes of the description are not
+ * used. */
+int32_t gtmoe_norm_workspace(const gtmoe_norm_desc *desc, size_t *bytes);
+int32_t gtmoe_norm_gradient(gtmoe_context *ctx, const gtmoe_norm_desc *desc, const void *output_gradients, const void *sums,
+                            const void *weights, const void *sum_gradients, void *input_gradients, void *weight_gradients,
+                            int32_t gradient_values, int32_t accumulate, void *workspace, size_t workspace_bytes,
+                            void *stream);
+
+/* Activations (activationfunction/activationfunction.go): GELU is z times the normal
+ * distribution at z, GELU_TANH its form with a tanh. */
+enum gtmoe_activation {
+    GTMOE_ACTIVATION_NONE = 0,
+    GTMOE_ACTIVATION_RELU = 1,
+    GTMOE_ACTIVATION_SILU = 2,
+    GTMOE_ACTIVATION_GELU = 3,
+    GTMOE_ACTIVATION_GELU_TANH = 4
+};
+
+/* A gated activation (GatedFeedForward, feedforward/gatedfeedforward.go:49-57):
+ *   outputs = act(min(gates, limit)) * clamp(ups, -limit, limit)
+ * limit 0: none (with a limit and SiLU: ClampedSiLU and ClampedLinear,
+ * activationfunction/moreactivationfunctions.go:207-244).  ups may be NULL: the
+ * activation alone.  With codes other than NONE gates and ups also go, as they came,
+ * into 8 bits: the checkpoint from which gtmoe_activation_gradient goes back. */
+typedef struct gtmoe_activation_desc {
+    int32_t values;
+    int32_t rows;          /* 0 .. 2^30 */
+    int32_t columns;       /* 1 .. 1048576 */
+    int32_t activation;    /* gtmoe_activation */
+    int32_t codes;         /* gtmoe_codes */
+    int32_t scale_columns; /* with codes: 16, 32, 64 or 128; else 0 */
+    double limit;          /* 0, or more than 0 */
+    int64_t gate_stride;   /* of gates and their gradients */
+    int64_t up_stride;     /* of ups and their gradients */
+    int64_t output_stride; /* of outputs and their gradients */
+    int64_t code_stride, scale_stride; /* of gates' and ups' alike */
+} gtmoe_activation_desc;
+int32_t gtmoe_activation_forward(gtmoe_context *ctx, const gtmoe_activation_desc *desc, const void *gates, const void *ups,
+                                 void *outputs, void *gate_codes, float *gate_scales, void *up_codes, float *up_scales,
+                                 void *stream);
+/* With a(z) = act(min(z, limit)) and c(z) = clamp(z, -limit, limit):
+ *   gate_gradients = output_gradients * c(ups) * act'(gates)   (0 above the limit)
+ *   up_gradients   = output_gradients * a(gates)               (0 beyond it)
+ *   outputs        = a(gates) * c(ups), as the forward's of what is read here
+ * With codes NONE gates and ups are values and the scales NULL; else they are the
+ * codes, with their scales, that the forward (or gtmoe_pack_rows) made.  ups NULL: the
+ * activation alone, without up_gradients.  Each result may be NULL.  A result may be a
+ * buffer of values that is read, at the same address and stride. */
+int32_t gtmoe_activation_gradient(gtmoe_context *ctx, const gtmoe_activation_desc *desc, const void *output_gradients,
+                                  const void *gates, const float *gate_scales, const void *ups, const float *up_scales,
+                                  void *gate_gradients, void *up_gradients, void *outputs, void *stream);
+
+/* Ragged products with biases, an activation, a factor and a residual (Layer.Forward,
+ * perceptron/layer.go:133-162, of every expert at once; with the factor the gate of a
+ * GatedFeedForward over its up projection's rows):
+ *   z[r] = W_g inputs[r] + biases_g
+ *   outputs[r] = act(z[r]) * factors[r] + residuals[r]
+ * z is rounded only where it is written to products, for the backward.  biases [groups]
+ * rows bias_stride apart, factors, residuals and products, in rows of `outputs` values
+ * and of the values' type, may each be NULL.  outputs may be factors or residuals
+ * themselves (same address and stride).  With one group offsets may be NULL: all rows.
+ * The gradients: gtmoe_activation_gradient (products as gates, factors as ups), then
+ * gtmoe_grouped_input_gradient, gtmoe_grouped_weight_gradient and
+ * gtmoe_grouped_bias_gradient. */
+typedef struct gtmoe_epilogue {
+    int32_t activation; /* gtmoe_activation */
+    int32_t reserved;   /* 0 */
+    const void *biases, *factors, *residuals;
+    void *products;
+    int64_t bias_stride, factor_stride, residual_stride, product_stride;
+} gtmoe_epilogue;
+int32_t gtmoe_grouped_fused_forward(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const gtmoe_epilogue *epilogue,
+                                    const int32_t *offsets, const void *inputs, const void *weights, void *outputs,
+                                    void *stream);
+/* bias_gradients[g] (+)= sum over g's rows of output_gradients[r] (Layer.Backward,
+ * perceptron/layer.go:164-210): groups rows of `outputs` values, contiguous, of type
+ * gradient_values, the rows' own or float32.  accumulate == 0: an empty group's become
+ * zero.  The inputs, weights and their strides of the description are not used.  With
+ * one group offsets may be NULL.  The workspace: gtmoe_grouped_bias_workspace bytes,
+ * 16-byte aligned. */
+int32_t gtmoe_grouped_bias_workspace(const gtmoe_grouped_desc *desc, size_t *bytes);
+int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
+                                    const void *output_gradients, void *bias_gradients, int32_t gradient_values,
+                                    int32_t accumulate, void *workspace, size_t workspace_bytes, void *stream);
+
+/* A token's choice of experts from its router logits (MixtureOfExperts.Forward,
+ * mixtureofexperts/mixtureofexperts.go:153-205, with scores of the usual kinds):
+ *   s = softmax(logits) over the experts, or 1 / (1 + e^-logits)
+ *   experts_per_token experts of the largest s + biases, best first; equal ones by
+ *   the lower index
+ *   gates[t][j] = scale * s_j / (renormalize ? the sum of the chosen s : 1)
+ * biases (float32, one per expert, MixtureOfExperts.BalanceBiases) move the choice,
+ * not the gates; without them (NULL) experts go by their logits.  With expert_groups
+ * above 1 only the experts of chosen_groups groups of consecutive experts can be
+ * chosen: those with the largest sums of their group_best (1 or 2) best s + biases
+ * (group_best 1 without biases: their largest logit); equal ones by the lower index.
+ * What is compared is computed in 64 bits.  A logit of -infinity or NaN comes after
+ * every other, whatever its bias, and counts in no group's sum; a token with
+ * nothing but -infinity has gates 0.  NaN, and in a softmax +infinity, leave the
+ * token's gates not finite; its choices are experts of the range all the same, each
+ * once.
+ * chosen [tokens][experts_per_token], gates alike (float32).  Where expert_offsets
+ * is not NULL the rows in expert order are listed as gtmoe_last_routing does:
+ * expert_offsets [experts + 1], rows_for_expert (the token of every row, may be
+ * NULL), places [tokens][experts_per_token] (the row of every choice, may be NULL);
+ * the workspace, of gtmoe_route_workspace bytes and 16-byte aligned, is only for them
+ * (NULL where the size is 0). */
+enum gtmoe_scores { GTMOE_SCORES_SOFTMAX = 0, GTMOE_SCORES_SIGMOID = 1 };
+typedef struct gtmoe_route_desc {
+    int32_t values;            /* of logits and their gradients */
+    int32_t tokens;            /* 0 .. 2^24 */
+    int32_t experts;           /* 1 .. 1024 */
+    int32_t experts_per_token; /* 1 .. 32, at most the experts of the chosen groups */
+    int32_t expert_groups;     /* 1 .. 64, divides experts */
+    int32_t chosen_groups;     /* 1 .. expert_groups */
+    int32_t group_best;        /* 1 or 2 */
+    int32_t scores;            /* gtmoe_scores */
+    int32_t renormalize;
+    int32_t reserved;          /* 0 */
+    double scale;              /* finite */
+    int64_t logit_stride;      /* of logits and their gradients */
+} gtmoe_route_desc;
+int32_t gtmoe_route_workspace(const gtmoe_route_desc *desc, size_t *bytes);
+int32_t gtmoe_route_forward(gtmoe_context *ctx, const gtmoe_route_desc *desc, const void *logits, const float *biases,
+                            int32_t *chosen, float *gates, int32_t *expert_offsets, int32_t *rows_for_expert,
+                            int32_t *places, void *workspace, size_t workspace_bytes, void *stream);
+/* The logits' gradients from the gates' (the choice itself has none): all experts'
+ * columns of every token are written.  A chosen value outside the experts takes part in
+ * nothing; one that stands twice counts twice, in the sum as well. */
+int32_t gtmoe_route_gradient(gtmoe_context *ctx, const gtmoe_route_desc *desc, const void *logits, const int32_t *chosen,
+                             const float *gate_gradients, void *logit_gradients, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
