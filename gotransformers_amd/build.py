@@ -27,6 +27,7 @@ SOURCES = [
     ("lora.hip", []),
     ("grouped.hip", []),
     ("grouped_large.hip", []),
+    ("grouped_fused.hip", []),
     ("grouped_few.hip", []),
     ("adapted.hip", []),
     ("dropout.hip", []),

@@ -21,7 +21,7 @@ struct AdapterTerm {
     const int32_t *adapter = nullptr;  // [rows]; outside [0, adapters): none
     const void *up = nullptr;
     int adapters = 0, rank = 0, ldu = 0;
-    // rows sorted by adapter (grouped_large.hip): the sorted rows' places, group
+    // rows sorted by adapter (grouped_large.h): the sorted rows' places, group
     // `adapters` those without an adapter
     const int32_t *index = nullptr;
 };
@@ -63,9 +63,10 @@ bool few_fits(const GroupedArgs &a);
 hipError_t launch_few(const GroupedArgs &a, int values, hipStream_t s);
 
 // The same for many rows of 16-bit values with both operands staged by LDS-DMA
-// (grouped_large.hip).
+// (grouped_large.h).
 bool large_fits(const GroupedArgs &a, int direction, int value_bytes);
 hipError_t launch_large(const GroupedArgs &a, int direction, int values, hipStream_t s);
+hipError_t launch_large_fused(const GroupedArgs &a, int values, hipStream_t s);
 constexpr int kMaxSortedRank = 64;  // ranks of u in two steps
 
 // u[t][j] = scales[a] sum_k down[a][j][k] x[t][k] for the rows with an adapter a,

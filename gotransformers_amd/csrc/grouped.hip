@@ -321,6 +321,15 @@ bool aligned16(const void *p, long long stride_bytes)
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride_bytes & 15) == 0;
 }
 
+// Whether every row an epilogue of 16-bit values reads or writes is whole 16 bytes.
+bool whole_epilogue(const GroupedArgs &a)
+{
+    const Epilogue &e = a.epilogue;
+    auto whole = [](const void *p, long long stride) { return !p || aligned16(p, stride * 2); };
+    return !e.on || (a.outputs % 8 == 0 && whole(a.out, a.ldo) && whole(e.factor, e.ldfactor) && whole(e.residual, e.ldresidual) &&
+                     whole(e.products, e.ldproducts));
+}
+
 // Workgroups of a product in bm x bn tiles: at most one partial tile per group.
 long long tile_blocks(const GroupedArgs &a, int direction, int bm, int bn)
 {
@@ -394,7 +403,7 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
             if (each <= 32) return launch_staged<T, DIR, 32, 128, 1, 4, 4>(a, da, db, s);
         return launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);
     } else {
-        if (da && db && large_fits(a, DIR, T::kBytes))
+        if (da && db && large_fits(a, DIR, T::kBytes) && (DIR != kGroupedForward || whole_epilogue(a)))
             return launch_large(a, DIR, std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
         if constexpr (DIR == kGroupedWeightGradient) {
             if (tile_blocks(a, DIR, 128, 128) < 256) return launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);

@@ -10,7 +10,7 @@
 //
 // A row stays in registers between its sum and its use: 16 lanes, a wave or a
 // workgroup hold one (`TEAM` threads of `NV` times eight values), rows wider than
-// 65536 are read again.  The gradient keeps dw's sums in registers over the rows
+// 16384 are read again.  The gradient keeps dw's sums in registers over the rows
 // of a team, one partial row per workgroup, which a second kernel adds in a fixed
 // order.
 #include "rows.h"
@@ -446,9 +446,8 @@ Shape shape_of(int rows, int columns)
     if (rows > kFewRows && eights <= 256) return {64, 4};
     if (eights <= 256) return {256, 1};
     if (eights <= 512) return {256, 2};
-    if (eights <= 1024) return {256, 4};
-    if (eights <= 2048) return {256, 8};
-    if (eights <= 8192) return {1024, 8};
+    if (eights <= 1024) return {1024, 1};
+    if (eights <= 2048) return {1024, 2};
     return {1024, 0};
 }
 
@@ -464,9 +463,8 @@ hipError_t with_shape(Shape s, F &&f)
     GTMOE_SHAPE(64, 4)
     GTMOE_SHAPE(256, 1)
     GTMOE_SHAPE(256, 2)
-    GTMOE_SHAPE(256, 4)
-    GTMOE_SHAPE(256, 8)
-    GTMOE_SHAPE(1024, 8)
+    GTMOE_SHAPE(1024, 1)
+    GTMOE_SHAPE(1024, 2)
 #undef GTMOE_SHAPE
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>());
 }

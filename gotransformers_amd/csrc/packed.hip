@@ -92,14 +92,26 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(PackArgs a, int per, l
     }
 }
 
-// gate and up within the limit (a NaN stays one), and whether they were
-template <int ACT>
-__device__ __forceinline__ void limited(float &g, float &u, float limit, bool &g_in, bool &u_in)
+// gate and up held within the limit (a NaN stays one); bit j: value j was beyond it.
+struct Beyond {
+    uint32_t gate = 0, up = 0;
+};
+__device__ __forceinline__ Beyond hold(float (&g)[8], float (&u)[8], float limit)
 {
-    g_in = !(g > limit);
-    u_in = !(fabsf(u) > limit);
-    g = g_in ? g : limit;
-    u = u_in ? u : copysignf(limit, u);
+    Beyond b;
+    if (limit == __builtin_inff()) return b;  // the same for all
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (g[j] > limit) {
+            g[j] = limit;
+            b.gate |= 1u << j;
+        }
+        if (fabsf(u[j]) > limit) {
+            u[j] = copysignf(limit, u[j]);
+            b.up |= 1u << j;
+        }
+    }
+    return b;
 }
 
 template <int VALUES, int ACT>
@@ -115,21 +127,23 @@ __global__ __launch_bounds__(kThreads) void activation_forward_kernel(Activation
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             g[j] = ge.get(j);
-            u[j] = a.up ? ue.get(j) : 1.f;
-            float gl = g[j], ul = u[j];
-            bool gi, ui;
-            limited<ACT>(gl, ul, a.limit, gi, ui);
-            y[j] = a.up ? activated<ACT>(gl) * ul : activated<ACT>(gl);
-        }
-        if (n > 0) {
-            Eight<VALUES> e;
-            e.set(y);
-            store_eight(e, a.out, p.row * a.ldo + p.column, n);
+            u[j] = a.up ? ue.get(j) : 0.f;
         }
         if (a.kept_gate.codes) {
             keep_eight(g, p, n, a.kept_gate);
             if (a.up) keep_eight(u, p, n, a.kept_up);
         }
+        if (n <= 0) continue;
+        hold(g, u, a.limit);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = activated<ACT>(g[j]);
+        if (a.up) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= u[j];
+        }
+        Eight<VALUES> e;
+        e.set(y);
+        store_eight(e, a.out, p.row * a.ldo + p.column, n);
     }
 }
 
@@ -157,19 +171,27 @@ __global__ __launch_bounds__(kThreads) void activation_gradient_kernel(Activatio
                 if (gated) u[j] = ue.get(j);
             }
         }
+        if (!gated) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = 0.f;
+        }
+        const Beyond beyond = hold(g, u, a.limit);
         float y[8], dg[8], du[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (!gated) u[j] = 1.f;
-            bool gi, ui;
-            limited<ACT>(g[j], u[j], a.limit, gi, ui);
-            if (!gated) u[j] = 1.f;
             float act, slope;
             activation_of<ACT, true>(g[j], act, slope);
-            const float d = de.get(j);
-            y[j] = act * u[j];
-            dg[j] = gi ? d * u[j] * slope : 0.f;
-            du[j] = ui ? d * act : 0.f;
+            const float d = de.get(j), c = gated ? u[j] : 1.f;
+            y[j] = act * c;
+            dg[j] = d * c * slope;
+            du[j] = d * act;
+        }
+        if (a.limit < __builtin_inff()) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (beyond.gate >> j & 1) dg[j] = 0.f;
+                if (beyond.up >> j & 1) du[j] = 0.f;
+            }
         }
         Eight<VALUES> e;
         if (a.dgate) {

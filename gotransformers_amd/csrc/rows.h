@@ -156,66 +156,83 @@ enum Codes { kCodesNone = 0, kCodesInt8 = 1, kCodesE4m3 = 2 };
 __device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct Scale {
-    float value;   // as it is stored
-    float times;   // a power of two that keeps value * times and its inverse normal
-    float scaled;  // value * times
-    float inverse; // 1 / scaled, rounded; 0 for codes of 0
+    float value;    // as it is stored
+    float inverse;  // 1 / value, rounded; 0 for a block of zeros
+    bool plain;     // value is 0 or well inside the normal numbers, and so is its inverse
     __device__ __forceinline__ Scale(uint32_t most_bits, int codes)
     {
         const float most = __uint_as_float(most_bits);
         value = codes == kCodesInt8 ? most / 127.f : most / 448.f;
+        plain = value == 0.f || (value >= 0x1p-60f && most_bits < 0x7f800000u);
         if (most_bits >= 0x7f800000u) value = __uint_as_float(0x7fc00000u);
-        times = value < 0x1p-60f ? 0x1p90f : 1.f;
-        scaled = value * times;
-        inverse = value > 0.f ? 1.f / scaled : 0.f;
+        inverse = value >= 0x1p-60f ? 1.f / value : 0.f;
     }
 };
 
-// The code of v as a number.  A quotient by its inverse may be off by a unit in the
-// last place; the remainder v - q scale, exact in an fma, puts it right.
-__device__ __forceinline__ float int8_code(float v, const Scale &s)
+// The size of an int8 code.  inverse is made 2^-22 too small, which is more than all the
+// roundings up to the sum with a half are, so that the whole number below it is the code or
+// one less: which, the remainder a - q scale tells, exact in an fma.
+__device__ __forceinline__ float int8_size(float a, float scale, float inverse, float half)
 {
-    const float a = fabsf(v) * s.times;
-    float q = rintf(a * s.inverse);
-    const float left = fmaf(-q, s.scaled, a), half = 0.5f * s.scaled;
-    q += left >= half ? 1.f : 0.f;
-    q -= left < -half ? 1.f : 0.f;
-    q = s.inverse > 0.f ? fminf(q, 127.f) : 0.f;
-    return copysignf(q, v);
+    const float q = floorf(fmaf(a, inverse, 0.5f));
+    return fminf(q + (fmaf(-q, scale, a) >= half ? 1.f : 0.f), 127.f);
 }
-__device__ __forceinline__ float e4m3_quotient(float v, const Scale &s)
+// The quotient v / scale, rounded: by the inverse, put right by its remainder.
+__device__ __forceinline__ float e4m3_quotient(float v, float scale, float inverse)
 {
-    const float a = v * s.times, q = a * s.inverse;
-    const float r = fmaf(fmaf(-q, s.scaled, a), s.inverse, q);
-    return s.inverse > 0.f ? fminf(fmaxf(r, -448.f), 448.f) : 0.f;
+    const float q = v * inverse;
+    return fminf(fmaxf(fmaf(fmaf(-q, scale, v), inverse, q), -448.f), 448.f);
 }
 
+__device__ __forceinline__ uint32_t int8_bytes(float a, float b, float c, float d)
+{
+    const uint32_t lo = __builtin_amdgcn_perm((uint32_t)(int)b, (uint32_t)(int)a, 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm((uint32_t)(int)d, (uint32_t)(int)c, 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t e4m3_bytes(float a, float b, float c, float d)
+{
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
+}
+
+// Codes of eight values of one block.
+template <int CODES>
+__device__ __forceinline__ uint2 encode_eight_of(const float (&v)[8], const Scale &s)
+{
+    float c[8], scale = s.value, inverse = s.inverse, times = 1.f;
+    const bool odd = __ballot(!s.plain) != 0;
+    if (odd) {
+        // scales next to the subnormal numbers: everything times a power of two; not
+        // finite: codes of 0
+        const bool tiny = scale < 0x1p-60f && scale > 0.f;
+        times = tiny ? 0x1p90f : 1.f;
+        scale = scale == scale ? scale * times : 0.f;
+        inverse = tiny ? 1.f / scale : inverse;
+    }
+    const float half = inverse > 0.f ? 0.5f * scale : __builtin_inff(), below = inverse - inverse * 0x1p-22f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float x = v[e];
+        if (odd) x = s.value == s.value ? x * times : 0.f;
+        c[e] = CODES == kCodesInt8 ? copysignf(int8_size(fabsf(x), scale, below, half), x) : e4m3_quotient(x, scale, inverse);
+    }
+    if constexpr (CODES == kCodesInt8)
+        return make_uint2(int8_bytes(c[0], c[1], c[2], c[3]), int8_bytes(c[4], c[5], c[6], c[7]));
+    else
+        return make_uint2(e4m3_bytes(c[0], c[1], c[2], c[3]), e4m3_bytes(c[4], c[5], c[6], c[7]));
+}
 __device__ __forceinline__ uint2 encode_eight(const float (&v)[8], const Scale &s, int codes)
 {
-    uint32_t w[2];
-    if (codes == kCodesInt8) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            w[i] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[i] |= ((uint32_t)(int)int8_code(v[4 * i + e], s) & 0xffu) << (8 * e);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            int p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_quotient(v[4 * i], s), e4m3_quotient(v[4 * i + 1], s), 0, false);
-            p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_quotient(v[4 * i + 2], s), e4m3_quotient(v[4 * i + 3], s), p, true);
-            w[i] = (uint32_t)p;
-        }
-    }
-    return make_uint2(w[0], w[1]);
+    return codes == kCodesInt8 ? encode_eight_of<kCodesInt8>(v, s) : encode_eight_of<kCodesE4m3>(v, s);
 }
 __device__ __forceinline__ void decode_eight(uint2 c, float scale, int codes, float (&v)[8])
 {
     const uint32_t w[2] = {c.x, c.y};
     if (codes == kCodesInt8) {
+        // a byte plus 128 is an unsigned number, which the hardware converts where it is
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))) * scale;
+        for (int e = 0; e < 8; ++e) v[e] = ((float)((w[e >> 2] ^ 0x80808080u) >> (8 * (e & 3)) & 0xffu) - 128.f) * scale;
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -282,7 +299,19 @@ __device__ __forceinline__ float logistic(float z)
     return z != z ? z : z >= 0.f ? r : e * r;
 }
 
-// act(z) and, where asked for, act'(z).  A NaN stays one.
+// The same where it is a factor of an activation: two of the hardware's functions, good to
+// a unit each, and an argument good to |z| 2^-24.  Below 2^-126 (z < -87) it is 0.
+__device__ __forceinline__ float logistic_factor(float z)
+{
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * z));
+}
+
+__device__ constexpr float kTail[10] = {0.25388533f, 0.25388303f,  0.22827554f, 0.17520681f,  0.12021917f,
+                                        -0.023251647f, 0.14413364f, -0.30252245f, 0.1918485f, -0.041677944f};
+
+// act(z) and, where asked for, act'(z).  A NaN stays one.  Arithmetic bounds these where
+// they stand beside 16-bit rows: SiLU takes 11 of the vector unit's slots, GELU 30, so
+// neither has the care for factors below 2^-126 that would double SiLU's.
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void activation_of(float z, float &a, float &slope)
 {
@@ -293,18 +322,26 @@ __device__ __forceinline__ void activation_of(float z, float &a, float &slope)
         a = z <= 0.f ? 0.f : z;
         slope = z <= 0.f ? 0.f : z != z ? z : 1.f;
     } else if constexpr (ACT == kActivationSilu) {
-        const float s = logistic(z);
+        const float s = logistic_factor(z);
         a = z * s;
         if constexpr (SLOPE) slope = fmaf(a, 1.f - s, s);
     } else if constexpr (ACT == kActivationGelu) {
-        // the normal distribution from its smaller tail: nothing cancels
-        const float c = 0.5f * erfcf(-0.70710678118654752440f * z);
+        // z times the normal distribution, from its smaller tail so that nothing
+        // cancels: with x = |z| / sqrt 2 the tail is e^(-x^2) / 2 times e^(x^2) erfc(x), which
+        // over t in (0, 1], t = 1 / (1 + 0.45 x), is t times a polynomial (a Chebyshev fit to
+        // 4e-8 over x up to 2000)
+        const float size = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(0.31819805153394638598f, size, 1.f));
+        const float e = __builtin_amdgcn_exp2f(-0.72134752044448170368f * (z * z));
+        float p = kTail[9];
+#pragma unroll
+        for (int i = 8; i >= 0; --i) p = fmaf(p, t, kTail[i]);
+        const float tail = 0.5f * e * (t * p), c = z > 0.f ? 1.f - tail : tail;
         a = z * c;
-        if constexpr (SLOPE) slope = fmaf(z * 0.39894228040143267794f, exp_minus(0.5f * z * z), c);
+        if constexpr (SLOPE) slope = fmaf(z * 0.39894228040143267794f, e, c);
     } else {
         // 0.5 z (1 + tanh(u)) = z logistic(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)
         constexpr float k = 1.59576912160573071176f, c3 = 0.044715f;
-        const float s = logistic(k * z * fmaf(c3 * z, z, 1.f));
+        const float s = logistic_factor(k * z * fmaf(c3 * z, z, 1.f));
         a = z * s;
         if constexpr (SLOPE) slope = fmaf(a * (1.f - s), k * fmaf(3.f * c3 * z, z, 1.f), s);
     }

@@ -331,7 +331,7 @@ def test_norm_gradient_without_rows(ctx):
 
 def act_error(z, name):
     """Relative to act(z) and to the sizes of act' 's terms: the library's function (2^-20 each of
-    two), and the rounded argument of an exponential: |z| for SiLU, twice z^2 for GELU (of
+    two; GELU's own polynomial is good to 4e-8 and its ten roundings, 2^-20), and the rounded argument of an exponential: |z| for SiLU, twice z^2 for GELU (of
     erfc about 2 x^2 = z^2 per relative error of its argument), for its tanh form 2 |u|, four roundings."""
     if name in ("none", "relu"):
         return np.zeros_like(z)
@@ -342,10 +342,11 @@ def act_error(z, name):
     return 2.0 ** -19 + 8 * np.abs(1.6 * (z + 0.044715 * z ** 3)) * U
 
 
-def act_last_steps(z):
-    """Absolutely, besides: a factor of act(z) below 2^-126 has steps of 2^-149, so that 16 units
-    of it are 2^-145, which the product with z (and act' with z and 1) multiplies."""
-    return (np.abs(z) + 1) * 2.0 ** -145
+def act_last_steps(z, name):
+    """Absolutely, besides: a factor s of act(z) below 2^-126 may be 0.  act(z) is z s, and act' is s + z s
+    (1 - s) d (GELU: z e / 2.5) with d = 1, for GELU's tanh form the slope of its argument."""
+    d = 1.6 * (1 + 3 * 0.044715 * z * z) if name == "gelu_tanh" else 1.0
+    return (np.abs(z) * d + 1) * 2.0 ** -126
 
 
 def z_values(rng, rows, columns):
@@ -387,7 +388,7 @@ def test_activation(ctx, kind, act, codes, scale_columns, rows, columns, layout,
         a, c, da, dc, size = plain.gated(gate, up, act, limit)
         z = np.minimum(gate, limit or np.inf)
         e = act_error(z, act)
-        near(out.get(), a * c, np.abs(a * c) * (e + 2 * U) + np.abs(c) * act_last_steps(z), kind)
+        near(out.get(), a * c, np.abs(a * c) * (e + 2 * U) + np.abs(c) * act_last_steps(z, act), kind)
         return a, c, da, dc, size, e
 
     check(y, g.get(), u.get() if u else None)
@@ -406,9 +407,9 @@ def test_activation(ctx, kind, act, codes, scale_columns, rows, columns, layout,
     a, c, da, dc, size, e = check(again, gv, uv)
     dyv = dy.get()
     inside = gv <= (limit or np.inf)
-    near(dg.get(), dyv * c * da, np.abs(dyv * c) * inside * (size * (2 * e + 4 * U) + act_last_steps(gv)), kind)
+    near(dg.get(), dyv * c * da, np.abs(dyv * c) * inside * (size * (2 * e + 4 * U) + act_last_steps(gv, act)), kind)
     if u:
-        near(du.get(), dyv * a * dc, np.abs(dyv * dc) * (np.abs(a) * (e + 2 * U) + act_last_steps(gv)), kind)
+        near(du.get(), dyv * a * dc, np.abs(dyv * dc) * (np.abs(a) * (e + 2 * U) + act_last_steps(gv, act)), kind)
         du.check_outside()
     for r in (y, again, dg):
         r.check_outside()
