@@ -718,6 +718,10 @@ def dropout(ctx, desc, inputs_ptr, base_ptr, outputs_ptr, rate, seed, offset, st
 # a block in plain rows (raw device addresses)
 # --------------------------------------------------------------------------
 
+# a workspace's size where the caller gives none: as large as the call needs
+_ENOUGH = C.c_size_t(-1).value
+
+
 def _scales_per_row(columns, scale_columns):
     return -(-columns // scale_columns) if scale_columns else 1
 
@@ -767,8 +771,8 @@ def norm_gradient(ctx, desc, output_gradients_ptr, sums_ptr, weights_ptr, sum_gr
                   weight_gradients_ptr, gradient_values, accumulate=False, workspace_ptr=None, stream=None,
                   workspace_bytes=None):
     """The gradients of inputs and weights (gtmoe_norm_gradient).
-    workspace_bytes: the workspace's size, norm_workspace_bytes(desc) unless given."""
-    n = norm_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    workspace_bytes: the workspace's size, taken for norm_workspace_bytes(desc) or more unless given."""
+    n = _ENOUGH if workspace_bytes is None else workspace_bytes
     ctx.check(library().gtmoe_norm_gradient(ctx.handle, C.byref(desc), output_gradients_ptr, sums_ptr, weights_ptr,
                                             sum_gradients_ptr, input_gradients_ptr, weight_gradients_ptr, gradient_values,
                                             1 if accumulate else 0, workspace_ptr, n, stream))
@@ -823,8 +827,8 @@ def grouped_bias_workspace_bytes(desc):
 def grouped_bias_gradient(ctx, desc, offsets_ptr, output_gradients_ptr, bias_gradients_ptr, gradient_values,
                           accumulate=False, workspace_ptr=None, stream=None, workspace_bytes=None):
     """bias_gradients[g] (+)= sum of output_gradients[r] over the group's rows.
-    workspace_bytes: the workspace's size, grouped_bias_workspace_bytes(desc) unless given."""
-    n = grouped_bias_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    workspace_bytes: the workspace's size, taken for grouped_bias_workspace_bytes(desc) or more unless given."""
+    n = _ENOUGH if workspace_bytes is None else workspace_bytes
     ctx.check(library().gtmoe_grouped_bias_gradient(ctx.handle, C.byref(desc), offsets_ptr, output_gradients_ptr,
                                                     bias_gradients_ptr, gradient_values, 1 if accumulate else 0,
                                                     workspace_ptr, n, stream))
@@ -847,8 +851,8 @@ def route_workspace_bytes(desc):
 def route_forward(ctx, desc, logits_ptr, biases_ptr, chosen_ptr, gates_ptr, expert_offsets_ptr=None,
                   rows_for_expert_ptr=None, places_ptr=None, workspace_ptr=None, stream=None, workspace_bytes=None):
     """Every token's experts and gates, and the rows in expert order (gtmoe_route_forward).
-    workspace_bytes: the workspace's size, route_workspace_bytes(desc) unless given."""
-    n = route_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    workspace_bytes: the workspace's size, taken for route_workspace_bytes(desc) or more unless given."""
+    n = _ENOUGH if workspace_bytes is None else workspace_bytes
     ctx.check(library().gtmoe_route_forward(ctx.handle, C.byref(desc), logits_ptr, biases_ptr, chosen_ptr, gates_ptr,
                                             expert_offsets_ptr, rows_for_expert_ptr, places_ptr, workspace_ptr, n, stream))
 

@@ -5,18 +5,21 @@
 //   gate_j = scale s_j / (renormalize ? sum over the chosen s : 1)
 // the rows in expert order (offsets, tokens, places), and the logits' gradient.
 //
-// Order.  Values that are compared become whole numbers of the same order: fp32
-// logits 32 bits, s + b and sums of two 64 bits of the fp64 value, because
-// sums of neighbouring fp32 values tie where the exact ones do not.  A round takes
-// the team's largest number; lanes hold consecutive experts, so the first lane
-// that has it holds the lowest index.  Keys 0 (not to be chosen: another group,
-// already chosen, past the last) and 1 (after everything else: a logit of -inf, a NaN)
-// lie below every number's.
+// Order.  Without biases experts compare by their logits, as whole numbers of the
+// same order; with them by s + b in fp64, because neighbouring fp32 values tie where
+// the exact ones do not.  16 lanes (64 above 256 experts) hold a token's experts,
+// consecutive ones in a lane.  A round takes their largest key; the first lane
+// that has it holds the lowest index.  Keys below every number's: of experts not to
+// be chosen (another group's, chosen already: 0 or NaN, which a maximum passes over)
+// and above them those that come after all others (logits of -inf and NaN: 1 or -inf;
+// places past the last expert too, which the lower indexes keep from being chosen).
 //
-// Gates come from differences of logarithms of the chosen scores, so that neither
-// large nor very negative logits leave 0 / 0:
-//   softmax   log s_j - log s_i = l_j - l_i
-//   logistic  log s = min(l, 0) - log(1 + e^-|l|)
+// Groups.  A group of one, two, four, ... lanes finds its best two by exchanges of
+// neighbours, any other through LDS; a group's place is the number of groups
+// before it.
+//
+// Renormalized gates take the chosen scores by their largest, so that neither large nor
+// very negative logits leave 0 / 0:  s = e^l, or e^min(l, 0) / (1 + e^-|l|).
 //
 // Lists.  A workgroup takes `each` consecutive tokens and writes how often each
 // expert was chosen among them; the second kernel adds the counts of the
@@ -34,9 +37,10 @@ namespace {
 
 constexpr int kThreads = 256;       // of every kernel but the one that does all
 constexpr int kAllThreads = 512;
+// Of the first kernel: a workgroup's tokens in one pass of its waves, four waves per SIMD.
+constexpr int choose_threads(int experts_per_lane) { return experts_per_lane > 8 ? 512 : 1024; }
 constexpr int kMostTokens = 256;    // of one workgroup: four words of a mask
 constexpr int kMostExperts = 1024;
-constexpr int kMostChosen = 32;
 constexpr int kMostGroups = 64;
 constexpr int kMostHeld = 256;      // workgroups whose counts the second kernel adds itself
 
@@ -47,26 +51,87 @@ __device__ __forceinline__ uint32_t order_of(float v)
     if (v != v || b == 0xff800000u) return 1;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ uint64_t order_of(double v)
-{
-    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
-    if (v != v) return 1;
-    return b >> 63 ? ~b : b | 0x8000000000000000ull;
-}
-__device__ __forceinline__ double value_of(uint64_t order)
-{
-    return __longlong_as_double((long long)(order >> 63 ? order & 0x7fffffffffffffffull : ~order));
-}
+// The logit a key above 1 stands for.
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 template <int CTRL>
-__device__ __forceinline__ uint64_t moved64(uint64_t v)
+__device__ __forceinline__ double moved64(double v)
 {
-    return (uint64_t)moved<CTRL>((uint32_t)(v >> 32)) << 32 | moved<CTRL>((uint32_t)v);
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)moved<CTRL>((uint32_t)(b >> 32)) << 32 | moved<CTRL>((uint32_t)b)));
 }
-__device__ __forceinline__ uint64_t read64(uint64_t v, int lane)
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved64(uint32_t v) { return moved<CTRL>(v); }
+__device__ __forceinline__ double lane_value64(double v, int lane)
 {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                            (uint32_t)__builtin_amdgcn_readlane((int)b, lane)));
+}
+__device__ __forceinline__ double permuted(int from, double v)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(b >> 32)) << 32 |
+                                            (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)b)));
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+__device__ __forceinline__ uint32_t smaller(uint32_t a, uint32_t b) { return min(a, b); }
+// (as one instruction each: nothing here is a signalling NaN, which fmax would first quiet)
+__device__ __forceinline__ double larger(double a, double b)
+{
+    double r;
+    asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ double smaller(double a, double b)
+{
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+// keys of what is never chosen, and of what comes last
+template <class Key>
+struct Never;
+template <>
+struct Never<uint32_t> {
+    static __device__ __forceinline__ uint32_t last() { return 1; }
+    static __device__ __forceinline__ uint32_t unless(bool gone, uint32_t k) { return gone ? 0 : k; }
+};
+template <>
+struct Never<double> {
+    static __device__ __forceinline__ double last() { return -__builtin_inf(); }
+    static __device__ __forceinline__ double unless(bool gone, double k)
+    {
+        return __hiloint2double(gone ? 0x7ff80000 : __double2hiint(k), __double2loint(k));
+    }
+};
+
+// e^x for x <= 0 in fp64: powers of two taken out, then the series to r^11 / 11! (below
+// 1e-14 of the whole for |r| <= log(2) / 2).
+__device__ __forceinline__ double exp64(double x)
+{
+    x = fmax(x, -750.0);
+    const double k = rint(x * 1.4426950408889634);
+    double r = fma(k, -6.93147180369123816490e-01, x);  // the first 32 bits of log 2
+    r = fma(k, -1.90821492927058770002e-10, r);
+    constexpr double inverse[12] = {1.0,       1.0,        1.0 / 2,     1.0 / 6,      1.0 / 24,      1.0 / 120,
+                                    1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
+    double p = inverse[11];
+#pragma unroll
+    for (int i = 10; i >= 0; --i) p = fma(p, r, inverse[i]);
+    return ldexp(p, (int)k);
+}
+// 1 / d for d of the size of a number of experts at most
+__device__ __forceinline__ double inverse64(double d)
+{
+    double x = __builtin_amdgcn_rcp(d);
+    x = fma(fma(-d, x, 1.0), x, x);
+    return fma(fma(-d, x, 1.0), x, x);
+}
+__device__ __forceinline__ double logistic64(float l)
+{
+    const double e = exp64(-fabs((double)l)), r = inverse64(1.0 + e);
+    return l >= 0.f ? r : e * r;
 }
 
 // The team's largest key and sums.
@@ -77,13 +142,14 @@ __device__ __forceinline__ uint32_t team_largest(uint32_t v)
     return wave_max(v);
 }
 template <int TEAM>
-__device__ __forceinline__ uint64_t team_largest(uint64_t v)
+__device__ __forceinline__ double team_largest(double v)
 {
-    v = max(v, moved64<kDppPairs>(v));
-    v = max(v, moved64<kDppFours>(v));
-    v = max(v, moved64<kDppEights>(v));
-    v = max(v, moved64<kDppSixteens>(v));
-    if constexpr (TEAM == 64) v = max(max(read64(v, 0), read64(v, 16)), max(read64(v, 32), read64(v, 48)));
+    v = larger(v, moved64<kDppPairs>(v));
+    v = larger(v, moved64<kDppFours>(v));
+    v = larger(v, moved64<kDppEights>(v));
+    v = larger(v, moved64<kDppSixteens>(v));
+    if constexpr (TEAM == 64)
+        v = larger(larger(lane_value64(v, 0), lane_value64(v, 16)), larger(lane_value64(v, 32), lane_value64(v, 48)));
     return v;
 }
 template <int TEAM>
@@ -130,62 +196,81 @@ __device__ __forceinline__ void load_logits(float (&l)[EPL], const void *base, l
     }
 }
 
-// log(logistic(l)) = upper + lower, upper = min(l, 0) exact, lower in (-log 2, 0]
-__device__ __forceinline__ float log_logistic_lower(float l) { return -log1pf(exp_minus(l)); }
-
-// The chosen ones' shares s_j / sum, `mine` of the team's slots in this lane: l, whether
-// there is one.  Two slots per lane where k exceeds the team.
-template <int TEAM, int SLOTS>
-__device__ __forceinline__ void shares_of(float (&share)[SLOTS], const float (&l)[SLOTS], const bool (&have)[SLOTS], bool logistic_scores)
+// The share s / sum of this lane's choice among the team's, l its logit.
+template <int TEAM>
+__device__ __forceinline__ float share_of(float l, bool have, bool logistic_scores)
 {
-    float upper[SLOTS], lower[SLOTS], most = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-        upper[i] = logistic_scores ? fminf(l[i], 0.f) : l[i];
-        if (l[i] != l[i]) upper[i] = l[i];
-        lower[i] = logistic_scores ? log_logistic_lower(l[i]) : 0.f;
-        if (have[i] && upper[i] > most) most = upper[i];
-    }
-    most = team_most<TEAM>(most);
+    // s = e^upper times a number between 1/2 and 1
+    const float upper = logistic_scores && l > 0.f ? 0.f : l;
+    float most = team_most<TEAM>(have ? upper : -__builtin_inff());
     if (most == -__builtin_inff()) most = 0.f;  // nothing but -inf: every share is 0
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-        const float d = upper[i] - most;
-        // (upper is at most `most`; +inf beside itself is NaN)
-        share[i] = have[i] ? exp_minus(d) * (logistic_scores ? expf(lower[i]) : 1.f) : 0.f;
-        sum += share[i];
-    }
-    sum = team_total<TEAM>(sum);
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) share[i] = sum == 0.f ? 0.f : share[i] / sum;
+    // (upper is at most `most`; +inf beside itself is NaN)
+    float s = exp_minus(upper - most);
+    if (logistic_scores) s *= inverse_of(1.f + exp_minus(l));
+    s = have ? s : 0.f;
+    const float sum = team_total<TEAM>(s);
+    return sum == 0.f ? 0.f : s / sum;
 }
 
 __device__ __forceinline__ int group_of(int e, uint32_t group_inverse) { return (int)((uint32_t)e * group_inverse >> 22); }
 
-// LDS of a wave for the groups' choice: its tokens' keys and the groups' keys and marks.
+// The best two keys of a group, and merged with another's.
+template <class Key>
+struct Best {
+    Key one = Never<Key>::last(), two = Never<Key>::last();
+    __device__ __forceinline__ void add(Key k)
+    {
+        two = larger(two, smaller(one, k));
+        one = larger(one, k);
+    }
+    template <int CTRL>
+    __device__ __forceinline__ void merge()
+    {
+        const Key o1 = moved64<CTRL>(one), o2 = moved64<CTRL>(two);
+        two = larger(smaller(one, o1), larger(two, o2));
+        one = larger(one, o1);
+    }
+};
+// What groups compare by: the sum of their best one or two.  Without biases the keys
+// are logits': of two, their scores (a softmax's without the common sum).
+__device__ __forceinline__ double group_total(const ChooseArgs &a, const Best<double> &b, float)
+{
+    return a.group_best == 2 && b.two > -__builtin_inf() ? b.one + b.two : b.one;
+}
+__device__ __forceinline__ double group_total(const ChooseArgs &a, const Best<uint32_t> &b, float most)
+{
+    if (b.one <= 1) return -__builtin_inf();
+    const float l1 = logit_of(b.one), l2 = logit_of(b.two);
+    if (a.group_best == 1) return (double)l1;
+    double s1 = a.logistic ? logistic64(l1) : exp64((double)l1 - (double)most);
+    if (b.two > 1) s1 += a.logistic ? logistic64(l2) : exp64((double)l2 - (double)most);
+    return s1;
+}
+
+// How groups are found: not at all; as 1, 2, 4, 8 or 16 lanes each; through LDS.
+enum GroupForm { kNoGroups = 0, kLaneGroups = 1, kAnyGroups = 2 };
 template <class Key, int EPL>
 struct WaveGroups {
     Key keys[64 * EPL];
-    Key best[4][kMostGroups];
-    uint32_t allowed[4][kMostGroups];
+    double total[4][kMostGroups];
+    uint8_t allowed[4][kMostGroups];
 };
-struct NoGroups {
+struct NoShared {
 };
 
-// tokens [first, last) of the workgroup.  Calls take(t, slot, expert) for each choice.
-template <int VALUES, class Key, int TEAM, int EPL, bool GROUPS, class Shared, class F>
+// tokens [first, last) of the workgroup.  Calls take(t, expert) for each choice.
+template <int VALUES, class Key, int TEAM, int EPL, int GROUPS, class Shared, class F>
 __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, int last, Shared *shared, F &&take)
 {
-    constexpr int TEAMS = 64 / TEAM, SLOTS = TEAM >= kMostChosen ? 1 : kMostChosen / TEAM;
-    constexpr bool WIDE = sizeof(Key) == 8;
+    constexpr int TEAMS = 64 / TEAM;
+    constexpr bool BIASED = sizeof(Key) == 8;
     const int lane = threadIdx.x & 63, in = lane % TEAM, team = lane / TEAM;
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int e0 = in * EPL;
     float b[EPL];
-    if constexpr (WIDE) {
+    if constexpr (BIASED) {
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) b[i] = a.biases && e0 + i < a.experts ? a.biases[e0 + i] : 0.f;
+        for (int i = 0; i < EPL; ++i) b[i] = e0 + i < a.experts ? a.biases[e0 + i] : 0.f;
     }
     for (int t0 = first + wave * TEAMS; t0 < last; t0 += waves * TEAMS) {
         const int t = min(t0 + team, last - 1);  // teams past the last repeat it and keep nothing
@@ -193,8 +278,7 @@ __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, in
         float l[EPL];
         load_logits<VALUES>(l, a.logits, (long long)t * a.ldlogits, e0, a.experts);
         float most = 0.f, sum = 0.f;  // of a softmax over all experts
-        const bool over_all = !a.logistic && (WIDE || !a.renormalize);
-        if (over_all) {
+        if (!a.logistic && (BIASED || !a.renormalize || GROUPS != kNoGroups)) {
             most = l[0];
 #pragma unroll
             for (int i = 1; i < EPL; ++i) most = l[i] > most || most != most ? l[i] : most;
@@ -207,28 +291,52 @@ __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, in
             }
         }
         Key key[EPL];
-        if constexpr (WIDE) {
-            double s[EPL], total = 0;
+        if constexpr (BIASED) {
+            double s[EPL], inverse = 1.0;
+            if (a.logistic) {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) s[i] = logistic64(l[i]);
+            } else {
+                double total = 0;
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) {
+                    s[i] = exp64((double)l[i] - (double)most);
+                    total += s[i];
+                }
+                inverse = inverse64(team_total<TEAM>(total));
+            }
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                s[i] = a.logistic ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - (double)most);
-                total += s[i];
-            }
-            if (!a.logistic) {
-                total = 1.0 / team_total<TEAM>(total);
-#pragma unroll
-                for (int i = 0; i < EPL; ++i) s[i] *= total;
-            }
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) {
-                const uint64_t o = order_of(s[i] + (double)b[i]);
-                key[i] = e0 + i >= a.experts ? 0 : l[i] != l[i] || l[i] == -__builtin_inff() ? 1 : o;
+                // (a bias of -inf stays before what comes last)
+                key[i] = l[i] > -__builtin_inff() ? larger(fma(s[i], inverse, (double)b[i]), -1e300) : Never<double>::last();
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) key[i] = e0 + i >= a.experts ? 0 : order_of(l[i]);
+            for (int i = 0; i < EPL; ++i) key[i] = order_of(l[i]);
         }
-        if constexpr (GROUPS) {
+        if constexpr (GROUPS == kLaneGroups) {
+            Best<Key> best;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) best.add(key[i]);
+            const int width = a.experts / a.groups / EPL;  // lanes of a group
+            if (width > 1) best.template merge<kDppPairs>();
+            if (width > 2) best.template merge<kDppFours>();
+            if (width > 4) best.template merge<kDppEights>();
+            if (width > 8) best.template merge<kDppSixteens>();
+            const double mine = group_total(a, best, most);
+            const int g = in / width;
+            int before = 0;
+            for (int o = 0; o < a.groups; o += 4) {
+                double other[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) other[i] = permuted(4 * (team * TEAM + (o + i) * width), mine);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    before += o + i < a.groups && (other[i] > mine || (other[i] == mine && o + i < g));
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) key[i] = Never<Key>::unless(before >= a.chosen_groups, key[i]);
+        } else if constexpr (GROUPS == kAnyGroups) {
             auto &w = shared[wave];
             Key *keys = w.keys + team * (TEAM * EPL);
 #pragma unroll
@@ -236,88 +344,69 @@ __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, in
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const int each = a.experts / a.groups;
             for (int g = in; g < a.groups; g += TEAM) {
-                Key one = 0, two = 0;
-                for (int i = 0; i < each; ++i) {
-                    const Key k = keys[g * each + i];
-                    two = k > one ? one : k > two ? k : two;
-                    one = k > one ? k : one;
-                }
-                if constexpr (WIDE)
-                    if (a.group_best == 2 && two > 1) one = order_of(value_of(one) + value_of(two));
-                w.best[team][g] = one;
+                Best<Key> best;
+                for (int i = 0; i < each; ++i) best.add(keys[g * each + i]);
+                w.total[team][g] = group_total(a, best, most);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             for (int g = in; g < a.groups; g += TEAM) {
-                const Key mine = w.best[team][g];
+                const double mine = w.total[team][g];
                 int before = 0;
                 for (int o = 0; o < a.groups; ++o) {
-                    const Key k = w.best[team][o];
-                    before += k > mine || (k == mine && o < g);
+                    const double other = w.total[team][o];
+                    before += other > mine || (other == mine && o < g);
                 }
                 w.allowed[team][g] = before < a.chosen_groups;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int i = 0; i < EPL; ++i)
-                if (e0 + i < a.experts && !w.allowed[team][group_of(e0 + i, a.group_inverse)]) key[i] = 0;
+                key[i] = Never<Key>::unless(e0 + i >= a.experts || !w.allowed[team][group_of(e0 + i, a.group_inverse)], key[i]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        // slot j is lane j % TEAM's
-        int expert[SLOTS];
-        float logit[SLOTS];
-        bool have[SLOTS];
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-            expert[i] = 0;
-            logit[i] = 0.f;
-            have[i] = in + i * TEAM < a.k;
-        }
+        // choice j is lane j's
+        int expert = 0;
         for (int j = 0; j < a.k; ++j) {
             Key top = key[0];
 #pragma unroll
-            for (int i = 1; i < EPL; ++i) top = max(top, key[i]);
+            for (int i = 1; i < EPL; ++i) top = larger(top, key[i]);
             top = team_largest<TEAM>(top);
-            int at = -1;
-            float l_at = 0.f;
+            // who has it, one bit a lane; the lowest bit of each team; of that lane the
+            // lowest expert (masks of lanes: the scalar unit's work)
+            uint64_t has[EPL], who = 0;
 #pragma unroll
-            for (int i = EPL - 1; i >= 0; --i)
-                if (key[i] == top) {
-                    at = i;
-                    l_at = l[i];
-                }
-            uint64_t who = __ballot(at >= 0);
-            if constexpr (TEAM < 64) who = who >> (team * TEAM) & ((1ull << (TEAM & 63)) - 1);
-            const int winner = __builtin_ctzll(who);
-            const bool won = in == winner;
-#pragma unroll
-            for (int i = 0; i < EPL; ++i)
-                if (won && i == at) key[i] = 0;
-            const int from = 4 * (team * TEAM + winner);
-            const int e = __builtin_amdgcn_ds_bpermute(from, e0 + at);
-            const float le = __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(l_at)));
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i)
-                if (j == in + i * TEAM) {
-                    expert[i] = e;
-                    logit[i] = le;
-                }
-        }
-        float gate[SLOTS];
-        if (a.renormalize) {
-            shares_of<TEAM>(gate, logit, have, a.logistic);
-        } else {
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i)
-                gate[i] = a.logistic ? logistic(logit[i]) : sum == 0.f ? 0.f : exp_minus(logit[i] - most) / sum;
-        }
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i)
-            if (have[i] && here) {
-                const long long at = (long long)t * a.k + in + i * TEAM;
-                a.chosen[at] = expert[i];
-                a.gates[at] = gate[i] * a.scale;
-                take(t, expert[i]);
+            for (int i = 0; i < EPL; ++i) {
+                has[i] = __ballot(key[i] == top);
+                who |= has[i];
             }
+            uint64_t first_lanes = who & ~(who - (TEAM == 16 ? 0x0001000100010001ull : 1ull));
+            const int winner = __builtin_ctzll(TEAM == 16 ? first_lanes >> (team * (TEAM & 63)) : first_lanes);
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                const bool it = __builtin_amdgcn_inverse_ballot_w64(first_lanes & has[i]);
+                first_lanes &= ~has[i];
+                at = it ? i : at;
+                key[i] = Never<Key>::unless(it, key[i]);
+            }
+            const int e = winner * EPL + __builtin_amdgcn_ds_bpermute(4 * (team * TEAM + winner), at);
+            expert = j == in ? e : expert;
+        }
+        float logit, gate;
+        {
+            float v[1];
+            load_logits<VALUES>(v, a.logits, (long long)t * a.ldlogits, expert, a.experts);
+            logit = v[0];
+        }
+        const bool have = in < a.k;
+        if (a.renormalize) gate = share_of<TEAM>(logit, have, a.logistic);
+        else gate = a.logistic ? logistic(logit) : sum == 0.f ? 0.f : exp_minus(logit - most) / sum;
+        if (have && here) {
+            const long long at = (long long)t * a.k + in;
+            a.chosen[at] = expert;
+            a.gates[at] = gate * a.scale;
+            take(t, expert);
+        }
     }
 }
 
@@ -354,44 +443,41 @@ __device__ __forceinline__ void add_before(int *start, const int *count, int exp
     }
 }
 
-// The places of tokens [first, last): behind start[e], in the order of the tokens, which
-// mask[w][e] has a bit for each.
-__device__ __forceinline__ void place_tokens(const ChooseArgs &a, int first, int last, const int *start,
-                                             const unsigned long long *mask)
+// The place of choice i of the tokens from `first` on, expert e: behind start[e], in the order of
+// the tokens, which mask[w][e] has a bit for each.
+__device__ __forceinline__ void place(const ChooseArgs &a, int first, int i, int e, const int *start, const unsigned long long *mask)
 {
-    const long long end = (long long)last * a.k;
-    for (long long i = (long long)first * a.k + threadIdx.x; i < end; i += blockDim.x) {
-        const int t = (int)(i / a.k), e = a.chosen[i], at = t - first;
-        int place = start[e];
-        for (int w = 0; w < at >> 6; ++w) place += __popcll(mask[w * a.experts + e]);
-        place += __popcll(mask[(at >> 6) * a.experts + e] & ((1ull << (at & 63)) - 1));
-        if (a.rows) a.rows[place] = t;
-        if (a.places) a.places[i] = place;
-    }
+    const int at = i / a.k;
+    int to = start[e];
+    for (int w = 0; w < at >> 6; ++w) to += __popcll(mask[w * a.experts + e]);
+    to += __popcll(mask[(at >> 6) * a.experts + e] & ((1ull << (at & 63)) - 1));
+    if (a.rows) a.rows[to] = first + at;
+    if (a.places) a.places[(long long)first * a.k + i] = to;
 }
 
-template <int VALUES, class Key, int TEAM, int EPL, bool GROUPS>
-__global__ __launch_bounds__(kThreads) void choose_kernel(ChooseArgs a)
+template <int VALUES, class Key, int TEAM, int EPL, int GROUPS>
+__global__ __launch_bounds__(choose_threads(EPL)) void choose_kernel(ChooseArgs a)
 {
-    typedef typename std::conditional<GROUPS, WaveGroups<Key, EPL>, NoGroups>::type Shared;
-    __shared__ Shared shared[GROUPS ? kThreads / 64 : 1];
+    constexpr int THREADS = choose_threads(EPL);
+    typedef typename std::conditional<GROUPS == kAnyGroups, WaveGroups<Key, EPL>, NoShared>::type Shared;
+    __shared__ Shared shared[GROUPS == kAnyGroups ? THREADS / 64 : 1];
     __shared__ int count[TEAM * EPL];
-    for (int e = threadIdx.x; e < TEAM * EPL; e += kThreads) count[e] = 0;
+    for (int e = threadIdx.x; e < TEAM * EPL; e += THREADS) count[e] = 0;
     __syncthreads();
     const int first = blockIdx.x * a.each, last = min(first + a.each, a.tokens);
     choose_tokens<VALUES, Key, TEAM, EPL, GROUPS>(a, first, last, shared, [&](int, int e) { atomicAdd(&count[e], 1); });
     if (!a.counts) return;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.ldcounts; e += kThreads)
+    for (int e = threadIdx.x; e < a.ldcounts; e += THREADS)
         a.counts[(long long)blockIdx.x * a.ldcounts + e] = e < a.experts ? (uint16_t)count[e] : (uint16_t)0;
 }
 
 // All tokens by one workgroup, lists included.
-template <int VALUES, class Key, int TEAM, int EPL, bool GROUPS>
+template <int VALUES, class Key, int TEAM, int EPL, int GROUPS>
 __global__ __launch_bounds__(kAllThreads) void choose_all_kernel(ChooseArgs a)
 {
-    typedef typename std::conditional<GROUPS, WaveGroups<Key, EPL>, NoGroups>::type Shared;
-    __shared__ Shared shared[GROUPS ? kAllThreads / 64 : 1];
+    typedef typename std::conditional<GROUPS == kAnyGroups, WaveGroups<Key, EPL>, NoShared>::type Shared;
+    __shared__ Shared shared[GROUPS == kAnyGroups ? kAllThreads / 64 : 1];
     __shared__ int start[TEAM * EPL], count[TEAM * EPL];
     __shared__ unsigned long long mask[kMostTokens / 64 * TEAM * EPL];
     const int words = (a.tokens + 63) >> 6;
@@ -410,7 +496,7 @@ __global__ __launch_bounds__(kAllThreads) void choose_all_kernel(ChooseArgs a)
     __syncthreads();
     add_before(start, count, a.experts, a.offsets);
     __syncthreads();
-    place_tokens(a, 0, a.tokens, start, mask);
+    for (int i = threadIdx.x; i < a.tokens * a.k; i += kAllThreads) place(a, 0, i, a.chosen[i], start, mask);
 }
 
 // Counts of up to eight experts of one workgroup.
@@ -456,102 +542,107 @@ __global__ __launch_bounds__(kThreads) void count_before_kernel(ChooseArgs a, in
     }
 }
 
+// HELD: the counts of all workgroups are added up here, by as many threads as their
+// loads can be in flight together.  The tokens' choices are on their way meanwhile.
+constexpr int kPlaceThreads = 1024, kAhead = 2;
+
 template <bool HELD>
-__global__ __launch_bounds__(kThreads) void place_kernel(ChooseArgs a, int blocks)
+__global__ __launch_bounds__(kPlaceThreads) void place_kernel(ChooseArgs a, int blocks)
 {
     __shared__ int start[kMostExperts], count[kMostExperts];
     __shared__ unsigned long long mask[kMostTokens / 64 * kMostExperts];
     const int first = blockIdx.x * a.each, last = min(first + a.each, a.tokens);
-    const int words = (last - first + 63) >> 6;
-    for (int i = threadIdx.x; i < words * a.experts; i += kThreads) mask[i] = 0;
-    for (int e = threadIdx.x; e < a.ldcounts; e += kThreads) {
+    const int words = (last - first + 63) >> 6, choices = (last - first) * a.k;
+    const int32_t *chosen = a.chosen + (long long)first * a.k;
+    int ahead[kAhead];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+        const int i = threadIdx.x + x * kPlaceThreads;
+        ahead[x] = i < choices ? chosen[i] : 0;
+    }
+    for (int i = threadIdx.x; i < words * a.experts; i += kPlaceThreads) mask[i] = 0;
+    for (int e = threadIdx.x; e < a.ldcounts; e += kPlaceThreads) {
         start[e] = HELD ? 0 : a.before[(long long)blockIdx.x * a.ldcounts + e];
         count[e] = HELD ? 0 : a.totals[e];
     }
-    __syncthreads();
-    if constexpr (HELD) {
-        const int columns = a.ldcounts / 8, column = threadIdx.x % columns;
-        int all[8] = {0, 0, 0, 0, 0, 0, 0, 0}, before[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if ((int)threadIdx.x < kThreads / columns * columns) {
-#pragma unroll 8
-            for (int b = threadIdx.x / columns; b < blocks; b += kThreads / columns) {
-                const Counts8 c = *reinterpret_cast<const Counts8 *>(a.counts + (long long)b * a.ldcounts + column * 8);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    all[i] += c.n[i];
-                    before[i] += b < (int)blockIdx.x ? c.n[i] : 0;
-                }
-            }
+    int all[8] = {0, 0, 0, 0, 0, 0, 0, 0}, before[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const int columns = a.ldcounts / 8, column = threadIdx.x % columns, row = threadIdx.x / columns, rows = kPlaceThreads / columns;
+    if (HELD && row < rows) {
+#pragma unroll 4
+        for (int b = row; b < blocks; b += rows) {
+            const Counts8 c = *reinterpret_cast<const Counts8 *>(a.counts + (long long)b * a.ldcounts + column * 8);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (all[i]) atomicAdd(&count[column * 8 + i], all[i]);
-                if (before[i]) atomicAdd(&start[column * 8 + i], before[i]);
+                all[i] += c.n[i];
+                before[i] += b < (int)blockIdx.x ? c.n[i] : 0;
             }
         }
     }
-    const long long end = (long long)last * a.k;
-    for (long long i = (long long)first * a.k + threadIdx.x; i < end; i += kThreads) {
-        const int at = (int)(i / a.k) - first;
-        atomicOr(&mask[(at >> 6) * a.experts + a.chosen[i]], 1ull << (at & 63));
+    __syncthreads();
+    // f(choice of the workgroup, its expert)
+    auto each_choice = [&](auto &&f) {
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            const int i = threadIdx.x + x * kPlaceThreads;
+            if (i < choices) f(i, ahead[x]);
+        }
+        for (int i = threadIdx.x + kAhead * kPlaceThreads; i < choices; i += kPlaceThreads) f(i, chosen[i]);
+    };
+    each_choice([&](int i, int e) {
+        const int at = i / a.k;
+        atomicOr(&mask[(at >> 6) * a.experts + e], 1ull << (at & 63));
+    });
+    if (HELD && row < rows) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (all[i]) atomicAdd(&count[column * 8 + i], all[i]);
+            if (before[i]) atomicAdd(&start[column * 8 + i], before[i]);
+        }
     }
     __syncthreads();
     add_before(start, count, a.experts, blockIdx.x == 0 ? a.offsets : nullptr);
     __syncthreads();
-    place_tokens(a, first, last, start, mask);
+    each_choice([&](int i, int e) { place(a, first, i, e, start, mask); });
 }
 
 // A choice outside the experts takes part in nothing.
 template <int VALUES, int TEAM, int EPL>
 __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradientArgs a)
 {
-    constexpr int TEAMS = 64 / TEAM, SLOTS = TEAM >= kMostChosen ? 1 : kMostChosen / TEAM;
+    constexpr int TEAMS = 64 / TEAM;
     const int lane = threadIdx.x & 63, in = lane % TEAM, team = lane / TEAM;
     const int e0 = in * EPL;
     const long long step = (long long)gridDim.x * (kThreads / TEAM);
     for (long long t0 = (long long)blockIdx.x * (kThreads / TEAM) + (threadIdx.x >> 6) * TEAMS; t0 < a.tokens; t0 += step) {
         const long long t = min(t0 + team, (long long)a.tokens - 1);
         const bool here = t0 + team < a.tokens;
-        int expert[SLOTS];
-        float l[SLOTS], dg[SLOTS];
-        bool have[SLOTS];
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-            const int j = in + i * TEAM;
-            expert[i] = -1;
-            dg[i] = l[i] = 0.f;
-            if (j < a.k) {
-                expert[i] = a.chosen[t * a.k + j];
-                dg[i] = a.gate_gradients[t * a.k + j] * a.scale;
-            }
-            have[i] = expert[i] >= 0 && expert[i] < a.experts;
-            if (have[i]) {
-                float v[1];
-                load_logits<VALUES>(v, a.logits, t * a.ldlogits, expert[i], a.experts);
-                l[i] = v[0];
-            } else {
-                expert[i] = -1;
-                dg[i] = 0.f;
-            }
+        int expert = -1;
+        float l = 0.f, dg = 0.f;
+        if (in < a.k) {
+            expert = a.chosen[t * a.k + in];
+            dg = a.gate_gradients[t * a.k + in] * a.scale;
         }
-        float out[EPL], d[SLOTS];  // d: what slot i adds to its expert's gradient
+        const bool have = expert >= 0 && expert < a.experts;
+        if (have) {
+            float v[1];
+            load_logits<VALUES>(v, a.logits, t * a.ldlogits, expert, a.experts);
+            l = v[0];
+        } else {
+            expert = -1;
+            dg = 0.f;
+        }
+        float out[EPL], d;  // d: what this lane's choice adds to its expert's gradient
 #pragma unroll
         for (int i = 0; i < EPL; ++i) out[i] = 0.f;
         if (a.renormalize) {
-            float share[SLOTS], dot = 0.f;
-            shares_of<TEAM>(share, l, have, a.logistic);
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i) dot += have[i] ? share[i] * dg[i] : 0.f;
-            dot = team_total<TEAM>(dot);
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i) {
-                d[i] = share[i] * (dg[i] - dot);
-                if (a.logistic) d[i] *= logistic(-l[i]);
-            }
+            const float share = share_of<TEAM>(l, have, a.logistic);
+            const float dot = team_total<TEAM>(have ? share * dg : 0.f);
+            d = share * (dg - dot);
+            if (a.logistic) d *= logistic(-l);
         } else if (a.logistic) {
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i) d[i] = dg[i] * logistic(l[i]) * logistic(-l[i]);
+            d = dg * logistic(l) * logistic(-l);
         } else {
-            float all[EPL], most, sum = 0.f, dot = 0.f;
+            float all[EPL], most, sum = 0.f;
             load_logits<VALUES>(all, a.logits, t * a.ldlogits, e0, a.experts);
             most = all[0];
 #pragma unroll
@@ -565,27 +656,15 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
             }
             sum = team_total<TEAM>(sum);
             const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i) {
-                d[i] = have[i] ? dg[i] * (exp_minus(l[i] - most) * inverse) : 0.f;
-                dot += d[i];
-            }
-            dot = team_total<TEAM>(dot);
+            d = have ? dg * (exp_minus(l - most) * inverse) : 0.f;
+            const float dot = team_total<TEAM>(d);
 #pragma unroll
             for (int i = 0; i < EPL; ++i) out[i] = -dot * (out[i] * inverse);
         }
         for (int j = 0; j < a.k; ++j) {
-            const int from = 4 * (team * TEAM + j % TEAM);
-            int e = -1;
-            float v = 0.f;
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i)
-                if (j / TEAM == i) {
-                    e = expert[i];
-                    v = d[i];
-                }
-            e = __builtin_amdgcn_ds_bpermute(from, e);
-            v = __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(v)));
+            const int from = 4 * (team * TEAM + j);
+            const int e = __builtin_amdgcn_ds_bpermute(from, expert);
+            const float v = __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(d)));
 #pragma unroll
             for (int i = 0; i < EPL; ++i)
                 if (e == e0 + i) out[i] += v;
@@ -619,10 +698,14 @@ hipError_t with_values(int values, F &&f)
     default: return f(std::integral_constant<int, kValuesF32>());
     }
 }
-// Lanes per token and experts per lane.
+// Lanes per token, one at least for each choice, and experts per lane.
 template <class F>
-hipError_t with_team(int experts, F &&f)
+hipError_t with_team(int experts, int k, F &&f)
 {
+    if (k > 16) {
+        if (experts <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
+        return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+    }
     if (experts <= 16) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
     if (experts <= 64) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
     if (experts <= 128) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
@@ -659,7 +742,6 @@ ChooseLayout choose_layout(int tokens, int experts)
 hipError_t launch_choose(ChooseArgs a, int values, void *workspace, hipStream_t s)
 {
     const ChooseLayout l = choose_layout(a.tokens, a.experts);
-    const bool wide = a.biases || (a.groups > 1 && a.group_best == 2);
     const bool grouped = a.groups > 1 && a.chosen_groups < a.groups;
     const bool lists = a.offsets != nullptr, all = lists && a.tokens <= kAllTokens;
     a.each = l.each;
@@ -672,26 +754,28 @@ hipError_t launch_choose(ChooseArgs a, int values, void *workspace, hipStream_t 
         a.before = reinterpret_cast<int *>(w + l.before);
     }
     const hipError_t e = with_values(values, [&](auto v) {
-        return with_team(a.experts, [&](auto team, auto epl) {
+        return with_team(a.experts, a.k, [&](auto team, auto epl) {
             constexpr int V = decltype(v)::value, T = decltype(team)::value, E = decltype(epl)::value;
+            const int each = a.experts / a.groups, width = each / E;
+            const bool lanes = each % E == 0 && width <= 16 && (width & (width - 1)) == 0;
             auto run = [&](auto key, auto g) {
                 typedef decltype(key) K;
-                if (all)
-                    hipLaunchKernelGGL((choose_all_kernel<V, K, T, E, decltype(g)::value>), dim3(1), dim3(kAllThreads), 0, s, a);
-                else
-                    hipLaunchKernelGGL((choose_kernel<V, K, T, E, decltype(g)::value>), dim3(l.blocks), dim3(kThreads), 0, s, a);
+                constexpr int G = decltype(g)::value;
+                if (all) hipLaunchKernelGGL((choose_all_kernel<V, K, T, E, G>), dim3(1), dim3(kAllThreads), 0, s, a);
+                else hipLaunchKernelGGL((choose_kernel<V, K, T, E, G>), dim3(l.blocks), dim3(choose_threads(E)), 0, s, a);
                 return hipGetLastError();
             };
-            if (wide) return grouped ? run(uint64_t(), std::true_type()) : run(uint64_t(), std::false_type());
-            return grouped ? run(uint32_t(), std::true_type()) : run(uint32_t(), std::false_type());
+            auto with = [&](auto g) { return a.biases ? run(double(), g) : run(uint32_t(), g); };
+            if (!grouped) return with(std::integral_constant<int, kNoGroups>());
+            return lanes ? with(std::integral_constant<int, kLaneGroups>()) : with(std::integral_constant<int, kAnyGroups>());
         });
     });
     if (e != hipSuccess || !lists || all) return e;
     if (l.blocks <= kMostHeld) {
-        hipLaunchKernelGGL(place_kernel<true>, dim3(l.blocks), dim3(kThreads), 0, s, a, l.blocks);
+        hipLaunchKernelGGL(place_kernel<true>, dim3(l.blocks), dim3(kPlaceThreads), 0, s, a, l.blocks);
     } else {
         hipLaunchKernelGGL(count_before_kernel, dim3(l.ldcounts / 8), dim3(kThreads), 0, s, a, l.blocks);
-        hipLaunchKernelGGL(place_kernel<false>, dim3(l.blocks), dim3(kThreads), 0, s, a, l.blocks);
+        hipLaunchKernelGGL(place_kernel<false>, dim3(l.blocks), dim3(kPlaceThreads), 0, s, a, l.blocks);
     }
     return hipGetLastError();
 }
@@ -699,7 +783,7 @@ hipError_t launch_choose(ChooseArgs a, int values, void *workspace, hipStream_t 
 hipError_t launch_choose_gradient(const ChooseGradientArgs &a, int values, hipStream_t s)
 {
     return with_values(values, [&](auto v) {
-        return with_team(a.experts, [&](auto team, auto epl) {
+        return with_team(a.experts, a.k, [&](auto team, auto epl) {
             constexpr int T = decltype(team)::value;
             const int tokens = kThreads / T;
             const unsigned blocks = (unsigned)std::min<long long>(((long long)a.tokens + tokens - 1) / tokens, 1 << 20);

@@ -23,58 +23,85 @@ namespace gtmoe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWideThreads = 1024;
 
-// The team's total of v: 16 lanes, a wave, or the whole workgroup.
-template <int TEAM>
-__device__ __forceinline__ float team_sum(float v, float *shared)
-{
-    if constexpr (TEAM == 16) return sixteen_sum(v);
-    v = wave_sum(v);
-    if constexpr (TEAM > 64) {
-        __syncthreads();  // the last total has been read
-        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.f;
-#pragma unroll
-        for (int w = 0; w < TEAM / 64; ++w) v += shared[w];
-    }
-    return v;
-}
-template <int TEAM>
-__device__ __forceinline__ uint32_t team_max(uint32_t v, float *shared)
-{
-    if constexpr (TEAM == 16) return lanes_max(v, 16);
-    v = wave_max(v);
-    if constexpr (TEAM > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = __uint_as_float(v);
-        __syncthreads();
-        v = 0;
-#pragma unroll
-        for (int w = 0; w < TEAM / 64; ++w) v = max(v, __float_as_uint(shared[w]));
-    }
-    return v;
-}
+// Totals over a team: 16 lanes, a wave, or the waves of a workgroup that hold a row.
+// Waves exchange by LDS, one barrier a total: two totals in turn use two places,
+// so that a place is written again only when a barrier has passed since its last
+// reading.  Every thread of the workgroup calls them together.
+template <int TEAM, int TEAMS>
+struct Totals {
+    static constexpr int kTeamWaves = TEAM > 64 ? TEAM / 64 : 1, kWaves = kTeamWaves * TEAMS;
+    double (*place)[kWaves];
+    int turn = 0;
 
-// Sums in 64 bits, for squares that fp32 does not hold: two halves through the
-// 32-bit exchanges would round, so lanes exchange whole doubles.
-template <int TEAM>
-__device__ double team_sum64(double v, float *shared)
-{
-#pragma unroll
-    for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) v += __shfl_xor(v, d);
-    if constexpr (TEAM > 64) {
-        double *s = reinterpret_cast<double *>(shared);
+    template <class T>
+    __device__ __forceinline__ T *exchange(T v)
+    {
+        T *p = reinterpret_cast<T *>(place[turn & 1]);
+        ++turn;
+        if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = v;
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0;
-        for (int w = 0; w < TEAM / 64; ++w) v += s[w];
-        __syncthreads();
+        return p;
     }
-    return v;
-}
+    // any: whether a team of the workgroup (TEAM <= 64: of the wave) has a total outside [least, most]
+    __device__ __forceinline__ float sum(float v, float least, float most, bool &any)
+    {
+        if constexpr (TEAM <= 64) {
+            v = TEAM == 16 ? sixteen_sum(v) : wave_sum(v);
+            any = __ballot(!(v >= least && v <= most)) != 0;
+            return v;
+        } else {
+            const float *p = exchange(wave_sum(v));
+            float mine = 0.f;
+            any = false;
+#pragma unroll
+            for (int t = 0; t < TEAMS; ++t) {
+                float total = 0.f;
+#pragma unroll
+                for (int w = 0; w < kTeamWaves; ++w) total += p[t * kTeamWaves + w];
+                any = any || !(total >= least && total <= most);
+                if (TEAMS == 1 || t == (int)(threadIdx.x / TEAM)) mine = total;
+            }
+            return mine;
+        }
+    }
+    __device__ __forceinline__ float sum(float v)
+    {
+        if constexpr (TEAM <= 64) {
+            return TEAM == 16 ? sixteen_sum(v) : wave_sum(v);
+        } else {
+            const float *p = exchange(wave_sum(v)) + threadIdx.x / TEAM * kTeamWaves;
+            v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kTeamWaves; ++w) v += p[w];
+            return v;
+        }
+    }
+    __device__ __forceinline__ uint32_t most(uint32_t v)
+    {
+        if constexpr (TEAM <= 64) {
+            return TEAM == 16 ? lanes_max(v, 16) : wave_max(v);
+        } else {
+            const uint32_t *p = exchange(wave_max(v)) + threadIdx.x / TEAM * kTeamWaves;
+            v = 0;
+#pragma unroll
+            for (int w = 0; w < kTeamWaves; ++w) v = max(v, p[w]);
+            return v;
+        }
+    }
+    // in 64 bits, for squares that fp32 does not hold
+    __device__ double sum64(double v)
+    {
+#pragma unroll
+        for (int d = 1; d < (TEAM < 64 ? TEAM : 64); d <<= 1) v += __shfl_xor(v, d);
+        if constexpr (TEAM > 64) {
+            const double *p = exchange(v) + threadIdx.x / TEAM * kTeamWaves;
+            v = 0;
+            for (int w = 0; w < kTeamWaves; ++w) v += p[w];
+        }
+        return v;
+    }
+};
 
 constexpr int team_threads(int team) { return team > kThreads ? team : kThreads; }
 
@@ -125,8 +152,8 @@ struct Row {
 
 // 1 / sqrt(mean(s^2) + epsilon) of a row.  Squares beyond fp32, or all below it
 // beside no epsilon, are added in 64 bits.
-template <int VALUES, int TEAM, int NV>
-__device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, double epsilon, float *shared)
+template <int VALUES, int TEAM, int NV, class T>
+__device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, int columns, double epsilon, T &totals)
 {
     float sum = 0.f;
     row.each([&](int i) {
@@ -134,20 +161,19 @@ __device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, 
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(e.get(j), e.get(j), sum);
     });
-    sum = team_sum<TEAM>(sum, shared);
-    float r = 1.f / sqrtf(sum / (float)row.columns + (float)epsilon);
-    const bool narrow = sum <= 1e37f && (sum >= 1e-25f || epsilon >= 1e-15);
-    // (the lanes of a wave exchange values below: all of them go if one has to)
-    if (TEAM > 64 ? !narrow : __ballot(!narrow) != 0) {
+    const float least = epsilon >= 1e-15 ? 0.f : 1e-25f;
+    bool any;
+    sum = totals.sum(sum, least, 1e37f, any);
+    float r = 1.f / sqrtf(sum / (float)columns + (float)epsilon);
+    if (any) {
         double wide = 0;
         row.each([&](int i) {
             const Eight<VALUES> e = row.get(i);
 #pragma unroll
             for (int j = 0; j < 8; ++j) wide += (double)e.get(j) * (double)e.get(j);
         });
-        wide = team_sum64<TEAM>(wide, shared);
-        const float again = (float)(1.0 / sqrt(wide / row.columns + epsilon));
-        if (!narrow) r = again;
+        wide = totals.sum64(wide);
+        if (!(sum >= least && sum <= 1e37f)) r = (float)(1.0 / sqrt(wide / columns + epsilon));
     }
     return r;
 }
@@ -156,7 +182,8 @@ template <int VALUES, int TEAM, int NV>
 __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormArgs a)
 {
     constexpr int TEAMS = team_threads(TEAM) / TEAM;
-    __shared__ float shared[2 * kWideThreads / 64];
+    __shared__ double place[2][Totals<TEAM, TEAMS>::kWaves];
+    Totals<TEAM, TEAMS> totals{place};
     const int scale_bits = a.scale_columns ? __builtin_ctz(a.scale_columns) : 31;
     for (long long r0 = (long long)blockIdx.x * TEAMS; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS) {
         // teams past the last row work on a row of no columns
@@ -187,12 +214,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
             row.fill(a.x, r * a.ldx);
         }
         float inverse = 1.f;
-        if (a.norm) {
-            row.columns = have ? a.columns : 1;  // (of the mean; no value is read)
-            if constexpr (NV == 0) row.columns = columns;
-            inverse = inverse_size(row, a.epsilon, shared);
-            row.columns = columns;
-        }
+        if (a.norm) inverse = inverse_size(row, a.columns, a.epsilon, totals);
         auto value = [&](int i, float (&y)[8]) {
             const int c = row.column(i), n = columns - c;
             const Eight<VALUES> e = row.get(i);
@@ -219,7 +241,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
                 value(i, y);
                 most = max(most, largest(y));
             });
-            most = team_max<TEAM>(most, shared);
+            most = totals.most(most);
         }
         row.each([&](int i) {
             const int c = row.column(i), n = columns - c;
@@ -246,7 +268,8 @@ template <int VALUES, int TEAM, int NV>
 __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormGradientArgs a)
 {
     constexpr int THREADS = team_threads(TEAM), TEAMS = THREADS / TEAM;
-    __shared__ float shared[2 * kWideThreads / 64];
+    __shared__ double place[2][Totals<TEAM, TEAMS>::kWaves];
+    Totals<TEAM, TEAMS> totals{place};
     __shared__ float part[TEAMS > 1 ? TEAMS : 1][TEAMS > 1 ? TEAM * NV * 8 : 1];
     float dw[NV ? NV : 1][8];
 #pragma unroll
@@ -254,44 +277,40 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
     const float mean = 1.f / (float)a.columns;
+    Row<VALUES, TEAM, NV> w(a.w, 0, a.columns);
+    if (a.w) w.fill(a.w, 0);
     for (long long r0 = (long long)blockIdx.x * TEAMS; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS) {
         const long long r = r0 + threadIdx.x / TEAM;
-        const bool have = r < a.rows;
-        const int columns = have ? a.columns : 0;
-        Row<VALUES, TEAM, NV> s(a.s, r * a.lds, columns), dy(a.dy, r * a.lddy, columns);
+        const int columns = r < a.rows ? a.columns : 0;
+        // all of a row's loads go out together
+        Row<VALUES, TEAM, NV> s(a.s, r * a.lds, columns), dy(a.dy, r * a.lddy, columns), ds(a.ds, r * a.ldds, columns);
         s.fill(a.s, r * a.lds);
         dy.fill(a.dy, r * a.lddy);
-        s.columns = NV && !have ? 1 : columns;
-        const float inverse = inverse_size(s, a.epsilon, shared);
-        s.columns = columns;
+        if (a.ds) ds.fill(a.ds, r * a.ldds);
+        const float inverse = inverse_size(s, a.columns, a.epsilon, totals);
         if (NV == 0 && a.inverse && threadIdx.x == 0) a.inverse[r] = inverse;
         float dot = 0.f;
         s.each([&](int i) {
-            const int c = s.column(i), n = columns - c;
-            const Eight<VALUES> v = s.get(i), g = dy.get(i);
-            Eight<VALUES> w;
-            if (a.w) load_eight(w, a.w, c, n);
+            const Eight<VALUES> v = s.get(i), g = dy.get(i), f = a.w ? w.get(i) : v;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float t = g.get(j) * (v.get(j) * inverse);
-                dot = a.w ? fmaf(w.get(j), t, dot) : dot + t;
+                dot = a.w ? fmaf(f.get(j), t, dot) : dot + t;
                 if constexpr (NV > 0) dw[i][j] += t;
             }
         });
-        dot = team_sum<TEAM>(dot, shared) * mean;
+        dot = totals.sum(dot) * mean;
         s.each([&](int i) {
             const int c = s.column(i), n = columns - c;
             if (n <= 0) return;
-            const Eight<VALUES> v = s.get(i), g = dy.get(i);
-            Eight<VALUES> w, e;
-            if (a.w) load_eight(w, a.w, c, n);
-            if (a.ds) load_eight(e, a.ds, r * a.ldds + c, n);
+            const Eight<VALUES> v = s.get(i), g = dy.get(i), f = a.w ? w.get(i) : v, p = a.ds ? ds.get(i) : v;
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float m = v.get(j) * inverse, t = a.w ? g.get(j) * w.get(j) : g.get(j);
-                y[j] = inverse * fmaf(-m, dot, t) + (a.ds ? e.get(j) : 0.f);
+                const float m = v.get(j) * inverse, t = a.w ? g.get(j) * f.get(j) : g.get(j);
+                y[j] = inverse * fmaf(-m, dot, t) + (a.ds ? p.get(j) : 0.f);
             }
+            Eight<VALUES> e;
             e.set(y);
             store_eight(e, a.dx, r * a.lddx + c, n);
         });
@@ -383,12 +402,15 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
     }
 }
 
-// out[g][c] (+)= the sum of partial rows: 16 columns per workgroup, 16 threads each.
+// out[g][c] (+)= the sum of partial rows: 16 columns per workgroup, 64 threads each.
 // The partial rows of group g are those of the row ranges it touches.
+constexpr int kAddThreads = 1024;
+
 template <int VALUES>
-__global__ __launch_bounds__(kThreads) void add_partials_kernel(AddPartialsArgs a)
+__global__ __launch_bounds__(kAddThreads) void add_partials_kernel(AddPartialsArgs a)
 {
-    __shared__ float part[16][17];
+    constexpr int EACH = kAddThreads / 16;
+    __shared__ float part[EACH][17];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4, g = blockIdx.y;
     const int c = blockIdx.x * 16 + x;
     int begin = 0, end = a.count;
@@ -401,9 +423,12 @@ __global__ __launch_bounds__(kThreads) void add_partials_kernel(AddPartialsArgs 
     float sum = 0.f;
     if (c < a.columns) {
 #pragma unroll 8
-        for (int p = begin + y; p < end; p += 16) sum += a.partial[(long long)p * a.columns + c];
+        for (int p = begin + y; p < end; p += EACH) sum += a.partial[(long long)p * a.columns + c];
     }
     part[y][x] = sum;
+    __syncthreads();
+    // the 64 sums of a column, four at a time, then the sixteen of them
+    if (y < 16) part[y][x] = (part[y][x] + part[y + 16][x]) + (part[y + 32][x] + part[y + 48][x]);
     __syncthreads();
     if (y == 0 && c < a.columns) {
         sum = 0.f;
@@ -431,8 +456,11 @@ __global__ __launch_bounds__(kThreads) void add_partials_kernel(AddPartialsArgs 
     }
 }
 
-// Threads and groups of eight values per thread that hold a row.  One wave per
-// row up to 2048 columns; from there, and while there are few rows, a workgroup.
+// Threads and groups of eight values per thread that hold a row: 16 lanes up to 128
+// columns, a wave up to 1024, from there, and while there are few rows, a workgroup.
+// (2048 columns by a wave, four groups a lane: the gradient 47.5 us without dw against
+// 29.5, fewer waves with so many registers; the forward 29.7 against 29.1, fp32 37.4
+// against 34.6.)
 constexpr int kFewRows = 512;
 struct Shape {
     int team, nv;
@@ -443,7 +471,6 @@ Shape shape_of(int rows, int columns)
     if (eights <= 16) return {16, 1};
     if (eights <= 64) return {64, 1};
     if (rows > kFewRows && eights <= 128) return {64, 2};
-    if (rows > kFewRows && eights <= 256) return {64, 4};
     if (eights <= 256) return {256, 1};
     if (eights <= 512) return {256, 2};
     if (eights <= 1024) return {1024, 1};
@@ -460,7 +487,6 @@ hipError_t with_shape(Shape s, F &&f)
     GTMOE_SHAPE(16, 1)
     GTMOE_SHAPE(64, 1)
     GTMOE_SHAPE(64, 2)
-    GTMOE_SHAPE(64, 4)
     GTMOE_SHAPE(256, 1)
     GTMOE_SHAPE(256, 2)
     GTMOE_SHAPE(1024, 1)
@@ -486,11 +512,15 @@ int blocks_of(long long rows, int team)
     return (int)std::min<long long>((rows + teams - 1) / teams, kMostBlocks);
 }
 
-// Workgroups of the gradient with dw: as many partial rows.
+// Workgroups of the gradient with dw, as many partial rows: sixteen waves per CU (8192 x
+// 2048 in bf16, us, both kernels: 50.9 with 512 workgroups of four waves, 37.8 with 1024,
+// 47.7 with 2048, whose partial rows take longer; 1024 x 16384: 50.7 with 256 of sixteen
+// waves, 66 with 512).
+constexpr int kGradientWaves = 4096;
 int gradient_blocks(int rows, int columns)
 {
     const Shape s = shape_of(rows, columns);
-    return std::min(blocks_of(rows, s.team), 512);
+    return std::min(blocks_of(rows, s.team), kGradientWaves / (team_threads(s.team) / 64));
 }
 
 }  // namespace
@@ -528,7 +558,7 @@ hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &ad
         if (a.rows > 0)
             hipLaunchKernelGGL(column_sums_kernel<V>, dim3((a.columns + kSumColumns - 1) / kSumColumns, (a.rows + a.each - 1) / a.each),
                                dim3(kThreads), 0, s, a);
-        hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16, a.groups), dim3(kThreads), 0, s, add);
+        hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16, a.groups), dim3(kAddThreads), 0, s, add);
         return hipGetLastError();
     });
 }
@@ -563,7 +593,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         if (shape.nv || a.rows == 0) {
             add.partial = workspace;
             add.count = a.rows ? blocks : 0;
-            hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16), dim3(kThreads), 0, s, add);
+            hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16), dim3(kAddThreads), 0, s, add);
             return hipGetLastError();
         }
         ColumnSumsArgs c;
