@@ -58,8 +58,9 @@ struct GroupedArgs {
 // Whether the product's tiles fit one launch.
 bool grouped_fits(const GroupedArgs &a, int direction, int values);
 hipError_t launch_grouped(const GroupedArgs &a, int direction, int values, hipStream_t s);
-// The forward of few rows with an epilogue, W streamed (grouped_few.hip).
-bool few_fits(const GroupedArgs &a);
+// The forward of few rows with an epilogue, W streamed (grouped_few.hip); staged: LDS-DMA
+// could take both operands.
+bool few_fits(const GroupedArgs &a, int value_bytes, bool staged);
 hipError_t launch_few(const GroupedArgs &a, int values, hipStream_t s);
 
 // The same for many rows of 16-bit values with both operands staged by LDS-DMA

@@ -293,21 +293,10 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a)
         if (!a.b && !a.bias) skip = without;
     }
     if constexpr (FUSED) {
-        const int lane = threadIdx.x & 63, h = lane >> 5;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int row = wm + 32 * i + (lane & 31);
-            if (row >= m) continue;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int col = wn + 32 * j + 8 * q + 4 * h;
-                    if (col >= n) continue;
-                    float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    store_fused<T>(a, g, (long long)tile_m + row, tile_n + col, v, n - col);
-                }
-        }
+        static_assert((BM + BN) * SB >= THREADS * 64, "4 KiB for every wave");
+        __syncthreads();  // every wave has read its last operands
+        finish_blocks<T, MI, NJ, 32, -1, false>(acc, a, g, tile_m, wm, min(m, BM), tile_n, wn, min(n, BN), s0 + wave * 4096,
+                                                threadIdx.x & 63);
         return;
     }
     if (DIR == kGroupedWeightGradient && a.out_f32)
@@ -395,7 +384,7 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
                                                            : launch_staged<T, DIR, 64, 64, 2, 2, 2, true>(a, da, db, s);
         }
     if constexpr (DIR == kGroupedForward)
-        if (a.epilogue.on && few_fits(a))
+        if (a.epilogue.on && few_fits(a, T::kBytes, da && db))
             return launch_few(a, T::kBytes == 4 ? kValuesF32 : std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
     const long long each = a.rows / a.groups;
     if constexpr (T::kBytes == 4) {

@@ -99,9 +99,24 @@ hipError_t launch_values(const GroupedArgs &a, hipStream_t s)
 
 }  // namespace
 
-bool few_fits(const GroupedArgs &a)
+// When the few rows' kernel is taken, against tiles of grouped.hip, both with SiLU and a
+// factor (us, MI355X):
+//   one group: 32 rows always (2048 -> 2048 bf16 9.6 against 11.0, fp32 14.8 against 37.3);
+//     more while 32 rows by 16 columns make at most one workgroup per CU (bf16, 128 rows of
+//     2048 -> 1024 9.5 against 11.0, 192 14.8 against 11.0), or three in fp32, whose tiles
+//     stream W worse (192 rows of 1024 -> 2048 20.2 against 22.3, 256 25.6 against 22.1)
+//   groups: a row per group on average (16 of 1024 -> 2048 bf16, 8 rows 8.2 against 9.1, 16
+//     rows 12.1 against 13.5, 32 rows 15.3 against 13.6; 64 of 2048 -> 1024, 64 rows 39.6
+//     against 47.8), two in fp32 (32 rows 33.7 against 33.3, 2 rows 8.3 against 20.9)
+//   16-bit rows that LDS-DMA cannot take: up to 192 (1201 -> 1000, 128 rows 12.0 against
+//     19.4, 192 19.6 against 19.7; 14 groups of 1000 -> 1201, 64 rows 11.6 against 12.5)
+bool few_fits(const GroupedArgs &a, int value_bytes, bool staged)
 {
-    return a.rows <= kMostRows && a.groups <= 64 && row_tiles(a, 16) * columns_of(a, 16) <= 1 << 22;
+    if (a.rows > kMostRows || a.groups > 64 || row_tiles(a, 16) * columns_of(a, 16) > 1 << 22) return false;
+    const bool wide = value_bytes == 4;
+    if (!wide && !staged) return a.rows <= 192;
+    if (a.groups > 1) return a.rows <= a.groups * (wide ? 2 : 1);
+    return a.rows <= 32 || (a.rows + 31) / 32 * ((a.outputs + 15) / 16) <= (wide ? 768 : 256);
 }
 
 hipError_t launch_few(const GroupedArgs &a, int values, hipStream_t s)

@@ -261,10 +261,7 @@ __device__ __forceinline__ void store_unit(typename O::Store *p, u32x4 v, int le
 // rows at the places of a.term.index.  The adapter's term is two steps more of
 // the same stream, u's parts against the adapter's up matrix.
 // FUSED (forward): at least 0, the activation of an epilogue, which the results pass in
-// registers, in the layout they have there.  The rows it reads and writes cross
-// between that layout and whole 128-byte pieces of rows in the wave's 4 KiB of
-// LDS, as the results do; the factors of a block of rows are on their way
-// while the block before is finished.
+// registers (finish_blocks), their rows crossing by the wave's 4 KiB of LDS.
 template <class T, int DIR, bool ADAPTED, int FUSED = -1>
 __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
 {
@@ -551,96 +548,8 @@ __global__ __launch_bounds__(kThreads) void grouped_large_kernel(GroupedArgs a)
         }
         if (DIR == kGroupedWeightGradient && a.accumulate && x.length == 0) return;
         if constexpr (FUSED >= 0) {
-            const Epilogue &e = a.epilogue;
-            // (rows and row starts are whole 16 bytes here: launch_grouped)
-            const int ur = el >> 3, unit = el & 7;  // the lane's row of eight and 16 bytes of it
-            const int col = wn + 8 * unit;
-            const bool in = col < x.n;
-            auto piece = [&](int p) { return stage + (8 * p + ur) * 128 + (unit ^ (((8 * p + ur) >> 1) & 7)) * 16; };
-            auto fours = [&](int j, int q) { return reinterpret_cast<uint2 *>(stage + ((slot ^ (4 * j + q) * 16) + (el >> 5) * 8)); };
-            // byte offset of row 64 i + wm + 8 p + ur of the tile, held inside it
-            // (`own` is ur, made again for each use: the sixteen of them were kept and spilled)
-            auto offset = [&](int own, int i, int p, long long ld) {
-                return ((uint32_t)min(64 * i + wm + 8 * p + own, x.m - 1) * (uint32_t)ld + (in ? col : 0)) * 2u;
-            };
-            auto again = [&]() {
-                int own = ur;
-                asm volatile("" : "+v"(own));
-                return own;
-            };
-            // rows of block i of a matrix, and into the wave's LDS
-            auto ask = [&](u32x4 (&v)[4], const void *from, long long ld, int i) {
-                const int own = again();
-                const char *base = reinterpret_cast<const char *>(reinterpret_cast<const Store *>(from) + (long long)x.m0 * ld + x.n0);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const u32x4 *>(base + offset(own, i, p, ld));
-            };
-            auto put = [&](const u32x4 (&v)[4]) {
-#pragma unroll
-                for (int p = 0; p < 4; ++p) *reinterpret_cast<u32x4 *>(piece(p)) = v[p];
-                __builtin_amdgcn_wave_barrier();
-            };
-            // the block's values, rounded, to rows of a matrix
-            auto take = [&](void *to, long long ld, int i) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const f32x16 &v = acc[i][j];
-                        *fours(j, q) = make_uint2(T::pack(v[4 * q], v[4 * q + 1]), T::pack(v[4 * q + 2], v[4 * q + 3]));
-                    }
-                __builtin_amdgcn_wave_barrier();
-                const int own = again();
-                char *base = reinterpret_cast<char *>(reinterpret_cast<Store *>(to) + (long long)x.m0 * ld + x.n0);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const u32x4 v = *reinterpret_cast<const u32x4 *>(piece(p));
-                    if (64 * i + wm + 8 * p + own < x.m && in) *reinterpret_cast<u32x4 *>(base + offset(own, i, p, ld)) = v;
-                }
-                __builtin_amdgcn_wave_barrier();
-            };
-            auto each = [&](int i, auto &&f) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint2 w = *fours(j, q);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            acc[i][j][4 * q + c] = f(acc[i][j][4 * q + c], T::load((uint16_t)((c < 2 ? w.x : w.y) >> (16 * (c & 1)))));
-                    }
-                __builtin_amdgcn_wave_barrier();
-            };
-            u32x4 rows[4];  // what is asked for next: block i's factors, then its residual
-            if (e.factor) ask(rows, e.factor, e.ldfactor, 0);
-            else if (e.residual) ask(rows, e.residual, e.ldresidual, 0);
-            if (e.bias)
-                add_bias<T>(acc, reinterpret_cast<const Store *>(e.bias) + x.g * e.ldbias, x.n0 + wn, a.outputs);
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                if (e.products) take(e.products, e.ldproducts, i);
-                if constexpr (FUSED != kActivationNone) {
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[i][j][r] = activated<FUSED>(acc[i][j][r]);
-                }
-                if (e.factor) {
-                    put(rows);
-                    if (e.residual) ask(rows, e.residual, e.ldresidual, i);
-                    else if (i + 1 < MI) ask(rows, e.factor, e.ldfactor, i + 1);
-                    each(i, [](float v, float w) { return v * w; });
-                }
-                if (e.residual) {
-                    put(rows);
-                    if (i + 1 < MI) {
-                        if (e.factor) ask(rows, e.factor, e.ldfactor, i + 1);
-                        else ask(rows, e.residual, e.ldresidual, i + 1);
-                    }
-                    each(i, [](float v, float w) { return v + w; });
-                }
-                take(a.out, a.ldo, i);
-            }
+            // (rows and row starts are whole 16 bytes here: launch_direction)
+            finish_blocks<T, MI, NJ, 64, FUSED, true>(acc, a, x.g, x.m0, wm, x.m, x.n0, wn, x.n, stage, el);
             return;
         }
         auto leave = [&](auto staged, auto type) {
