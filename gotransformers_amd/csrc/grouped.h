@@ -154,7 +154,7 @@ struct ColumnSumsArgs {
     long long ldx = 0, ldv = 0;
     int rows = 0, columns = 0, groups = 1, each = 0;
 };
-int sum_rows_each(int rows, int groups, int columns);
+int sum_rows_each(int rows, int columns);
 size_t sum_floats(int rows, int groups, int columns);
 hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &add, int values, hipStream_t s);
 

@@ -370,9 +370,21 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
             todo &= todo - 1;
             const int begin = __builtin_amdgcn_readlane(lo, src), end = __builtin_amdgcn_readlane(hi, src);
             float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (n > 0) {
-#pragma unroll 4
-                for (int r = begin + wave; r < end; r += kThreads / 64) {
+            // eight rows' loads of a wave go out together
+            constexpr int WAVES = kThreads / 64, AHEAD = 8;
+            int r = begin + wave;
+            if (n >= 8 && !a.v)
+                for (; r + (AHEAD - 1) * WAVES < end; r += AHEAD * WAVES) {
+                    Eight<VALUES> e[AHEAD];
+#pragma unroll
+                    for (int x = 0; x < AHEAD; ++x) load_eight(e[x], a.x, (r + x * WAVES) * a.ldx + c, 8);
+#pragma unroll
+                    for (int x = 0; x < AHEAD; ++x)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum[j] += e[x].get(j);
+                }
+            if (n > 0)
+                for (; r < end; r += WAVES) {
                     Eight<VALUES> e;
                     load_eight(e, a.x, r * a.ldx + c, n);
                     if (a.v) {
@@ -386,7 +398,6 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
                         for (int j = 0; j < 8; ++j) sum[j] += e.get(j);
                     }
                 }
-            }
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < 8; ++j) part[wave][8 * lane + j] = sum[j];
@@ -402,14 +413,11 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
     }
 }
 
-// out[g][c] (+)= the sum of partial rows: 16 columns per workgroup, 64 threads each.
+// out[g][c] (+)= the sum of partial rows: 16 columns per workgroup, EACH threads each.
 // The partial rows of group g are those of the row ranges it touches.
-constexpr int kAddThreads = 1024;
-
-template <int VALUES>
-__global__ __launch_bounds__(kAddThreads) void add_partials_kernel(AddPartialsArgs a)
+template <int VALUES, int EACH>
+__global__ __launch_bounds__(16 * EACH) void add_partials_kernel(AddPartialsArgs a)
 {
-    constexpr int EACH = kAddThreads / 16;
     __shared__ float part[EACH][17];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4, g = blockIdx.y;
     const int c = blockIdx.x * 16 + x;
@@ -427,9 +435,11 @@ __global__ __launch_bounds__(kAddThreads) void add_partials_kernel(AddPartialsAr
     }
     part[y][x] = sum;
     __syncthreads();
-    // the 64 sums of a column, four at a time, then the sixteen of them
-    if (y < 16) part[y][x] = (part[y][x] + part[y + 16][x]) + (part[y + 32][x] + part[y + 48][x]);
-    __syncthreads();
+    if constexpr (EACH == 64) {
+        // the 64 sums of a column, four at a time, then the sixteen of them
+        if (y < 16) part[y][x] = (part[y][x] + part[y + 16][x]) + (part[y + 32][x] + part[y + 48][x]);
+        __syncthreads();
+    }
     if (y == 0 && c < a.columns) {
         sum = 0.f;
 #pragma unroll
@@ -538,16 +548,31 @@ hipError_t launch_norm_forward(const NormArgs &a, int values, hipStream_t s)
     });
 }
 
-int sum_rows_each(int rows, int groups, int columns)
+namespace {
+
+// many: partial rows of a group.
+template <int V>
+hipError_t launch_add(const AddPartialsArgs &a, int many, hipStream_t s)
 {
-    // about 1024 workgroups, of 32 rows at least
+    const dim3 grid((a.columns + 15) / 16, a.groups);
+    if (many > 32) hipLaunchKernelGGL((add_partials_kernel<V, 64>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((add_partials_kernel<V, 16>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int sum_rows_each(int rows, int columns)
+{
+    // a workgroup per CU, of 32 rows at least (16384 x 2048 bf16 both kernels, us: 15.2 with
+    // 256 workgroups, 16.7 with 512, 18.2 with 1024)
     const int strips = (columns + kSumColumns - 1) / kSumColumns;
-    const int slices = std::max(1, std::min(1024 / std::min(strips, 1024), 65535));
+    const int slices = std::max(1, 256 / std::min(strips, 256));
     return std::max(32, (rows + slices - 1) / slices);
 }
 size_t sum_floats(int rows, int groups, int columns)
 {
-    const int each = sum_rows_each(rows, groups, columns);
+    const int each = sum_rows_each(rows, columns);
     return (size_t)((rows + each - 1) / each + groups) * columns;
 }
 
@@ -558,8 +583,7 @@ hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &ad
         if (a.rows > 0)
             hipLaunchKernelGGL(column_sums_kernel<V>, dim3((a.columns + kSumColumns - 1) / kSumColumns, (a.rows + a.each - 1) / a.each),
                                dim3(kThreads), 0, s, a);
-        hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16, a.groups), dim3(kAddThreads), 0, s, add);
-        return hipGetLastError();
+        return launch_add<V>(add, a.rows / a.each / a.groups, s);
     });
 }
 
@@ -593,8 +617,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         if (shape.nv || a.rows == 0) {
             add.partial = workspace;
             add.count = a.rows ? blocks : 0;
-            hipLaunchKernelGGL(add_partials_kernel<V>, dim3((a.columns + 15) / 16), dim3(kAddThreads), 0, s, add);
-            return hipGetLastError();
+            return launch_add<V>(add, add.count, s);
         }
         ColumnSumsArgs c;
         c.x = a.dy;
@@ -606,7 +629,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         c.rows = add.rows = a.rows;
         c.columns = a.columns;
         c.groups = 1;
-        c.each = add.each = sum_rows_each(a.rows, 1, a.columns);
+        c.each = add.each = sum_rows_each(a.rows, a.columns);
         add.partial = c.partial;
         return launch_column_sums(c, add, V, s);
     });
