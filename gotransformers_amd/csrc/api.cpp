@@ -3560,7 +3560,9 @@ ActivationArgs activation_args(const gtmoe_activation_desc *d)
     return a;
 }
 
-PackedRows kept_rows(const gtmoe_activation_desc *d, const void *codes, const float *scales)
+// Of a norm's or an activation's description.
+template <class Desc>
+PackedRows kept_rows(const Desc *d, const void *codes, const float *scales)
 {
     PackedRows k;
     k.codes = (uint8_t *)codes;
@@ -3707,12 +3709,7 @@ int32_t gtmoe_norm_forward(gtmoe_context *ctx, const gtmoe_norm_desc *desc, cons
         a.columns = desc->columns;
         a.epsilon = desc->epsilon;
         if (coded) {
-            a.codes = (uint8_t *)codes;
-            a.scales = scales;
-            a.ldcodes = desc->code_stride;
-            a.ldscales = desc->scale_stride;
-            a.code_type = desc->codes;
-            a.scale_columns = desc->scale_columns;
+            a.kept = kept_rows(desc, codes, scales);
         }
         return GTMOE_OK;
     };

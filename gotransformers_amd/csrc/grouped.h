@@ -109,15 +109,20 @@ struct DropoutArgs {
 };
 hipError_t launch_dropout(const DropoutArgs &a, int values, hipStream_t s);
 
+// Rows in 8 bits: codes and, per scale_columns columns (0: per row), a scale.
+struct PackedRows {
+    uint8_t *codes = nullptr;
+    float *scales = nullptr;
+    long long ldcodes = 0, ldscales = 0;
+    int code_type = 0, scale_columns = 0;
+};
 // Norm forward (norm.hip); norm 0: the rows as they are, into codes.
 struct NormArgs {
     const void *x = nullptr, *residual = nullptr, *w = nullptr;
     void *sums = nullptr, *out = nullptr;
-    uint8_t *codes = nullptr;
-    float *scales = nullptr;
-    long long ldx = 0, ldresidual = 0, ldsums = 0, ldo = 0, ldcodes = 0, ldscales = 0;
+    PackedRows kept;  // without codes: none
+    long long ldx = 0, ldresidual = 0, ldsums = 0, ldo = 0;
     int rows = 0, columns = 0, norm = 1;
-    int code_type = 0, scale_columns = 0;  // scale_columns 0: one scale per row
     double epsilon = 0;
 };
 hipError_t launch_norm_forward(const NormArgs &a, int values, hipStream_t s);
@@ -158,13 +163,6 @@ int sum_rows_each(int rows, int columns);
 size_t sum_floats(int rows, int groups, int columns);
 hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &add, int values, hipStream_t s);
 
-// Rows in 8 bits: codes and, per scale_columns columns (0: per row), a scale.
-struct PackedRows {
-    uint8_t *codes = nullptr;
-    float *scales = nullptr;
-    long long ldcodes = 0, ldscales = 0;
-    int code_type = 0, scale_columns = 0;
-};
 struct PackArgs {
     const void *x = nullptr;  // packed from,
     void *out = nullptr;      // or unpacked into; rows ldx apart

@@ -123,16 +123,18 @@ struct Row {
     {
         if constexpr (NV > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) load_eight(v[i], from, row + column(i), columns - column(i));
+            for (int i = 0; i < NV; ++i) load_eight(v[i], from, row, column(i), columns);
         }
     }
+    // whether the thread has columns in its i-th group
+    __device__ __forceinline__ bool any(int i) const { return any_column<VALUES>(column(i), columns); }
     __device__ __forceinline__ Eight<VALUES> get(int i) const
     {
         if constexpr (NV > 0) {
             return v[i];
         } else {
             Eight<VALUES> e;
-            load_eight(e, base, at + column(i), columns - column(i));
+            load_eight(e, base, at, column(i), columns);
             return e;
         }
     }
@@ -184,7 +186,6 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
     constexpr int TEAMS = team_threads(TEAM) / TEAM;
     __shared__ double place[2][Totals<TEAM, TEAMS>::kWaves];
     Totals<TEAM, TEAMS> totals{place};
-    const int scale_bits = a.scale_columns ? __builtin_ctz(a.scale_columns) : 31;
     for (long long r0 = (long long)blockIdx.x * TEAMS; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS) {
         // teams past the last row work on a row of no columns
         const long long r = r0 + threadIdx.x / TEAM;
@@ -194,21 +195,21 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
         if (a.residual || a.sums) {
             row.fill(a.x, r * a.ldx);
             row.each([&](int i) {
-                const int c = row.column(i), n = columns - c;
-                if (n <= 0) return;
+                const int c = row.column(i);
+                if (!row.any(i)) return;
                 Eight<VALUES> e;
                 if constexpr (NV > 0) e = row.v[i];
-                else load_eight(e, a.x, r * a.ldx + c, n);
+                else load_eight(e, a.x, r * a.ldx, c, columns);
                 if (a.residual) {
                     Eight<VALUES> b;
-                    load_eight(b, a.residual, r * a.ldresidual + c, n);
+                    load_eight(b, a.residual, r * a.ldresidual, c, columns);
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = e.get(j) + b.get(j);
                     e.set(v);
                 }
                 if constexpr (NV > 0) row.v[i] = e;
-                store_eight(e, a.sums, r * a.ldsums + c, n);
+                store_eight(e, a.sums, r * a.ldsums, c, columns);
             });
         } else {
             row.fill(a.x, r * a.ldx);
@@ -216,11 +217,10 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
         float inverse = 1.f;
         if (a.norm) inverse = inverse_size(row, a.columns, a.epsilon, totals);
         auto value = [&](int i, float (&y)[8]) {
-            const int c = row.column(i), n = columns - c;
             const Eight<VALUES> e = row.get(i);
             if (a.norm) {
                 Eight<VALUES> w;
-                if (a.w) load_eight(w, a.w, c, n);
+                if (a.w) load_eight(w, a.w, 0, row.column(i), columns);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = a.w ? e.get(j) * inverse * w.get(j) : e.get(j) * inverse;
             } else {
@@ -228,37 +228,24 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
                 for (int j = 0; j < 8; ++j) y[j] = e.get(j);
             }
         };
-        auto largest = [](const float (&y)[8]) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, size_bits(y[j]));
-            return m;
-        };
         uint32_t most = 0;
-        if (a.codes && !a.scale_columns) {
+        if (a.kept.codes && !a.kept.scale_columns) {
             row.each([&](int i) {
                 float y[8];
                 value(i, y);
-                most = max(most, largest(y));
+                most = max(most, max(largest_of_four(y), largest_of_four(y + 4)));
             });
             most = totals.most(most);
         }
         row.each([&](int i) {
-            const int c = row.column(i), n = columns - c;
             float y[8];
             value(i, y);
-            if (a.out && n > 0) {
+            if (a.out && row.any(i)) {
                 Eight<VALUES> e;
                 e.set(y);
-                store_eight(e, a.out, r * a.ldo + c, n);
+                store_eight(e, a.out, r * a.ldo, row.column(i), columns);
             }
-            if (a.codes) {
-                const Scale s(a.scale_columns ? lanes_max(largest(y), a.scale_columns / 8) : most, a.code_type);
-                if (n > 0) {
-                    store_codes(encode_eight(y, s, a.code_type), a.codes + r * a.ldcodes + c, n);
-                    if ((c & ((1u << scale_bits) - 1)) == 0) a.scales[r * a.ldscales + (c >> scale_bits)] = s.value;
-                }
-            }
+            if (a.kept.codes) keep_eight<VALUES>(y, r, row.column(i), columns, a.kept, most);
         });
     }
 }
@@ -301,8 +288,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
         });
         dot = totals.sum(dot) * mean;
         s.each([&](int i) {
-            const int c = s.column(i), n = columns - c;
-            if (n <= 0) return;
+            if (!s.any(i)) return;
             const Eight<VALUES> v = s.get(i), g = dy.get(i), f = a.w ? w.get(i) : v, p = a.ds ? ds.get(i) : v;
             float y[8];
 #pragma unroll
@@ -312,7 +298,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
             }
             Eight<VALUES> e;
             e.set(y);
-            store_eight(e, a.dx, r * a.lddx + c, n);
+            store_eight(e, a.dx, r * a.lddx, s.column(i), columns);
         });
     }
     if constexpr (NV > 0) {
@@ -323,7 +309,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) part[team][8 * (i * TEAM + thread) + j] = dw[i][j];
+                for (int j = 0; j < 8; ++j) part[team][column_of<VALUES>(8 * (i * TEAM + thread), j)] = dw[i][j];
             __syncthreads();
             for (int c = threadIdx.x; c < a.columns; c += THREADS) {
                 float v = 0.f;
@@ -336,7 +322,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int c = 8 * (i * TEAM + thread) + j;
+                    const int c = column_of<VALUES>(8 * (i * TEAM + thread), j);
                     if (c < a.columns) out[c] = dw[i][j];
                 }
         }
@@ -354,7 +340,8 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
 {
     __shared__ float part[kThreads / 64][kSumColumns];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = blockIdx.x * kSumColumns + 8 * lane, n = a.columns - c;
+    const int c = blockIdx.x * kSumColumns + 8 * lane;
+    const bool any = any_column<VALUES>(c, a.columns), whole = column_of<VALUES>(c, 7) < a.columns;
     const int first = blockIdx.y * a.each, last = min(first + a.each, a.rows);
     for (int g0 = 0; g0 < a.groups; g0 += 64) {
         int lo = 0, hi = 0;
@@ -373,23 +360,23 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
             // eight rows' loads of a wave go out together
             constexpr int WAVES = kThreads / 64, AHEAD = 8;
             int r = begin + wave;
-            if (n >= 8 && !a.v)
+            if (whole && !a.v)
                 for (; r + (AHEAD - 1) * WAVES < end; r += AHEAD * WAVES) {
                     Eight<VALUES> e[AHEAD];
 #pragma unroll
-                    for (int x = 0; x < AHEAD; ++x) load_eight(e[x], a.x, (r + x * WAVES) * a.ldx + c, 8);
+                    for (int x = 0; x < AHEAD; ++x) load_whole_eight(e[x], a.x, (r + x * WAVES) * a.ldx, c);
 #pragma unroll
                     for (int x = 0; x < AHEAD; ++x)
 #pragma unroll
                         for (int j = 0; j < 8; ++j) sum[j] += e[x].get(j);
                 }
-            if (n > 0)
+            if (any)
                 for (; r < end; r += WAVES) {
                     Eight<VALUES> e;
-                    load_eight(e, a.x, r * a.ldx + c, n);
+                    load_eight(e, a.x, r * a.ldx, c, a.columns);
                     if (a.v) {
                         Eight<VALUES> v;
-                        load_eight(v, a.v, r * a.ldv + c, n);
+                        load_eight(v, a.v, r * a.ldv, c, a.columns);
                         const float inverse = a.inverse[r];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) sum[j] += e.get(j) * (v.get(j) * inverse);
@@ -400,7 +387,7 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
                 }
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) part[wave][8 * lane + j] = sum[j];
+            for (int j = 0; j < 8; ++j) part[wave][column_of<VALUES>(8 * lane, j)] = sum[j];
             __syncthreads();
             float *out = a.partial + (long long)(blockIdx.y + g0 + src) * a.columns + blockIdx.x * kSumColumns;
             for (int i = threadIdx.x; i < min(kSumColumns, a.columns - blockIdx.x * kSumColumns); i += kThreads) {

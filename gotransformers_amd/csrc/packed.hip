@@ -35,45 +35,18 @@ __device__ __forceinline__ Place place_of(long long i, int per, bool narrow)
     return {r, (int)(i - r * per) * 8};
 }
 
-__device__ __forceinline__ uint32_t largest_of(const float (&v)[8])
-{
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, size_bits(v[e]));
-    return m;
-}
-
-// Codes of eight values and, by its first lane, their block's scale.  Every lane of
-// the block calls it.
-__device__ __forceinline__ void keep_eight(const float (&v)[8], const Place &p, int n, const PackedRows &k)
-{
-    const Scale s(lanes_max(largest_of(v), k.scale_columns / 8), k.code_type);
-    if (n <= 0) return;
-    store_codes(encode_eight(v, s, k.code_type), k.codes + p.row * k.ldcodes + p.column, n);
-    const int bits = __builtin_ctz(k.scale_columns);
-    if ((p.column & (k.scale_columns - 1)) == 0) k.scales[p.row * k.ldscales + (p.column >> bits)] = s.value;
-}
-
-// The eight values that codes stand for (scale_columns 0: one scale per row).
-__device__ __forceinline__ void kept_eight(float (&v)[8], const Place &p, int n, const PackedRows &k)
-{
-    const int bits = k.scale_columns ? __builtin_ctz(k.scale_columns) : 31;
-    decode_eight(load_codes(k.codes + p.row * k.ldcodes + p.column, n), k.scales[p.row * k.ldscales + (p.column >> bits)],
-                 k.code_type, v);
-}
-
 template <int VALUES>
 __global__ __launch_bounds__(kThreads) void pack_kernel(PackArgs a, int per, long long total, bool narrow)
 {
     for (long long i0 = (long long)blockIdx.x * kThreads; i0 < total; i0 += (long long)gridDim.x * kThreads) {
         const Place p = place_of(i0 + threadIdx.x, per, narrow);
-        const int n = p.row < a.rows ? a.columns - p.column : 0;
+        const int columns = p.row < a.rows ? a.columns : 0;
         Eight<VALUES> e;
-        load_eight(e, a.x, p.row * a.ldx + p.column, n);
+        load_eight(e, a.x, p.row * a.ldx, p.column, columns);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = e.get(j);
-        keep_eight(v, p, n, a.kept);
+        keep_eight<VALUES>(v, p.row, p.column, columns, a.kept);
     }
 }
 
@@ -82,13 +55,12 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(PackArgs a, int per, l
 {
     for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
         const Place p = place_of(i, per, narrow);
-        const int n = a.columns - p.column;
-        if (n <= 0) continue;
+        if (!any_column<VALUES>(p.column, a.columns)) continue;
         float v[8];
-        kept_eight(v, p, n, a.kept);
+        kept_eight<VALUES>(v, p.row, p.column, a.columns, a.kept);
         Eight<VALUES> e;
         e.set(v);
-        store_eight(e, a.out, p.row * a.ldx + p.column, n);
+        store_eight(e, a.out, p.row * a.ldx, p.column, a.columns);
     }
 }
 
@@ -119,10 +91,10 @@ __global__ __launch_bounds__(kThreads) void activation_forward_kernel(Activation
 {
     for (long long i0 = (long long)blockIdx.x * kThreads; i0 < total; i0 += (long long)gridDim.x * kThreads) {
         const Place p = place_of(i0 + threadIdx.x, per, narrow);
-        const int n = p.row < a.rows ? a.columns - p.column : 0;
+        const int columns = p.row < a.rows ? a.columns : 0;
         Eight<VALUES> ge, ue;
-        load_eight(ge, a.gate, p.row * a.ldgate + p.column, n);
-        if (a.up) load_eight(ue, a.up, p.row * a.ldup + p.column, n);
+        load_eight(ge, a.gate, p.row * a.ldgate, p.column, columns);
+        if (a.up) load_eight(ue, a.up, p.row * a.ldup, p.column, columns);
         float g[8], u[8], y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -130,10 +102,10 @@ __global__ __launch_bounds__(kThreads) void activation_forward_kernel(Activation
             u[j] = a.up ? ue.get(j) : 0.f;
         }
         if (a.kept_gate.codes) {
-            keep_eight(g, p, n, a.kept_gate);
-            if (a.up) keep_eight(u, p, n, a.kept_up);
+            keep_eight<VALUES>(g, p.row, p.column, columns, a.kept_gate);
+            if (a.up) keep_eight<VALUES>(u, p.row, p.column, columns, a.kept_up);
         }
-        if (n <= 0) continue;
+        if (!any_column<VALUES>(p.column, columns)) continue;
         hold(g, u, a.limit);
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = activated<ACT>(g[j]);
@@ -143,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void activation_forward_kernel(Activation
         }
         Eight<VALUES> e;
         e.set(y);
-        store_eight(e, a.out, p.row * a.ldo + p.column, n);
+        store_eight(e, a.out, p.row * a.ldo, p.column, columns);
     }
 }
 
@@ -152,19 +124,18 @@ __global__ __launch_bounds__(kThreads) void activation_gradient_kernel(Activatio
 {
     for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
         const Place p = place_of(i, per, narrow);
-        const int n = a.columns - p.column;
-        if (n <= 0) continue;
+        if (!any_column<VALUES>(p.column, a.columns)) continue;
         const bool gated = a.up || a.kept_up.codes;
         Eight<VALUES> de;
-        load_eight(de, a.dy, p.row * a.lddy + p.column, n);
+        load_eight(de, a.dy, p.row * a.lddy, p.column, a.columns);
         float g[8], u[8];
         if (a.kept_gate.codes) {
-            kept_eight(g, p, n, a.kept_gate);
-            if (gated) kept_eight(u, p, n, a.kept_up);
+            kept_eight<VALUES>(g, p.row, p.column, a.columns, a.kept_gate);
+            if (gated) kept_eight<VALUES>(u, p.row, p.column, a.columns, a.kept_up);
         } else {
             Eight<VALUES> ge, ue;
-            load_eight(ge, a.gate, p.row * a.ldgate + p.column, n);
-            if (gated) load_eight(ue, a.up, p.row * a.ldup + p.column, n);
+            load_eight(ge, a.gate, p.row * a.ldgate, p.column, a.columns);
+            if (gated) load_eight(ue, a.up, p.row * a.ldup, p.column, a.columns);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 g[j] = ge.get(j);
@@ -196,28 +167,29 @@ __global__ __launch_bounds__(kThreads) void activation_gradient_kernel(Activatio
         Eight<VALUES> e;
         if (a.dgate) {
             e.set(dg);
-            store_eight(e, a.dgate, p.row * a.lddgate + p.column, n);
+            store_eight(e, a.dgate, p.row * a.lddgate, p.column, a.columns);
         }
         if (a.dup) {
             e.set(du);
-            store_eight(e, a.dup, p.row * a.lddup + p.column, n);
+            store_eight(e, a.dup, p.row * a.lddup, p.column, a.columns);
         }
         if (a.out) {
             e.set(y);
-            store_eight(e, a.out, p.row * a.ldo + p.column, n);
+            store_eight(e, a.out, p.row * a.ldo, p.column, a.columns);
         }
     }
 }
 
-// Threads of a row: whole scales, or groups of eight where there are none.
+// Threads of a row: whole scales, or groups of eight where there are none; of fp32
+// whole 128 columns (column_of).
 struct Grid {
     int per;
     long long total;
     bool narrow;
     dim3 blocks;
-    Grid(int rows, int columns, int scale_columns)
+    Grid(int rows, int columns, int scale_columns, int values)
     {
-        const int unit = std::max(scale_columns, 8);
+        const int unit = values == kValuesF32 ? 128 : std::max(scale_columns, 8);
         per = (columns + unit - 1) / unit * (unit / 8);
         total = (long long)rows * per;
         narrow = total < (1ll << 31);
@@ -255,17 +227,13 @@ hipError_t launch_pack(const PackArgs &a, int values, hipStream_t s)
         NormArgs n;
         n.x = a.x;
         n.ldx = a.ldx;
-        n.codes = a.kept.codes;
-        n.scales = a.kept.scales;
-        n.ldcodes = a.kept.ldcodes;
-        n.ldscales = a.kept.ldscales;
+        n.kept = a.kept;
         n.rows = a.rows;
         n.columns = a.columns;
         n.norm = 0;
-        n.code_type = a.kept.code_type;
         return launch_norm_forward(n, values, s);
     }
-    const Grid g(a.rows, a.columns, a.kept.scale_columns);
+    const Grid g(a.rows, a.columns, a.kept.scale_columns, values);
     return with_values(values, [&](auto v) {
         hipLaunchKernelGGL(pack_kernel<decltype(v)::value>, g.blocks, dim3(kThreads), 0, s, a, g.per, g.total, g.narrow);
         return hipGetLastError();
@@ -274,7 +242,7 @@ hipError_t launch_pack(const PackArgs &a, int values, hipStream_t s)
 
 hipError_t launch_unpack(const PackArgs &a, int values, hipStream_t s)
 {
-    const Grid g(a.rows, a.columns, 0);
+    const Grid g(a.rows, a.columns, 0, values);
     return with_values(values, [&](auto v) {
         hipLaunchKernelGGL(unpack_kernel<decltype(v)::value>, g.blocks, dim3(kThreads), 0, s, a, g.per, g.total, g.narrow);
         return hipGetLastError();
@@ -283,7 +251,7 @@ hipError_t launch_unpack(const PackArgs &a, int values, hipStream_t s)
 
 hipError_t launch_activation(const ActivationArgs &a, bool gradient, int values, hipStream_t s)
 {
-    const Grid g(a.rows, a.columns, gradient ? 0 : a.kept_gate.scale_columns);
+    const Grid g(a.rows, a.columns, gradient ? 0 : a.kept_gate.scale_columns, values);
     return with_values(values, [&](auto v) {
         return with_activation(a.activation, [&](auto act) {
             constexpr int V = decltype(v)::value, A = decltype(act)::value;
