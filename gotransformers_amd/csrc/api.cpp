@@ -4000,7 +4000,7 @@ int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc
         a.rows = add.rows = desc->rows;
         a.columns = add.columns = desc->outputs;
         a.groups = add.groups = desc->groups;
-        a.each = add.each = sum_rows_each(desc->rows, desc->outputs);
+        a.each = add.each = sum_rows_each(desc->rows, desc->groups, desc->outputs);
         add.out = bias_gradients;
         add.ldo = desc->outputs;
         add.out_f32 = gradient_values == GTMOE_VALUES_FLOAT32;

@@ -127,15 +127,6 @@ struct NormArgs {
 };
 hipError_t launch_norm_forward(const NormArgs &a, int values, hipStream_t s);
 
-struct NormGradientArgs {
-    const void *dy = nullptr, *s = nullptr, *w = nullptr, *ds = nullptr;
-    void *dx = nullptr;
-    float *partial = nullptr;  // a row of dw's sums per workgroup
-    float *inverse = nullptr;  // of every row, where dw is summed apart
-    long long lddy = 0, lds = 0, ldds = 0, lddx = 0;
-    int rows = 0, columns = 0;
-    double epsilon = 0;
-};
 // Sums of partial rows: of all `count`, or (each > 0) of those of group g's rows.
 struct AddPartialsArgs {
     const float *partial = nullptr;
@@ -144,6 +135,16 @@ struct AddPartialsArgs {
     long long ldo = 0;
     int columns = 0, count = 0, each = 0, rows = 0, groups = 1;
     int out_f32 = 0, accumulate = 0;
+};
+struct NormGradientArgs {
+    const void *dy = nullptr, *s = nullptr, *w = nullptr, *ds = nullptr;
+    void *dx = nullptr;
+    float *partial = nullptr;  // a row of dw's sums per workgroup
+    float *inverse = nullptr;  // of every row, where dw is summed apart
+    AddPartialsArgs into;      // set by the launcher: dw itself
+    long long lddy = 0, lds = 0, ldds = 0, lddx = 0;
+    int rows = 0, columns = 0;
+    double epsilon = 0;
 };
 // Floats of workspace with dw.
 size_t norm_gradient_floats(int rows, int columns);
@@ -158,10 +159,11 @@ struct ColumnSumsArgs {
     float *partial = nullptr;
     long long ldx = 0, ldv = 0;
     int rows = 0, columns = 0, groups = 1, each = 0;
+    AddPartialsArgs into;  // set by the launcher: the sums themselves
 };
-int sum_rows_each(int rows, int columns);
+int sum_rows_each(int rows, int groups, int columns);
 size_t sum_floats(int rows, int groups, int columns);
-hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &add, int values, hipStream_t s);
+hipError_t launch_column_sums(ColumnSumsArgs a, const AddPartialsArgs &add, int values, hipStream_t s);
 
 struct PackArgs {
     const void *x = nullptr;  // packed from,

@@ -250,7 +250,32 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
     }
 }
 
-// One partial row of dw per workgroup (a.partial), none without it.
+// out[g][c] (+)= sum, rounded once.
+template <int VALUES>
+__device__ __forceinline__ void store_sum(const AddPartialsArgs &a, int g, int c, float sum)
+{
+    const long long at = g * a.ldo + c;
+    if (a.out_f32) {
+        float *o = reinterpret_cast<float *>(a.out) + at;
+        *o = a.accumulate ? *o + sum : sum;
+    } else {
+        typedef typename Eight<VALUES>::Store Store;
+        Eight<VALUES> e;
+        Store *o = reinterpret_cast<Store *>(a.out) + at, w[8] = {};
+        if (a.accumulate) {
+            w[0] = *o;
+            __builtin_memcpy(e.raw, w, sizeof w);
+            sum += e.get(0);
+        }
+        const float v[8] = {sum, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        e.set(v);
+        __builtin_memcpy(w, e.raw, sizeof w);
+        *o = w[0];
+    }
+}
+
+// One partial row of dw per workgroup (a.partial); of few rows one workgroup, which
+// writes dw itself (a.into.out); or none.
 template <int VALUES, int TEAM, int NV>
 __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormGradientArgs a)
 {
@@ -302,9 +327,12 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
         });
     }
     if constexpr (NV > 0) {
-        if (!a.partial) return;
+        if (!a.partial && !a.into.out) return;
         const int thread = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-        float *out = a.partial + (long long)blockIdx.x * a.columns;
+        auto keep = [&](int c, float v) {
+            if (a.partial) a.partial[(long long)blockIdx.x * a.columns + c] = v;
+            else store_sum<VALUES>(a.into, 0, c, v);
+        };
         if constexpr (TEAMS > 1) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -315,7 +343,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
                 float v = 0.f;
 #pragma unroll
                 for (int t = 0; t < TEAMS; ++t) v += part[t][c];
-                out[c] = v;
+                keep(c, v);
             }
         } else {
 #pragma unroll
@@ -323,7 +351,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int c = column_of<VALUES>(8 * (i * TEAM + thread), j);
-                    if (c < a.columns) out[c] = dw[i][j];
+                    if (c < a.columns) keep(c, dw[i][j]);
                 }
         }
     }
@@ -332,7 +360,9 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
 // Sums over rows by group, in two steps: a workgroup adds `each` consecutive rows of
 // 512 columns, one partial row for every group among them; the pair (workgroup b,
 // group g) has slot b + g, and no other pair has it, since rows are in group order.
-// With v: of the rows' values times v's times inverse[r].
+// With v: of the rows' values times v's times inverse[r].  All rows by one workgroup per
+// 512 columns (few rows): it writes the sums themselves (a.into.out), zero for the
+// groups without rows.
 constexpr int kSumColumns = 512;
 
 template <int VALUES>
@@ -351,7 +381,8 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
         }
         lo = max(lo, first);
         hi = min(hi, last);
-        uint64_t todo = __ballot(lo < hi);
+        const bool own = a.into.out != nullptr;
+        uint64_t todo = __ballot(lo < hi || (own && !a.into.accumulate && g0 + lane < a.groups));
         while (todo) {
             const int src = __builtin_ctzll(todo);
             todo &= todo - 1;
@@ -394,7 +425,8 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
                 float v = 0.f;
 #pragma unroll
                 for (int w = 0; w < kThreads / 64; ++w) v += part[w][i];
-                out[i] = v;
+                if (own) store_sum<VALUES>(a.into, g0 + src, blockIdx.x * kSumColumns + i, v);
+                else out[i] = v;
             }
         }
     }
@@ -432,24 +464,7 @@ __global__ __launch_bounds__(16 * EACH) void add_partials_kernel(AddPartialsArgs
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += part[i][x];
         if (begin == end && a.accumulate) return;
-        const long long at = g * a.ldo + c;
-        if (a.out_f32) {
-            float *o = reinterpret_cast<float *>(a.out) + at;
-            *o = a.accumulate ? *o + sum : sum;
-        } else {
-            typedef typename Eight<VALUES>::Store Store;
-            Eight<VALUES> e;
-            Store *o = reinterpret_cast<Store *>(a.out) + at, w[8] = {};
-            if (a.accumulate) {
-                w[0] = *o;
-                __builtin_memcpy(e.raw, w, sizeof w);
-                sum += e.get(0);
-            }
-            const float v[8] = {sum, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            e.set(v);
-            __builtin_memcpy(w, e.raw, sizeof w);
-            *o = w[0];
-        }
+        store_sum<VALUES>(a, g, c, sum);
     }
 }
 
@@ -549,28 +564,35 @@ hipError_t launch_add(const AddPartialsArgs &a, int many, hipStream_t s)
 
 }  // namespace
 
-int sum_rows_each(int rows, int columns)
+// (64 rows of 2048 columns in 16 groups 15.1 us by one workgroup per 512 columns, 9.8 by two kernels; 32 rows
+// of one group 7.5 and 9.8)
+static bool few_sums(int rows, int groups) { return rows <= 64 && groups <= 4; }
+
+int sum_rows_each(int rows, int groups, int columns)
 {
-    // a workgroup per CU, of 32 rows at least (16384 x 2048 bf16 both kernels, us: 15.2 with
+    // few rows one range, whose sums need no second kernel; else a workgroup per CU, of 32 rows
+    // at least (16384 x 2048 bf16 both kernels, us: 15.2 with
     // 256 workgroups, 16.7 with 512, 18.2 with 1024)
     const int strips = (columns + kSumColumns - 1) / kSumColumns;
     const int slices = std::max(1, 256 / std::min(strips, 256));
-    return std::max(32, (rows + slices - 1) / slices);
+    return few_sums(rows, groups) ? 64 : std::max(32, (rows + slices - 1) / slices);
 }
 size_t sum_floats(int rows, int groups, int columns)
 {
-    const int each = sum_rows_each(rows, columns);
+    const int each = sum_rows_each(rows, groups, columns);
     return (size_t)((rows + each - 1) / each + groups) * columns;
 }
 
-hipError_t launch_column_sums(const ColumnSumsArgs &a, const AddPartialsArgs &add, int values, hipStream_t s)
+hipError_t launch_column_sums(ColumnSumsArgs a, const AddPartialsArgs &add, int values, hipStream_t s)
 {
+    const bool one = a.rows > 0 && few_sums(a.rows, a.groups);
+    if (one) a.into = add;
     return with_values(values, [&](auto v) {
         constexpr int V = decltype(v)::value;
         if (a.rows > 0)
             hipLaunchKernelGGL(column_sums_kernel<V>, dim3((a.columns + kSumColumns - 1) / kSumColumns, (a.rows + a.each - 1) / a.each),
                                dim3(kThreads), 0, s, a);
-        return launch_add<V>(add, a.rows / a.each / a.groups, s);
+        return one ? hipGetLastError() : launch_add<V>(add, a.rows / a.each / a.groups, s);
     });
 }
 
@@ -585,8 +607,15 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
 {
     const Shape shape = shape_of(a.rows, a.columns);
     const bool weights = into.out != nullptr;
-    if (weights) (shape.nv ? a.partial : a.inverse) = workspace;
-    const int blocks = weights && shape.nv ? gradient_blocks(a.rows, a.columns) : blocks_of(a.rows, shape.team);
+    int blocks = weights && shape.nv ? gradient_blocks(a.rows, a.columns) : blocks_of(a.rows, shape.team);
+    // few rows, four for each of a workgroup's teams: a second launch would take longer
+    const bool one = weights && shape.nv && shape.team <= 256 && a.rows > 0 && blocks <= 4;
+    if (one) {
+        blocks = 1;
+        a.into = into;
+    } else if (weights) {
+        (shape.nv ? a.partial : a.inverse) = workspace;
+    }
     return with_values(values, [&](auto v) -> hipError_t {
         constexpr int V = decltype(v)::value;
         if (a.rows > 0) {
@@ -597,7 +626,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
             });
             if (e != hipSuccess) return e;
         }
-        if (!weights) return hipSuccess;
+        if (!weights || one) return hipSuccess;
         AddPartialsArgs add = into;
         add.columns = a.columns;
         add.groups = 1;
@@ -616,7 +645,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         c.rows = add.rows = a.rows;
         c.columns = a.columns;
         c.groups = 1;
-        c.each = add.each = sum_rows_each(a.rows, a.columns);
+        c.each = add.each = sum_rows_each(a.rows, 1, a.columns);
         add.partial = c.partial;
         return launch_column_sums(c, add, V, s);
     });

@@ -596,7 +596,7 @@ typedef struct gtmoe_norm_desc {
     int32_t rows;          /* 0 .. 2^30 */
     int32_t columns;       /* 1 .. 1048576 */
     int32_t codes;         /* gtmoe_codes */
-    int32_t scale_columns; /* with codes: 0, 16, 32, 64 or 128; else 0 */
+    int32_t scale_columns; /* with codes: 0, 16, 32, 64 or 128; else not used */
     int32_t reserved;      /* 0 */
     double epsilon;        /* at least 0 */
     int64_t input_stride;    /* of inputs and input gradients */
@@ -646,7 +646,7 @@ typedef struct gtmoe_activation_desc {
     int32_t columns;       /* 1 .. 1048576 */
     int32_t activation;    /* gtmoe_activation */
     int32_t codes;         /* gtmoe_codes */
-    int32_t scale_columns; /* with codes: 16, 32, 64 or 128; else 0 */
+    int32_t scale_columns; /* with codes: 16, 32, 64 or 128; else not used */
     double limit;          /* 0, or more than 0 */
     int64_t gate_stride;   /* of gates and their gradients */
     int64_t up_stride;     /* of ups and their gradients */
