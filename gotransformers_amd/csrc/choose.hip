@@ -26,6 +26,12 @@
 // workgroups before it and of the experts before, and finds a token's place among
 // its workgroup's by a bit mask of tokens per expert.  Nothing depends on the order
 // in which anything ran.  Few tokens are one workgroup and one launch.
+//
+// What bounds it (MI355X): the vector unit and the chain of the rounds; the bytes would
+// take 1 us.  16384 tokens x 128 experts, k = 8, sigmoid with biases, 4 of 8 groups by their best
+// two: 14.6 us (of some 850 vector instructions per four tokens, 235 are the scores, 420
+// the rounds), lists 6.5.  8192 x 64, k = 4, softmax: 4.4, lists 5.9, gradient 3.9.  32 x 64,
+// k = 6, with lists 4.8, one launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -76,7 +82,9 @@ __device__ __forceinline__ double permuted(int from, double v)
 }
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
 __device__ __forceinline__ uint32_t smaller(uint32_t a, uint32_t b) { return min(a, b); }
-// (as one instruction each: nothing here is a signalling NaN, which fmax would first quiet)
+// (as one instruction each: nothing here is a signalling NaN, which fmax would first quiet.
+// No transcendental's result goes in, and the compiler keeps the wait states that DPP
+// needs behind whatever wrote its operand.)
 __device__ __forceinline__ double larger(double a, double b)
 {
     double r;

@@ -7,6 +7,10 @@
 // device, as in grouped.hip; columns are dealt to the XCDs in turn, so that
 // however few rows there are every XCD streams its share of W, and the row tiles of
 // a group, a multiple of eight workgroups apart, find W in the same L2.
+//
+// What bounds it (MI355X): a launch and two trips to memory.  32 rows of 1024 -> 2048 bf16 with
+// bias, SiLU and factor 6.8 us, W's 4 MB alone 0.8; 64 groups of 2048 -> 1024, a row each, 58.6,
+// W's 268 MB at 4.6 TB/s.
 #include "grouped_rows.h"
 
 namespace gtmoe {
@@ -106,8 +110,8 @@ hipError_t launch_values(const GroupedArgs &a, hipStream_t s)
 //     2048 -> 1024 9.5 against 11.0, 192 14.8 against 11.0), or three in fp32, whose tiles
 //     stream W worse (192 rows of 1024 -> 2048 20.2 against 22.3, 256 25.6 against 22.1)
 //   groups: a row per group on average (16 of 1024 -> 2048 bf16, 8 rows 8.2 against 9.1, 16
-//     rows 12.1 against 13.5, 32 rows 15.3 against 13.6; 64 of 2048 -> 1024, 64 rows 39.6
-//     against 47.8), two in fp32 (32 rows 33.7 against 33.3, 2 rows 8.3 against 20.9)
+//     rows 12.1 against 13.5, 32 rows 15.3 against 13.6; 64 of 2048 -> 1024, 64 rows, W
+//     partly cached, 39.6 against 47.8), two in fp32 (32 rows 33.7 against 33.3, 2 rows 8.3 against 20.9)
 //   16-bit rows that LDS-DMA cannot take: up to 192 (1201 -> 1000, 128 rows 12.0 against
 //     19.4, 192 19.6 against 19.7; 14 groups of 1000 -> 1201, 64 rows 11.6 against 12.5)
 bool few_fits(const GroupedArgs &a, int value_bytes, bool staged)
