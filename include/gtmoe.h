@@ -615,8 +615,8 @@ int32_t gtmoe_norm_forward(gtmoe_context *ctx, const gtmoe_norm_desc *desc, cons
  * the gradient of inputs and residuals alike, may be sum_gradients themselves where
  * the strides are the same.  weight_gradients (one row, of type gradient_values: the
  * values' own or float32) may be NULL.  The workspace, of gtmoe_norm_workspace
- * bytes, 16-byte aligned, is only for them.  The codes of the description are not
- * used. */
+ * bytes, 16-byte aligned, is only for them.  The codes of the description are
+ * checked but not used. */
 int32_t gtmoe_norm_workspace(const gtmoe_norm_desc *desc, size_t *bytes);
 int32_t gtmoe_norm_gradient(gtmoe_context *ctx, const gtmoe_norm_desc *desc, const void *output_gradients, const void *sums,
                             const void *weights, const void *sum_gradients, void *input_gradients, void *weight_gradients,
@@ -693,8 +693,8 @@ int32_t gtmoe_grouped_fused_forward(gtmoe_context *ctx, const gtmoe_grouped_desc
 /* bias_gradients[g] (+)= sum over g's rows of output_gradients[r] (Layer.Backward,
  * perceptron/layer.go:164-210): groups rows of `outputs` values, contiguous, of type
  * gradient_values, the rows' own or float32.  accumulate == 0: an empty group's become
- * zero.  The inputs, weights and their strides of the description are not used.  With
- * one group offsets may be NULL.  The workspace: gtmoe_grouped_bias_workspace bytes,
+ * zero.  The inputs, weights and their strides of the description are checked but
+ * not used.  With one group offsets may be NULL.  The workspace: gtmoe_grouped_bias_workspace bytes,
  * 16-byte aligned. */
 int32_t gtmoe_grouped_bias_workspace(const gtmoe_grouped_desc *desc, size_t *bytes);
 int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc *desc, const int32_t *offsets,
