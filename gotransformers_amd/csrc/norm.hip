@@ -300,13 +300,16 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
     if (a.w) w.fill(a.w, 0);
     for (long long r0 = (long long)blockIdx.x * TEAMS; r0 < a.rows; r0 += (long long)gridDim.x * TEAMS) {
         const long long r = r0 + threadIdx.x / TEAM;
-        const int columns = r < a.rows ? a.columns : 0;
+        const bool have = r < a.rows;
+        const int columns = have ? a.columns : 0;
         // all of a row's loads go out together
         Row<VALUES, TEAM, NV> s(a.s, r * a.lds, columns), dy(a.dy, r * a.lddy, columns), ds(a.ds, r * a.ldds, columns);
         s.fill(a.s, r * a.lds);
         dy.fill(a.dy, r * a.lddy);
         if (a.ds) ds.fill(a.ds, r * a.ldds);
-        const float inverse = inverse_size(s, a.columns, a.epsilon, totals);
+        float inverse = inverse_size(s, a.columns, a.epsilon, totals);
+        // a team past the last row adds nothing to dw (without epsilon its row of zeros has no inverse)
+        if (!have) inverse = 0.f;
         if (NV == 0 && a.inverse && threadIdx.x == 0) a.inverse[r] = inverse;
         float dot = 0.f;
         s.each([&](int i) {
