@@ -140,7 +140,7 @@ struct NormGradientArgs {
     const void *dy = nullptr, *s = nullptr, *w = nullptr, *ds = nullptr;
     void *dx = nullptr;
     float *partial = nullptr;  // a row of dw's sums per workgroup
-    float *inverse = nullptr;  // of every row, where dw is summed apart
+    float *inverse = nullptr;  // of every row, as two factors, where dw is summed apart
     AddPartialsArgs into;      // set by the launcher: dw itself
     long long lddy = 0, lds = 0, ldds = 0, lddx = 0;
     int rows = 0, columns = 0;

@@ -119,6 +119,7 @@ struct Row {
     const void *base;
     long long at;
     int columns, thread;
+    float times = 1.f;  // of what is read again
 
     __device__ __forceinline__ Row(const void *base_, long long at_, int columns_)
         : base(base_), at(at_), columns(columns_), thread(threadIdx.x % TEAM)
@@ -142,7 +143,24 @@ struct Row {
         } else {
             Eight<VALUES> e;
             load_eight(e, base, at, column(i), columns);
+            if (times != 1.f) scale(e, times);
             return e;
+        }
+    }
+    static __device__ __forceinline__ void scale(Eight<VALUES> &e, float by)
+    {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = e.get(j) * by;
+        e.set(y);
+    }
+    __device__ __forceinline__ void scale(float by)
+    {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) scale(v[i], by);
+        } else {
+            times = by;
         }
     }
     // f(i) for every group of eight of the thread; i is a constant of the compiler's
@@ -159,10 +177,15 @@ struct Row {
     }
 };
 
-// 1 / sqrt(mean(s^2) + epsilon) of a row.  Squares beyond fp32, or all below it
-// beside no epsilon, are added in 64 bits.
+// r = 1 / sqrt(mean(s^2) + epsilon) of a row, as value * times, times a power of two.
+struct Inverse {
+    float value, times = 1.f;
+};
+// Squares beyond fp32, or all below it beside no epsilon, are added in 64 bits.  r itself
+// may then be none of fp32's normal numbers (rows of size 2^-128 and less, or 2^126 and more):
+// the row is left times a power of two, so that s r is what it holds times value.
 template <int VALUES, int TEAM, int NV, class T>
-__device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, int columns, double epsilon, T &totals)
+__device__ __forceinline__ Inverse inverse_size(Row<VALUES, TEAM, NV> &row, int columns, double epsilon, T &totals)
 {
     float sum = 0.f;
     row.each([&](int i) {
@@ -173,7 +196,7 @@ __device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, 
     const float least = epsilon >= 1e-15 ? 0.f : 1e-25f;
     bool any;
     sum = totals.sum(sum, least, 1e37f, any);
-    float r = 1.f / sqrtf(sum / (float)columns + (float)epsilon);
+    Inverse r{1.f / sqrtf(sum / (float)columns + (float)epsilon)};
     if (any) {
         double wide = 0;
         row.each([&](int i) {
@@ -182,7 +205,12 @@ __device__ __forceinline__ float inverse_size(const Row<VALUES, TEAM, NV> &row, 
             for (int j = 0; j < 8; ++j) wide += (double)e.get(j) * (double)e.get(j);
         });
         wide = totals.sum64(wide);
-        if (!(sum >= least && sum <= 1e37f)) r = (float)(1.0 / sqrt(wide / columns + epsilon));
+        if (!(sum >= least && sum <= 1e37f)) {
+            const double exact = 1.0 / sqrt(wide / columns + epsilon);
+            r.times = exact > 0x1p64 ? 0x1p64f : exact < 0x1p-64 ? 0x1p-32f : 1.f;
+            r.value = (float)(exact / (double)r.times);
+        }
+        row.scale(r.times);
     }
     return r;
 }
@@ -222,7 +250,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
             row.fill(a.x, r * a.ldx);
         }
         float inverse = 1.f;
-        if (a.norm) inverse = inverse_size(row, a.columns, a.epsilon, totals);
+        if (a.norm) inverse = inverse_size(row, a.columns, a.epsilon, totals).value;
         auto value = [&](int i, float (&y)[8]) {
             const Eight<VALUES> e = row.get(i);
             if (a.norm) {
@@ -307,10 +335,14 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
         s.fill(a.s, r * a.lds);
         dy.fill(a.dy, r * a.lddy);
         if (a.ds) ds.fill(a.ds, r * a.ldds);
-        float inverse = inverse_size(s, a.columns, a.epsilon, totals);
+        Inverse size = inverse_size(s, a.columns, a.epsilon, totals);
         // a team past the last row adds nothing to dw (without epsilon its row of zeros has no inverse)
-        if (!have) inverse = 0.f;
-        if (NV == 0 && a.inverse && threadIdx.x == 0) a.inverse[r] = inverse;
+        if (!have) size.value = 0.f;
+        const float inverse = size.value;
+        if (NV == 0 && a.inverse && threadIdx.x == 0) {
+            a.inverse[2 * r] = size.value;
+            a.inverse[2 * r + 1] = size.times;
+        }
         float dot = 0.f;
         s.each([&](int i) {
             const Eight<VALUES> v = s.get(i), g = dy.get(i), f = a.w ? w.get(i) : v;
@@ -329,7 +361,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float m = v.get(j) * inverse, t = a.w ? g.get(j) * f.get(j) : g.get(j);
-                y[j] = inverse * fmaf(-m, dot, t) + (a.ds ? p.get(j) : 0.f);
+                y[j] = fmaf(inverse * fmaf(-m, dot, t), size.times, a.ds ? p.get(j) : 0.f);
             }
             Eight<VALUES> e;
             e.set(y);
@@ -370,7 +402,7 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
 // Sums over rows by group, in two steps: a workgroup adds `each` consecutive rows of
 // 512 columns, one partial row for every group among them; the pair (workgroup b,
 // group g) has slot b + g, and no other pair has it, since rows are in group order.
-// With v: of the rows' values times v's times inverse[r].  All rows by one workgroup per
+// With v: of the rows' values times v's times r's two inverses.  All rows by one workgroup per
 // 512 columns (few rows): it writes the sums themselves (a.into.out), zero for the
 // groups without rows.
 constexpr int kSumColumns = 512;
@@ -431,9 +463,9 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
                     if (a.v) {
                         Eight<VALUES> v;
                         load_eight(v, a.v, r * a.ldv, c, a.columns);
-                        const float inverse = a.inverse[r];
+                        const float inverse = a.inverse[2 * (long long)r], times = a.inverse[2 * (long long)r + 1];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[j] += e.get(j) * (v.get(j) * inverse);
+                        for (int j = 0; j < 8; ++j) sum[j] += e.get(j) * (v.get(j) * times * inverse);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) sum[j] += e.get(j);
@@ -623,7 +655,7 @@ size_t norm_gradient_floats(int rows, int columns)
 {
     if (rows == 0) return 0;
     if (shape_of(rows, columns).nv) return (size_t)gradient_blocks(rows, columns) * columns;
-    return (size_t)rows + sum_floats(rows, 1, columns);
+    return 2 * (size_t)rows + sum_floats(rows, 1, columns);
 }
 
 hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddPartialsArgs &into, int values, hipStream_t s)
@@ -664,7 +696,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         c.v = a.s;
         c.ldv = a.lds;
         c.inverse = a.inverse;
-        c.partial = workspace + a.rows;
+        c.partial = workspace + 2 * (size_t)a.rows;
         c.rows = add.rows = a.rows;
         c.columns = a.columns;
         c.groups = 1;

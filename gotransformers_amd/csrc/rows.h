@@ -27,7 +27,6 @@ struct Eight<kValuesF32> {
 #pragma unroll
         for (int e = 0; e < 8; ++e) raw[e] = v[e];
     }
-    static __device__ __forceinline__ float rounded(float v) { return v; }
 };
 template <>
 struct Eight<kValuesBf16> {
@@ -44,7 +43,6 @@ struct Eight<kValuesBf16> {
 #pragma unroll
         for (int e = 0; e < 4; ++e) raw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[2 * e], v[2 * e + 1]}, b2));
     }
-    static __device__ __forceinline__ float rounded(float v) { return (float)(__bf16)v; }
 };
 template <>
 struct Eight<kValuesF16> {
@@ -61,7 +59,6 @@ struct Eight<kValuesF16> {
 #pragma unroll
         for (int e = 0; e < 4; ++e) raw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[2 * e], v[2 * e + 1]}, h2));
     }
-    static __device__ __forceinline__ float rounded(float v) { return (float)(_Float16)v; }
 };
 
 // The columns of a thread's eight values, `column` being eight times its place in the row:

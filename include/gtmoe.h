@@ -590,7 +590,8 @@ int32_t gtmoe_unpack_rows(gtmoe_context *ctx, const gtmoe_packed_desc *desc, con
  * may be NULL without residuals and may be inputs or residuals themselves (same
  * address and stride).  With codes other than NONE the result, before it is rounded
  * to the values' type, also goes to codes and scales; outputs may then be NULL.
- * Squares that float32 does not hold are added in 64 bits. */
+ * Squares that float32 does not hold are added in 64 bits, and rows of any size are
+ * normed, subnormal ones beside epsilon 0 among them (a row of zeros is then 0 / 0). */
 typedef struct gtmoe_norm_desc {
     int32_t values;
     int32_t rows;          /* 0 .. 2^30 */

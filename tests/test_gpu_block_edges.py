@@ -96,3 +96,41 @@ def test_norm_gradient_onto_the_sums_gradients(ctx, kind, rows, columns):
     apart = gradient_of_norm(ctx, kind, s, dy, w, 1e-6, ds)
     onto = gradient_of_norm(ctx, kind, s, dy, w, 1e-6, ds, True)
     assert np.array_equal(apart[4], onto[4]) and np.array_equal(apart[5], onto[5])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, columns", SHAPES)
+def test_norm_of_rows_next_to_the_ends_of_fp32(ctx, kind, rows, columns):
+    """Without epsilon 1 / sqrt(mean(s^2)) of rows of subnormal numbers is beyond fp32, of the largest
+    subnormal: the quotient and the weights' gradients are of the size of one all the same."""
+    rng = np.random.default_rng(rows + 5 * columns)
+    say(f"norm at the ends {kind} {rows} x {columns}")
+    top = 3.4e38 if kind == "f32" else 3.3e38
+    size = np.resize([1e-40, 2e38, 1e-38, 3e-37, top], rows)[:, None]
+    v = rng.uniform(-1, 1, size=(rows, columns)) * size
+    v[0, 1::2] = 0.0
+    x, y, w = Rows(kind, rows, columns, data=v), Rows(kind, rows, columns), rng.normal(size=columns) + 1
+    hw = Rows(kind, 1, columns, data=w[None])
+    d = gt.norm_desc(VALUES[kind], rows, columns, 0.0)
+    gt.norm_forward(ctx, d, x.ptr, None, hw.ptr, None, y.ptr, None, None, stream())
+    want, _ = plain.norm(x.get(), hw.get()[0], 0.0)
+    # the inverse from 64 bits and two products; a product with the power of two may leave subnormal bits, half a
+    # step of 2^-149 beside s r of the row's size 1
+    near(y.get(), want, (4 * np.abs(want) + np.abs(hw.get())) * U, kind)
+    # output gradients so small that the input gradients are numbers of fp32, and no smaller: their products
+    # with s r, of the size of one, stay normal numbers
+    dy = rng.normal(size=(rows, columns)) * np.where(size < 1e-30, 1e-10, 0.01)
+    check_gradient_of_norm(ctx, kind, v, dy, w, 0.0)
+
+
+@pytest.mark.parametrize("columns", [100, 2048, 20000])
+def test_norm_of_the_smallest_numbers(ctx, columns):
+    """A row of 2^-149, the next with zeros in it; codes of their quotients."""
+    v = np.zeros((3, columns))
+    v[0], v[1, ::3], v[2] = 2.0 ** -149, -2.0 ** -149, 1.0
+    x, y, q, k = Rows("f32", 3, columns, data=v), Rows("f32", 3, columns), Rows("u8", 3, columns), Rows("f32", 3, 1)
+    d = gt.norm_desc(gt.VALUES_FLOAT32, 3, columns, 0.0, gt.CODES_INT8, 0)
+    gt.norm_forward(ctx, d, x.ptr, None, None, None, y.ptr, q.ptr, k.ptr, stream())
+    want, _ = plain.norm(x.get(), None, 0.0)
+    near(y.get(), want, 4 * np.abs(want) * U, "f32")
+    assert np.array_equal(q.get().view(np.int8), np.sign(v) * 127)
