@@ -445,7 +445,11 @@ __device__ __forceinline__ void activation_of(float z, float &a, float &slope)
         constexpr float k = 1.59576912160573071176f, c3 = 0.044715f;
         const float s = logistic_factor(k * z * fmaf(c3 * z, z, 1.f));
         a = z * s;
-        if constexpr (SLOPE) slope = fmaf(a * (1.f - s), k * fmaf(3.f * c3 * z, z, 1.f), s);
+        if constexpr (SLOPE) {
+            // (beyond 16 in size a (1 - s) is 0, whose product with an infinite square would be none)
+            const float held = __builtin_amdgcn_fmed3f(z, -64.f, 64.f);
+            slope = fmaf(a * (1.f - s), k * fmaf(3.f * c3 * held, held, 1.f), s);
+        }
     }
 }
 template <int ACT>

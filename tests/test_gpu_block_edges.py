@@ -134,3 +134,30 @@ def test_norm_of_the_smallest_numbers(ctx, columns):
     want, _ = plain.norm(x.get(), None, 0.0)
     near(y.get(), want, 4 * np.abs(want) * U, "f32")
     assert np.array_equal(q.get().view(np.int8), np.sign(v) * 127)
+
+
+# --------------------------------------------------------------------------
+# activations
+# --------------------------------------------------------------------------
+
+ACTS = {"none": gt.ACTIVATION_NONE, "relu": gt.ACTIVATION_RELU, "silu": gt.ACTIVATION_SILU, "gelu": gt.ACTIVATION_GELU,
+        "gelu_tanh": gt.ACTIVATION_GELU_TANH}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act", list(ACTS))
+def test_activation_of_the_largest_gates(ctx, kind, act):
+    """Where act(z) is z or 0, and act' 1 or 0, all but exactly: up to the type's largest number."""
+    top = float(torch.finfo({"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[kind]).max)
+    z = np.array([1e3, 1e4, 65504.0] + ([] if kind == "f16" else [1e10, 1.8e19, 1e20, 1e30]) + [top])
+    z = np.concatenate([z, -z])[None]
+    n = z.shape[1]
+    g, u, dy = Rows(kind, 1, n, data=z), Rows(kind, 1, n, data=np.full((1, n), 0.5)), Rows(kind, 1, n, data=np.full((1, n), 0.25))
+    y, dg, du = (Rows(kind, 1, n) for _ in range(3))
+    d = gt.activation_desc(VALUES[kind], 1, n, ACTS[act])
+    gt.activation_forward(ctx, d, g.ptr, u.ptr, y.ptr, stream=stream())
+    z = g.get()
+    on = np.ones_like(z) if act == "none" else (z > 0).astype(float)
+    assert np.array_equal(y.get(), z * on / 2)
+    gt.activation_gradient(ctx, d, dy.ptr, g.ptr, None, u.ptr, None, dg.ptr, du.ptr, y.ptr, stream())
+    assert np.array_equal(y.get(), z * on / 2) and np.array_equal(dg.get(), on / 8) and np.array_equal(du.get(), z * on / 4)
