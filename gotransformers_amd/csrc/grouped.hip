@@ -385,7 +385,7 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
         }
     if constexpr (DIR == kGroupedForward)
         if (a.epilogue.on && few_fits(a, T::kBytes, da && db))
-            return launch_few(a, T::kBytes == 4 ? kValuesF32 : std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
+            return launch_few(a, values_of<T>(), s);
     const long long each = a.rows / a.groups;
     if constexpr (T::kBytes == 4) {
         if constexpr (DIR != kGroupedWeightGradient)
@@ -393,7 +393,7 @@ hipError_t launch_direction(const GroupedArgs &a, hipStream_t s)
         return launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);
     } else {
         if (da && db && large_fits(a, DIR, T::kBytes) && (DIR != kGroupedForward || whole_epilogue(a)))
-            return launch_large(a, DIR, std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16, s);
+            return launch_large(a, DIR, values_of<T>(), s);
         if constexpr (DIR == kGroupedWeightGradient) {
             if (tile_blocks(a, DIR, 128, 128) < 256) return launch_staged<T, DIR, 64, 64, 2, 2, 2>(a, da, db, s);
             return launch_staged<T, DIR, 64, 128, 2, 2, 2>(a, da, db, s);

@@ -102,15 +102,22 @@ __device__ __forceinline__ void multiply_rows(const typename T::Store *const (&p
     }
 }
 
+template <class T>
+constexpr int values_of()
+{
+    return T::kBytes == 4 ? kValuesF32 : std::is_same<T, Bf16>::value ? kValuesBf16 : kValuesF16;
+}
+
 // y = act(z + b) factor + residual of four columns of a row, z kept first where it
 // is asked for; `left` of the columns exist, the first a multiple of four.
+template <int VALUES>
 __device__ __forceinline__ float epilogue_activated(float z, int activation)
 {
     switch (activation) {
-    case kActivationRelu: return activated<kActivationRelu>(z);
-    case kActivationSilu: return activated<kActivationSilu>(z);
-    case kActivationGelu: return activated<kActivationGelu>(z);
-    case kActivationGeluTanh: return activated<kActivationGeluTanh>(z);
+    case kActivationRelu: return activated<VALUES, kActivationRelu>(z);
+    case kActivationSilu: return activated<VALUES, kActivationSilu>(z);
+    case kActivationGelu: return activated<VALUES, kActivationGelu>(z);
+    case kActivationGeluTanh: return activated<VALUES, kActivationGeluTanh>(z);
     default: return z;
     }
 }
@@ -134,7 +141,7 @@ __device__ __forceinline__ void store_fused(const GroupedArgs &a, int g, long lo
         store4<T>(reinterpret_cast<Store *>(e.products) + row * e.ldproducts + col, v, left, whole_fours<T>(e.products, e.ldproducts));
     if (e.activation != kActivationNone) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = epilogue_activated(v[i], e.activation);
+        for (int i = 0; i < 4; ++i) v[i] = epilogue_activated<values_of<T>()>(v[i], e.activation);
     }
     if (e.factor) {
         float f[4];
@@ -267,7 +274,7 @@ __device__ __forceinline__ void finish_blocks(f32x16 (&acc)[MI][NJ], const Group
 #pragma unroll
         for (int j = j0; j < j0 + EACH; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = activated<decltype(kind)::value>(acc[i][j][r]);
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = activated<values_of<T>(), decltype(kind)::value>(acc[i][j][r]);
     };
     u32x4 rows[PASSES];  // what was asked for last: a block's factors, then its residual
     auto ask_first = [&](int i, int j0) {

@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void activation_forward_kernel(Activation
         if (!any_column<VALUES>(p.column, columns)) continue;
         hold(g, u, a.limit);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = activated<ACT>(g[j]);
+        for (int j = 0; j < 8; ++j) y[j] = activated<VALUES, ACT>(g[j]);
         if (a.up) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] *= u[j];
@@ -157,11 +157,13 @@ __global__ __launch_bounds__(kThreads) void activation_gradient_kernel(Activatio
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float act, slope;
-            activation_of<ACT, true>(g[j], act, slope);
+            activation_of<VALUES, ACT, true>(g[j], act, slope);
             const float d = de.get(j), c = gated ? u[j] : 1.f;
             y[j] = act * c;
             dg[j] = d * c * slope;
             du[j] = d * act;
+            // (eight at once would take registers, and so waves: GELU in bf16 79 instead of 66)
+            if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
         if (a.limit < __builtin_inff()) {
 #pragma unroll

@@ -389,7 +389,7 @@ __device__ __forceinline__ float exp_minus(float x)
     const float e = __builtin_amdgcn_exp2f(small ? t + 64.f : t);
     return a < -1e4f ? 0.f : fmaf(e, lo * 0.69314718055994530942f, e) * (small ? 0x1p-64f : 1.f);
 }
-__device__ __forceinline__ float inverse_of(float d)  // d in [1, 2]
+__device__ __forceinline__ float inverse_of(float d)  // d at least 1, far from the largest numbers
 {
     const float x = __builtin_amdgcn_rcpf(d);
     return fmaf(fmaf(-d, x, 1.f), x, x);
@@ -401,22 +401,64 @@ __device__ __forceinline__ float logistic(float z)
     return z != z ? z : z >= 0.f ? r : e * r;
 }
 
-// The same where it is a factor of an activation: two of the hardware's functions, good to
-// a unit each, and an argument good to |z| 2^-24.  Below 2^-126 (z < -87) it is 0.
-__device__ __forceinline__ float logistic_factor(float z)
-{
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * z));
-}
+// Activations z times a factor.  The hardware's functions know no subnormal numbers, and
+// z e^z may still be one, or a normal number of bf16 and fp32, where e^z is none (z = -88): there
+// e^z is taken times a power of two, and that put right behind the product with z.
+
+// 1 / (1 + e^-z) = value * times for 16-bit rows: a power of two and a reciprocal of the
+// hardware's, good to a unit each, of an argument good to |z| 2^-24.  fp16 has no numbers as small.
+template <int VALUES>
+struct Logistic {
+    float value, times;
+    __device__ __forceinline__ Logistic(float z)
+    {
+        constexpr float by = (float)-1.44269504088896340736;
+        const bool far = VALUES == kValuesBf16 && z < 0.f;
+        times = far ? 0x1p-32f : 1.f;
+        value = __builtin_amdgcn_rcpf(times + __builtin_amdgcn_exp2f(VALUES == kValuesBf16 ? fmaf(by, z, far ? -32.f : 0.f) : by * z));
+    }
+};
+
+// 2^(whole + fraction) = e * times for fp32 rows: an exponent t rounded to fp32 would cost |t|
+// units, the fraction holds what is left of it beside its whole part.
+struct Power {
+    float e, times;
+    __device__ __forceinline__ Power(float whole, float fraction)
+    {
+        const bool far = whole < -64.f;
+        times = far ? 0x1p-64f : 1.f;
+        e = ldexpf(__builtin_amdgcn_exp2f(fraction), (int)whole + (far ? 64 : 0));
+    }
+};
+constexpr double kLog2e = 1.44269504088896340736;
+// what fp32 leaves of a constant
+constexpr float rest_of(double c) { return (float)(c - (double)(float)c); }
+// s = value * times = 1 / (1 + e^-y) and rest = 1 - s, of y's sign and p = e^-|y|.
+struct WideLogistic {
+    float value, times, rest;
+    __device__ __forceinline__ WideLogistic(bool below, const Power &p)
+    {
+        const float e = p.e * p.times, r = inverse_of(1.f + e);
+        value = below ? p.e * r : r;
+        times = below ? p.times : 1.f;
+        rest = below ? r : e * r;
+    }
+};
 
 __device__ constexpr float kTail[10] = {0.25388533f, 0.25388303f,  0.22827554f, 0.17520681f,  0.12021917f,
                                         -0.023251647f, 0.14413364f, -0.30252245f, 0.1918485f, -0.041677944f};
 
-// act(z) and, where asked for, act'(z).  A NaN stays one.  Arithmetic bounds these where
-// they stand beside 16-bit rows: SiLU takes 11 of the vector unit's slots, GELU 30, so
-// neither has the care for factors below 2^-126 that would double SiLU's.
-template <int ACT, bool SLOPE>
+// act(z) and, where asked for, act'(z).  A NaN stays one.  16-bit rows keep 8 or 11 bits of them
+// and take short forms, whose arithmetic bounds kernels beside their bytes; fp32 rows have both
+// the time and the use for exponents of more bits than fp32: rms errors of SiLU 5.1e-8 of the value,
+// GELU 7.3e-8, its tanh form 4.8e-8 (an exponent rounded to fp32: 8e-8 for SiLU below 4, 4e-7 from 10 on).  What
+// both cost (us, against factors that end at 2^-126 and fp32 by the short forms): SiLU 4096 x 2048
+// bf16 forward with codes 15.8 -> 16.3, gradient from them 18.7 -> 19.0, fp32 26.4 -> 27.8 and 34.4 -> 35.3;
+// without codes fp32 20.5 -> 20.7 and 42.7 -> 42.8.
+template <int VALUES, int ACT, bool SLOPE>
 __device__ __forceinline__ void activation_of(float z, float &a, float &slope)
 {
+    constexpr bool WIDE = VALUES == kValuesF32;
     if constexpr (ACT == kActivationNone) {
         a = z;
         slope = 1.f;
@@ -424,42 +466,75 @@ __device__ __forceinline__ void activation_of(float z, float &a, float &slope)
         a = z <= 0.f ? 0.f : z;
         slope = z <= 0.f ? 0.f : z != z ? z : 1.f;
     } else if constexpr (ACT == kActivationSilu) {
-        const float s = logistic_factor(z);
-        a = z * s;
-        if constexpr (SLOPE) slope = fmaf(a, 1.f - s, s);
+        if constexpr (WIDE) {
+            constexpr float by = (float)-kLog2e, by_rest = rest_of(-kLog2e);
+            const float size = fminf(fabsf(z), 200.f), whole = rintf(size * by);
+            const Power e(whole, fmaf(size, by_rest, fmaf(size, by, -whole)));
+            const WideLogistic l(z < 0.f, e);
+            a = z * l.value * l.times;
+            if constexpr (SLOPE) slope = fmaf(z, l.rest, 1.f) * l.value * l.times;
+        } else {
+            const Logistic<VALUES> l(z);
+            a = z * l.value * l.times;
+            const float s = l.value * l.times;
+            if constexpr (SLOPE) slope = fmaf(a, 1.f - s, s);
+        }
     } else if constexpr (ACT == kActivationGelu) {
         // z times the normal distribution, from its smaller tail so that nothing
         // cancels: with x = |z| / sqrt 2 the tail is e^(-x^2) / 2 times e^(x^2) erfc(x), which
-        // over t in (0, 1], t = 1 / (1 + 0.45 x), is t times a polynomial (a Chebyshev fit to
-        // 4e-8 over x up to 2000)
-        const float size = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(0.31819805153394638598f, size, 1.f));
-        const float e = __builtin_amdgcn_exp2f(-0.72134752044448170368f * (z * z));
-        float p = kTail[9];
+        // over r in (0, 1], r = 1 / (1 + 0.45 x), is r times a polynomial (a Chebyshev fit, as
+        // rounded good to 6.2e-8 over x up to 2000)
+        constexpr float density = 0.39894228040143267794f, by = (float)(-0.5 * kLog2e);
+        // e and the tail are taken 2^32 times as large but for fp16, which has no numbers there
+        constexpr float shift = VALUES == kValuesF16 ? 0.f : 32.f, half = VALUES == kValuesF16 ? 0.5f : 0x1p-33f;
+        const float size = WIDE ? fminf(fabsf(z), 32.f) : fabsf(z), r = __builtin_amdgcn_rcpf(fmaf(0.31819805153394638598f, size, 1.f));
+        const float square = size * size;
+        float e, p = kTail[9];
+        if constexpr (WIDE) {
+            const float whole = rintf(square * by), rest = fmaf(square, rest_of(-0.5 * kLog2e), fmaf(size, size, -square) * by);
+            e = ldexpf(__builtin_amdgcn_exp2f(fmaf(square, by, -whole) + rest), (int)whole + 32);
+        } else {
+            e = __builtin_amdgcn_exp2f(fmaf(square, by, shift));
+        }
 #pragma unroll
-        for (int i = 8; i >= 0; --i) p = fmaf(p, t, kTail[i]);
-        const float tail = 0.5f * e * (t * p), c = z > 0.f ? 1.f - tail : tail;
-        a = z * c;
-        if constexpr (SLOPE) slope = fmaf(z * 0.39894228040143267794f, e, c);
+        for (int i = 8; i >= 0; --i) p = fmaf(p, r, kTail[i]);
+        const float w = e * (r * p);
+        const float c = z > 0.f ? fmaf(w, -half, 1.f) : w, times = z > 0.f ? 1.f : half;
+        a = z * c * times;
+        if constexpr (SLOPE) slope = fmaf(z * (2.f * half * density), e, c * times);
     } else {
         // 0.5 z (1 + tanh(u)) = z logistic(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)
-        constexpr float k = 1.59576912160573071176f, c3 = 0.044715f;
-        const float s = logistic_factor(k * z * fmaf(c3 * z, z, 1.f));
-        a = z * s;
-        if constexpr (SLOPE) {
-            // (beyond 16 in size a (1 - s) is 0, whose product with an infinite square would be none)
-            const float held = __builtin_amdgcn_fmed3f(z, -64.f, 64.f);
-            slope = fmaf(a * (1.f - s), k * fmaf(3.f * c3 * held, held, 1.f), s);
+        constexpr double k64 = 1.59576912160573071176, c64 = 0.044715;
+        constexpr float k = (float)k64, c3 = (float)c64;
+        // (beyond 16 in size the slope is 0 or 1; of infinite squares it would be no number)
+        const float held = __builtin_amdgcn_fmed3f(z, -64.f, 64.f), dy = k * fmaf(3.f * c3 * held, held, 1.f);
+        if constexpr (WIDE) {
+            // -|y| log2 e = u v, u = -k log2 e |z| and v = 1 + c3 z^2, each with what its rounding left
+            constexpr float by = (float)(-k64 * kLog2e), by_rest = rest_of(-k64 * kLog2e);
+            const float size = fminf(fabsf(z), 16.f), square = size * size;
+            const float u = size * by, u_rest = fmaf(size, by_rest, fmaf(size, by, -u));
+            const float v = fmaf(c3, square, 1.f);
+            const float v_rest = fmaf(c3, square, 1.f - v) + fmaf(rest_of(c64), square, c3 * fmaf(size, size, -square));
+            const float whole = rintf(u * v);
+            const Power e(whole, fmaf(u, v, -whole) + fmaf(u, v_rest, v * u_rest));
+            const WideLogistic l(z < 0.f, e);
+            a = z * l.value * l.times;
+            if constexpr (SLOPE) slope = z != z ? z : fmaf(held * l.rest, dy, 1.f) * l.value * l.times;
+        } else {
+            const Logistic<VALUES> l(k * z * fmaf(c3 * z, z, 1.f));
+            a = z * l.value * l.times;
+            const float s = l.value * l.times;
+            if constexpr (SLOPE) slope = fmaf(a * (1.f - s), dy, s);
         }
     }
 }
-template <int ACT>
+template <int VALUES, int ACT>
 __device__ __forceinline__ float activated(float z)
 {
     float a, slope;
-    activation_of<ACT, false>(z, a, slope);
+    activation_of<VALUES, ACT, false>(z, a, slope);
     return a;
 }
-
 }  // namespace
 
 }  // namespace gtmoe

@@ -626,7 +626,8 @@ int32_t gtmoe_norm_gradient(gtmoe_context *ctx, const gtmoe_norm_desc *desc, con
 
 /* Activations (activationfunction/activationfunction.go): GELU is z times the normal
  * distribution at z, GELU_TANH its form with a tanh.  They are good to about
- * 2^-19 + z^2 2^-22 of their value; where a factor of z falls below 2^-126 they may be 0. */
+ * 2^-20 of their value on float32 rows and to 2^-19 + z^2 2^-22 on 16-bit rows before
+ * these are rounded, down to the type's smallest numbers. */
 enum gtmoe_activation {
     GTMOE_ACTIVATION_NONE = 0,
     GTMOE_ACTIVATION_RELU = 1,

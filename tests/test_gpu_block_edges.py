@@ -161,3 +161,48 @@ def test_activation_of_the_largest_gates(ctx, kind, act):
     assert np.array_equal(y.get(), z * on / 2)
     gt.activation_gradient(ctx, d, dy.ptr, g.ptr, None, u.ptr, None, dg.ptr, du.ptr, y.ptr, stream())
     assert np.array_equal(y.get(), z * on / 2) and np.array_equal(dg.get(), on / 8) and np.array_equal(du.get(), z * on / 4)
+
+
+def curve(ctx, kind, act, z):
+    """(act, act') at z by the operators."""
+    n = z.size
+    g, one = Rows(kind, 1, n, data=z[None]), Rows(kind, 1, n, data=np.ones((1, n)))
+    y, again, dg = Rows(kind, 1, n), Rows(kind, 1, n), Rows(kind, 1, n)
+    d = gt.activation_desc(VALUES[kind], 1, n, ACTS[act])
+    gt.activation_forward(ctx, d, g.ptr, None, y.ptr, stream=stream())
+    gt.activation_gradient(ctx, d, one.ptr, g.ptr, None, None, None, dg.ptr, None, again.ptr, stream())
+    assert bool((again.buffer == y.buffer).all())
+    return g.get()[0], y.get()[0], dg.get()[0]
+
+
+# where act(z) is 2^-150: half of the smallest number
+TAILS = {"silu": -108.6, "gelu": -14.3, "gelu_tanh": -10.9}
+
+
+@pytest.mark.parametrize("act", list(TAILS))
+def test_activation_of_fp32_rows(ctx, act):
+    """Bounds, in units of 2^-24 of the value, or for the slope of its terms: SiLU's and the tanh form's
+    power of two 2.2 (a unit of the hardware's, the argument's fraction), the reciprocal 3.2, two products: 8.
+    GELU's power 2.2, its t 2.6, the polynomial's fit 1.1 and roundings 4, three products: 14.  Slopes take three
+    more roundings of each term, the tanh form's four of the argument's slope."""
+    rng = np.random.default_rng(1)
+    z = np.concatenate([np.linspace(TAILS[act], 20, 20001), rng.normal(size=20000) * 3, rng.normal(size=200) * 1e-30])
+    z, y, slope = curve(ctx, "f32", act, z)
+    want, d, size = plain.activation(z, act)
+    near(y, want, 16 * U * np.abs(want), "f32")
+    near(slope, d, 24 * U * size + 2.0 ** -148, "f32")
+    near_by = (z > -8) & (z < 8) & (np.abs(z) > 1e-3)
+    rms = lambda e: float(np.sqrt(np.mean(e * e)))
+    say(f"{act} rms relative error {rms((y / want - 1)[near_by]):.2e}")
+
+
+@pytest.mark.parametrize("act", list(TAILS))
+def test_activation_of_bf16_rows_to_the_smallest_numbers(ctx, act):
+    """2^-14 is 1024 units of 2^-24: of |z|, of z^2 / 2 (GELU) or of five times the argument (the tanh form), up
+    to 109, at most 550, and 40 for the functions and products."""
+    z = np.linspace(TAILS[act], 4, 4001)
+    z, y, slope = curve(ctx, "bf16", act, z)
+    want, d, size = plain.activation(z, act)
+    assert np.abs(want[z < 0]).min() < 2.0 ** -133
+    near(y, want, 2.0 ** -14 * np.abs(want) + 2.0 ** -149, "bf16")
+    near(slope, d, 2.0 ** -14 * size + 2.0 ** -148, "bf16")
