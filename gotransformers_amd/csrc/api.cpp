@@ -4073,7 +4073,7 @@ int32_t gtmoe_route_forward(gtmoe_context *ctx, const gtmoe_route_desc *desc, co
         a.group_best = desc->group_best;
         a.logistic = desc->scores == GTMOE_SCORES_SIGMOID;
         a.renormalize = desc->renormalize != 0;
-        a.scale = (float)desc->scale;
+        a.scale = desc->scale;
         return GTMOE_OK;
     };
     if (!ctx) return check_only(check);
@@ -4111,7 +4111,7 @@ int32_t gtmoe_route_gradient(gtmoe_context *ctx, const gtmoe_route_desc *desc, c
         a.k = desc->experts_per_token;
         a.logistic = desc->scores == GTMOE_SCORES_SIGMOID;
         a.renormalize = desc->renormalize != 0;
-        a.scale = (float)desc->scale;
+        a.scale = desc->scale;
         return GTMOE_OK;
     };
     if (!ctx) return check_only(check);

@@ -20,6 +20,8 @@
 //
 // Renormalized gates take the chosen scores by their largest, so that neither large nor
 // very negative logits leave 0 / 0:  s = e^l, or e^min(l, 0) / (1 + e^-|l|).
+// Gates and gradients are taken in fp64 and rounded once (16384 tokens below: 20.8 -> 21.4 us with
+// the lists; in fp32 with its sums they were off by 2.2 times a rounding).
 //
 // Lists.  A workgroup takes `each` consecutive tokens and writes how often each
 // expert was chosen among them; the second kernel adds the counts of the
@@ -136,10 +138,16 @@ __device__ __forceinline__ double inverse64(double d)
     x = fma(fma(-d, x, 1.0), x, x);
     return fma(fma(-d, x, 1.0), x, x);
 }
+// e^(a - b), a at most b but for NaN, which stays one
+__device__ __forceinline__ double exp_between(float a, float b)
+{
+    const double x = (double)a - (double)b;
+    return x != x ? x : exp64(x);
+}
 __device__ __forceinline__ double logistic64(float l)
 {
     const double e = exp64(-fabs((double)l)), r = inverse64(1.0 + e);
-    return l >= 0.f ? r : e * r;
+    return l != l ? (double)l : l >= 0.f ? r : e * r;
 }
 
 // The team's largest key and sums.
@@ -161,16 +169,14 @@ __device__ __forceinline__ double team_largest(double v)
     return v;
 }
 template <int TEAM>
-__device__ __forceinline__ float team_total(float v)
-{
-    if constexpr (TEAM == 16) return sixteen_sum(v);
-    return wave_sum(v);
-}
-template <int TEAM>
 __device__ __forceinline__ double team_total(double v)
 {
-#pragma unroll
-    for (int d = 1; d < TEAM; d <<= 1) v += __shfl_xor(v, d);
+    v += moved64<kDppPairs>(v);
+    v += moved64<kDppFours>(v);
+    v += moved64<kDppEights>(v);
+    v += moved64<kDppSixteens>(v);
+    if constexpr (TEAM == 64)
+        v = (lane_value64(v, 0) + lane_value64(v, 16)) + (lane_value64(v, 32) + lane_value64(v, 48));
     return v;
 }
 template <int TEAM>
@@ -206,18 +212,18 @@ __device__ __forceinline__ void load_logits(float (&l)[EPL], const void *base, l
 
 // The share s / sum of this lane's choice among the team's, l its logit.
 template <int TEAM>
-__device__ __forceinline__ float share_of(float l, bool have, bool logistic_scores)
+__device__ __forceinline__ double share_of(float l, bool have, bool logistic_scores)
 {
     // s = e^upper times a number between 1/2 and 1
     const float upper = logistic_scores && l > 0.f ? 0.f : l;
     float most = team_most<TEAM>(have ? upper : -__builtin_inff());
     if (most == -__builtin_inff()) most = 0.f;  // nothing but -inf: every share is 0
     // (upper is at most `most`; +inf beside itself is NaN)
-    float s = exp_minus(upper - most);
-    if (logistic_scores) s *= inverse_of(1.f + exp_minus(l));
-    s = have ? s : 0.f;
-    const float sum = team_total<TEAM>(s);
-    return sum == 0.f ? 0.f : s / sum;
+    double s = exp_between(upper, most);
+    if (logistic_scores) s *= inverse64(1.0 + exp64(-fabs((double)l)));
+    s = have ? s : 0.0;
+    const double sum = team_total<TEAM>(s);
+    return sum == 0.0 ? 0.0 : s * inverse64(sum);
 }
 
 __device__ __forceinline__ int group_of(int e, uint32_t group_inverse) { return (int)((uint32_t)e * group_inverse >> 22); }
@@ -285,7 +291,8 @@ __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, in
         const bool here = t0 + team < last;
         float l[EPL];
         load_logits<VALUES>(l, a.logits, (long long)t * a.ldlogits, e0, a.experts);
-        float most = 0.f, sum = 0.f;  // of a softmax over all experts
+        float most = 0.f;  // of a softmax over all experts
+        double sum = 0;
         if (!a.logistic && (BIASED || !a.renormalize || GROUPS != kNoGroups)) {
             most = l[0];
 #pragma unroll
@@ -294,7 +301,7 @@ __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, in
             if (most == -__builtin_inff()) most = 0.f;
             if (!a.renormalize) {
 #pragma unroll
-                for (int i = 0; i < EPL; ++i) sum += exp_minus(l[i] - most);
+                for (int i = 0; i < EPL; ++i) sum += exp_between(l[i], most);
                 sum = team_total<TEAM>(sum);
             }
         }
@@ -400,19 +407,20 @@ __device__ __forceinline__ void choose_tokens(const ChooseArgs &a, int first, in
             const int e = winner * EPL + __builtin_amdgcn_ds_bpermute(4 * (team * TEAM + winner), at);
             expert = j == in ? e : expert;
         }
-        float logit, gate;
+        float logit;
         {
             float v[1];
             load_logits<VALUES>(v, a.logits, (long long)t * a.ldlogits, expert, a.experts);
             logit = v[0];
         }
         const bool have = in < a.k;
+        double gate;
         if (a.renormalize) gate = share_of<TEAM>(logit, have, a.logistic);
-        else gate = a.logistic ? logistic(logit) : sum == 0.f ? 0.f : exp_minus(logit - most) / sum;
+        else gate = a.logistic ? logistic64(logit) : sum == 0.0 ? 0.0 : exp_between(logit, most) * inverse64(sum);
         if (have && here) {
             const long long at = (long long)t * a.k + in;
             a.chosen[at] = expert;
-            a.gates[at] = gate * a.scale;
+            a.gates[at] = (float)(gate * a.scale);
             take(t, expert);
         }
     }
@@ -625,10 +633,11 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
         const long long t = min(t0 + team, (long long)a.tokens - 1);
         const bool here = t0 + team < a.tokens;
         int expert = -1;
-        float l = 0.f, dg = 0.f;
+        float l = 0.f;
+        double dg = 0;
         if (in < a.k) {
             expert = a.chosen[t * a.k + in];
-            dg = a.gate_gradients[t * a.k + in] * a.scale;
+            dg = (double)a.gate_gradients[t * a.k + in] * a.scale;
         }
         const bool have = expert >= 0 && expert < a.experts;
         if (have) {
@@ -637,20 +646,21 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
             l = v[0];
         } else {
             expert = -1;
-            dg = 0.f;
+            dg = 0;
         }
-        float out[EPL], d;  // d: what this lane's choice adds to its expert's gradient
+        double out[EPL], d;  // d: what this lane's choice adds to its expert's gradient
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) out[i] = 0.f;
+        for (int i = 0; i < EPL; ++i) out[i] = 0;
         if (a.renormalize) {
-            const float share = share_of<TEAM>(l, have, a.logistic);
-            const float dot = team_total<TEAM>(have ? share * dg : 0.f);
+            const double share = share_of<TEAM>(l, have, a.logistic);
+            const double dot = team_total<TEAM>(have ? share * dg : 0.0);
             d = share * (dg - dot);
-            if (a.logistic) d *= logistic(-l);
+            if (a.logistic) d *= logistic64(-l);
         } else if (a.logistic) {
-            d = dg * logistic(l) * logistic(-l);
+            d = dg * logistic64(l) * logistic64(-l);
         } else {
-            float all[EPL], most, sum = 0.f;
+            float all[EPL], most;
+            double sum = 0;
             load_logits<VALUES>(all, a.logits, t * a.ldlogits, e0, a.experts);
             most = all[0];
 #pragma unroll
@@ -659,20 +669,20 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
             if (most == -__builtin_inff()) most = 0.f;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) {
-                out[i] = exp_minus(all[i] - most);
+                out[i] = exp_between(all[i], most);
                 sum += out[i];
             }
             sum = team_total<TEAM>(sum);
-            const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-            d = have ? dg * (exp_minus(l - most) * inverse) : 0.f;
-            const float dot = team_total<TEAM>(d);
+            const double inverse = sum == 0.0 ? 0.0 : inverse64(sum);
+            d = have ? dg * (exp_between(l, most) * inverse) : 0.0;
+            const double by = -team_total<TEAM>(d) * inverse;
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) out[i] = -dot * (out[i] * inverse);
+            for (int i = 0; i < EPL; ++i) out[i] *= by;
         }
         for (int j = 0; j < a.k; ++j) {
             const int from = 4 * (team * TEAM + j);
             const int e = __builtin_amdgcn_ds_bpermute(from, expert);
-            const float v = __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint(d)));
+            const double v = permuted(from, d);
 #pragma unroll
             for (int i = 0; i < EPL; ++i)
                 if (e == e0 + i) out[i] += v;
@@ -683,9 +693,10 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
         Store w[EPL];
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
-            if constexpr (VALUES == kValuesF32) w[i] = out[i];
-            else if constexpr (VALUES == kValuesBf16) w[i] = __builtin_bit_cast(uint16_t, (__bf16)out[i]);
-            else w[i] = __builtin_bit_cast(uint16_t, (_Float16)out[i]);
+            const float v = (float)out[i];
+            if constexpr (VALUES == kValuesF32) w[i] = v;
+            else if constexpr (VALUES == kValuesBf16) w[i] = __builtin_bit_cast(uint16_t, (__bf16)v);
+            else w[i] = __builtin_bit_cast(uint16_t, (_Float16)v);
         }
         if (e0 + EPL <= a.experts) {
             __builtin_memcpy(p, w, sizeof w);

@@ -198,7 +198,7 @@ struct ChooseArgs {
     long long ldlogits = 0;
     int tokens = 0, experts = 0, k = 0, groups = 1, chosen_groups = 1, group_best = 1;
     int logistic = 0, renormalize = 0;
-    float scale = 1.f;
+    double scale = 1.0;
     // set by the launcher: tokens per workgroup, what each counted, the sums before it
     int each = 0, ldcounts = 0;
     uint32_t group_inverse = 0;
@@ -220,7 +220,7 @@ struct ChooseGradientArgs {
     void *logit_gradients = nullptr;
     long long ldlogits = 0, ldgradients = 0;
     int tokens = 0, experts = 0, k = 0, logistic = 0, renormalize = 0;
-    float scale = 1.f;
+    double scale = 1.0;
 };
 hipError_t launch_choose_gradient(const ChooseGradientArgs &a, int values, hipStream_t s);
 

@@ -377,28 +377,10 @@ __device__ __forceinline__ void kept_eight(float (&v)[8], long long row, int col
 // ---------------------------------------------------------------------------
 enum Activation { kActivationNone = 0, kActivationRelu = 1, kActivationSilu = 2, kActivationGelu = 3, kActivationGeluTanh = 4 };
 
-// e^-|x|, about a unit in the last place: the exponent's product with log2 e in two
-// parts.  The hardware's power of two gives zero where the result is below 2^-126:
-// there it takes 64 less, and the product with 2^-64 keeps the subnormal bits.
-__device__ __forceinline__ float exp_minus(float x)
-{
-    constexpr float log2e = 1.44269504088896340736f, rest = (float)(1.44269504088896340736 - (double)1.44269504088896340736f);
-    const float a = -fabsf(x), t = a * log2e;
-    const float lo = fmaf(a, rest, fmaf(a, log2e, -t));
-    const bool small = t < -125.f;
-    const float e = __builtin_amdgcn_exp2f(small ? t + 64.f : t);
-    return a < -1e4f ? 0.f : fmaf(e, lo * 0.69314718055994530942f, e) * (small ? 0x1p-64f : 1.f);
-}
 __device__ __forceinline__ float inverse_of(float d)  // d at least 1, far from the largest numbers
 {
     const float x = __builtin_amdgcn_rcpf(d);
     return fmaf(fmaf(-d, x, 1.f), x, x);
-}
-// 1 / (1 + e^-z)
-__device__ __forceinline__ float logistic(float z)
-{
-    const float e = exp_minus(z), r = inverse_of(1.f + e);
-    return z != z ? z : z >= 0.f ? r : e * r;
 }
 
 // Activations z times a factor.  The hardware's functions know no subnormal numbers, and

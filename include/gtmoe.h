@@ -714,11 +714,12 @@ int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc
  * above 1 only the experts of chosen_groups groups of consecutive experts can be
  * chosen: those with the largest sums of their group_best (1 or 2) best s + biases
  * (group_best 1 without biases: their largest logit); equal ones by the lower index.
- * What is compared is computed in 64 bits.  A logit of -infinity or NaN comes after
- * every other, whatever its bias, and counts in no group's sum; a token with
- * nothing but -infinity has gates 0.  NaN, and in a softmax +infinity, leave the
- * token's gates not finite; its choices are experts of the range all the same, each
- * once.
+ * What is compared, the gates and their gradients are computed in 64 bits.  A logit of
+ * -infinity or NaN comes after every other, whatever its bias, and counts in no group's
+ * sum; a token with nothing but -infinity has gates 0.  NaN, and in a softmax
+ * +infinity, leave the gates not finite whose sum they are in (renormalized: of the
+ * chosen; a softmax: of all); the token's choices are experts of the range all the same,
+ * each once.
  * chosen [tokens][experts_per_token], gates alike (float32).  Where expert_offsets
  * is not NULL the rows in expert order are listed as gtmoe_last_routing does:
  * expert_offsets [experts + 1], rows_for_expert (the token of every row, may be

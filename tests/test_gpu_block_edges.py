@@ -206,3 +206,52 @@ def test_activation_of_bf16_rows_to_the_smallest_numbers(ctx, act):
     assert np.abs(want[z < 0]).min() < 2.0 ** -133
     near(y, want, 2.0 ** -14 * np.abs(want) + 2.0 ** -149, "bf16")
     near(slope, d, 2.0 ** -14 * size + 2.0 ** -148, "bf16")
+
+
+# --------------------------------------------------------------------------
+# the choice of experts
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens, experts, k, biased", [(300, 64, 6, False), (40, 128, 8, True), (33, 24, 3, False), (20, 700, 20, True)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_route_gates_and_gradients_are_rounded_once(ctx, kind, tokens, experts, k, biased, scores, renormalize):
+    """Scores, their sums and the gradients are taken in 64 bits (the exponential to 1e-14, 1024 terms): 1e-12 of
+    the terms, and one rounding; a 16-bit gradient is rounded to fp32 first.  Small scores stay as exact."""
+    rng = np.random.default_rng(tokens + experts)
+    say(f"gates {kind} {tokens} {experts} {k} {biased} {scores} {renormalize}")
+    far = np.repeat([1.0, 20.0, 60.0], -(-tokens // 3))[:tokens, None]
+    l, dg = rng.normal(size=(tokens, experts)) * far, rng.normal(size=(tokens, k))
+    l, dg = Rows(kind, tokens, experts, data=l), Rows("f32", tokens, k, data=dg)
+    b = torch.as_tensor(rng.normal(size=experts) * 0.1, dtype=torch.float32).cuda() if biased else None
+    chosen, gates, dl = Rows("i32", tokens, k), Rows("f32", tokens, k), Rows(kind, tokens, experts)
+    d = gt.route_desc(VALUES[kind], tokens, experts, k, scores=gt.SCORES_SIGMOID if scores == "sigmoid" else gt.SCORES_SOFTMAX,
+                      renormalize=renormalize, scale=0.1)
+    gt.route_forward(ctx, d, l.ptr, None if b is None else b.data_ptr(), chosen.ptr, gates.ptr, stream=stream())
+    want, wgates = plain.route(l.get(), None if b is None else b.double().cpu().numpy(), k, scores, renormalize=renormalize, scale=0.1)
+    assert np.array_equal(chosen.get(), want)
+    near(gates.get(), wgates, 1e-12 * np.abs(wgates), "f32")
+    gt.route_gradient(ctx, d, l.ptr, chosen.ptr, dg.ptr, dl.ptr, stream())
+    ref, size = plain.route_gradient(l.get(), want, dg.get(), scores, renormalize, 0.1)
+    near(dl.get(), ref, 1e-12 * size + (0.0 if kind == "f32" else np.abs(ref) * U + 2.0 ** -150), kind)
+
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_route_gates_of_what_is_not_finite(ctx, biased, renormalize):
+    """Of a softmax: a sum that NaN or +infinity is in leaves no gate finite, other tokens' gates stay."""
+    rng = np.random.default_rng(3)
+    l = rng.normal(size=(40, 32))
+    l[3, 5], l[8, 0], l[9] = np.nan, np.inf, np.nan
+    l = Rows("f32", 40, 32, data=l)
+    b = torch.zeros(32, device="cuda") if biased else None
+    chosen, gates = Rows("i32", 40, 4), Rows("f32", 40, 4)
+    d = gt.route_desc(0, 40, 32, 4, renormalize=renormalize)
+    gt.route_forward(ctx, d, l.ptr, None if b is None else b.data_ptr(), chosen.ptr, gates.ptr, stream=stream())
+    got = gates.get()
+    sums = [9] if renormalize else [3, 8, 9]
+    if 0 in chosen.get()[8]:
+        sums.append(8)
+    assert not np.isfinite(got[sums]).any()
+    assert np.isfinite(got[np.setdiff1d(np.arange(40), [3, 8, 9])]).all()
