@@ -3725,7 +3725,7 @@ int32_t gtmoe_norm_workspace(const gtmoe_norm_desc *desc, size_t *bytes)
 {
     if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
     TRY(check_norm(nullptr, desc));
-    *bytes = norm_gradient_floats(desc->rows, desc->columns) * 4;
+    *bytes = norm_gradient_bytes(desc->rows, desc->columns);
     return GTMOE_OK;
 }
 
@@ -3747,7 +3747,7 @@ int32_t gtmoe_norm_gradient(gtmoe_context *ctx, const gtmoe_norm_desc *desc, con
             TRY(check_gradient_values(c, "weight gradients", gradient_values, desc->values));
             gs = value_bytes(gradient_values);
             TRY(check_pointer(c, "weight gradients", weight_gradients, gs));
-            need = norm_gradient_floats(desc->rows, desc->columns) * 4;
+            need = norm_gradient_bytes(desc->rows, desc->columns);
             TRY(check_workspace(c, workspace, workspace_bytes, need));
         }
         if (desc->rows > 0) {
@@ -3969,7 +3969,7 @@ int32_t gtmoe_grouped_bias_workspace(const gtmoe_grouped_desc *desc, size_t *byt
     static const int32_t offsets[2] = {0, 0};
     if (!bytes) return GTMOE_ERR_INVALID_ARGUMENT;
     TRY(check_grouped(nullptr, desc, offsets));
-    *bytes = sum_floats(desc->rows, desc->groups, desc->outputs) * 4;
+    *bytes = sum_bytes(desc->rows, desc->groups, desc->outputs);
     return GTMOE_OK;
 }
 
@@ -3983,7 +3983,7 @@ int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc
         TRY(check_grouped_or_whole(c, desc, offsets));
         TRY(check_gradient_values(c, "bias gradients", gradient_values, desc->values));
         const int es = value_bytes(desc->values), gs = value_bytes(gradient_values);
-        const size_t need = sum_floats(desc->rows, desc->groups, desc->outputs) * 4;
+        const size_t need = sum_bytes(desc->rows, desc->groups, desc->outputs);
         TRY(check_pointer(c, "bias gradients", bias_gradients, gs));
         if (desc->rows > 0) TRY(check_pointer(c, "output gradients", output_gradients, es));
         TRY(check_workspace(c, workspace, workspace_bytes, need));
@@ -3995,7 +3995,7 @@ int32_t gtmoe_grouped_bias_gradient(gtmoe_context *ctx, const gtmoe_grouped_desc
         a.x = output_gradients;
         a.ldx = desc->output_stride;
         a.offsets = add.offsets = offsets;
-        a.partial = (float *)workspace;
+        a.partial = (double *)workspace;
         add.partial = a.partial;
         a.rows = add.rows = desc->rows;
         a.columns = add.columns = desc->outputs;

@@ -129,7 +129,7 @@ hipError_t launch_norm_forward(const NormArgs &a, int values, hipStream_t s);
 
 // Sums of partial rows: of all `count`, or (each > 0) of those of group g's rows.
 struct AddPartialsArgs {
-    const float *partial = nullptr;
+    const void *partial = nullptr;  // fp32, or fp64 those of column sums
     void *out = nullptr;
     const int32_t *offsets = nullptr;
     long long ldo = 0;
@@ -146,23 +146,23 @@ struct NormGradientArgs {
     int rows = 0, columns = 0;
     double epsilon = 0;
 };
-// Floats of workspace with dw.
-size_t norm_gradient_floats(int rows, int columns);
+// Bytes of workspace with dw.
+size_t norm_gradient_bytes(int rows, int columns);
 // into.out null: no dw.
 hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddPartialsArgs &into, int values, hipStream_t s);
 
-// Sums of rows by group, partial rows of `each` consecutive rows first.
+// Sums of rows by group in fp64, partial rows of `each` consecutive rows first.
 struct ColumnSumsArgs {
     const void *x = nullptr, *v = nullptr;
     const float *inverse = nullptr;
     const int32_t *offsets = nullptr;
-    float *partial = nullptr;
+    double *partial = nullptr;
     long long ldx = 0, ldv = 0;
     int rows = 0, columns = 0, groups = 1, each = 0;
     AddPartialsArgs into;  // set by the launcher: the sums themselves
 };
 int sum_rows_each(int rows, int groups, int columns);
-size_t sum_floats(int rows, int groups, int columns);
+size_t sum_bytes(int rows, int groups, int columns);
 hipError_t launch_column_sums(ColumnSumsArgs a, const AddPartialsArgs &add, int values, hipStream_t s);
 
 struct PackArgs {

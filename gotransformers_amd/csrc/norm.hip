@@ -287,12 +287,12 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_forward_kernel(NormAr
 
 // out[g][c] (+)= sum, rounded once.
 template <int VALUES>
-__device__ __forceinline__ void store_sum(const AddPartialsArgs &a, int g, int c, float sum)
+__device__ __forceinline__ void store_sum(const AddPartialsArgs &a, int g, int c, double sum)
 {
     const long long at = g * a.ldo + c;
     if (a.out_f32) {
         float *o = reinterpret_cast<float *>(a.out) + at;
-        *o = a.accumulate ? *o + sum : sum;
+        *o = (float)(a.accumulate ? *o + sum : sum);
     } else {
         typedef typename Eight<VALUES>::Store Store;
         Eight<VALUES> e;
@@ -302,7 +302,7 @@ __device__ __forceinline__ void store_sum(const AddPartialsArgs &a, int g, int c
             __builtin_memcpy(e.raw, w, sizeof w);
             sum += e.get(0);
         }
-        const float v[8] = {sum, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const float v[8] = {(float)sum, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         e.set(v);
         __builtin_memcpy(w, e.raw, sizeof w);
         *o = w[0];
@@ -399,18 +399,19 @@ __global__ __launch_bounds__(team_threads(TEAM)) void norm_gradient_kernel(NormG
     }
 }
 
-// Sums over rows by group, in two steps: a workgroup adds `each` consecutive rows of
-// 512 columns, one partial row for every group among them; the pair (workgroup b,
-// group g) has slot b + g, and no other pair has it, since rows are in group order.
-// With v: of the rows' values times v's times r's two inverses.  All rows by one workgroup per
-// 512 columns (few rows): it writes the sums themselves (a.into.out), zero for the
-// groups without rows.
+// Sums over rows by group, in fp64 (fp32 sums of terms that cancel lose the difference's bits; 16
+// uneven groups of 16384 x 2048 bf16 16.8 -> 17.7 us, 14 of 2331 x 1201 fp32 12.1 -> 13.6), in two
+// steps: a workgroup adds `each` consecutive rows of 512 columns, one partial row for every group
+// among them; the pair (workgroup b, group g) has slot b + g, and no other pair has it, since
+// rows are in group order.  With v: of the rows' values times v's times r's two inverses.  All
+// rows by one workgroup per 512 columns (few rows): it writes the sums themselves (a.into.out),
+// zero for the groups without rows.
 constexpr int kSumColumns = 512;
 
 template <int VALUES>
 __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
 {
-    __shared__ float part[kThreads / 64][kSumColumns];
+    __shared__ double part[kThreads / 64][kSumColumns];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = blockIdx.x * kSumColumns + 8 * lane;
     const bool any = any_column<VALUES>(c, a.columns), whole = column_of<VALUES>(c, 7) < a.columns;
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
             const int src = __builtin_ctzll(todo);
             todo &= todo - 1;
             const int begin = __builtin_amdgcn_readlane(lo, src), end = __builtin_amdgcn_readlane(hi, src);
-            float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             // eight rows' loads of a wave go out together
             constexpr int WAVES = kThreads / 64, AHEAD = 8;
             int r = begin + wave;
@@ -441,19 +442,21 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
 #pragma unroll
                     for (int x = 0; x < AHEAD; ++x)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[j] += e[x].get(j);
+                        for (int j = 0; j < 8; ++j) sum[j] += (double)e[x].get(j);
                 }
-            // and the rest's of them, the last row in the place of those past the end (16 uneven
-            // groups of 16384 x 2048 bf16 19.9 -> 16.7 us, of 16384 x 2048 fp32 34.2 -> 30.3; 14 of
-            // 2331 x 1201 fp32 10.8 -> 11.9)
+            // and the rest's of them, the last row in the place of those past the end, which are not
+            // added (16 uneven groups of 16384 x 2048 bf16 with sums in fp32 19.9 -> 16.7 us, fp32
+            // 34.2 -> 30.3; 14 of 2331 x 1201 fp32 10.8 -> 11.9)
             if (whole && !a.v && r < end) {
                 Eight<VALUES> e[AHEAD];
 #pragma unroll
                 for (int x = 0; x < AHEAD; ++x) load_whole_eight(e[x], a.x, min(r + x * WAVES, end - 1) * a.ldx, c);
 #pragma unroll
-                for (int x = 0; x < AHEAD; ++x)
+                for (int x = 0; x < AHEAD; ++x) {
+                    if (r + x * WAVES >= end) continue;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[j] += r + x * WAVES < end ? e[x].get(j) : 0.f;
+                    for (int j = 0; j < 8; ++j) sum[j] += (double)e[x].get(j);
+                }
                 r = end;
             }
             if (any)
@@ -465,19 +468,19 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
                         load_eight(v, a.v, r * a.ldv, c, a.columns);
                         const float inverse = a.inverse[2 * (long long)r], times = a.inverse[2 * (long long)r + 1];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[j] += e.get(j) * (v.get(j) * times * inverse);
+                        for (int j = 0; j < 8; ++j) sum[j] += (double)e.get(j) * (double)(v.get(j) * times * inverse);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[j] += e.get(j);
+                        for (int j = 0; j < 8; ++j) sum[j] += (double)e.get(j);
                     }
                 }
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < 8; ++j) part[wave][column_of<VALUES>(8 * lane, j)] = sum[j];
             __syncthreads();
-            float *out = a.partial + (long long)(blockIdx.y + g0 + src) * a.columns + blockIdx.x * kSumColumns;
+            double *out = a.partial + (long long)(blockIdx.y + g0 + src) * a.columns + blockIdx.x * kSumColumns;
             for (int i = threadIdx.x; i < min(kSumColumns, a.columns - blockIdx.x * kSumColumns); i += kThreads) {
-                float v = 0.f;
+                double v = 0;
 #pragma unroll
                 for (int w = 0; w < kThreads / 64; ++w) v += part[w][i];
                 if (own) store_sum<VALUES>(a.into, g0 + src, blockIdx.x * kSumColumns + i, v);
@@ -489,10 +492,10 @@ __global__ __launch_bounds__(kThreads) void column_sums_kernel(ColumnSumsArgs a)
 
 // out[g][c] (+)= the sum of partial rows: 16 columns per workgroup, EACH threads each.
 // The partial rows of group g are those of the row ranges it touches.
-template <int VALUES, int EACH>
+template <int VALUES, int EACH, class Partial>
 __global__ __launch_bounds__(16 * EACH) void add_partials_kernel(AddPartialsArgs a)
 {
-    __shared__ float part[EACH][17];
+    __shared__ double part[EACH][17];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4, g = blockIdx.y;
     const int c = blockIdx.x * 16 + x;
     int begin = 0, end = a.count;
@@ -502,10 +505,11 @@ __global__ __launch_bounds__(16 * EACH) void add_partials_kernel(AddPartialsArgs
         begin = lo < hi ? lo / a.each + g : 0;
         end = lo < hi ? (hi - 1) / a.each + g + 1 : 0;
     }
-    float sum = 0.f;
+    double sum = 0;
     if (c < a.columns) {
+        const Partial *partial = reinterpret_cast<const Partial *>(a.partial) + c;
 #pragma unroll 8
-        for (int p = begin + y; p < end; p += EACH) sum += a.partial[(long long)p * a.columns + c];
+        for (int p = begin + y; p < end; p += EACH) sum += (double)partial[(long long)p * a.columns];
     }
     part[y][x] = sum;
     __syncthreads();
@@ -515,7 +519,7 @@ __global__ __launch_bounds__(16 * EACH) void add_partials_kernel(AddPartialsArgs
         __syncthreads();
     }
     if (y == 0 && c < a.columns) {
-        sum = 0.f;
+        sum = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += part[i][x];
         if (begin == end && a.accumulate) return;
@@ -608,12 +612,12 @@ hipError_t launch_norm_forward(const NormArgs &a, int values, hipStream_t s)
 namespace {
 
 // many: partial rows of a group.
-template <int V>
+template <int V, class Partial>
 hipError_t launch_add(const AddPartialsArgs &a, int many, hipStream_t s)
 {
     const dim3 grid((a.columns + 15) / 16, a.groups);
-    if (many > 32) hipLaunchKernelGGL((add_partials_kernel<V, 64>), grid, dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL((add_partials_kernel<V, 16>), grid, dim3(256), 0, s, a);
+    if (many > 32) hipLaunchKernelGGL((add_partials_kernel<V, 64, Partial>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((add_partials_kernel<V, 16, Partial>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -632,10 +636,10 @@ int sum_rows_each(int rows, int groups, int columns)
     const int slices = std::max(1, 256 / std::min(strips, 256));
     return few_sums(rows, groups) ? 64 : std::max(32, (rows + slices - 1) / slices);
 }
-size_t sum_floats(int rows, int groups, int columns)
+size_t sum_bytes(int rows, int groups, int columns)
 {
     const int each = sum_rows_each(rows, groups, columns);
-    return (size_t)((rows + each - 1) / each + groups) * columns;
+    return (size_t)((rows + each - 1) / each + groups) * columns * sizeof(double);
 }
 
 hipError_t launch_column_sums(ColumnSumsArgs a, const AddPartialsArgs &add, int values, hipStream_t s)
@@ -647,15 +651,15 @@ hipError_t launch_column_sums(ColumnSumsArgs a, const AddPartialsArgs &add, int 
         if (a.rows > 0)
             hipLaunchKernelGGL(column_sums_kernel<V>, dim3((a.columns + kSumColumns - 1) / kSumColumns, (a.rows + a.each - 1) / a.each),
                                dim3(kThreads), 0, s, a);
-        return one ? hipGetLastError() : launch_add<V>(add, a.rows / a.each / a.groups, s);
+        return one ? hipGetLastError() : launch_add<V, double>(add, a.rows / a.each / a.groups, s);
     });
 }
 
-size_t norm_gradient_floats(int rows, int columns)
+size_t norm_gradient_bytes(int rows, int columns)
 {
     if (rows == 0) return 0;
-    if (shape_of(rows, columns).nv) return (size_t)gradient_blocks(rows, columns) * columns;
-    return 2 * (size_t)rows + sum_floats(rows, 1, columns);
+    if (shape_of(rows, columns).nv) return (size_t)gradient_blocks(rows, columns) * columns * sizeof(float);
+    return 2 * (size_t)rows * sizeof(float) + sum_bytes(rows, 1, columns);
 }
 
 hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddPartialsArgs &into, int values, hipStream_t s)
@@ -688,7 +692,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         if (shape.nv || a.rows == 0) {
             add.partial = workspace;
             add.count = a.rows ? blocks : 0;
-            return launch_add<V>(add, add.count, s);
+            return launch_add<V, float>(add, add.count, s);
         }
         ColumnSumsArgs c;
         c.x = a.dy;
@@ -696,7 +700,7 @@ hipError_t launch_norm_gradient(NormGradientArgs a, float *workspace, const AddP
         c.v = a.s;
         c.ldv = a.lds;
         c.inverse = a.inverse;
-        c.partial = workspace + 2 * (size_t)a.rows;
+        c.partial = reinterpret_cast<double *>(workspace + 2 * (size_t)a.rows);
         c.rows = add.rows = a.rows;
         c.columns = a.columns;
         c.groups = 1;

@@ -694,8 +694,8 @@ int32_t gtmoe_grouped_fused_forward(gtmoe_context *ctx, const gtmoe_grouped_desc
                                     void *stream);
 /* bias_gradients[g] (+)= sum over g's rows of output_gradients[r] (Layer.Backward,
  * perceptron/layer.go:164-210): groups rows of `outputs` values, contiguous, of type
- * gradient_values, the rows' own or float32.  accumulate == 0: an empty group's become
- * zero.  The inputs, weights and their strides of the description are checked but
+ * gradient_values, the rows' own or float32, added in 64 bits and rounded once.
+ * accumulate == 0: an empty group's become zero.  The inputs, weights and their strides of the description are checked but
  * not used.  With one group offsets may be NULL.  The workspace: gtmoe_grouped_bias_workspace bytes,
  * 16-byte aligned. */
 int32_t gtmoe_grouped_bias_workspace(const gtmoe_grouped_desc *desc, size_t *bytes);

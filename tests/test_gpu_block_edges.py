@@ -255,3 +255,26 @@ def test_route_gates_of_what_is_not_finite(ctx, biased, renormalize):
         sums.append(8)
     assert not np.isfinite(got[sums]).any()
     assert np.isfinite(got[np.setdiff1d(np.arange(40), [3, 8, 9])]).all()
+
+
+# --------------------------------------------------------------------------
+# bias gradients
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sizes, columns", [([300], 130), ([32], 2048), ([9000, 0, 3, 4000], 70), ([1, 700] * 40, 33)])
+def test_bias_gradients_are_rounded_once(ctx, kind, sizes, columns):
+    """Sums in 64 bits: below 2^-40 of the terms, 2^14 at most, and one rounding, also where terms of 1e4 cancel."""
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    R, G = int(off[-1]), len(sizes)
+    rng = np.random.default_rng(R)
+    v = rng.normal(size=(R, columns)) + 1e4 * (-1.0) ** np.arange(R)[:, None]
+    dy, db = Rows(kind, R, columns, data=v), Rows("f32", G, columns)
+    d = gt.grouped_desc(VALUES[kind], G, R, 8, columns)
+    dev, ws = torch.from_numpy(off).cuda(), workspace(gt.grouped_bias_workspace_bytes(d))
+    gt.grouped_bias_gradient(ctx, d, dev.data_ptr(), dy.ptr, db.ptr, gt.VALUES_FLOAT32, False, ws.data_ptr(), stream())
+    v = dy.get()
+    want = np.stack([v[off[g]:off[g + 1]].sum(axis=0) for g in range(G)])
+    size = np.stack([np.abs(v[off[g]:off[g + 1]]).sum(axis=0) for g in range(G)])
+    near(db.get(), want, size * 2.0 ** -40, "f32")
+    assert bool((ws[-64:] == 0xA5).all())
