@@ -679,6 +679,15 @@ def adapted_desc(values, rows, inputs, outputs, adapters, rank, input_stride=Non
                        inputs if weight_stride is None else weight_stride)
 
 
+def _workspace(workspace, size):
+    """(address, bytes) of a workspace.  A buffer (a tensor: data_ptr() and nbytes) has its own size, or
+    the smaller one given with it, and the library refuses one that is too small; so it does an address
+    with a size.  An address alone cannot be checked: it is taken for as large as the call needs."""
+    if hasattr(workspace, "data_ptr"):
+        return workspace.data_ptr(), workspace.nbytes if size is None else min(size, workspace.nbytes)
+    return workspace, C.c_size_t(-1).value if size is None else size
+
+
 def adapted_workspace_bytes(desc):
     """Bytes of the workspace adapted_forward needs: the rows' products with
     their Down matrices in fp32, padded to eight ranks, the rows' order by
@@ -692,10 +701,11 @@ def adapted_forward(ctx, desc, inputs_ptr, weights_ptr, biases_ptr, adapter_ptr,
                     outputs_ptr, workspace_ptr, stream=None, workspace_bytes=None):
     """outputs[t] = W inputs[t] + b + s_a Up_a (Down_a inputs[t]) with each
     row's own adapter a; weights_ptr None: added to outputs (gtmoe_adapted_forward).
-    workspace_bytes: the workspace's size, adapted_workspace_bytes(desc) unless given."""
-    n = adapted_workspace_bytes(desc) if workspace_bytes is None else workspace_bytes
+    workspace_ptr: a buffer of adapted_workspace_bytes(desc), or an address and workspace_bytes; an address
+    alone is not checked."""
+    workspace, n = _workspace(workspace_ptr, workspace_bytes)
     ctx.check(library().gtmoe_adapted_forward(ctx.handle, C.byref(desc), inputs_ptr, weights_ptr, biases_ptr,
-                                              adapter_ptr, down_ptr, up_ptr, scales_ptr, outputs_ptr, workspace_ptr, n,
+                                              adapter_ptr, down_ptr, up_ptr, scales_ptr, outputs_ptr, workspace, n,
                                               stream))
 
 
@@ -717,10 +727,6 @@ def dropout(ctx, desc, inputs_ptr, base_ptr, outputs_ptr, rate, seed, offset, st
 # --------------------------------------------------------------------------
 # a block in plain rows (raw device addresses)
 # --------------------------------------------------------------------------
-
-# a workspace's size where the caller gives none: as large as the call needs
-_ENOUGH = C.c_size_t(-1).value
-
 
 def _scales_per_row(columns, scale_columns):
     return -(-columns // scale_columns) if scale_columns else 1
@@ -771,11 +777,12 @@ def norm_gradient(ctx, desc, output_gradients_ptr, sums_ptr, weights_ptr, sum_gr
                   weight_gradients_ptr, gradient_values, accumulate=False, workspace_ptr=None, stream=None,
                   workspace_bytes=None):
     """The gradients of inputs and weights (gtmoe_norm_gradient).
-    workspace_bytes: the workspace's size, taken for norm_workspace_bytes(desc) or more unless given."""
-    n = _ENOUGH if workspace_bytes is None else workspace_bytes
+    workspace_ptr: a buffer of norm_workspace_bytes(desc), or an address and workspace_bytes; an address
+    alone is not checked."""
+    workspace, n = _workspace(workspace_ptr, workspace_bytes)
     ctx.check(library().gtmoe_norm_gradient(ctx.handle, C.byref(desc), output_gradients_ptr, sums_ptr, weights_ptr,
                                             sum_gradients_ptr, input_gradients_ptr, weight_gradients_ptr, gradient_values,
-                                            1 if accumulate else 0, workspace_ptr, n, stream))
+                                            1 if accumulate else 0, workspace, n, stream))
 
 
 def activation_desc(values, rows, columns, activation, limit=0.0, codes=CODES_NONE, scale_columns=None, gate_stride=None,
@@ -827,11 +834,12 @@ def grouped_bias_workspace_bytes(desc):
 def grouped_bias_gradient(ctx, desc, offsets_ptr, output_gradients_ptr, bias_gradients_ptr, gradient_values,
                           accumulate=False, workspace_ptr=None, stream=None, workspace_bytes=None):
     """bias_gradients[g] (+)= sum of output_gradients[r] over the group's rows.
-    workspace_bytes: the workspace's size, taken for grouped_bias_workspace_bytes(desc) or more unless given."""
-    n = _ENOUGH if workspace_bytes is None else workspace_bytes
+    workspace_ptr: a buffer of grouped_bias_workspace_bytes(desc), or an address and workspace_bytes; an address
+    alone is not checked."""
+    workspace, n = _workspace(workspace_ptr, workspace_bytes)
     ctx.check(library().gtmoe_grouped_bias_gradient(ctx.handle, C.byref(desc), offsets_ptr, output_gradients_ptr,
                                                     bias_gradients_ptr, gradient_values, 1 if accumulate else 0,
-                                                    workspace_ptr, n, stream))
+                                                    workspace, n, stream))
 
 
 def route_desc(values, tokens, experts, experts_per_token, expert_groups=1, chosen_groups=1, group_best=1,
@@ -851,10 +859,11 @@ def route_workspace_bytes(desc):
 def route_forward(ctx, desc, logits_ptr, biases_ptr, chosen_ptr, gates_ptr, expert_offsets_ptr=None,
                   rows_for_expert_ptr=None, places_ptr=None, workspace_ptr=None, stream=None, workspace_bytes=None):
     """Every token's experts and gates, and the rows in expert order (gtmoe_route_forward).
-    workspace_bytes: the workspace's size, taken for route_workspace_bytes(desc) or more unless given."""
-    n = _ENOUGH if workspace_bytes is None else workspace_bytes
+    workspace_ptr: a buffer of route_workspace_bytes(desc), or an address and workspace_bytes; an address
+    alone is not checked."""
+    workspace, n = _workspace(workspace_ptr, workspace_bytes)
     ctx.check(library().gtmoe_route_forward(ctx.handle, C.byref(desc), logits_ptr, biases_ptr, chosen_ptr, gates_ptr,
-                                            expert_offsets_ptr, rows_for_expert_ptr, places_ptr, workspace_ptr, n, stream))
+                                            expert_offsets_ptr, rows_for_expert_ptr, places_ptr, workspace, n, stream))
 
 
 def route_gradient(ctx, desc, logits_ptr, chosen_ptr, gate_gradients_ptr, logit_gradients_ptr, stream=None):

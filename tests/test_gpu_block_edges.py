@@ -272,7 +272,10 @@ def test_bias_gradients_are_rounded_once(ctx, kind, sizes, columns):
     dy, db = Rows(kind, R, columns, data=v), Rows("f32", G, columns)
     d = gt.grouped_desc(VALUES[kind], G, R, 8, columns)
     dev, ws = torch.from_numpy(off).cuda(), workspace(gt.grouped_bias_workspace_bytes(d))
-    gt.grouped_bias_gradient(ctx, d, dev.data_ptr(), dy.ptr, db.ptr, gt.VALUES_FLOAT32, False, ws.data_ptr(), stream())
+    # (the workspace as a buffer, whose size is checked)
+    with pytest.raises(gt.InvalidArgument, match="the workspace has 16 bytes"):
+        gt.grouped_bias_gradient(ctx, d, dev.data_ptr(), dy.ptr, db.ptr, gt.VALUES_FLOAT32, False, ws[:16], stream())
+    gt.grouped_bias_gradient(ctx, d, dev.data_ptr(), dy.ptr, db.ptr, gt.VALUES_FLOAT32, False, ws, stream())
     v = dy.get()
     want = np.stack([v[off[g]:off[g + 1]].sum(axis=0) for g in range(G)])
     size = np.stack([np.abs(v[off[g]:off[g + 1]]).sum(axis=0) for g in range(G)])
