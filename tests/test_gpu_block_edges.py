@@ -7,8 +7,9 @@ import torch
 
 import gotransformers_amd as gt
 from tests import plain_block as plain
-from tests.device_rows import Rows, say, stream
+from tests.device_rows import Rows, rounded, say, stream
 from tests.plain_rows import HALF_LAST_STEP, HALF_STEP, VALUES
+from tests.test_gpu_block_rows import Product, whole
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -281,3 +282,27 @@ def test_bias_gradients_are_rounded_once(ctx, kind, sizes, columns):
     size = np.stack([np.abs(v[off[g]:off[g + 1]]).sum(axis=0) for g in range(G)])
     near(db.get(), want, size * 2.0 ** -40, "f32")
     assert bool((ws[-64:] == 0xA5).all())
+
+
+# --------------------------------------------------------------------------
+# products with an epilogue
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("groups, rows", [(65, 13), (130, 5), (300, 13), (300, 14), (200, 200)])
+@pytest.mark.parametrize("widths", [(72, 136), (129, 130)])
+@pytest.mark.parametrize("layout", ["packed", "odd"])
+def test_fused_product_of_few_rows_in_many_groups(ctx, kind, groups, rows, widths, layout):
+    """Whole numbers, exact in fp32; the 64th group, the next and the last are among those with rows.  Three
+    rows more are of no group: 16 of all are the few rows' kernel's, 17 the tiles'."""
+    rng = np.random.default_rng(groups + rows)
+    sizes = np.bincount(np.concatenate([[63, 64, groups - 1], rng.integers(0, groups, size=rows - 3)]), minlength=groups)
+    p = Product(kind, (list(sizes), 1), widths, layout, "bfrp", "relu", whole)
+    say(f"few rows {kind} {groups} {rows} {widths} {layout}")
+    p.call(ctx)
+    z, _, _, y = p.reference()
+    inside = slice(p.off[0], p.off[-1])
+    for have, want in ((p.y, y), (p.z, z)):
+        got = have.get()
+        assert np.array_equal(got[inside], rounded(want, kind)[inside]) and p.untouched(got)
+        have.check_outside()
