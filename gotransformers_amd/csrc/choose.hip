@@ -621,8 +621,9 @@ __global__ __launch_bounds__(kPlaceThreads) void place_kernel(ChooseArgs a, int 
     each_choice([&](int i, int e) { place(a, first, i, e, start, mask); });
 }
 
-// A choice outside the experts takes part in nothing.
-template <int VALUES, int TEAM, int EPL>
+// A choice outside the experts takes part in nothing.  ALL: every expert has a term (of a softmax
+// over all of them), not the chosen alone.
+template <int VALUES, int TEAM, int EPL, bool ALL>
 __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradientArgs a)
 {
     constexpr int TEAMS = 64 / TEAM;
@@ -648,19 +649,42 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
             expert = -1;
             dg = 0;
         }
-        double out[EPL], d;  // d: what this lane's choice adds to its expert's gradient
+        double d;  // what this lane's choice adds to its expert's gradient
+        // the choices' terms to those of all experts, and the row
+        auto finish = [&](auto (&out)[EPL]) {
+            typedef typename std::remove_reference<decltype(out[0])>::type Sum;
+            for (int j = 0; j < a.k; ++j) {
+                const int from = 4 * (team * TEAM + j);
+                const int e = __builtin_amdgcn_ds_bpermute(from, expert);
+                Sum v;
+                if constexpr (sizeof(Sum) == 8) v = permuted(from, d);
+                else v = __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)__float_as_uint((float)d)));
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) out[i] = 0;
-        if (a.renormalize) {
-            const double share = share_of<TEAM>(l, have, a.logistic);
-            const double dot = team_total<TEAM>(have ? share * dg : 0.0);
-            d = share * (dg - dot);
-            if (a.logistic) d *= logistic64(-l);
-        } else if (a.logistic) {
-            d = dg * logistic64(l) * logistic64(-l);
-        } else {
+                for (int i = 0; i < EPL; ++i)
+                    if (e == e0 + i) out[i] += v;
+            }
+            if (!here) return;
+            typedef typename Eight<VALUES>::Store Store;
+            Store *p = reinterpret_cast<Store *>(a.logit_gradients) + t * a.ldgradients + e0;
+            Store w[EPL];
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                const float v = (float)out[i];
+                if constexpr (VALUES == kValuesF32) w[i] = v;
+                else if constexpr (VALUES == kValuesBf16) w[i] = __builtin_bit_cast(uint16_t, (__bf16)v);
+                else w[i] = __builtin_bit_cast(uint16_t, (_Float16)v);
+            }
+            if (e0 + EPL <= a.experts) {
+                __builtin_memcpy(p, w, sizeof w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i)
+                    if (e0 + i < a.experts) p[i] = w[i];
+            }
+        };
+        if constexpr (ALL) {
             float all[EPL], most;
-            double sum = 0;
+            double out[EPL], sum = 0;
             load_logits<VALUES>(all, a.logits, t * a.ldlogits, e0, a.experts);
             most = all[0];
 #pragma unroll
@@ -678,32 +702,18 @@ __global__ __launch_bounds__(kThreads) void choose_gradient_kernel(ChooseGradien
             const double by = -team_total<TEAM>(d) * inverse;
 #pragma unroll
             for (int i = 0; i < EPL; ++i) out[i] *= by;
-        }
-        for (int j = 0; j < a.k; ++j) {
-            const int from = 4 * (team * TEAM + j);
-            const int e = __builtin_amdgcn_ds_bpermute(from, expert);
-            const double v = permuted(from, d);
-#pragma unroll
-            for (int i = 0; i < EPL; ++i)
-                if (e == e0 + i) out[i] += v;
-        }
-        if (!here) continue;
-        typedef typename Eight<VALUES>::Store Store;
-        Store *p = reinterpret_cast<Store *>(a.logit_gradients) + t * a.ldgradients + e0;
-        Store w[EPL];
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            const float v = (float)out[i];
-            if constexpr (VALUES == kValuesF32) w[i] = v;
-            else if constexpr (VALUES == kValuesBf16) w[i] = __builtin_bit_cast(uint16_t, (__bf16)v);
-            else w[i] = __builtin_bit_cast(uint16_t, (_Float16)v);
-        }
-        if (e0 + EPL <= a.experts) {
-            __builtin_memcpy(p, w, sizeof w);
+            finish(out);
         } else {
-#pragma unroll
-            for (int i = 0; i < EPL; ++i)
-                if (e0 + i < a.experts) p[i] = w[i];
+            if (a.renormalize) {
+                const double share = share_of<TEAM>(l, have, a.logistic);
+                const double dot = team_total<TEAM>(have ? share * dg : 0.0);
+                d = share * (dg - dot);
+                if (a.logistic) d *= logistic64(-l);
+            } else {
+                d = dg * logistic64(l) * logistic64(-l);
+            }
+            float out[EPL] = {};  // an expert has one choice's term alone, but for one that stands twice
+            finish(out);
         }
     }
 }
@@ -806,7 +816,9 @@ hipError_t launch_choose_gradient(const ChooseGradientArgs &a, int values, hipSt
             constexpr int T = decltype(team)::value;
             const int tokens = kThreads / T;
             const unsigned blocks = (unsigned)std::min<long long>(((long long)a.tokens + tokens - 1) / tokens, 1 << 20);
-            hipLaunchKernelGGL((choose_gradient_kernel<decltype(v)::value, T, decltype(epl)::value>), dim3(blocks), dim3(kThreads), 0, s, a);
+            constexpr int V = decltype(v)::value, E = decltype(epl)::value;
+            if (a.renormalize || a.logistic) hipLaunchKernelGGL((choose_gradient_kernel<V, T, E, false>), dim3(blocks), dim3(kThreads), 0, s, a);
+            else hipLaunchKernelGGL((choose_gradient_kernel<V, T, E, true>), dim3(blocks), dim3(kThreads), 0, s, a);
             return hipGetLastError();
         });
     });
