@@ -21,7 +21,8 @@
 // Renormalized gates take the chosen scores by their largest, so that neither large nor
 // very negative logits leave 0 / 0:  s = e^l, or e^min(l, 0) / (1 + e^-|l|).
 // Gates and gradients are taken in fp64 and rounded once (16384 tokens below: 20.8 -> 21.4 us with
-// the lists; in fp32 with its sums they were off by 2.2 times a rounding).
+// the lists, the gradient's kernel 5.0 -> 6.3; in fp32 with its sums they were off by 2.2 times a
+// rounding).
 //
 // Lists.  A workgroup takes `each` consecutive tokens and writes how often each
 // expert was chosen among them; the second kernel adds the counts of the
@@ -31,9 +32,12 @@
 //
 // What bounds it (MI355X): the vector unit and the chain of the rounds; the bytes would
 // take 1 us.  16384 tokens x 128 experts, k = 8, sigmoid with biases, 4 of 8 groups by their best
-// two: 14.6 us (of some 850 vector instructions per four tokens, 235 are the scores, 420
-// the rounds), lists 6.5.  8192 x 64, k = 4, softmax: 4.4, lists 5.9, gradient 3.9.  32 x 64,
-// k = 6, with lists 4.8, one launch.
+// two: 15.4 us (of some 850 vector instructions per four tokens besides the gates, 235 are the
+// scores, 420 the rounds; issue alone would take some 6), lists 6.8 (every workgroup adds the counts of
+// all, one wave of it scans, three barriers between).  8192 x 64, k = 4, softmax: 5.3, lists 5.9,
+// gradient 4.2.  32 x 64, k = 6, with lists 5.0, one launch.  131072 x 64, k = 6: 22.9, sums before each
+// workgroup 5.9, lists 7.1.  16384 x 700, k = 20: 86.5, lists 19.5.  16384 x 60, k = 5, 2 of 5 groups,
+// found through LDS: 8.7.
 #include <algorithm>
 #include <type_traits>
 

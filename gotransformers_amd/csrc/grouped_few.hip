@@ -8,9 +8,11 @@
 // however few rows there are every XCD streams its share of W, and the row tiles of
 // a group, a multiple of eight workgroups apart, find W in the same L2.
 //
-// What bounds it (MI355X): a launch and two trips to memory.  32 rows of 1024 -> 2048 bf16 with
-// bias, SiLU and factor 6.8 us, W's 4 MB alone 0.8; 64 groups of 2048 -> 1024, a row each, 58.6,
-// W's 268 MB at 4.6 TB/s.
+// What bounds it (MI355X): a launch and a wave's trips to memory one after the other.  32 rows of
+// 1024 -> 2048 bf16 with bias, SiLU and factor 6.8 us, W's 4 MB alone 0.8: a wave has four steps of the
+// reduction, too few for the batch of multiply_rows, and waits for each one's loads; then the factor's.
+// 128 workgroups stream W, half of the CUs.  The same in fp32 10.  64 groups of 2048 -> 1024, a row
+// each, 58.6, W's 268 MB at 4.6 TB/s.
 #include "grouped_rows.h"
 
 namespace gtmoe {

@@ -60,8 +60,10 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c)
 
 // acc[p][q] += a_p b_q^T over the reduction [0, length) that falls to this
 // wave (every WAVES-th 64 bytes), a_p and b_q the lane's rows of NP and NQ
-// 16-row operands.  Loads go straight to MFMA operands; `ahead` steps of them
-// are requested together.
+// 16-row operands.  Loads go straight to MFMA operands, those of `ahead` steps from
+// one loop, in which the compiler keeps up to seven loads in flight (one and two operands of
+// 16 bits: 18 loads, the first wait behind seven).  Steps that are fewer, and the last
+// ones, go one by one, each behind its loads.
 template <class T, int WAVES, int NP, int NQ>
 __device__ __forceinline__ void multiply_rows(const typename T::Store *const (&pa)[NP], const typename T::Store *const (&pb)[NQ],
                                               int length, int wave, f32x4 (&acc)[NP][NQ])

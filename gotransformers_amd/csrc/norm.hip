@@ -14,12 +14,14 @@
 // of a team, one partial row per workgroup, which a second kernel adds in a fixed
 // order; few rows are one workgroup's, which writes dw itself.
 //
-// What bounds it (MI355X): memory.  8192 x 2048 bf16, residual and sums: forward 28.0 us (134 MB
-// at 4.8 TB/s, a large copy reaches 5.0), gradient 33.3 and its partial rows' sums 4.9.
-// 2331 x 1201 fp32, rows that begin anywhere: 12.5 (3.6 TB/s), 12.2 and 4.  One row: 4.2, a
-// launch and two trips to memory.  The gradient's gap is the work between a row's loads and
-// its store; the next row's loads ahead of it, or two rows at a time, took more registers
-// and fewer waves: 40 to 53 and 54 us.
+// What bounds it (MI355X): memory.  8192 x 2048 bf16, residual and sums: forward 28.6 us (134 MB
+// at 4.7 TB/s, a large copy reaches 5.0), gradient 31.5 (4.5 TB/s) and its partial rows' sums 4.9,
+// which read their lines two to three times over, sixteen columns a workgroup.  2331 x 1201 fp32,
+// rows that begin anywhere: 13.2 (3.5 TB/s), 12.4 and 4.3.  Into 8 bits 8192 x 2048 bf16: int8 with
+// a scale per 128 columns 20.7, E4M3 with one per row 22.2.  512 rows of 40000, read again: 19.6, gradient 36.7
+// and, for the weights, 39 and 5.  One row: 4.0, a launch and two trips to memory.  The gradient's
+// gap is the work between a row's loads and its store; the next row's loads ahead of it, or two
+// rows at a time, took more registers and fewer waves: 40 to 53 and 54 us.
 #include "rows.h"
 
 #include <algorithm>

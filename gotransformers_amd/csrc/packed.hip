@@ -10,10 +10,10 @@
 // neighbouring lanes, whose maximum they find by DPP.
 //
 // What bounds it (MI355X): memory, with arithmetic close behind in the forward with codes.
-// 16384 x 2048 bf16, SiLU, int8 with a scale per 128 columns: forward 59 us (273 MB, 4.6 TB/s),
-// gradient with y again 65 (340 MB, 5.2 TB/s); per 16 columns 59 and 66; without codes 39 and 75
-// (201 and 403 MB).  2331 x 1201 fp32, GELU, E4M3 per 32: 12.8 and 14.7.  Packing 8192 x 2048
-// fp16 rows per 16 columns 15.9, back 10.7.
+// 16384 x 2048 bf16, SiLU, int8 with a scale per 128 columns: forward 61 us (273 MB, 4.5 TB/s),
+// gradient with y again 64 (340 MB, 5.3 TB/s); per 16 columns 59 and 66; without codes 39 and 75
+// (201 and 403 MB).  2331 x 1201 fp32, GELU, E4M3 per 32: 13.6 and 15.0.  Packing 8192 x 2048
+// fp16 rows per 16 columns 13.5 to 15, back 10.2.
 #include <algorithm>
 #include <type_traits>
 
