@@ -116,16 +116,18 @@ hipError_t launch_values(const GroupedArgs &a, hipStream_t s)
 //     partly cached, 39.6 against 47.8), two in fp32 (32 rows 33.7 against 33.3, 2 rows 8.3 against 20.9)
 //   16-bit rows that LDS-DMA cannot take: up to 192 (1201 -> 1000, 128 rows 12.0 against
 //     19.4, 192 19.6 against 19.7; 14 groups of 1000 -> 1201, 64 rows 11.6 against 12.5)
-//   more than 64 groups, with a bias and SiLU, rows dealt at random: 16 rows (128 of 2048 -> 1024
-//     bf16, 4 rows 6.5 against 11.8, 16 rows 14.2 against 14.3, 24 rows 20.6 against 19.1; 256 of
-//     1024 -> 512, 16 rows 7.1 against 9.9, 128 rows 27.2 against 23.4; 128 of 1001 -> 1201, 16 rows 18.8
-//     against 20.3, 24 rows 23.9 against 20.4), in fp32 a row per group (256 of 1024 -> 512, 32 rows
-//     14.9 against 23.8, 64 rows 27.7 against 25.8, 128 rows 45.2 against 54.3, 256 rows 76 against 85)
+//   more than 64 groups, with a bias and SiLU, rows dealt at random: 48 rows that make at most four
+//     workgroups per CU, were each a group's only one (bf16: 128 of 2048 -> 1024, 4 rows 6.5 against 11.8, 16 rows 14.2
+//     against 14.3, 24 rows 20.6 against 19.1; 256 of 1024 -> 512, 24 rows 8.5 against 9.9, 128 rows 27.2
+//     against 23.4; 128 of 1001 -> 1201, 4 rows 9.2 against 18.2, 24 rows 23.9 against 20.4; 128 of 64 ->
+//     8192, a row 4.1 against 6.8, 16 rows 22.5 against 14.3; of 16384 -> 64, 16 rows 22 against 54, 256
+//     rows 98 against 76; fp32: 256 of 1024 -> 512, 32 rows 14.9
+//     against 23.8, 64 rows 27.7 against 25.8; 1024 of 256 -> 256, 16 rows 9.8 against 19.0, 256 rows 42.0 against 28.5)
 bool few_fits(const GroupedArgs &a, int value_bytes, bool staged)
 {
     if (a.rows > kMostRows || row_tiles(a, 16) * columns_of(a, 16) > 1 << 22) return false;
     const bool wide = value_bytes == 4;
-    if (a.groups > 64) return a.rows <= (wide ? a.groups : 16);
+    if (a.groups > 64) return a.rows <= 48 && a.rows * ((a.outputs + 15) / 16) <= 1024;
     if (!wide && !staged) return a.rows <= 192;
     if (a.groups > 1) return a.rows <= a.groups * (wide ? 2 : 1);
     return a.rows <= 32 || (a.rows + 31) / 32 * ((a.outputs + 15) / 16) <= (wide ? 768 : 256);

@@ -289,12 +289,12 @@ def test_bias_gradients_are_rounded_once(ctx, kind, sizes, columns):
 # --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("groups, rows", [(65, 13), (130, 5), (300, 13), (300, 14), (200, 200)])
+@pytest.mark.parametrize("groups, rows", [(65, 13), (130, 5), (300, 45), (300, 46), (200, 200)])
 @pytest.mark.parametrize("widths", [(72, 136), (129, 130)])
 @pytest.mark.parametrize("layout", ["packed", "odd"])
 def test_fused_product_of_few_rows_in_many_groups(ctx, kind, groups, rows, widths, layout):
     """Whole numbers, exact in fp32; the 64th group, the next and the last are among those with rows.  Three
-    rows more are of no group: 16 of all are the few rows' kernel's, 17 the tiles'."""
+    rows more are of no group: 48 of all are the few rows' kernel's, 49 the tiles'."""
     rng = np.random.default_rng(groups + rows)
     sizes = np.bincount(np.concatenate([[63, 64, groups - 1], rng.integers(0, groups, size=rows - 3)]), minlength=groups)
     p = Product(kind, (list(sizes), 1), widths, layout, "bfrp", "relu", whole)
